@@ -116,6 +116,18 @@ SIGNATURES = {
                                           c_int],
     "ecd_layer_stack": [_P, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
                         c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P],
+    "ecd_page_free": [_P, c_int, _P, c_int, _P, c_int, c_int, _P, c_int, _P, _P],
+    "ecd_page_fork": [_P, _P, c_int, _P, c_int, _P, c_int, _P, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P],
+    "ecd_page_extend": [_P, c_int, _P, c_int, _P, c_int, c_int, _P, _P, _P],
+    "ecd_page_compact": [_P, _P, c_int, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int,
+                         c_int, _P],
+    "ecd_paged_write": [_P, c_long, _P, c_int, _P, _P, _P, _P, _P, c_long, c_int, c_int, c_int, c_int, c_int, c_int,
+                        c_int, c_int, _P],
+    "ecd_paged_attn": [_P, c_long, _P, _P, _P, c_long, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
+                       c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
+    "ecd_quant_a8": [_P, c_long, _P, c_float, _P, c_long, _P, c_int, c_int, _P],
+    "ecd_gemm_a8": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, _P],
+    "ecd_gemm_a8_silu": [_P, c_long, _P, _P, _P, _P, c_long, c_int, c_int, c_int, _P],
 }
 
 _lib = None

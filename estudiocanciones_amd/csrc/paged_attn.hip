@@ -1,0 +1,397 @@
+// Decode attention over pages of a KV cache, the prefix that a group of rows shares read once for all of them (gfx950).
+//
+// Row r (sequence r / S) attends slots [0, pos[r]] of its sequence: o = softmax(q k^T scale) v per query head, G = Hq / Hk
+// of them on each kv head.  The rows of a group hold the same slots [0, prefix).  Softmax splits over slots: with
+//   m = max s,  l = sum exp(s - m),  a = sum exp(s - m) v   over any part of the slots,
+// the whole is  o = sum_parts exp(m_part - M) a_part / sum_parts exp(m_part - M) l_part,  M = max m_part.
+// So a workgroup takes one part: an item of the plan (slots [lo, hi) of a group's prefix, for up to 16 CT columns, a
+// column being one query head of one row), or a share of one row's own slots.  A second kernel joins the parts.
+//
+// A row takes the shared parts only if it attends the whole prefix; else its own part covers [0, pos].  The shared slots
+// are read through the first such row's pages.
+#include "common.h"
+
+namespace ecd {
+
+constexpr int PQ_W = 4;       // waves of a workgroup
+constexpr int PQ_T = 32;      // slots of a wave's tile
+constexpr int PQ_MIN = PQ_W * PQ_T;  // slots of a row's own share at least
+
+// what does not change over a call
+struct PagedArgs {
+  const f16* q;      // row r at q + r ldq
+  const f16* kp;     // [NP, Hk, P, HD]
+  const f16* vp;
+  const int* table;  // row of sequence b at table + b ldt, MP entries
+  const int64_t* pos;
+  f16* o;            // [R, Hq, HD]
+  float* pm;         // [R Hq, parts]: maximum and sum of each part, then its unnormalised output
+  float* pl;
+  float* pa;         // [R Hq, parts, HD]
+  const int* items;  // {first row, rows, lo, hi, part} of each shared part
+  const int* rows;   // {shared slots, shared parts} of each row
+  long ldq, ldt;
+  int MP, NP, S, Hq, Hk, G, PS, nitems, nown, parts;  // PS: log2 of the page size
+  float c2;          // scale log2(e)
+};
+
+__device__ __forceinline__ float max_groups(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// One tile of 32 slots in registers.  Lane l: K of slots 16 j + (l & 15), dims 8 (l >> 4) + 32 i; V of slots
+// 16 j + 4 (l >> 4) + e, dims VW (l & 15) + 128 x.
+template <int HD>
+struct PTile {
+  static constexpr int KC = HD / 32, VW = HD >= 128 ? 8 : HD / 16, ND = (HD + 127) / 128;
+  typedef f16 vec __attribute__((ext_vector_type(VW)));
+  f16x8 k[2][KC];
+  vec v[2][4][ND];
+};
+
+// slots t0 .. t0 + 31 (t0 a multiple of 32) of the sequence whose page numbers are at `tab`; slots from hi on repeat a
+// slot before it (masked later)
+template <int HD>
+__device__ __forceinline__ void tile_load(PTile<HD>& t, const PagedArgs& a, const int* tab, int kh, int t0, int hi,
+                                          int lane) {
+  const int grp = lane >> 4, col = lane & 15, mask = (1 << a.PS) - 1;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int h0 = min(t0 + 16 * j, (hi - 1) & ~15);  // a half tile lies in one page
+    const int page = min(max(__builtin_amdgcn_readfirstlane(tab[h0 >> a.PS]), 0), a.NP - 1);
+    const long base = ((((long)page * a.Hk + kh) << a.PS) + (h0 & mask)) * HD;
+    const f16* k = a.kp + base + col * HD + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < PTile<HD>::KC; ++i) t.k[j][i] = *(const f16x8*)(k + 32 * i);
+    const f16* v = a.vp + base + 4 * grp * HD + PTile<HD>::VW * col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int x = 0; x < PTile<HD>::ND; ++x) t.v[j][e][x] = *(const typename PTile<HD>::vec*)(v + e * HD + 128 * x);
+  }
+}
+
+// The running softmax of CT tiles of 16 columns (lane l: column l & 15 of each).  acc[c][x][b]: row i of lane l is dim
+// 128 x + VW (4 (l >> 4) + i) + b.  l: this lane's share of the sum.
+template <int HD, int CT>
+struct PState {
+  static constexpr int VW = PTile<HD>::VW, ND = PTile<HD>::ND;
+  f16x8 q[CT][HD / 32];
+  f32x4 acc[CT][ND][VW];
+  float m[CT], l[CT];
+};
+
+// slots outside [lo, hi) of the tile at t0 do not count, whatever they hold
+template <int HD, int CT>
+__device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, float c2, int t0, int lo, int hi, int lane) {
+  using T = PTile<HD>;
+  const int grp = lane >> 4;
+  const bool edge = t0 < lo || t0 + PQ_T > hi;  // uniform
+  if (edge) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = t0 + 16 * j + 4 * grp + e;
+        if (k < lo || k >= hi)
+#pragma unroll
+          for (int x = 0; x < T::ND; ++x) t.v[j][e][x] = (typename T::vec)((f16)0);
+      }
+  }
+  f16x8 p[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    f32x4 sc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < T::KC; ++i) sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[j][i], s.q[c][i], sc[j], 0, 0, 0);
+    }
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = t0 + 16 * j + 4 * grp + e;
+          if (k < lo || k >= hi) sc[j][e] = -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[j][e]);
+    const float mn = fmaxf(s.m[c], max_groups(mx));
+    const float mb = mn == -INFINITY ? 0.f : mn * c2;
+    float ps = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][e], c2, -mb));
+        ps += w;
+        p[c][4 * j + e] = (f16)w;
+      }
+    if (__any(mn != s.m[c])) {
+      const float alpha = __builtin_amdgcn_exp2f(s.m[c] * c2 - mb);
+      s.l[c] *= alpha;
+#pragma unroll
+      for (int x = 0; x < T::ND; ++x)
+#pragma unroll
+        for (int b = 0; b < T::VW; ++b) s.acc[c][x][b] = s.acc[c][x][b] * alpha;
+    }
+    s.l[c] += ps;
+    s.m[c] = mn;
+  }
+#pragma unroll
+  for (int x = 0; x < T::ND; ++x)
+#pragma unroll
+    for (int b = 0; b < T::VW; ++b) {
+      const f16x8 va = {t.v[0][0][x][b], t.v[0][1][x][b], t.v[0][2][x][b], t.v[0][3][x][b],
+                        t.v[1][0][x][b], t.v[1][1][x][b], t.v[1][2][x][b], t.v[1][3][x][b]};
+#pragma unroll
+      for (int c = 0; c < CT; ++c) s.acc[c][x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[c], s.acc[c][x][b], 0, 0, 0);
+    }
+}
+
+// One part on one workgroup: `cols` columns (query head c % G of row row0 + c / G), slots [lo, hi) through `tab`.
+// `live(row)`: whether the row takes this part.  Its result goes to place `part`, or with `whole` normalised to o.
+template <int HD, int CT, typename Live>
+__device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0, int cols, int kh, const int* tab, int lo,
+                                       int hi, int part, bool whole, Live&& live) {
+  constexpr int ST = HD + 4;  // floats of a column in LDS
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = lane >> 4, col = lane & 15;
+  PState<HD, CT> s;
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int n = 16 * c + col;
+    const int cc = n < cols ? n : 0;
+    const f16* q = a.q + (long)(row0 + cc / a.G) * a.ldq + (long)(kh * a.G + cc % a.G) * HD + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) s.q[c][i] = *(const f16x8*)(q + 32 * i);
+    s.m[c] = -INFINITY;
+    s.l[c] = 0.f;
+#pragma unroll
+    for (int x = 0; x < PTile<HD>::ND; ++x)
+#pragma unroll
+      for (int b = 0; b < PTile<HD>::VW; ++b) s.acc[c][x][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  PTile<HD> t;
+  for (int t0 = (lo & ~(PQ_T - 1)) + wv * PQ_T; t0 < hi; t0 += PQ_W * PQ_T) {
+    tile_load<HD>(t, a, tab, kh, t0, hi, lane);
+    tile_attend<HD, CT>(s, t, a.c2, t0, lo, hi, lane);
+  }
+
+  // the waves' states to one: maxima and sums first, then the outputs on the common maximum
+  float* sm = lds;                    // [PQ_W][16 CT]
+  float* sl = lds + PQ_W * 16 * CT;
+  float* sa = lds + 2 * PQ_W * 16 * CT;  // [PQ_W][16 CT][ST]
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const float l = sum_groups(s.l[c]);
+    if (grp == 0) {
+      sm[wv * 16 * CT + 16 * c + col] = l == l ? s.m[c] : l;  // (a sum that is no number is not an empty part)
+      sl[wv * 16 * CT + 16 * c + col] = l;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < PQ_W; ++w) M = fmaxf(M, sm[w * 16 * CT + 16 * c + col]);
+    const float m = sm[wv * 16 * CT + 16 * c + col];
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * a.c2);
+    float* d = sa + (wv * 16 * CT + 16 * c + col) * ST;
+#pragma unroll
+    for (int x = 0; x < PTile<HD>::ND; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < PTile<HD>::VW; b += 4)
+          *(f32x4*)(d + 128 * x + PTile<HD>::VW * (4 * grp + i) + b) =
+              (f32x4){s.acc[c][x][b][i] * f, s.acc[c][x][b + 1][i] * f, s.acc[c][x][b + 2][i] * f, s.acc[c][x][b + 3][i] * f};
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < cols * (HD / 4); i += 64 * PQ_W) {
+    const int n = i / (HD / 4), d = 4 * (i - n * (HD / 4));
+    const int row = row0 + n / a.G;
+    const long head = (long)row * a.Hq + kh * a.G + n % a.G;
+    float M = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < PQ_W; ++w) M = fmaxf(M, sm[w * 16 * CT + n]);
+    f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < PQ_W; ++w) {
+      const float m = sm[w * 16 * CT + n];
+      l += m == -INFINITY ? 0.f : sl[w * 16 * CT + n] * __builtin_amdgcn_exp2f((m - M) * a.c2);
+      v = v + *(const f32x4*)(sa + (w * 16 * CT + n) * ST + d);
+    }
+    if (whole) {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a sum that is no number stays none)
+      *(f16x4*)(a.o + head * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
+    } else {
+      const long pi = head * a.parts + part;
+      M = !live(row) ? -INFINITY : l == l ? M : l;
+      if (d == 0) {
+        a.pm[pi] = M;
+        a.pl[pi] = l;
+      }
+      *(f32x4*)(a.pa + pi * HD + d) = v;
+    }
+  }
+}
+
+template <int HD, int CT>
+constexpr int attend_lds() {
+  return PQ_W * 16 * CT * (2 + HD + 4);
+}
+
+template <int HD, int CT>
+__global__ __launch_bounds__(64 * PQ_W) void paged_attn_kernel(PagedArgs a) {
+  __shared__ __align__(16) float lds[attend_lds<HD, CT>()];
+  __shared__ int s_lead;
+  const int kh = blockIdx.y;
+  if ((int)blockIdx.x < a.nitems) {
+    const int* it = a.items + 5 * blockIdx.x;
+    const int row0 = it[0], n = it[1], lo = it[2], hi = it[3];
+    // the first row that attends the whole prefix leads: its pages hold every shared slot
+    if (threadIdx.x < 64) {
+      const int r = row0 + threadIdx.x;
+      const bool in = (int)threadIdx.x < n && a.pos[r] + 1 >= a.rows[2 * r];
+      const uint64_t b = __ballot(in);
+      if (threadIdx.x == 0) s_lead = b ? row0 + __builtin_ctzll(b) : -1;
+    }
+    __syncthreads();
+    const int lead = __builtin_amdgcn_readfirstlane(s_lead);
+    const int hi1 = lead < 0 ? lo : min(hi, a.MP << a.PS);
+    attend<HD, CT>(a, lds, row0, n * a.G, kh, a.table + (long)max(lead, 0) / a.S * a.ldt, min(lo, hi1), hi1, it[4], false,
+                   [&](int row) { return a.pos[row] + 1 >= a.rows[2 * row]; });
+    return;
+  }
+  const int x = blockIdx.x - a.nitems, r = x / a.nown, k = x - r * a.nown;
+  const long p = a.pos[r];
+  const int end = (int)min(p < 0 ? 0l : p + 1, (long)a.MP << a.PS);
+  const int shared = a.rows[2 * r], np = a.rows[2 * r + 1];
+  const int from = end >= shared ? shared : 0;
+  const int per = (max(PQ_MIN, (end - from + a.nown - 1) / a.nown) + PQ_T - 1) & ~(PQ_T - 1);
+  const int lo = min(from + k * per, end), hi = min(lo + per, end);
+  attend<HD, 1>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1,
+                [](int) { return true; });
+}
+
+// One workgroup per (row, kv head): its parts in order.
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int HD) {
+  extern __shared__ float w[];  // [G][parts]
+  __shared__ float s_inv[16];
+  const int r = blockIdx.x, kh = blockIdx.y;
+  const int n = a.rows[2 * r + 1] + a.nown;
+  if (n == 1) return;
+  const long head = (long)r * a.Hq + kh * a.G;
+  for (int i = threadIdx.x; i < a.G * n; i += 256) {
+    const int g = i / n, k = i - g * n;
+    w[g * a.parts + k] = a.pm[(head + g) * a.parts + k];
+  }
+  __syncthreads();
+  for (int g = threadIdx.x >> 6; g < a.G; g += 4) {
+    const int lane = threadIdx.x & 63;
+    float M = -INFINITY, l = 0.f;
+    for (int k = lane; k < n; k += 64) M = fmaxf(M, w[g * a.parts + k]);
+    M = wave_max(M);
+    for (int k = lane; k < n; k += 64) {
+      const float m = w[g * a.parts + k];
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * a.c2);
+      w[g * a.parts + k] = f;
+      if (f != 0.f) l += f * a.pl[(head + g) * a.parts + k];
+    }
+    l = wave_sum(l);
+    if (lane == 0) s_inv[g] = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.G * (HD / 4); i += 256) {
+    const int g = i / (HD / 4), d = 4 * (i - g * (HD / 4));
+    f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < n; ++k) {
+      const float f = w[g * a.parts + k];
+      if (f != 0.f) v = v + *(const f32x4*)(a.pa + ((head + g) * a.parts + k) * HD + d) * f;
+    }
+    const float inv = s_inv[g];
+    *(f16x4*)(a.o + (head + g) * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
+  }
+}
+
+template <int HD, int CT>
+static int launch_paged(const PagedArgs& a, int R, hipStream_t st) {
+  hipLaunchKernelGGL((paged_attn_kernel<HD, CT>), dim3(a.nitems + R * a.nown, a.Hk), dim3(64 * PQ_W), 0, st, a);
+  return ecd_launch_status();
+}
+
+}  // namespace ecd
+
+using namespace ecd;
+
+extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const void* vp, const int32_t* table, long ldt,
+                              const int64_t* pos, void* o, float* ws, const int32_t* items, const int32_t* rows,
+                              int nitems, int nown, int parts, int ctiles, int R, int S, int MP, int NP, int Hq, int Hk,
+                              int P, int HD, float scale, void* stream) {
+  if (!q || !kp || !vp || !table || !pos || !o || !rows || (nitems > 0 && !items) || nitems < 0 || nown < 1 ||
+      parts < nown || (parts > 1 && !ws) || R <= 0 || S <= 0 || MP <= 0 || NP <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
+      Hq / Hk > 16 || P < 16 || (P & (P - 1)) || ldt < MP || ldq < (long)Hq * HD || (ldq % 8) ||
+      ((uintptr_t)q & 15) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)o & 7) || ((uintptr_t)ws & 15) ||
+      !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown + nitems > 0x7FFFFFFFL || Hk > 65535)
+    return ECD_EINVAL;
+  if ((HD != 64 && HD != 128 && HD != 256) || parts > 512) return ECD_ENOTSUP;
+  const long heads = (long)R * Hq, n2 = (heads * parts + 3) & ~3l;
+  PagedArgs a;
+  a.q = (const f16*)q;
+  a.kp = (const f16*)kp;
+  a.vp = (const f16*)vp;
+  a.table = table;
+  a.pos = pos;
+  a.o = (f16*)o;
+  a.pm = ws;
+  a.pl = ws + n2;
+  a.pa = ws + 2 * n2;
+  a.items = items;
+  a.rows = rows;
+  a.ldq = ldq;
+  a.ldt = ldt;
+  a.MP = MP;
+  a.NP = NP;
+  a.S = S;
+  a.Hq = Hq;
+  a.Hk = Hk;
+  a.G = Hq / Hk;
+  a.PS = __builtin_ctz((unsigned)P);
+  a.nitems = nitems;
+  a.nown = nown;
+  a.parts = parts;
+  a.c2 = scale * 1.44269504088896341f;
+  const hipStream_t st = (hipStream_t)stream;
+  int rc = ECD_ENOTSUP;
+#define PQ(HD_, CT_)                     \
+  if (HD == HD_ && ctiles == CT_) rc = launch_paged<HD_, CT_>(a, R, st)
+  PQ(64, 1);
+  PQ(64, 2);
+  PQ(64, 4);
+  PQ(128, 1);
+  PQ(128, 2);
+  PQ(128, 4);
+  PQ(256, 1);
+  PQ(256, 2);
+#undef PQ
+  if (rc != ECD_OK || parts == 1) return rc;
+  hipLaunchKernelGGL(paged_join_kernel, dim3(R, Hk), dim3(256), (size_t)a.G * parts * sizeof(float), st, a, HD);
+  return ecd_launch_status();
+}

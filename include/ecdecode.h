@@ -603,6 +603,78 @@ int ecd_codec_euler(void* x, const void* noise, const void* ic, const void* dphi
  * counterpart: a kernel of known HBM traffic used to calibrate hardware byte counters. */
 int ecd_copy_bytes(const void* src, void* dst, long nbytes, void* stream);
 
+/* ---- Pages of a KV cache, one prompt shared by many takes (no counterpart in the reference: its takes hold a dense
+ * cache each and compute the prompt once per take, app/engine.py:380-388).  The state lives on the device:
+ *   kv [planes, NP, Hk, P, HD] f16: NP pages of P slots in each plane (layer by layer, keys then values);
+ *   ref [NP] int32 owners of each page (0: free); table [B, MP] int32: page of slots j P .. of each sequence, -1 behind
+ *   its last one; length [B] int64 slots held; err [1] int32, bits set by a call that cannot be done:
+ *     1 a sequence or page number out of range, 2 the target of a fork holds slots or is named twice,
+ *     4 no free page, 8 a slot or length beyond the table, 16 the other pool is too small.
+ * Such a call changes nothing but err (ecd_page_free skips the numbers out of range).  Free pages are taken lowest number
+ * first, in the order of the call's sequences.  Calls on one state have to be ordered (one stream, or events). */
+
+/* The n sequences of seqs give their pages back (a page is free once its last owner has); a sequence named twice is
+ * freed once.  Their table rows become -1, their lengths 0. */
+int ecd_page_free(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B, int P,
+                  const int32_t* seqs, int n, int32_t* err, void* stream);
+
+/* Sequence dst[i] becomes a copy of src[i] (as it was before the call), i < n <= 1024: it shares the whole pages and
+ * gets the slots of a last page that is not full copied, in every plane, into a page of its own.  Targets hold no slots.
+ *   plan: [4 n] int32 workspace (any contents). */
+int ecd_page_fork(void* kv, int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B,
+                  const int32_t* src, const int32_t* dst, int n, int32_t* plan, int32_t* err, int planes, int Hk,
+                  int P, int HD, void* stream);
+
+/* Every sequence b < B <= 1024 holds slot pos[b] afterwards: new pages up to it, length[b] = max(length[b], pos[b] + 1).
+ * Calling it again with the same pos changes nothing; pos[b] = -1 leaves b alone. */
+int ecd_page_extend(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B, int P,
+                    const int64_t* pos, int32_t* err, void* stream);
+
+/* The pages in use, in ascending order, to pages 0 .. of another pool kv2 [planes, NP2, Hk, P, HD], and the state that
+ * goes with them to ref2 [NP2], table2 [B, MP], length2 [B]; the pages of kv2 behind them are left as they are.
+ *   ws: [1 + 2 NP] int32 workspace (any contents).  kv and kv2 must not overlap. */
+int ecd_page_compact(const void* kv, const int32_t* ref, int NP, const int32_t* table, const int64_t* length, void* kv2,
+                     int32_t* ref2, int NP2, int32_t* table2, int64_t* length2, int B, int MP, int32_t* ws,
+                     int32_t* err, int planes, int Hk, int P, int HD, void* stream);
+
+/* RoPE and the write of M rows into pages: row m of qkv (q | k | v heads, row stride ld) belongs to sequence m / S
+ * (table row stride ldt) at slot pos[m].  With rope [LR, HD / 2, 2] f32 the q and k pairs are rotated as by
+ * ecd_rope_kv_write and q goes to [M, Hq * HD]; without it k and v are written as they are and q may be NULL.  A row
+ * whose slot is outside [0, MP P) (or [0, LR)), or whose page is outside [0, NP), writes no k and v.
+ *   kp, vp [NP, Hk, P, HD]; HD % 8 == 0; 16-byte aligned rows. */
+int ecd_paged_write(const void* qkv, long ld, const float* rope, int LR, const int64_t* pos, void* q, void* kp,
+                    void* vp, const int32_t* table, long ldt, int MP, int NP, int M, int S, int Hq, int Hk, int P,
+                    int HD, void* stream);
+
+/* Decode attention over pages: row r (sequence r / S) attends slots [0, pos[r]] (pos -1: nothing, its output is 0); the
+ * slots that a group of rows shares are read once for all of them.
+ *   q row stride ldq; o [R, Hq * HD]; table row stride ldt; P a power of two from 16; HD in {64, 128, 256};
+ *   Hq / Hk <= 16; MP P <= 2^30.
+ *   rows [R, 2] int32: shared slots and number of shared parts of each row; items [nitems, 5] int32: first row, rows (at
+ *   most 16 ctiles / (Hq / Hk)), first slot, last slot + 1 and part number of each shared part; nown: parts of each
+ *   row's own slots; parts: the most parts of any row (<= 512); ctiles 1, 2 or 4 (HD 256: 1 or 2).  A row that does not
+ *   attend all shared slots takes none of the shared parts and attends its own slots from 0.
+ *   ws: fp32 workspace of 2 ceil4(R Hq parts) + R Hq parts HD values (any contents; NULL where parts is 1). */
+int ecd_paged_attn(const void* q, long ldq, const void* kp, const void* vp, const int32_t* table, long ldt,
+                   const int64_t* pos, void* o, float* ws, const int32_t* items, const int32_t* rows, int nitems,
+                   int nown, int parts, int ctiles, int R, int S, int MP, int NP, int Hq, int Hk, int P, int HD,
+                   float scale, void* stream);
+
+/* Rows of x [M, K] f16 (or, with nw [K], of their RMS norm in fp32) as int8 codes and an fp32 scale each:
+ * sx[m] = max |y[m]| / 127, c[m, k] = rint(127 y[m, k] / max |y[m]|), ties to even; columns K .. ldc - 1 are 0.
+ * A row that holds an infinity or a NaN gets the scale NaN.  K % 64 == 0, K <= 2^17, ldc % 128 == 0. */
+int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, long ldc, float* sx, int M, int K,
+                 void* stream);
+
+/* y[m, n] = f16(sx[m] s[n] sum_k c[m, k] q[n, k] (+ res[m, n])) with weights packed by ecd_pack_i8: the sum is an
+ * integer, one rounding at the end.  c from ecd_quant_a8 (zero columns behind K). */
+int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
+                void* y, long ldy, int M, int N, int K, void* stream);
+
+/* mm[m, j] = f16(silu(z[m, 2j]) z[m, 2j + 1]), z the fp32 product of ecd_gemm_a8 on row-interleaved w1 | w3. */
+int ecd_gemm_a8_silu(const void* c, long ldc, const float* sx, const void* wp, const void* s, void* mm, long ldm,
+                     int M, int F, int K, void* stream);
+
 /* Library version string (static storage). */
 const char* ecd_version(void);
 
