@@ -127,6 +127,7 @@ SIGNATURES = {
                        c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "ecd_quant_a8": [_P, c_long, _P, c_float, _P, c_long, _P, c_int, c_int, _P],
     "ecd_gemm_a8": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, _P],
+    "ecd_gemm_a8_tuned": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P],
     "ecd_gemm_a8_silu": [_P, c_long, _P, _P, _P, _P, c_long, c_int, c_int, c_int, _P],
 }
 

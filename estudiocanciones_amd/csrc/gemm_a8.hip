@@ -85,61 +85,352 @@ struct A8Out {
   long ldy;
 };
 
-// 64 features x 64 rows per workgroup, fragments straight from memory
+// One row's results of 8 consecutive features n .. (fewer at the end) from their integer sums; sn: the features' scales
 template <bool SILU>
-__global__ __launch_bounds__(256) void gemm_a8_kernel(const int8_t* __restrict__ c, long ldc,
-                                                      const int8_t* __restrict__ wp, A8Out out, int M, int N, int K) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int nt = (N + 15) >> 4, tile = min((int)blockIdx.x * 4 + wv, nt - 1), m0 = blockIdx.y * 64;
-  const int8_t* w = wp + (long)tile * 16 * K + 16 * lane;
-  const int8_t* x[4];
-  i32x4 acc[4];
+__device__ __forceinline__ void a8_finish(const A8Out& out, const int (&v)[8], float sm, const float (&sn)[8], long m, int n, int N) {
+  float z[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = c + (long)min(m0 + 16 * i + (lane & 15), M - 1) * ldc + 16 * (lane >> 4);
-    acc[i] = (i32x4){0, 0, 0, 0};
-  }
-  for (int k = 0; k < K; k += 64) {
-    const i32x4 a = *(const i32x4*)(w + 16L * k);
+  for (int j = 0; j < 8; ++j) z[j] = (float)v[j] * (sm * sn[j]);
+  if constexpr (SILU) {
+    f16x4 o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const i32x4*)(x[i] + k), acc[i], 0, 0, 0);
-  }
-  const int n0 = ((int)blockIdx.x * 4 + wv) * 16 + 4 * (lane >> 4);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + 16 * i + (lane & 15);
-    if (m >= M) continue;
-    const float sm = out.sx[m];
-    float z[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) z[j] = (float)acc[i][j] * (sm * (float)out.s[min(n0 + j, N - 1)]);
-    if constexpr (SILU) {
-#pragma unroll
-      for (int j = 0; j < 4; j += 2)
-        if (n0 + j < N) out.y[m * out.ldy + (n0 + j) / 2] = (f16)(z[j] / (1.f + __expf(-z[j])) * z[j + 1]);
+    for (int j = 0; j < 4; ++j) o[j] = (f16)(z[2 * j] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[2 * j] * -1.44269504088896341f)) * z[2 * j + 1]);
+    f16* d = out.y + m * out.ldy + (n >> 1);
+    if (n + 7 < N) {
+      *(f16x4u*)d = o;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (n0 + j < N) out.y[m * out.ldy + n0 + j] = (f16)(out.res ? z[j] + (float)out.res[m * out.ldr + n0 + j] : z[j]);
+        if (n + 2 * j < N) d[j] = o[j];
+    }
+  } else {
+    const f16* r = out.res ? out.res + m * out.ldr + n : nullptr;
+    f16* d = out.y + m * out.ldy + n;
+    f16x8 o;
+    if (n + 7 < N) {
+      f16x8 rv = (f16x8)((f16)0);
+      if (r) rv = *(const f16x8u*)r;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = (f16)(r ? z[j] + (float)rv[j] : z[j]);
+      *(f16x8u*)d = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < N) d[j] = (f16)(r ? z[j] + (float)r[j] : z[j]);
     }
   }
 }
 
-template <bool SILU>
-static int launch_a8(const void* c, long ldc, const void* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
-  const int mb = (M + 63) / 64;
-  if (mb > 65535) return ECD_ENOTSUP;
-  hipLaunchKernelGGL(gemm_a8_kernel<SILU>, dim3((N + 63) / 64, mb), dim3(256), 0, st, (const int8_t*)c, ldc,
-                     (const int8_t*)wp, out, M, N, K);
+__device__ __forceinline__ void a8_scales(const f16* s, int n, int N, float (&sn)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sn[j] = (float)s[min(n + j, N - 1)];
+}
+
+// ---- few rows: the weights stream once from memory into registers
+// One workgroup per 16 features and up to 16 RT rows; its WV waves take an equal share of K each and add their integer
+// sums in LDS.
+template <bool SILU, int RT, int WV>
+__global__ __launch_bounds__(64 * WV) void gemm_a8_few_kernel(const int8_t* __restrict__ c, long ldc,
+                                                              const int8_t* __restrict__ wp, A8Out out, int M, int N, int K) {
+  __shared__ __align__(16) int part[WV][RT * 16][20];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * RT;
+  const int steps = K >> 6, s0 = steps * wv / WV, s1 = steps * (wv + 1) / WV;
+  const int8_t* w = wp + (long)blockIdx.x * 16 * K + 16 * lane;
+  const int8_t* x[RT];
+  i32x4 acc[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    x[i] = c + (long)min(m0 + 16 * i + (lane & 15), M - 1) * ldc + 16 * (lane >> 4);
+    acc[i] = (i32x4){0, 0, 0, 0};
+  }
+  constexpr int U = RT <= 2 ? 8 : 4;
+  int k = s0;
+  for (; k + U <= s1; k += U) {
+    i32x4 a[U], b[U][RT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      a[u] = __builtin_nontemporal_load((const i32x4*)(w + 1024L * (k + u)));
+#pragma unroll
+      for (int i = 0; i < RT; ++i) b[u][i] = *(const i32x4*)(x[i] + 64 * (k + u));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][i], acc[i], 0, 0, 0);
+  }
+  for (; k < s1; ++k) {
+    const i32x4 a = __builtin_nontemporal_load((const i32x4*)(w + 1024L * k));
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const i32x4*)(x[i] + 64 * k), acc[i], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) *(i32x4*)&part[wv][16 * i + (lane & 15)][4 * (lane >> 4)] = acc[i];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 32 * RT; t += 64 * WV) {
+    const int r = t >> 1, h = 8 * (t & 1), m = m0 + r, n = n0 + h;
+    if (m >= M || n >= N) continue;
+    int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < WV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += part[i][r][h + j];
+    float sn[8];
+    a8_scales(out.s, n, N, sn);
+    a8_finish<SILU>(out, v, out.sx[m], sn, m, n, N);
+  }
+}
+
+// ---- many rows: tiles of 32 WN FT features x 32 WM RT rows through an LDS ring of NS stages of 128 k
+// The loads, the stages and the order of a loop pass are those of GemmTile (gemm_core.h) on bytes: 16 bytes of a row or a
+// feature are 16 k of v_mfma_i32_32x32x32_i8 instead of 8 of the fp16 product.
+template <int FT, int RT>
+struct A8Frags {
+  i32x4 w[2][FT], x[2][RT];
+};
+
+template <int WN, int WM, int FT, int RT, int NS>
+struct A8Tile {
+  static constexpr int NW = WN * WM, BN = 32 * WN * FT, BM = 32 * WM * RT;
+  static constexpr int WI = BN / 8 / NW, XI = BM / 8 / NW, PER = WI + XI;  // DMA instructions (1 KB) per wave and chunk
+  static_assert(WI * NW * 8 == BN && XI * NW * 8 == BM, "whole DMA instructions per wave");
+  static_assert(NS >= 2 && PER * (NS - 1) < 64, "vmcnt range");
+  static constexpr int LW = BN * 128, LX = BM * 128, STG = LW + LX;  // bytes of a stage
+  // the sums leave through LDS as int32, some row tiles of each wave at a time
+  static constexpr int ROW = BN + 4;  // ints of an output row
+  static constexpr int fit(int n) { return n == 1 || 32 * WM * n * ROW * 4 <= NS * STG ? n : fit(n / 2); }
+  static constexpr int RP = fit(RT);  // row tiles of a pass
+  static_assert(RT % RP == 0, "whole passes");
+  static constexpr int PASS_BYTES = 32 * WM * RP * ROW * 4;
+  static constexpr int LDS = NS * STG > PASS_BYTES ? NS * STG : PASS_BYTES;
+
+  // Sums of chunks c0 .. c0 + nch - 1 of 128 k.  `odd`: the last of them is half a chunk (its second half of the weights
+  // re-reads the first; the codes behind K are 0).
+  static __device__ __forceinline__ void run(unsigned char* lds, i32x16 (&acc)[FT][RT], const int8_t* __restrict__ c, long ldc,
+                                             const int8_t* __restrict__ wp, int M, int N, int K, int n0, int m0, int c0,
+                                             int nch, bool odd) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wv % WN, wm = wv / WN;
+    const int ntiles = (N + 15) >> 4, t0 = min(n0 / 16, ntiles - 1);
+    const long tile_bytes = 16L * K;
+    const int8_t* wb = wp + t0 * tile_bytes + 2048L * c0;
+    const int8_t* xb = c + (long)m0 * ldc + 128L * c0;
+    uint32_t woff[WI], xoff[XI];
+#pragma unroll
+    for (int j = 0; j < WI; ++j) {
+      const int i = wv + NW * j;
+      woff[j] = (uint32_t)((min(n0 / 16 + (i >> 1), ntiles - 1) - t0) * tile_bytes) + 1024 * (i & 1) + 16 * lane;
+    }
+#pragma unroll
+    for (int j = 0; j < XI; ++j) {
+      const int r = 8 * (wv + NW * j) + (lane >> 3);
+      xoff[j] = (uint32_t)((min(m0 + r, M - 1) - m0) * ldc) + 16 * ((lane & 7) ^ x_swz(r));
+    }
+    const uint32_t lds0 = lds_addr(lds) + wv * 1024;
+    int left = nch;  // chunks not yet asked for
+    const uint32_t back = wv & 1 ? 1024u : 0u;  // (NW is even: this wave's weight instructions are all first or all second halves)
+    static_assert(NW % 2 == 0, "a wave keeps its half");
+    auto dma = [&](auto J, uint32_t sa) {
+      constexpr int j = decltype(J)::value;
+      if constexpr (j < WI)
+        lds_dma16_at<NW * j * 1024>(wb, odd && left == 1 ? woff[j] - back : woff[j], sa);
+      else
+        lds_dma16_at<LW + NW * (j - WI) * 1024>(xb, xoff[j - WI], sa);
+    };
+    auto next_chunk = [&]() {
+      wb += 2048;
+      xb += 128;
+      --left;
+    };
+    static_for<0, FT * RT>([&](auto I) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[I.value / RT][I.value % RT][e] = 0;
+    });
+    // fragment addresses: 32 features are two packed 16-row tiles of 2 KB, piece o = 2 s + (lane >> 5) of k-step s lies in
+    // 1 KB half o >> 2 at unit 16 (o & 3) + row; piece o of x row r at position o ^ x_swz(r)
+    const int wfo = (wn * FT * 2 + ((lane >> 4) & 1)) * 2048 + (lane >> 5) * 256 + (lane & 15) * 16;
+    int xfo[4];
+    static_for<0, 4>([&](auto S) {
+      xfo[S.value] = LW + (wm * RT * 32 + (lane & 31)) * 128 + 16 * ((2 * S.value + (lane >> 5)) ^ x_swz(lane & 31));
+    });
+    constexpr int NM = 2 * FT * RT, NR = 2 * (FT + RT);
+    auto read1 = [&](auto I, auto H, const unsigned char* base, A8Frags<FT, RT>& f) {
+      constexpr int i = decltype(I)::value, h = decltype(H)::value;
+      if constexpr (i < 2 * FT) {
+        constexpr int s = i / FT, ft = i % FT;
+        f.w[s][ft] = *(const i32x4*)(base + wfo + 1024 * h + 512 * s + ft * 4096);
+      } else {
+        constexpr int k = i - 2 * FT, s = k / RT, rt = k % RT;
+        f.x[s][rt] = *(const i32x4*)(base + xfo[2 * h + s] + rt * 4096);
+      }
+    };
+    // the products of a half chunk, with the reads of the next half's fragments and DMA instructions D0 .. D1 - 1 between
+    auto half = [&](const A8Frags<FT, RT>& f, auto H, const unsigned char* base, A8Frags<FT, RT>& nf, auto D0, auto D1, uint32_t sa) {
+      static_for<0, NM>([&](auto I) {
+        constexpr int m = decltype(I)::value, s = m / (FT * RT), ft = m % (FT * RT) / RT, rt = m % RT;
+        acc[ft][rt] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[s][ft], f.x[s][rt], acc[ft][rt], 0, 0, 0);
+        constexpr int d0 = decltype(D0)::value, nd = decltype(D1)::value - d0;
+        static_for<d0 + m * nd / NM, d0 + (m + 1) * nd / NM>([&](auto J) { dma(J, sa); });
+        static_for<m * NR / NM, (m + 1) * NR / NM>([&](auto J) { read1(J, H, base, nf); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    auto barrier = [&]() {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+
+    for (int s = 0; s < NS; ++s)
+      if (s < nch) {
+        static_for<0, PER>([&](auto J) { dma(J, lds0 + s * STG); });
+        next_chunk();
+      }
+    wait_chunk<PER, NS - 1, false>(min(NS - 1, nch - 1));
+    barrier();
+    A8Frags<FT, RT> fa, fc;
+    static_for<0, NR>([&](auto I) { read1(I, IC<0>{}, lds, fa); });
+    // as in GemmTile: each pass runs chunk i's second half and chunk i + 1's first, and loads chunk i + NS
+    constexpr int DS = NS > 2 ? (PER + 1) / 2 : PER;
+    int i = 0, st = 0;
+    half(fa, IC<1>{}, lds, fc, IC<0>{}, IC<0>{}, 0);
+    for (; i < nch - NS; ++i) {
+      wait_vm_lgkm0<(NS - 2) * PER>();
+      barrier();
+      const int sn = st + 1 == NS ? 0 : st + 1;
+      const unsigned char* base = lds + sn * STG;
+      const uint32_t sa = lds0 + st * STG;
+      half(fc, IC<0>{}, base, fa, IC<0>{}, IC<DS>{}, sa);
+      half(fa, IC<1>{}, base, fc, IC<DS>{}, IC<PER>{}, sa);
+      next_chunk();
+      st = sn;
+    }
+    for (; i < nch - 1; ++i) {
+      wait_chunk<PER, NS - 2, true>(min(NS - 2, nch - 2 - i));
+      barrier();
+      const int sn = st + 1 == NS ? 0 : st + 1;
+      const unsigned char* base = lds + sn * STG;
+      half(fc, IC<0>{}, base, fa, IC<0>{}, IC<0>{}, 0);
+      half(fa, IC<1>{}, base, fc, IC<0>{}, IC<0>{}, 0);
+      st = sn;
+    }
+    half(fc, IC<0>{}, lds, fa, IC<0>{}, IC<0>{}, 0);  // (its reads are never used)
+  }
+
+  // f(row of the tile, feature of the tile, 8 sums) for every piece of 8 features, rows in passes through LDS
+  template <typename F>
+  static __device__ __forceinline__ void sums(unsigned char* lds, const i32x16 (&acc)[FT][RT], F&& f) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wv % WN, wm = wv / WN;
+    int* buf = (int*)lds;
+    constexpr int PR = BN / 8, RS = 64 * NW / PR, ROWS = 32 * WM * RP;
+    static_assert(64 * NW % PR == 0 && ROWS % RS == 0, "whole rows per step");
+    const int p = threadIdx.x % PR;
+    static_for<0, RT / RP>([&](auto P) {
+      __syncthreads();
+      static_for<0, FT * RP>([&](auto I) {
+        constexpr int ft = decltype(I)::value / RP, q = decltype(I)::value % RP, rt = decltype(P)::value * RP + q;
+        int* d = buf + (long)((wm * RP + q) * 32 + (lane & 31)) * ROW + (wn * FT + ft) * 32 + 4 * (lane >> 5);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(i32x4*)(d + 8 * g) = (i32x4){acc[ft][rt][4 * g], acc[ft][rt][4 * g + 1], acc[ft][rt][4 * g + 2], acc[ft][rt][4 * g + 3]};
+      });
+      __syncthreads();
+#pragma unroll 2
+      for (int r = threadIdx.x / PR; r < ROWS; r += RS) {
+        const i32x4 a = *(const i32x4*)(buf + (long)r * ROW + 8 * p), b = *(const i32x4*)(buf + (long)r * ROW + 8 * p + 4);
+        const int v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        const int w = r / (32 * RP), q = r - w * 32 * RP;
+        f((w * RT + decltype(P)::value * RP) * 32 + q, 8 * p, v);
+      }
+    });
+  }
+};
+
+// Block b of an order in which the row blocks of a feature block have numbers that are equal modulo 8: one XCD, whose L2
+// then holds the weights.
+__device__ __forceinline__ void a8_block(int b, int nfb, int nmb, int& fb, int& mb) {
+  const int full = nfb & ~7;
+  if (b < full * nmb) {
+    const int g = b / (8 * nmb), rem = b - g * 8 * nmb;
+    mb = rem >> 3;
+    fb = g * 8 + (rem & 7);
+  } else {
+    const int rem = b - full * nmb, tw = nfb - full;
+    mb = rem / tw;
+    fb = full + rem - mb * tw;
+  }
+}
+
+template <bool SILU, int WN, int WM, int FT, int RT, int NS>
+__global__ __launch_bounds__(64 * WN * WM, 1) void gemm_a8_kernel(const int8_t* __restrict__ c, long ldc,
+                                                                  const int8_t* __restrict__ wp, A8Out out, int M, int N, int K,
+                                                                  int nfb, int nmb) {
+  using T = A8Tile<WN, WM, FT, RT, NS>;
+  __shared__ __align__(16) unsigned char lds[T::LDS];
+  int fb, mb;
+  a8_block(blockIdx.x, nfb, nmb, fb, mb);
+  const int n0 = fb * T::BN, m0 = mb * T::BM;
+  i32x16 acc[FT][RT];
+  T::run(lds, acc, c, ldc, wp, M, N, K, n0, m0, 0, (K + 127) >> 7, K & 64);
+  const int nb = n0 + 8 * (threadIdx.x % (T::BN / 8));
+  float sn[8];
+  a8_scales(out.s, nb, N, sn);
+  T::sums(lds, acc, [&](int r, int, const int (&v)[8]) {
+    const int m = m0 + r;
+    if (m < M && nb < N) a8_finish<SILU>(out, v, out.sx[m], sn, m, nb, N);
+  });
+}
+
+template <bool SILU, int WN, int WM, int FT, int RT, int NS>
+static int launch_tile(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
+  using T = A8Tile<WN, WM, FT, RT, NS>;
+  const int nfb = (N + T::BN - 1) / T::BN, nmb = (M + T::BM - 1) / T::BM;
+  if ((long)nfb * nmb > 0x7FFFFFFFL) return ECD_ENOTSUP;
+  hipLaunchKernelGGL((gemm_a8_kernel<SILU, WN, WM, FT, RT, NS>), dim3((unsigned)(nfb * nmb)), dim3(64 * WN * WM), 0, st, c, ldc, wp, out, M,
+                     N, K, nfb, nmb);
   return ecd_launch_status();
+}
+
+template <bool SILU, int RT, int WV>
+static int launch_few(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
+  if ((M + 16 * RT - 1) / (16 * RT) > 65535) return ECD_ENOTSUP;
+  hipLaunchKernelGGL((gemm_a8_few_kernel<SILU, RT, WV>), dim3((N + 15) / 16, (M + 16 * RT - 1) / (16 * RT)), dim3(64 * WV), 0, st, c, ldc,
+                     wp, out, M, N, K);
+  return ecd_launch_status();
+}
+
+template <bool SILU>
+static int launch_a8(const void* cv, long ldc, const void* wv, const A8Out& out, int M, int N, int K, hipStream_t st, int cfg = 0) {
+  const int8_t *c = (const int8_t*)cv, *wp = (const int8_t*)wv;
+#define A8_TILE(...) return launch_tile<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
+#define A8_FEW(...) return launch_few<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
+  if (!cfg) cfg = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 3 : M <= 256 ? 7 : 10;
+  switch (cfg) {
+    case 1: A8_FEW(1, 4);
+    case 2: A8_FEW(2, 4);
+    case 3: A8_FEW(4, 4);
+    case 4: A8_FEW(1, 8);
+    case 5: A8_FEW(2, 8);
+    case 6: A8_FEW(4, 8);
+    case 7: A8_TILE(2, 2, 1, 1, 8);   // 64 x 64
+    case 8: A8_TILE(2, 2, 1, 2, 6);   // 64 x 128
+    case 9: A8_TILE(2, 2, 2, 2, 4);   // 128 x 128
+    case 10: A8_TILE(2, 2, 4, 4, 2);  // 256 x 256, 4 waves
+    case 11: A8_TILE(4, 2, 2, 4, 2);  // 256 x 256, 8 waves
+    case 12: A8_TILE(2, 2, 4, 2, 3);  // 256 x 128, 4 waves
+    case 13: A8_TILE(2, 2, 2, 4, 3);  // 128 x 256
+    default: return ECD_EINVAL;
+  }
+#undef A8_TILE
+#undef A8_FEW
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static bool a8_ok(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* y, int M, int N,
                   int K) {
   return c && sx && wp && s && y && M > 0 && N > 0 && K > 0 && K % 64 == 0 && K <= 1 << 17 && ldc >= K &&
-         ldc % 128 == 0 && aligned16(c) && aligned16(wp);
+         ldc % 128 == 0 && ldc <= 1 << 23 && aligned16(c) && aligned16(wp);
 }
 
 }  // namespace ecd
@@ -168,6 +459,13 @@ int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const 
   if (!a8_ok(c, ldc, sx, wp, s, y, M, N, K) || ldy < N || (res && ldr < N)) return ECD_EINVAL;
   return launch_a8<false>(c, ldc, wp, A8Out{sx, (const f16*)s, (const f16*)res, ldr, (f16*)y, ldy}, M, N, K,
                           (hipStream_t)stream);
+}
+
+int ecd_gemm_a8_tuned(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
+                      void* y, long ldy, int M, int N, int K, int cfg, void* stream) {
+  if (!a8_ok(c, ldc, sx, wp, s, y, M, N, K) || ldy < N || (res && ldr < N) || cfg < 0) return ECD_EINVAL;
+  return launch_a8<false>(c, ldc, wp, A8Out{sx, (const f16*)s, (const f16*)res, ldr, (f16*)y, ldy}, M, N, K,
+                          (hipStream_t)stream, cfg);
 }
 
 int ecd_gemm_a8_silu(const void* c, long ldc, const float* sx, const void* wp, const void* s, void* mm, long ldm,

@@ -28,7 +28,7 @@ struct PagedArgs {
   float* pm;         // [R Hq, parts]: maximum and sum of each part, then its unnormalised output
   float* pl;
   float* pa;         // [R Hq, parts, HD]
-  const int* items;  // {first row, rows, lo, hi, part} of each shared part
+  const int* items;  // {first row, rows, lo, hi, part, kv head} of each shared part
   const int* rows;   // {shared slots, shared parts} of each row
   long ldq, ldt;
   int MP, NP, S, Hq, Hk, G, PS, nitems, nown, parts;  // PS: log2 of the page size
@@ -58,25 +58,41 @@ struct PTile {
   vec v[2][4][ND];
 };
 
-// slots t0 .. t0 + 31 (t0 a multiple of 32) of the sequence whose page numbers are at `tab`; slots from hi on repeat a
-// slot before it (masked later)
-template <int HD>
-__device__ __forceinline__ void tile_load(PTile<HD>& t, const PagedArgs& a, const int* tab, int kh, int t0, int hi,
-                                          int lane) {
-  const int grp = lane >> 4, col = lane & 15, mask = (1 << a.PS) - 1;
+// Where the tiles of a wave lie: lane i holds the pool row (page Hk + kh) P + slot of the halves of tile i.  Slots from hi
+// on repeat a half before it (masked later); a number that is no page reads page 0 or the last one.
+struct Places {
+  uint32_t r[2];
+};
+__device__ __forceinline__ Places places(const PagedArgs& a, const int* tab, int kh, int t0, int hi, int lane) {
+  Places p;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int h0 = min(t0 + 16 * j, (hi - 1) & ~15);  // a half tile lies in one page
-    const int page = min(max(__builtin_amdgcn_readfirstlane(tab[h0 >> a.PS]), 0), a.NP - 1);
-    const long base = ((((long)page * a.Hk + kh) << a.PS) + (h0 & mask)) * HD;
-    const f16* k = a.kp + base + col * HD + 8 * grp;
+    const int h = min(t0 + lane * (PQ_W * PQ_T) + 16 * j, (hi - 1) & ~15);  // a half tile lies in one page
+    const int page = min(max(tab[h >> a.PS], 0), a.NP - 1);
+    p.r[j] = (((uint32_t)page * a.Hk + kh) << a.PS) + (h & ((1 << a.PS) - 1));
+  }
+  return p;
+}
+
+template <int HD>
+__device__ __forceinline__ void load_k(PTile<HD>& t, const PagedArgs& a, const Places& p, int i, int lane) {
 #pragma unroll
-    for (int i = 0; i < PTile<HD>::KC; ++i) t.k[j][i] = *(const f16x8*)(k + 32 * i);
-    const f16* v = a.vp + base + 4 * grp * HD + PTile<HD>::VW * col;
+  for (int j = 0; j < 2; ++j) {
+    const f16* k = a.kp + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.r[j], i) * HD;
+#pragma unroll
+    for (int x = 0; x < PTile<HD>::KC; ++x) t.k[j][x] = *(const f16x8*)(k + (uint32_t)((lane & 15) * HD + 8 * (lane >> 4) + 32 * x));
+  }
+}
+template <int HD>
+__device__ __forceinline__ void load_v(PTile<HD>& t, const PagedArgs& a, const Places& p, int i, int lane) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const f16* v = a.vp + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.r[j], i) * HD;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int x = 0; x < PTile<HD>::ND; ++x) t.v[j][e][x] = *(const typename PTile<HD>::vec*)(v + e * HD + 128 * x);
+      for (int x = 0; x < PTile<HD>::ND; ++x)
+        t.v[j][e][x] = *(const typename PTile<HD>::vec*)(v + (uint32_t)((4 * (lane >> 4) + e) * HD + PTile<HD>::VW * (lane & 15) + 128 * x));
   }
 }
 
@@ -90,47 +106,39 @@ struct PState {
   float m[CT], l[CT];
 };
 
-// slots outside [lo, hi) of the tile at t0 do not count, whatever they hold
-template <int HD, int CT>
-__device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, float c2, int t0, int lo, int hi, int lane) {
+// Slots outside [lo, hi) of the tile at t0 do not count, whatever they hold.  `after_scores` runs once K is used.
+template <int HD, int CT, typename F>
+__device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, float c2, int t0, int lo, int hi, int lane, F&& after_scores) {
   using T = PTile<HD>;
   const int grp = lane >> 4;
   const bool edge = t0 < lo || t0 + PQ_T > hi;  // uniform
-  if (edge) {
+  f32x4 sc[CT][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+  for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = t0 + 16 * j + 4 * grp + e;
-        if (k < lo || k >= hi)
+    for (int j = 0; j < 2; ++j) {
+      sc[c][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int x = 0; x < T::ND; ++x) t.v[j][e][x] = (typename T::vec)((f16)0);
-      }
-  }
+      for (int i = 0; i < T::KC; ++i) sc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[j][i], s.q[c][i], sc[c][j], 0, 0, 0);
+    }
+  after_scores();
   f16x8 p[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    f32x4 sc[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      sc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < T::KC; ++i) sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[j][i], s.q[c][i], sc[j], 0, 0, 0);
-    }
     if (edge) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int k = t0 + 16 * j + 4 * grp + e;
-          if (k < lo || k >= hi) sc[j][e] = -INFINITY;
+          if (k < lo || k >= hi) sc[c][j][e] = -INFINITY;
         }
     }
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[j][e]);
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[c][j][e]);
     const float mn = fmaxf(s.m[c], max_groups(mx));
     const float mb = mn == -INFINITY ? 0.f : mn * c2;
     float ps = 0.f;
@@ -138,7 +146,7 @@ __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, flo
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][e], c2, -mb));
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][j][e], c2, -mb));
         ps += w;
         p[c][4 * j + e] = (f16)w;
       }
@@ -152,6 +160,17 @@ __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, flo
     }
     s.l[c] += ps;
     s.m[c] = mn;
+  }
+  if (edge) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = t0 + 16 * j + 4 * grp + e;
+        if (k < lo || k >= hi)
+#pragma unroll
+          for (int x = 0; x < T::ND; ++x) t.v[j][e][x] = (typename T::vec)((f16)0);
+      }
   }
 #pragma unroll
   for (int x = 0; x < T::ND; ++x)
@@ -187,10 +206,28 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
 #pragma unroll
       for (int b = 0; b < PTile<HD>::VW; ++b) s.acc[c][x][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
+  // K of the next tile is asked for once this one's scores are formed, V once this one's is used: one tile is always in
+  // flight, in the registers of the last one
   PTile<HD> t;
-  for (int t0 = (lo & ~(PQ_T - 1)) + wv * PQ_T; t0 < hi; t0 += PQ_W * PQ_T) {
-    tile_load<HD>(t, a, tab, kh, t0, hi, lane);
-    tile_attend<HD, CT>(s, t, a.c2, t0, lo, hi, lane);
+  const int first = (lo & ~(PQ_T - 1)) + wv * PQ_T;
+  const int n = hi > first ? (hi - first + PQ_W * PQ_T - 1) / (PQ_W * PQ_T) : 0;
+  Places at;
+  if (n > 0) {
+    at = places(a, tab, kh, first, hi, lane);
+    load_k<HD>(t, a, at, 0, lane);
+    load_v<HD>(t, a, at, 0, lane);
+  }
+  for (int i = 0; i < n; ++i) {
+    const bool more = i + 1 < n;
+    if (more && ((i + 1) & 63) == 0) at = places(a, tab, kh, first + (i + 1) * (PQ_W * PQ_T), hi, lane);
+    tile_attend<HD, CT>(s, t, a.c2, first + i * (PQ_W * PQ_T), lo, hi, lane, [&]() {
+      asm volatile("" ::: "memory");
+      if (more) load_k<HD>(t, a, at, (i + 1) & 63, lane);
+      asm volatile("" ::: "memory");
+    });
+    asm volatile("" ::: "memory");
+    if (more) load_v<HD>(t, a, at, (i + 1) & 63, lane);
+    asm volatile("" ::: "memory");
   }
 
   // the waves' states to one: maxima and sums first, then the outputs on the common maximum
@@ -259,13 +296,12 @@ constexpr int attend_lds() {
 }
 
 template <int HD, int CT>
-__global__ __launch_bounds__(64 * PQ_W) void paged_attn_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * PQ_W, 2) void paged_attn_kernel(PagedArgs a) {
   __shared__ __align__(16) float lds[attend_lds<HD, CT>()];
   __shared__ int s_lead;
-  const int kh = blockIdx.y;
   if ((int)blockIdx.x < a.nitems) {
-    const int* it = a.items + 5 * blockIdx.x;
-    const int row0 = it[0], n = it[1], lo = it[2], hi = it[3];
+    const int* it = a.items + 6 * blockIdx.x;
+    const int row0 = it[0], n = it[1], lo = it[2], hi = it[3], kh = it[5];
     // the first row that attends the whole prefix leads: its pages hold every shared slot
     if (threadIdx.x < 64) {
       const int r = row0 + threadIdx.x;
@@ -280,7 +316,7 @@ __global__ __launch_bounds__(64 * PQ_W) void paged_attn_kernel(PagedArgs a) {
                    [&](int row) { return a.pos[row] + 1 >= a.rows[2 * row]; });
     return;
   }
-  const int x = blockIdx.x - a.nitems, r = x / a.nown, k = x - r * a.nown;
+  const int x = blockIdx.x - a.nitems, u = x / a.Hk, kh = x - u * a.Hk, r = u / a.nown, k = u - r * a.nown;
   const long p = a.pos[r];
   const int end = (int)min(p < 0 ? 0l : p + 1, (long)a.MP << a.PS);
   const int shared = a.rows[2 * r], np = a.rows[2 * r + 1];
@@ -291,49 +327,51 @@ __global__ __launch_bounds__(64 * PQ_W) void paged_attn_kernel(PagedArgs a) {
                 [](int) { return true; });
 }
 
-// One workgroup per (row, kv head): its parts in order.
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int HD) {
-  extern __shared__ float w[];  // [G][parts]
-  __shared__ float s_inv[16];
-  const int r = blockIdx.x, kh = blockIdx.y;
-  const int n = a.rows[2 * r + 1] + a.nown;
+// One thread per four dims of a head: JB parts at a time, all their loads at once, in the order of the parts.
+constexpr int JB = 8;
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int HD, int heads) {
+  const int i = blockIdx.x * 256 + threadIdx.x, per = HD / 4;
+  const int head = i / per, d = 4 * (i - head * per);
+  if (head >= heads) return;
+  const int r = head / a.Hq, n = a.rows[2 * r + 1] + a.nown;
   if (n == 1) return;
-  const long head = (long)r * a.Hq + kh * a.G;
-  for (int i = threadIdx.x; i < a.G * n; i += 256) {
-    const int g = i / n, k = i - g * n;
-    w[g * a.parts + k] = a.pm[(head + g) * a.parts + k];
-  }
-  __syncthreads();
-  for (int g = threadIdx.x >> 6; g < a.G; g += 4) {
-    const int lane = threadIdx.x & 63;
-    float M = -INFINITY, l = 0.f;
-    for (int k = lane; k < n; k += 64) M = fmaxf(M, w[g * a.parts + k]);
-    M = wave_max(M);
-    for (int k = lane; k < n; k += 64) {
-      const float m = w[g * a.parts + k];
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * a.c2);
-      w[g * a.parts + k] = f;
-      if (f != 0.f) l += f * a.pl[(head + g) * a.parts + k];
+  const float *pm = a.pm + (long)head * a.parts, *pl = a.pl + (long)head * a.parts, *pa = a.pa + (long)head * a.parts * HD + d;
+  float M = -INFINITY, l = 0.f;
+  f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < n; k0 += JB) {
+    float m[JB], s[JB];
+    f32x4 x[JB];
+#pragma unroll
+    for (int k = 0; k < JB; ++k) {
+      const int kk = min(k0 + k, n - 1);
+      m[k] = k0 + k < n ? pm[kk] : -INFINITY;
+      s[k] = pl[kk];
+      x[k] = *(const f32x4*)(pa + (long)kk * HD);
     }
-    l = wave_sum(l);
-    if (lane == 0) s_inv[g] = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.G * (HD / 4); i += 256) {
-    const int g = i / (HD / 4), d = 4 * (i - g * (HD / 4));
-    f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < n; ++k) {
-      const float f = w[g * a.parts + k];
-      if (f != 0.f) v = v + *(const f32x4*)(a.pa + ((head + g) * a.parts + k) * HD + d) * f;
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < JB; ++k) mn = fmaxf(mn, m[k]);
+    if (mn != M) {
+      const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mn) * a.c2);
+      l *= f;
+      v = v * f;
+      M = mn;
     }
-    const float inv = s_inv[g];
-    *(f16x4*)(a.o + (head + g) * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
+#pragma unroll
+    for (int k = 0; k < JB; ++k)
+      if (m[k] != -INFINITY) {  // (an empty part's output is not looked at)
+        const float f = __builtin_amdgcn_exp2f((m[k] - M) * a.c2);
+        l += f * s[k];
+        v = v + x[k] * f;
+      }
   }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  *(f16x4*)(a.o + (long)head * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
 }
 
 template <int HD, int CT>
 static int launch_paged(const PagedArgs& a, int R, hipStream_t st) {
-  hipLaunchKernelGGL((paged_attn_kernel<HD, CT>), dim3(a.nitems + R * a.nown, a.Hk), dim3(64 * PQ_W), 0, st, a);
+  hipLaunchKernelGGL((paged_attn_kernel<HD, CT>), dim3(a.nitems + R * a.nown * a.Hk), dim3(64 * PQ_W), 0, st, a);
   return ecd_launch_status();
 }
 
@@ -349,7 +387,8 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
       parts < nown || (parts > 1 && !ws) || R <= 0 || S <= 0 || MP <= 0 || NP <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
       Hq / Hk > 16 || P < 16 || (P & (P - 1)) || ldt < MP || ldq < (long)Hq * HD || (ldq % 8) ||
       ((uintptr_t)q & 15) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)o & 7) || ((uintptr_t)ws & 15) ||
-      !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown + nitems > 0x7FFFFFFFL || Hk > 65535)
+      !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown * Hk + nitems > 0x7FFFFFFFL || (long)R * Hq > 0x7FFFFFFFL / 64 ||
+      (long)NP * Hk * P > 0xFFFFFFFFL)
     return ECD_EINVAL;
   if ((HD != 64 && HD != 128 && HD != 256) || parts > 512) return ECD_ENOTSUP;
   const long heads = (long)R * Hq, n2 = (heads * parts + 3) & ~3l;
@@ -384,14 +423,11 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
   if (HD == HD_ && ctiles == CT_) rc = launch_paged<HD_, CT_>(a, R, st)
   PQ(64, 1);
   PQ(64, 2);
-  PQ(64, 4);
   PQ(128, 1);
   PQ(128, 2);
-  PQ(128, 4);
   PQ(256, 1);
-  PQ(256, 2);
 #undef PQ
   if (rc != ECD_OK || parts == 1) return rc;
-  hipLaunchKernelGGL(paged_join_kernel, dim3(R, Hk), dim3(256), (size_t)a.G * parts * sizeof(float), st, a, HD);
+  hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)((heads * (HD / 4) + 255) / 256)), dim3(256), 0, st, a, HD, (int)heads);
   return ecd_launch_status();
 }

@@ -973,6 +973,10 @@ class PagedAttnPlan:
         self.dev = flat.device
 
 
+PLAN_SHARED_WG = 384  # workgroups that the shared parts are cut for
+PLAN_OWN_WG = 512     # and the rows' own parts
+
+
 def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda"):
     """The plan of paged_attn for rows in ``groups``: a list of (rows, prefix), consecutive rows whose first ``prefix``
     slots are the same (0: nothing shared).  ``max_len``: the most slots that a row may come to hold.  Made once for all
@@ -991,25 +995,30 @@ def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda"):
 def _make_plan(groups, Hq, Hk, HD, max_len, dev):
     G = Hq // Hk
     R = sum(n for n, _ in groups)
-    cols = max([n * G for n, p in groups if p and n > 1], default=0)
-    ct = 1 if cols <= 16 else 2 if cols <= 32 or HD > 128 else 4
+    shared = [n > 1 and p > 0 for n, p in groups]
+    cols = max([n * G for (n, p), s in zip(groups, shared) if s], default=0)
+    ct = 2 if cols > 16 and HD <= 128 else 1
     fit = 16 * ct // G  # rows of a shared part
-    items, rows, r0, most = [], [], 0, 0
-    for n, p in groups:
-        if n == 1 or p == 0:
-            rows += [(0, 0)] * n
-        else:
-            per = max(256, -(-p // (16 * 128)) * 128)
-            splits = -(-p // per)
-            chunks = -(-n // fit)
-            for c in range(chunks):
-                a, b = n * c // chunks, n * (c + 1) // chunks
-                items += [(r0 + a, b - a, k * per, min(p, (k + 1) * per), k) for k in range(splits)]
-            rows += [(p, splits)] * n
-            most = max(most, splits)
+    slots = sum(p * -(-n // fit) for (n, p), s in zip(groups, shared) if s) * Hk
+    per = max(128, -(-slots // (PLAN_SHARED_WG * 128)) * 128)
+    units, rows, r0, most = [], [], 0, 0
+    for (n, p), s in zip(groups, shared):
+        splits = -(-p // per) if s else 0
+        chunks = -(-n // fit)
+        for k in range(splits):
+            units += [[(r0 + n * c // chunks, n * (c + 1) // chunks - n * c // chunks, k * per, min(p, (k + 1) * per), k, h)
+                       for c in range(chunks)] for h in range(Hk)]
+        rows += [(p if s else 0, splits)] * n
+        most = max(most, splits)
         r0 += n
-    longest = max(max_len - (p if n > 1 else 0) for n, p in groups)
-    nown = max(1, min(16, -(-512 // (R * Hk)), -(-longest // 128)))
+    # the parts that read the same slots get numbers that are equal modulo 8: one XCD, whose L2 then holds the slots
+    items = []
+    for u in range(0, len(units), 8):
+        eight = units[u:u + 8]
+        for c in range(max(len(x) for x in eight)):
+            items += [x[c] for x in eight if c < len(x)]
+    longest = max(max_len - (p if s else 0) for (n, p), s in zip(groups, shared))
+    nown = max(1, min(16, -(-PLAN_OWN_WG // (R * Hk)), -(-longest // 128)))
     return PagedAttnPlan(items, rows, nown, most + nown, ct, Hq, Hk, HD, dev)
 
 

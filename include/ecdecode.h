@@ -650,9 +650,9 @@ int ecd_paged_write(const void* qkv, long ld, const float* rope, int LR, const i
  * slots that a group of rows shares are read once for all of them.
  *   q row stride ldq; o [R, Hq * HD]; table row stride ldt; P a power of two from 16; HD in {64, 128, 256};
  *   Hq / Hk <= 16; MP P <= 2^30.
- *   rows [R, 2] int32: shared slots and number of shared parts of each row; items [nitems, 5] int32: first row, rows (at
- *   most 16 ctiles / (Hq / Hk)), first slot, last slot + 1 and part number of each shared part; nown: parts of each
- *   row's own slots; parts: the most parts of any row (<= 512); ctiles 1, 2 or 4 (HD 256: 1 or 2).  A row that does not
+ *   rows [R, 2] int32: shared slots and number of shared parts of each row; items [nitems, 6] int32: first row, rows (at
+ *   most 16 ctiles / (Hq / Hk)), first slot, last slot + 1, part number and kv head of each shared part; nown: parts of
+ *   each row's own slots; parts: the most parts of any row (<= 512); ctiles 1 or 2 (HD 256: 1).  A row that does not
  *   attend all shared slots takes none of the shared parts and attends its own slots from 0.
  *   ws: fp32 workspace of 2 ceil4(R Hq parts) + R Hq parts HD values (any contents; NULL where parts is 1). */
 int ecd_paged_attn(const void* q, long ldq, const void* kp, const void* vp, const int32_t* table, long ldt,
@@ -670,6 +670,10 @@ int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, lo
  * integer, one rounding at the end.  c from ecd_quant_a8 (zero columns behind K). */
 int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                 void* y, long ldy, int M, int N, int K, void* stream);
+
+/* ecd_gemm_a8 with the kernel chosen by cfg (0: the library's choice); the results are the same bits. */
+int ecd_gemm_a8_tuned(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
+                      void* y, long ldy, int M, int N, int K, int cfg, void* stream);
 
 /* mm[m, j] = f16(silu(z[m, 2j]) z[m, 2j + 1]), z the fp32 product of ecd_gemm_a8 on row-interleaved w1 | w3. */
 int ecd_gemm_a8_silu(const void* c, long ldc, const float* sx, const void* wp, const void* s, void* mm, long ldm,
