@@ -171,4 +171,6 @@ def check(rc: int, name: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    rc = getattr(_lib or lib(), name)(*args)
+    if rc:
+        check(rc, name)

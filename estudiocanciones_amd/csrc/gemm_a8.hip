@@ -189,32 +189,38 @@ struct A8Frags {
   i32x4 w[2][FT], x[2][RT];
 };
 
-template <int WN, int WM, int FT, int RT, int NS>
+template <int WN, int WM, int FT, int RT, int NS, int KG>
 struct A8Tile {
   static constexpr int NW = WN * WM, BN = 32 * WN * FT, BM = 32 * WM * RT;
   static constexpr int WI = BN / 8 / NW, XI = BM / 8 / NW, PER = WI + XI;  // DMA instructions (1 KB) per wave and chunk
   static_assert(WI * NW * 8 == BN && XI * NW * 8 == BM, "whole DMA instructions per wave");
   static_assert(NS >= 2 && PER * (NS - 1) < 64, "vmcnt range");
-  static constexpr int LW = BN * 128, LX = BM * 128, STG = LW + LX;  // bytes of a stage
+  static constexpr int LW = BN * 128, LX = BM * 128, STG = LW + LX, RING = NS * STG;  // bytes of a stage, of a group's ring
   // the sums leave through LDS as int32, some row tiles of each wave at a time
   static constexpr int ROW = BN + 4;  // ints of an output row
-  static constexpr int fit(int n) { return n == 1 || 32 * WM * n * ROW * 4 <= NS * STG ? n : fit(n / 2); }
+  static constexpr int fit(int n) { return n == 1 || 32 * WM * n * ROW * 4 <= RING ? n : fit(n / 2); }
   static constexpr int RP = fit(RT);  // row tiles of a pass
   static_assert(RT % RP == 0, "whole passes");
-  static constexpr int PASS_BYTES = 32 * WM * RP * ROW * 4;
-  static constexpr int LDS = NS * STG > PASS_BYTES ? NS * STG : PASS_BYTES;
+  static constexpr int PASS = 32 * WM * RP * ROW;  // ints of a pass
+  static constexpr int LDS = KG * (RING > PASS * 4 ? RING : PASS * 4);
+  static constexpr int THREADS = 64 * NW * KG;
 
-  // Sums of chunks c0 .. c0 + nch - 1 of 128 k.  `odd`: the last of them is half a chunk (its second half of the weights
-  // re-reads the first; the codes behind K are 0).
-  static __device__ __forceinline__ void run(unsigned char* lds, i32x16 (&acc)[FT][RT], const int8_t* __restrict__ c, long ldc,
-                                             const int8_t* __restrict__ wp, int M, int N, int K, int n0, int m0, int c0,
-                                             int nch, bool odd) {
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wn = wv % WN, wm = wv / WN;
+  // The sums of this wave's group: KG groups of NW waves take an equal share of K each, from a ring of their own (a CU
+  // with one workgroup then has KG times the loads in flight, where there are too few tiles for all CUs).  A chunk of 128 k
+  // that K ends in: the second half of the weights re-reads the first, the codes behind K are 0.
+  static __device__ __forceinline__ void run(unsigned char* all, i32x16 (&acc)[FT][RT], const int8_t* __restrict__ c, long ldc,
+                                             const int8_t* __restrict__ wp, int M, int N, int K, int n0, int m0) {
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wv = wid % NW, kg = wid / NW, wn = wv % WN, wm = wv / WN;
+    unsigned char* lds = all + kg * RING;
+    const int chunks = (K + 127) >> 7, most = (chunks + KG - 1) / KG;
+    const int c0 = chunks * kg / KG, nch = chunks * (kg + 1) / KG - c0;
+    const bool odd = (K & 64) && kg == KG - 1;
     const int ntiles = (N + 15) >> 4, t0 = min(n0 / 16, ntiles - 1);
     const long tile_bytes = 16L * K;
     const int8_t* wb = wp + t0 * tile_bytes + 2048L * c0;
     const int8_t* xb = c + (long)m0 * ldc + 128L * c0;
+    int left = nch;  // chunks not yet asked for
     uint32_t woff[WI], xoff[XI];
 #pragma unroll
     for (int j = 0; j < WI; ++j) {
@@ -227,7 +233,6 @@ struct A8Tile {
       xoff[j] = (uint32_t)((min(m0 + r, M - 1) - m0) * ldc) + 16 * ((lane & 7) ^ x_swz(r));
     }
     const uint32_t lds0 = lds_addr(lds) + wv * 1024;
-    int left = nch;  // chunks not yet asked for
     const uint32_t back = wv & 1 ? 1024u : 0u;  // (NW is even: this wave's weight instructions are all first or all second halves)
     static_assert(NW % 2 == 0, "a wave keeps its half");
     auto dma = [&](auto J, uint32_t sa) {
@@ -275,12 +280,16 @@ struct A8Tile {
         __builtin_amdgcn_sched_barrier(0);
       });
     };
-    auto barrier = [&]() {
+    auto barrier = [&]() {  // (of the whole workgroup: each group passes `most` of them)
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
 
+    if (KG > 1 && nch == 0) {
+      for (int b = 0; b < most; ++b) barrier();
+      return;
+    }
     for (int s = 0; s < NS; ++s)
       if (s < nch) {
         static_for<0, PER>([&](auto J) { dma(J, lds0 + s * STG); });
@@ -315,22 +324,24 @@ struct A8Tile {
       st = sn;
     }
     half(fc, IC<0>{}, lds, fa, IC<0>{}, IC<0>{}, 0);  // (its reads are never used)
+    if (KG > 1 && nch < most) barrier();
   }
 
-  // f(row of the tile, feature of the tile, 8 sums) for every piece of 8 features, rows in passes through LDS
+  // f(row of the tile, 8 sums) for every row and this thread's piece of 8 features, rows in passes through LDS, where the
+  // groups' sums are added
   template <typename F>
   static __device__ __forceinline__ void sums(unsigned char* lds, const i32x16 (&acc)[FT][RT], F&& f) {
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wn = wv % WN, wm = wv / WN;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wv = wid % NW, kg = wid / NW, wn = wv % WN, wm = wv / WN;
     int* buf = (int*)lds;
-    constexpr int PR = BN / 8, RS = 64 * NW / PR, ROWS = 32 * WM * RP;
-    static_assert(64 * NW % PR == 0 && ROWS % RS == 0, "whole rows per step");
+    constexpr int PR = BN / 8, RS = THREADS / PR, ROWS = 32 * WM * RP;
+    static_assert(THREADS % PR == 0, "whole rows per step");
     const int p = threadIdx.x % PR;
     static_for<0, RT / RP>([&](auto P) {
       __syncthreads();
       static_for<0, FT * RP>([&](auto I) {
         constexpr int ft = decltype(I)::value / RP, q = decltype(I)::value % RP, rt = decltype(P)::value * RP + q;
-        int* d = buf + (long)((wm * RP + q) * 32 + (lane & 31)) * ROW + (wn * FT + ft) * 32 + 4 * (lane >> 5);
+        int* d = buf + kg * PASS + ((wm * RP + q) * 32 + (lane & 31)) * ROW + (wn * FT + ft) * 32 + 4 * (lane >> 5);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *(i32x4*)(d + 8 * g) = (i32x4){acc[ft][rt][4 * g], acc[ft][rt][4 * g + 1], acc[ft][rt][4 * g + 2], acc[ft][rt][4 * g + 3]};
@@ -338,10 +349,15 @@ struct A8Tile {
       __syncthreads();
 #pragma unroll 2
       for (int r = threadIdx.x / PR; r < ROWS; r += RS) {
-        const i32x4 a = *(const i32x4*)(buf + (long)r * ROW + 8 * p), b = *(const i32x4*)(buf + (long)r * ROW + 8 * p + 4);
+        i32x4 a = *(const i32x4*)(buf + r * ROW + 8 * p), b = *(const i32x4*)(buf + r * ROW + 8 * p + 4);
+#pragma unroll
+        for (int k = 1; k < KG; ++k) {
+          a += *(const i32x4*)(buf + k * PASS + r * ROW + 8 * p);
+          b += *(const i32x4*)(buf + k * PASS + r * ROW + 8 * p + 4);
+        }
         const int v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         const int w = r / (32 * RP), q = r - w * 32 * RP;
-        f((w * RT + decltype(P)::value * RP) * 32 + q, 8 * p, v);
+        f((w * RT + decltype(P)::value * RP) * 32 + q, v);
       }
     });
   }
@@ -362,33 +378,33 @@ __device__ __forceinline__ void a8_block(int b, int nfb, int nmb, int& fb, int& 
   }
 }
 
-template <bool SILU, int WN, int WM, int FT, int RT, int NS>
-__global__ __launch_bounds__(64 * WN * WM, 1) void gemm_a8_kernel(const int8_t* __restrict__ c, long ldc,
-                                                                  const int8_t* __restrict__ wp, A8Out out, int M, int N, int K,
-                                                                  int nfb, int nmb) {
-  using T = A8Tile<WN, WM, FT, RT, NS>;
+template <bool SILU, int WN, int WM, int FT, int RT, int NS, int KG>
+__global__ __launch_bounds__(64 * WN * WM * KG, 1) void gemm_a8_kernel(const int8_t* __restrict__ c, long ldc,
+                                                                       const int8_t* __restrict__ wp, A8Out out, int M, int N,
+                                                                       int K, int nfb, int nmb) {
+  using T = A8Tile<WN, WM, FT, RT, NS, KG>;
   __shared__ __align__(16) unsigned char lds[T::LDS];
   int fb, mb;
   a8_block(blockIdx.x, nfb, nmb, fb, mb);
   const int n0 = fb * T::BN, m0 = mb * T::BM;
   i32x16 acc[FT][RT];
-  T::run(lds, acc, c, ldc, wp, M, N, K, n0, m0, 0, (K + 127) >> 7, K & 64);
+  T::run(lds, acc, c, ldc, wp, M, N, K, n0, m0);
   const int nb = n0 + 8 * (threadIdx.x % (T::BN / 8));
   float sn[8];
   a8_scales(out.s, nb, N, sn);
-  T::sums(lds, acc, [&](int r, int, const int (&v)[8]) {
+  T::sums(lds, acc, [&](int r, const int (&v)[8]) {
     const int m = m0 + r;
     if (m < M && nb < N) a8_finish<SILU>(out, v, out.sx[m], sn, m, nb, N);
   });
 }
 
-template <bool SILU, int WN, int WM, int FT, int RT, int NS>
+template <bool SILU, int WN, int WM, int FT, int RT, int NS, int KG = 1>
 static int launch_tile(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
-  using T = A8Tile<WN, WM, FT, RT, NS>;
+  using T = A8Tile<WN, WM, FT, RT, NS, KG>;
   const int nfb = (N + T::BN - 1) / T::BN, nmb = (M + T::BM - 1) / T::BM;
   if ((long)nfb * nmb > 0x7FFFFFFFL) return ECD_ENOTSUP;
-  hipLaunchKernelGGL((gemm_a8_kernel<SILU, WN, WM, FT, RT, NS>), dim3((unsigned)(nfb * nmb)), dim3(64 * WN * WM), 0, st, c, ldc, wp, out, M,
-                     N, K, nfb, nmb);
+  hipLaunchKernelGGL((gemm_a8_kernel<SILU, WN, WM, FT, RT, NS, KG>), dim3((unsigned)(nfb * nmb)), dim3(T::THREADS), 0, st, c, ldc, wp, out,
+                     M, N, K, nfb, nmb);
   return ecd_launch_status();
 }
 
@@ -405,7 +421,7 @@ static int launch_a8(const void* cv, long ldc, const void* wv, const A8Out& out,
   const int8_t *c = (const int8_t*)cv, *wp = (const int8_t*)wv;
 #define A8_TILE(...) return launch_tile<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
 #define A8_FEW(...) return launch_few<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
-  if (!cfg) cfg = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 3 : M <= 256 ? 7 : 10;
+  if (!cfg) cfg = M <= 16 ? 4 : M <= 256 ? 14 : 11;
   switch (cfg) {
     case 1: A8_FEW(1, 4);
     case 2: A8_FEW(2, 4);
@@ -420,6 +436,21 @@ static int launch_a8(const void* cv, long ldc, const void* wv, const A8Out& out,
     case 11: A8_TILE(4, 2, 2, 4, 2);  // 256 x 256, 8 waves
     case 12: A8_TILE(2, 2, 4, 2, 3);  // 256 x 128, 4 waves
     case 13: A8_TILE(2, 2, 2, 4, 3);  // 128 x 256
+    case 14: A8_TILE(2, 2, 1, 1, 4);     // 64 x 64, two per CU
+    case 15: A8_TILE(2, 2, 1, 1, 3);     // 64 x 64, three per CU
+    case 16: A8_TILE(2, 2, 1, 2, 3);     // 64 x 128, two per CU
+    case 17: A8_TILE(2, 2, 2, 1, 3);     // 128 x 64
+    case 18: A8_TILE(2, 2, 2, 2, 2);     // 128 x 128, two per CU
+    case 20: A8_FEW(1, 16);
+    case 21: A8_TILE(2, 2, 1, 1, 4, 2);  // 64 x 64, K in two
+    case 22: A8_TILE(2, 2, 1, 1, 2, 4);  // 64 x 64, K in four
+    case 23: A8_TILE(1, 2, 1, 1, 3, 4);  // 32 x 64, K in four
+    case 24: A8_TILE(2, 1, 1, 1, 3, 4);  // 64 x 32, K in four
+    case 25: A8_TILE(2, 2, 1, 2, 3, 2);  // 64 x 128, K in two
+    case 26: A8_TILE(2, 2, 2, 1, 3, 2);  // 128 x 64, K in two
+    case 27: A8_TILE(2, 2, 1, 1, 2, 2);  // 64 x 64, K in two, two per CU
+    case 28: A8_TILE(1, 2, 1, 1, 3, 2);  // 32 x 64, K in two, two per CU
+    case 29: A8_TILE(2, 2, 2, 2, 2, 2);  // 128 x 128, K in two
     default: return ECD_EINVAL;
   }
 #undef A8_TILE
@@ -463,7 +494,8 @@ int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const 
 
 int ecd_gemm_a8_tuned(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                       void* y, long ldy, int M, int N, int K, int cfg, void* stream) {
-  if (!a8_ok(c, ldc, sx, wp, s, y, M, N, K) || ldy < N || (res && ldr < N) || cfg < 0) return ECD_EINVAL;
+  if (!a8_ok(c, ldc, sx, wp, s, y, M, N, K) || ldy < N || (res && ldr < N) || cfg < 0)
+    return ECD_EINVAL;
   return launch_a8<false>(c, ldc, wp, A8Out{sx, (const f16*)s, (const f16*)res, ldr, (f16*)y, ldy}, M, N, K,
                           (hipStream_t)stream, cfg);
 }

@@ -58,27 +58,23 @@ struct PTile {
   vec v[2][4][ND];
 };
 
-// Where the tiles of a wave lie: lane i holds the pool row (page Hk + kh) P + slot of the halves of tile i.  Slots from hi
+// Where tiles lie: lane i holds the pool row (page Hk + kh) P + slot of the halves of the tile at t0 + step i.  Slots from hi
 // on repeat a half before it (masked later); a number that is no page reads page 0 or the last one.
 struct Places {
-  uint32_t r[2];
+  uint32_t r0, r1;
 };
-__device__ __forceinline__ Places places(const PagedArgs& a, const int* tab, int kh, int t0, int hi, int lane) {
-  Places p;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int h = min(t0 + lane * (PQ_W * PQ_T) + 16 * j, (hi - 1) & ~15);  // a half tile lies in one page
-    const int page = min(max(tab[h >> a.PS], 0), a.NP - 1);
-    p.r[j] = (((uint32_t)page * a.Hk + kh) << a.PS) + (h & ((1 << a.PS) - 1));
-  }
-  return p;
+__device__ __forceinline__ Places places(const PagedArgs& a, const int* tab, int kh, int t0, int step, int hi, int lane) {
+  const int last = (hi - 1) & ~15, mask = (1 << a.PS) - 1;  // a half tile lies in one page
+  const int h0 = min(t0 + lane * step, last), h1 = min(t0 + lane * step + 16, last);
+  const uint32_t p0 = min(max(tab[h0 >> a.PS], 0), a.NP - 1), p1 = min(max(tab[h1 >> a.PS], 0), a.NP - 1);
+  return {((p0 * a.Hk + kh) << a.PS) + (h0 & mask), ((p1 * a.Hk + kh) << a.PS) + (h1 & mask)};
 }
 
 template <int HD>
 __device__ __forceinline__ void load_k(PTile<HD>& t, const PagedArgs& a, const Places& p, int i, int lane) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const f16* k = a.kp + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.r[j], i) * HD;
+    const f16* k = a.kp + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(j ? p.r1 : p.r0), i) * HD;
 #pragma unroll
     for (int x = 0; x < PTile<HD>::KC; ++x) t.k[j][x] = *(const f16x8*)(k + (uint32_t)((lane & 15) * HD + 8 * (lane >> 4) + 32 * x));
   }
@@ -87,7 +83,7 @@ template <int HD>
 __device__ __forceinline__ void load_v(PTile<HD>& t, const PagedArgs& a, const Places& p, int i, int lane) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const f16* v = a.vp + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.r[j], i) * HD;
+    const f16* v = a.vp + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(j ? p.r1 : p.r0), i) * HD;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -173,30 +169,26 @@ __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, flo
       }
   }
 #pragma unroll
-  for (int x = 0; x < T::ND; ++x)
+  for (int x = 0; x < T::ND; ++x) {
+    const typename T::vec v0 = t.v[0][0][x], v1 = t.v[0][1][x], v2 = t.v[0][2][x], v3 = t.v[0][3][x];
+    const typename T::vec v4 = t.v[1][0][x], v5 = t.v[1][1][x], v6 = t.v[1][2][x], v7 = t.v[1][3][x];
 #pragma unroll
     for (int b = 0; b < T::VW; ++b) {
-      const f16x8 va = {t.v[0][0][x][b], t.v[0][1][x][b], t.v[0][2][x][b], t.v[0][3][x][b],
-                        t.v[1][0][x][b], t.v[1][1][x][b], t.v[1][2][x][b], t.v[1][3][x][b]};
+      const f16x8 va = {v0[b], v1[b], v2[b], v3[b], v4[b], v5[b], v6[b], v7[b]};
 #pragma unroll
       for (int c = 0; c < CT; ++c) s.acc[c][x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[c], s.acc[c][x][b], 0, 0, 0);
     }
+  }
 }
 
-// One part on one workgroup: `cols` columns (query head c % G of row row0 + c / G), slots [lo, hi) through `tab`.
-// `live(row)`: whether the row takes this part.  Its result goes to place `part`, or with `whole` normalised to o.
-template <int HD, int CT, typename Live>
-__device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0, int cols, int kh, const int* tab, int lo,
-                                       int hi, int part, bool whole, Live&& live) {
-  constexpr int ST = HD + 4;  // floats of a column in LDS
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int grp = lane >> 4, col = lane & 15;
-  PState<HD, CT> s;
+// nothing attended yet; q of columns 16 first .. (query head n % G of row row0 + n / G; columns from cols on repeat one)
+template <int HD, int CT>
+__device__ __forceinline__ void begin(PState<HD, CT>& s, const PagedArgs& a, int row0, int cols, int first, int kh, int lane) {
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const int n = 16 * c + col;
+    const int n = 16 * (first + c) + (lane & 15);
     const int cc = n < cols ? n : 0;
-    const f16* q = a.q + (long)(row0 + cc / a.G) * a.ldq + (long)(kh * a.G + cc % a.G) * HD + 8 * grp;
+    const f16* q = a.q + (long)(row0 + cc / a.G) * a.ldq + (long)(kh * a.G + cc % a.G) * HD + 8 * (lane >> 4);
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) s.q[c][i] = *(const f16x8*)(q + 32 * i);
     s.m[c] = -INFINITY;
@@ -206,6 +198,18 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
 #pragma unroll
       for (int b = 0; b < PTile<HD>::VW; ++b) s.acc[c][x][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
+}
+
+// One part on one workgroup whose waves share out the slots: `cols` columns, slots [lo, hi) through `tab`.
+// `live`: bit i says whether row row0 + i takes this part.  Its result goes to place `part`, or with `whole` normalised to o.
+template <int HD, int CT>
+__device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0, int cols, int kh, const int* tab, int lo,
+                                       int hi, int part, bool whole, uint64_t live) {
+  constexpr int ST = HD + 4;  // floats of a column in LDS
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = lane >> 4, col = lane & 15;
+  PState<HD, CT> s;
+  begin(s, a, row0, cols, 0, kh, lane);
   // K of the next tile is asked for once this one's scores are formed, V once this one's is used: one tile is always in
   // flight, in the registers of the last one
   PTile<HD> t;
@@ -213,13 +217,13 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
   const int n = hi > first ? (hi - first + PQ_W * PQ_T - 1) / (PQ_W * PQ_T) : 0;
   Places at;
   if (n > 0) {
-    at = places(a, tab, kh, first, hi, lane);
+    at = places(a, tab, kh, first, PQ_W * PQ_T, hi, lane);
     load_k<HD>(t, a, at, 0, lane);
     load_v<HD>(t, a, at, 0, lane);
   }
   for (int i = 0; i < n; ++i) {
     const bool more = i + 1 < n;
-    if (more && ((i + 1) & 63) == 0) at = places(a, tab, kh, first + (i + 1) * (PQ_W * PQ_T), hi, lane);
+    if (more && ((i + 1) & 63) == 0) at = places(a, tab, kh, first + (i + 1) * (PQ_W * PQ_T), PQ_W * PQ_T, hi, lane);
     tile_attend<HD, CT>(s, t, a.c2, first + i * (PQ_W * PQ_T), lo, hi, lane, [&]() {
       asm volatile("" ::: "memory");
       if (more) load_k<HD>(t, a, at, (i + 1) & 63, lane);
@@ -280,7 +284,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
       *(f16x4*)(a.o + head * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
     } else {
       const long pi = head * a.parts + part;
-      M = !live(row) ? -INFINITY : l == l ? M : l;
+      M = !(live >> (row - row0) & 1) ? -INFINITY : l == l ? M : l;
       if (d == 0) {
         a.pm[pi] = M;
         a.pl[pi] = l;
@@ -295,36 +299,32 @@ constexpr int attend_lds() {
   return PQ_W * 16 * CT * (2 + HD + 4);
 }
 
+// slots that row r attends
+__device__ __forceinline__ int attended(const PagedArgs& a, int r) {
+  const long p = a.pos[r];
+  return (int)min(p < 0 ? 0l : p + 1, (long)a.MP << a.PS);
+}
+
 template <int HD, int CT>
-__global__ __launch_bounds__(64 * PQ_W, 2) void paged_attn_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * PQ_W, HD > 128 ? 1 : 2) void paged_attn_kernel(PagedArgs a) {
   __shared__ __align__(16) float lds[attend_lds<HD, CT>()];
-  __shared__ int s_lead;
+  const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < a.nitems) {
     const int* it = a.items + 6 * blockIdx.x;
     const int row0 = it[0], n = it[1], lo = it[2], hi = it[3], kh = it[5];
     // the first row that attends the whole prefix leads: its pages hold every shared slot
-    if (threadIdx.x < 64) {
-      const int r = row0 + threadIdx.x;
-      const bool in = (int)threadIdx.x < n && a.pos[r] + 1 >= a.rows[2 * r];
-      const uint64_t b = __ballot(in);
-      if (threadIdx.x == 0) s_lead = b ? row0 + __builtin_ctzll(b) : -1;
-    }
-    __syncthreads();
-    const int lead = __builtin_amdgcn_readfirstlane(s_lead);
-    const int hi1 = lead < 0 ? lo : min(hi, a.MP << a.PS);
-    attend<HD, CT>(a, lds, row0, n * a.G, kh, a.table + (long)max(lead, 0) / a.S * a.ldt, min(lo, hi1), hi1, it[4], false,
-                   [&](int row) { return a.pos[row] + 1 >= a.rows[2 * row]; });
+    const int r = row0 + min(lane, n - 1);
+    const uint64_t live = __ballot(lane < n && attended(a, r) >= a.rows[2 * r]);
+    const int* tab = a.table + (long)((row0 + (live ? __builtin_ctzll(live) : 0)) / a.S) * a.ldt;
+    attend<HD, CT>(a, lds, row0, n * a.G, kh, tab, lo, live ? hi : lo, it[4], false, live);
     return;
   }
   const int x = blockIdx.x - a.nitems, u = x / a.Hk, kh = x - u * a.Hk, r = u / a.nown, k = u - r * a.nown;
-  const long p = a.pos[r];
-  const int end = (int)min(p < 0 ? 0l : p + 1, (long)a.MP << a.PS);
-  const int shared = a.rows[2 * r], np = a.rows[2 * r + 1];
+  const int end = attended(a, r), shared = a.rows[2 * r], np = a.rows[2 * r + 1];
   const int from = end >= shared ? shared : 0;
   const int per = (max(PQ_MIN, (end - from + a.nown - 1) / a.nown) + PQ_T - 1) & ~(PQ_T - 1);
   const int lo = min(from + k * per, end), hi = min(lo + per, end);
-  attend<HD, 1>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1,
-                [](int) { return true; });
+  attend<HD, 1>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1, ~0ull);
 }
 
 // One thread per four dims of a head: JB parts at a time, all their loads at once, in the order of the parts.

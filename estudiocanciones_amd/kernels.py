@@ -830,108 +830,129 @@ def embed_gemv_packed(tok, table, tscale, cb, vocab, wp, s, N, even=None, stream
 
 
 # ---------------------------------------------------------------- pages of a KV cache
-def _on(t, dev, name, dtype, shape):
-    """t is a contiguous tensor of dtype and shape on dev (-1: any size)."""
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+def _on(t, dev, call, name, dtype, shape):
+    """t is a contiguous tensor of dtype and shape on dev."""
+    if t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous():
+        return
+    if t.dtype is not dtype:
+        raise TypeError(f"{call}: {name}: expected {dtype}, got {t.dtype}")
     if t.device != dev:
-        raise ValueError(f"{name}: is on {t.device}, the call's other tensors on {dev}")
-    if t.dim() != len(shape) or any(a not in (-1, b) for a, b in zip(shape, t.shape)) or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
+        raise ValueError(f"{call}: {name} is on {t.device}, the call's other tensors on {dev}")
+    raise ValueError(f"{call}: {name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _call_on(dev, name, *args):
-    """_ffi.call with the tensors' device as the current one, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        _ffi.call(name, *args, stream_ptr(dev))
+    """_ffi.call with the tensors' device as the current one, on its current stream (asked for as its handle: a stream
+    object costs as much as a launch)."""
+    i = dev.index
+    if i == torch._C._cuda_getDevice():
+        _ffi.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
-            _ffi.call(name, *args, stream_ptr(dev))
+            _ffi.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
 
 
 def _page_state(name, ref, table, length, err):
     dev = _dev(ref, name)
-    _on(ref, dev, f"{name} ref", torch.int32, (-1,))
-    _on(table, dev, f"{name} table", torch.int32, (-1, -1))
-    _on(length, dev, f"{name} length", torch.int64, (table.shape[0],))
-    _on(err, dev, f"{name} err", torch.int32, (1,))
-    return dev
+    if table.dim() != 2:
+        raise ValueError(f"{name}: table must be [B, MP]")
+    B, MP = table.shape
+    _on(ref, dev, name, "ref", torch.int32, (ref.numel(),))
+    _on(table, dev, name, "table", torch.int32, (B, MP))
+    _on(length, dev, name, "length", torch.int64, (B,))
+    _on(err, dev, name, "err", torch.int32, (1,))
+    return dev, ref.numel(), B, MP
 
 
 def _page_pool(name, kv, ref):
-    _on(kv, ref.device, f"{name} kv", torch.float16, (-1, 2, ref.shape[0], -1, -1, -1))
-    if kv.shape[5] % 8:
-        raise ValueError(f"{name}: head_dim must be a multiple of 8")
-    return kv.shape[0] * 2, kv.shape[3], kv.shape[4], kv.shape[5]
+    if kv.dim() != 6:
+        raise ValueError(f"{name}: kv must be [layers, 2, NP, Hk, P, HD]")
+    layers, _, NP, Hk, P, HD = kv.shape
+    _on(kv, ref.device, name, "kv", torch.float16, (layers, 2, ref.numel(), Hk, P, HD))
+    if HD % 8 or kv.data_ptr() % 16:
+        raise ValueError(f"{name}: head_dim must be a multiple of 8 and kv 16-byte aligned")
+    return layers * 2, Hk, P, HD
 
 
 def page_free(ref, table, length, seqs, page, err):
     """The sequences ``seqs`` [n] int32 give their pages back: a page whose last owner goes is free.  ``ref`` [NP] int32
     owners of each page, ``table`` [B, MP] int32 page numbers (-1 behind a sequence's last), ``length`` [B] int64 slots
     held, ``page`` slots of a page; ``err`` [1] int32 collects what was refused (include/ecdecode.h lists its bits)."""
-    dev = _page_state("page_free", ref, table, length, err)
-    _on(seqs, dev, "page_free seqs", torch.int32, (-1,))
-    if seqs.shape[0]:
-        _call_on(dev, "ecd_page_free", ref.data_ptr(), ref.shape[0], table.data_ptr(), table.shape[1], length.data_ptr(),
-                 table.shape[0], int(page), seqs.data_ptr(), seqs.shape[0], err.data_ptr())
+    dev, NP, B, MP = _page_state("page_free", ref, table, length, err)
+    n = seqs.numel()
+    _on(seqs, dev, "page_free", "seqs", torch.int32, (n,))
+    if n:
+        _call_on(dev, "ecd_page_free", ref.data_ptr(), NP, table.data_ptr(), MP, length.data_ptr(), B, int(page),
+                 seqs.data_ptr(), n, err.data_ptr())
 
 
 def page_fork(kv, ref, table, length, src, dst, err):
     """Sequence dst[i] (holding nothing) becomes a copy of src[i] (int32 [n], n <= 1024): whole pages shared, the slots
     of a last page that is not full copied into a page of its own in every layer of ``kv`` [layers, 2, NP, Hk, P, HD]."""
-    dev = _page_state("page_fork", ref, table, length, err)
+    dev, NP, B, MP = _page_state("page_fork", ref, table, length, err)
     planes, Hk, P, HD = _page_pool("page_fork", kv, ref)
-    _on(src, dev, "page_fork src", torch.int32, (-1,))
-    _on(dst, dev, "page_fork dst", torch.int32, src.shape)
-    n = src.shape[0]
+    n = src.numel()
+    _on(src, dev, "page_fork", "src", torch.int32, (n,))
+    _on(dst, dev, "page_fork", "dst", torch.int32, (n,))
     if n:
         plan = torch.empty(4 * n, device=dev, dtype=torch.int32)
-        _call_on(dev, "ecd_page_fork", kv.data_ptr(), ref.data_ptr(), ref.shape[0], table.data_ptr(), table.shape[1],
-                 length.data_ptr(), table.shape[0], src.data_ptr(), dst.data_ptr(), n, plan.data_ptr(), err.data_ptr(),
-                 planes, Hk, P, HD)
+        _call_on(dev, "ecd_page_fork", kv.data_ptr(), ref.data_ptr(), NP, table.data_ptr(), MP, length.data_ptr(), B,
+                 src.data_ptr(), dst.data_ptr(), n, plan.data_ptr(), err.data_ptr(), planes, Hk, P, HD)
 
 
 def page_extend(ref, table, length, pos, page, err):
     """Every sequence b holds slot pos[b] (int64 [B], B <= 1024) afterwards; -1, or a slot it holds, leaves it alone."""
-    dev = _page_state("page_extend", ref, table, length, err)
-    _on(pos, dev, "page_extend pos", torch.int64, length.shape)
-    _call_on(dev, "ecd_page_extend", ref.data_ptr(), ref.shape[0], table.data_ptr(), table.shape[1], length.data_ptr(),
-             table.shape[0], int(page), pos.data_ptr(), err.data_ptr())
+    dev, NP, B, MP = _page_state("page_extend", ref, table, length, err)
+    _on(pos, dev, "page_extend", "pos", torch.int64, (B,))
+    _call_on(dev, "ecd_page_extend", ref.data_ptr(), NP, table.data_ptr(), MP, length.data_ptr(), B, int(page),
+             pos.data_ptr(), err.data_ptr())
 
 
 def page_compact(kv, ref, table, length, kv2, ref2, table2, length2, err):
     """The pages in use, in ascending order, to the first pages of another pool kv2 [layers, 2, NP2, Hk, P, HD], with the
     state ref2 [NP2], table2 [B, MP], length2 [B] that goes with them.  The first pool and its state stay as they are."""
-    dev = _page_state("page_compact", ref, table, length, err)
+    dev, NP, B, MP = _page_state("page_compact", ref, table, length, err)
     planes, Hk, P, HD = _page_pool("page_compact", kv, ref)
-    _on(ref2, dev, "page_compact ref2", torch.int32, (-1,))
-    _on(kv2, dev, "page_compact kv2", torch.float16, (kv.shape[0], 2, ref2.shape[0], Hk, P, HD))
-    _on(table2, dev, "page_compact table2", torch.int32, table.shape)
-    _on(length2, dev, "page_compact length2", torch.int64, length.shape)
+    NP2 = ref2.numel()
+    _on(ref2, dev, "page_compact", "ref2", torch.int32, (NP2,))
+    _on(kv2, dev, "page_compact", "kv2", torch.float16, (kv.shape[0], 2, NP2, Hk, P, HD))
+    _on(table2, dev, "page_compact", "table2", torch.int32, (B, MP))
+    _on(length2, dev, "page_compact", "length2", torch.int64, (B,))
     for a, b in ((kv, kv2), (ref, ref2), (table, table2), (length, length2)):
         lo, hi = a.data_ptr(), a.data_ptr() + a.numel() * a.element_size()
         if b.data_ptr() < hi and lo < b.data_ptr() + b.numel() * b.element_size():
             raise ValueError("page_compact: the two pools and their states must not overlap")
-    ws = torch.empty(1 + 2 * ref.shape[0], device=dev, dtype=torch.int32)
-    _call_on(dev, "ecd_page_compact", kv.data_ptr(), ref.data_ptr(), ref.shape[0], table.data_ptr(), length.data_ptr(),
-             kv2.data_ptr(), ref2.data_ptr(), ref2.shape[0], table2.data_ptr(), length2.data_ptr(), table.shape[0],
-             table.shape[1], ws.data_ptr(), err.data_ptr(), planes, Hk, P, HD)
+    ws = torch.empty(1 + 2 * NP, device=dev, dtype=torch.int32)
+    _call_on(dev, "ecd_page_compact", kv.data_ptr(), ref.data_ptr(), NP, table.data_ptr(), length.data_ptr(),
+             kv2.data_ptr(), ref2.data_ptr(), NP2, table2.data_ptr(), length2.data_ptr(), B, MP, ws.data_ptr(),
+             err.data_ptr(), planes, Hk, P, HD)
 
 
 def _paged(name, kp, vp, table, dev):
-    _on(kp, dev, f"{name} kp", torch.float16, (-1, -1, -1, -1))
-    _on(vp, dev, f"{name} vp", torch.float16, kp.shape)
-    if table.dtype != torch.int32 or table.device != dev or table.dim() != 2 or table.stride(1) != 1 or \
-            table.stride(0) < table.shape[1]:
+    """(NP, Hk, P, HD, MP, table stride) of the pages and the table of a call."""
+    if kp.dim() != 4 or table.dim() != 2:
+        raise ValueError(f"{name}: kp / vp must be [NP, Hk, P, HD] and table [B, MP]")
+    shape = kp.shape
+    _on(kp, dev, name, "kp", torch.float16, shape)
+    _on(vp, dev, name, "vp", torch.float16, shape)
+    MP, (ld, one) = table.shape[1], table.stride()
+    if table.dtype is not torch.int32 or table.device != dev or one != 1 or ld < MP:
         raise ValueError(f"{name}: table must be int32 [B, MP] with contiguous rows on {dev}")
     if kp.data_ptr() % 16 or vp.data_ptr() % 16:
         raise ValueError(f"{name}: kp and vp must be 16-byte aligned")
+    return *shape, MP, ld
 
 
-def _rows16(t, dev, name):
+def _rows16(t, name):
+    """(device, row stride) of a [M, N] fp16 GPU tensor with unit inner stride and 16-byte rows."""
+    dev = t.device
+    if t.dtype is torch.float16 and t.is_cuda and t.dim() == 2:
+        ld, one = t.stride()
+        if one == 1 and ld % 8 == 0 and t.data_ptr() % 16 == 0:
+            return dev, ld
+    _dev(t, name)
     _f16(t, name)
-    if t.device != dev or t.dim() != 2 or t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: must be [M, N] on {dev} with unit inner stride and 16-byte rows")
+    raise ValueError(f"{name}: must be [M, N] with unit inner stride and 16-byte rows")
 
 
 def paged_write(qkv, kp, vp, table, pos, S, Hq, Hk, rope=None, q=None):
@@ -939,24 +960,24 @@ def paged_write(qkv, kp, vp, table, pos, S, Hq, Hk, rope=None, q=None):
     (int64 [M]); ``kp`` / ``vp`` [NP, Hk, P, HD], ``table`` [B, MP] int32 with B S >= M.  With ``rope`` [L, HD/2, 2]
     float32, q and k are rotated first (the numerics of _rope_cache) and q [M, Hq HD] is returned (``q``: its
     destination); without it nothing is.  A row whose slot has no page writes nothing into the cache."""
-    dev = _dev(qkv, "paged_write")
-    _rows16(qkv, dev, "paged_write qkv")
-    _paged("paged_write", kp, vp, table, dev)
-    M, (NP, _, P, HD) = qkv.shape[0], kp.shape
-    if kp.shape[1] != Hk or qkv.shape[1] != (Hq + 2 * Hk) * HD or HD % 8 or S < 1 or table.shape[0] * S < M:
+    dev, ld = _rows16(qkv, "paged_write qkv")
+    NP, hk, P, HD, MP, ldt = _paged("paged_write", kp, vp, table, dev)
+    M, W = qkv.shape
+    if hk != Hk or W != (Hq + 2 * Hk) * HD or HD % 8 or S < 1 or table.shape[0] * S < M:
         raise ValueError("paged_write: qkv must be [M, (Hq + 2 Hk) HD], kp / vp [NP, Hk, P, HD], table [B, MP] with "
                          "B * S >= M")
-    _on(pos, dev, "paged_write pos", torch.int64, (M,))
+    _on(pos, dev, "paged_write", "pos", torch.int64, (M,))
+    L = 0
     if rope is not None:
-        _on(rope, dev, "paged_write rope", torch.float32, (-1, HD // 2, 2))
+        L = rope.shape[0]
+        _on(rope, dev, "paged_write", "rope", torch.float32, (L, HD // 2, 2))
         q = torch.empty(M, Hq * HD, device=dev, dtype=torch.float16) if q is None else q
-        _on(q, dev, "paged_write q", torch.float16, (M, Hq * HD))
+        _on(q, dev, "paged_write", "q", torch.float16, (M, Hq * HD))
     else:
         q = None
     if M:
-        _call_on(dev, "ecd_paged_write", qkv.data_ptr(), qkv.stride(0), _ptr(rope), 0 if rope is None else rope.shape[0],
-                 pos.data_ptr(), _ptr(q), kp.data_ptr(), vp.data_ptr(), table.data_ptr(), table.stride(0),
-                 table.shape[1], NP, M, int(S), Hq, Hk, P, HD)
+        _call_on(dev, "ecd_paged_write", qkv.data_ptr(), ld, _ptr(rope), L, pos.data_ptr(), _ptr(q), kp.data_ptr(),
+                 vp.data_ptr(), table.data_ptr(), ldt, MP, NP, M, int(S), Hq, Hk, P, HD)
     return q
 
 
@@ -967,14 +988,17 @@ class PagedAttnPlan:
         self.nitems, self.R, self.nown, self.parts, self.ctiles = len(items), len(rows), nown, parts, ctiles
         self.Hq, self.Hk, self.HD = Hq, Hk, HD
         flat = torch.tensor([v for x in rows for v in x] + [v for x in items for v in x], dtype=torch.int32, device=dev)
-        self.rows, self.items = flat[:2 * self.R], flat[2 * self.R:]
+        self.flat = flat
+        self.rows_ptr, self.items_ptr = flat.data_ptr(), flat.data_ptr() + 8 * self.R
         heads = self.R * Hq
         self.ws = 0 if parts == 1 else 2 * (-(-heads * parts // 4) * 4) + heads * parts * HD
         self.dev = flat.device
 
 
-PLAN_SHARED_WG = 384  # workgroups that the shared parts are cut for
-PLAN_OWN_WG = 512     # and the rows' own parts
+PLAN_SHARED_WG = 256  # workgroups that the shared parts are cut for
+PLAN_OWN_WG = 128     # and the rows' own parts at least
+PLAN_OWN_SLOTS = 1024
+PLAN_CAP = 16
 
 
 def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda"):
@@ -1018,7 +1042,7 @@ def _make_plan(groups, Hq, Hk, HD, max_len, dev):
         for c in range(max(len(x) for x in eight)):
             items += [x[c] for x in eight if c < len(x)]
     longest = max(max_len - (p if s else 0) for (n, p), s in zip(groups, shared))
-    nown = max(1, min(16, -(-PLAN_OWN_WG // (R * Hk)), -(-longest // 128)))
+    nown = max(1, min(PLAN_CAP, max(-(-PLAN_OWN_WG // (R * Hk)), -(-longest // PLAN_OWN_SLOTS)), -(-longest // 128)))
     return PagedAttnPlan(items, rows, nown, most + nown, ct, Hq, Hk, HD, dev)
 
 
@@ -1028,30 +1052,33 @@ def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
     ``kp`` / ``vp`` [NP, Hk, P, HD], P a power of two from 16; ``pos`` int64 [>= R], -1: the row attends nothing and its
     output is 0.  Rows of ``out`` behind the plan's are left as they are.  The result of a row does not depend on what
     lies in slots that it does not attend."""
-    dev = _dev(q, "paged_attn")
-    _rows16(q, dev, "paged_attn q")
-    _paged("paged_attn", kp, vp, table, dev)
+    dev, ldq = _rows16(q, "paged_attn q")
+    NP, hk, P, hd, MP, ldt = _paged("paged_attn", kp, vp, table, dev)
     R, Hq, Hk, HD = plan.R, plan.Hq, plan.Hk, plan.HD
-    NP, hk, P, hd = kp.shape
+    rows, wide = q.shape
     if plan.dev != dev:
         raise ValueError(f"paged_attn: the plan is on {plan.dev}, the tensors on {dev}")
-    if hk != Hk or hd != HD or q.shape[1] != Hq * HD or q.shape[0] < R or S < 1 or table.shape[0] * S < R:
+    if hk != Hk or hd != HD or wide != Hq * HD or rows < R or S < 1 or table.shape[0] * S < R:
         raise ValueError("paged_attn: q [>= R, Hq HD], kp / vp [NP, Hk, P, HD] and table [B, MP] (B * S >= R) must fit "
                          "the plan")
     if P < 16 or P & (P - 1):
         raise ValueError("paged_attn: the page size must be a power of two from 16")
-    _on(pos, dev, "paged_attn pos", torch.int64, (-1,))
-    if pos.shape[0] < R:
+    n = pos.numel()
+    _on(pos, dev, "paged_attn", "pos", torch.int64, (n,))
+    if n < R:
         raise ValueError("paged_attn: pos must hold a slot for each row")
-    scale = 1.0 / math.sqrt(HD) if scale is None else float(scale)
+    scale = HD ** -0.5 if scale is None else float(scale)
     if not scale > 0:
         raise ValueError("paged_attn: scale must be positive")
-    o = torch.empty(q.shape[0], Hq * HD, device=dev, dtype=torch.float16) if out is None else out
-    _on(o, dev, "paged_attn out", torch.float16, (q.shape[0], Hq * HD))
-    ws = torch.empty(plan.ws, device=dev, dtype=torch.float32) if plan.ws else None
-    _call_on(dev, "ecd_paged_attn", q.data_ptr(), q.stride(0), kp.data_ptr(), vp.data_ptr(), table.data_ptr(),
-             table.stride(0), pos.data_ptr(), o.data_ptr(), _ptr(ws), plan.items.data_ptr(), plan.rows.data_ptr(),
-             plan.nitems, plan.nown, plan.parts, plan.ctiles, R, int(S), table.shape[1], NP, Hq, Hk, P, HD, scale)
+    if out is None:
+        o = torch.empty(rows, wide, device=dev, dtype=torch.float16)
+    else:
+        o = out
+        _on(o, dev, "paged_attn", "out", torch.float16, (rows, wide))
+    ws = torch.empty(plan.ws, device=dev, dtype=torch.float32).data_ptr() if plan.ws else None
+    _call_on(dev, "ecd_paged_attn", q.data_ptr(), ldq, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), ldt,
+             pos.data_ptr(), o.data_ptr(), ws, plan.items_ptr, plan.rows_ptr, plan.nitems, plan.nown, plan.parts,
+             plan.ctiles, R, int(S), MP, NP, Hq, Hk, P, HD, scale)
     return o
 
 
@@ -1061,32 +1088,31 @@ def quant_a8(x, nw=None, eps=1e-5):
     rounded to fp16): scale[m] = max |y[m]| / 127 fp32, codes int8 [M, K] = rint(127 y / max |y|), ties to even.  A row
     of zeros has scale 0; one that holds an infinity or a NaN has scale NaN.  The codes' rows are zero padded to a
     multiple of 128 (their stride)."""
-    dev = _dev(x, "quant_a8")
-    _rows16(x, dev, "quant_a8 x")
+    dev, ld = _rows16(x, "quant_a8 x")
     M, K = x.shape
-    if K % 64 or K > 1 << 17:
+    if K % 64 or not 0 < K <= 1 << 17:
         raise ValueError("quant_a8: K must be a multiple of 64, at most 131072")
     if nw is not None:
-        _on(nw, dev, "quant_a8 nw", torch.float16, (K,))
+        _on(nw, dev, "quant_a8", "nw", torch.float16, (K,))
         if nw.data_ptr() % 16:
             raise ValueError("quant_a8: nw must be 16-byte aligned")
-    c = torch.empty(M, -(-K // 128) * 128, device=dev, dtype=torch.int8)
+    ldc = -(-K // 128) * 128
+    c = torch.empty(M, ldc, device=dev, dtype=torch.int8)
     s = torch.empty(M, device=dev, dtype=torch.float32)
     if M:
-        _call_on(dev, "ecd_quant_a8", x.data_ptr(), x.stride(0), _ptr(nw), float(eps), c.data_ptr(), c.stride(0),
-                 s.data_ptr(), M, K)
-    return c[:, :K], s
+        _call_on(dev, "ecd_quant_a8", x.data_ptr(), ld, _ptr(nw), float(eps), c.data_ptr(), ldc, s.data_ptr(), M, K)
+    return (c if ldc == K else c[:, :K]), s
 
 
 def _a8_args(name, c, sx, wp, s, N, K):
     dev = _dev(c, name)
-    if c.dtype != torch.int8 or c.dim() != 2 or c.shape[1] != K or c.stride(1) != 1 or c.stride(0) % 128 or \
+    if c.dtype is not torch.int8 or c.dim() != 2 or c.shape[1] != K or c.stride(1) != 1 or c.stride(0) % 128 or \
             c.data_ptr() % 16:
         raise ValueError(f"{name}: codes must come from quant_a8 (int8 [M, {K}], rows padded to a multiple of 128)")
     M = c.shape[0]
-    _on(sx, dev, f"{name} scale", torch.float32, (M,))
-    _on(s, dev, f"{name} s", torch.float16, (N,))
-    if wp.dtype != torch.int8 or wp.device != dev or not wp.is_contiguous() or wp.numel() < -(-N // 16) * 16 * K:
+    _on(sx, dev, name, "scale", torch.float32, (M,))
+    _on(s, dev, name, "s", torch.float16, (N,))
+    if wp.dtype is not torch.int8 or wp.device != dev or not wp.is_contiguous() or wp.numel() < -(-N // 16) * 16 * K:
         raise ValueError(f"{name}: wp must be pack_i8 of an [N, K] matrix on {dev}")
     return dev, M
 
