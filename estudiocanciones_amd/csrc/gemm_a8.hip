@@ -14,66 +14,66 @@ namespace ecd {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-// One workgroup per row.  A row that holds an infinity or a NaN gets the scale NaN (and codes 0).
-template <bool NORM>
+// One workgroup per row, its values in registers (NV pieces of 8 per thread; rows of more than 2048 NV values are read
+// again).  A row that holds an infinity or a NaN gets the scale NaN (and codes 0).
+template <bool NORM, int NV>
 __global__ __launch_bounds__(256) void quant_a8_kernel(const f16* __restrict__ x, long ldx, const f16* __restrict__ w,
                                                        float eps, int8_t* __restrict__ c, long ldc,
                                                        float* __restrict__ sx, int K) {
   __shared__ float red[8];
-  __shared__ int s_bad;
   const int t = threadIdx.x;
   const long m = blockIdx.x;
   const f16* xr = x + m * ldx;
-  if (t == 0) s_bad = 0;
+  f16x8 v[NV], g[NORM ? NV : 1];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = 8 * t + 2048 * i;
+    v[i] = k < K ? *(const f16x8*)(xr + k) : (f16x8)((f16)0);
+    if constexpr (NORM) g[i] = k < K ? *(const f16x8*)(w + k) : (f16x8)((f16)0);
+  }
+  auto each = [&](auto&& f) {  // f(k, 8 values, 8 weights) over this thread's pieces of the row
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f(8 * t + 2048 * i, v[i], g[NORM ? i : 0]);
+    for (int k = 8 * t + 2048 * NV; k < K; k += 2048) f(k, *(const f16x8*)(xr + k), *(const f16x8*)((NORM ? w : xr) + k));
+  };
   float r = 1.f;
   if constexpr (NORM) {
     float s = 0.f;
-    for (int k = 8 * t; k < K; k += 2048) {
-      const f16x8 v = *(const f16x8*)(xr + k);
+    each([&](int, const f16x8& a, const f16x8&) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += (float)v[j] * (float)v[j];
-    }
-    s = wave_sum(s);
+      for (int j = 0; j < 8; ++j) s += (float)a[j] * (float)a[j];
+    });
+    s = wave_sum_dpp(s);
     if ((t & 63) == 0) red[t >> 6] = s;
     __syncthreads();
     r = 1.0f / sqrtf((red[0] + red[1] + red[2] + red[3]) / (float)K + eps);
   }
-  auto value = [&](int k, float* y) {
-    const f16x8 v = *(const f16x8*)(xr + k);
-    f16x8 g;
-    if constexpr (NORM) g = *(const f16x8*)(w + k);
+  auto value = [&](f16 a, f16 b) { return NORM ? (float)a * r * (float)b : (float)a; };
+  // the largest magnitude as bits: an infinity or a NaN is larger than every number
+  uint32_t top = 0;
+  each([&](int, const f16x8& a, const f16x8& b) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = NORM ? (float)v[j] * r * (float)g[j] : (float)v[j];
-  };
-  float top = 0.f;
-  bool bad = false;
-  for (int k = 8 * t; k < K; k += 2048) {
-    float y[8];
-    value(k, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      top = fmaxf(top, fabsf(y[j]));
-      bad |= !(fabsf(y[j]) < INFINITY);
-    }
-  }
-  top = wave_max(top);
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(value(a[j], b[j])) & 0x7FFFFFFFu);
+  });
+  top = wave_max_u32(top);
+  if ((t & 63) == 0) red[4 + (t >> 6)] = __uint_as_float(top);
   __syncthreads();
-  if ((t & 63) == 0) red[4 + (t >> 6)] = top;
-  if (bad) atomicOr(&s_bad, 1);
-  __syncthreads();
-  top = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
-  const bool none = s_bad || top == 0.f;
-  if (t == 0) sx[m] = s_bad ? NAN : top / 127.f;
-  for (int k = 8 * t; k < ldc; k += 2048) {
+  top = max(max(__float_as_uint(red[4]), __float_as_uint(red[5])), max(__float_as_uint(red[6]), __float_as_uint(red[7])));
+  const bool bad = top >= 0x7F800000u, none = bad || top == 0;
+  const float big = __uint_as_float(top);
+  if (t == 0) sx[m] = bad ? NAN : big / 127.f;
+  int8_t* cr = c + m * ldc;
+  each([&](int k, const f16x8& a, const f16x8& b) {
+    if (k >= ldc) return;
     uint32_t o[2] = {0u, 0u};
-    if (k < K && !none) {
-      float y[8];
-      value(k, y);
+    if (!none) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j >> 2] |= (uint32_t)((int)rintf(y[j] * 127.f / top) & 255) << (8 * (j & 3));
+      for (int j = 0; j < 8; ++j) o[j >> 2] |= (uint32_t)((int)rintf(value(a[j], b[j]) * 127.f / big) & 255) << (8 * (j & 3));
     }
-    *(u32x2*)(c + m * ldc + k) = (u32x2){o[0], o[1]};
-  }
+    *(u32x2*)(cr + k) = (u32x2){o[0], o[1]};
+  });
+  // the columns behind K that lie behind the last piece (K is a multiple of 64, ldc of 128)
+  for (int k = max(K, 2048 * NV) + 8 * t; k < ldc; k += 2048) *(u32x2*)(cr + k) = (u32x2){0u, 0u};
 }
 
 struct A8Out {
@@ -85,38 +85,48 @@ struct A8Out {
   long ldy;
 };
 
-// One row's results of 8 consecutive features n .. (fewer at the end) from their integer sums; sn: the features' scales
-template <bool SILU>
-__device__ __forceinline__ void a8_finish(const A8Out& out, const int (&v)[8], float sm, const float (&sn)[8], long m, int n, int N) {
-  float z[8];
+// The results of 8 consecutive features n .. (fewer at the end) of U rows from their integer sums; sm, sn: the scales of
+// the rows and the features.  Rows from M on are left out.
+template <bool SILU, int U>
+__device__ __forceinline__ void a8_finish(const A8Out& out, const int (&v)[U][8], const float (&sm)[U], const float (&sn)[8],
+                                          const int (&m)[U], int n, int M, int N) {
+  const bool whole = n + 7 < N;
+  f16x8 r[U];
+  if (!SILU && out.res && whole) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = (float)v[j] * (sm * sn[j]);
-  if constexpr (SILU) {
-    f16x4 o;
+    for (int u = 0; u < U; ++u) r[u] = *(const f16x8u*)(out.res + min(m[u], M - 1) * out.ldr + n);
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = (f16)(z[2 * j] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[2 * j] * -1.44269504088896341f)) * z[2 * j + 1]);
-    f16* d = out.y + m * out.ldy + (n >> 1);
-    if (n + 7 < N) {
-      *(f16x4u*)d = o;
-    } else {
+  for (int u = 0; u < U; ++u) {
+    if (m[u] >= M) break;
+    float z[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = (float)v[u][j] * (sm[u] * sn[j]);
+    if constexpr (SILU) {
+      f16x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (n + 2 * j < N) d[j] = o[j];
-    }
-  } else {
-    const f16* r = out.res ? out.res + m * out.ldr + n : nullptr;
-    f16* d = out.y + m * out.ldy + n;
-    f16x8 o;
-    if (n + 7 < N) {
-      f16x8 rv = (f16x8)((f16)0);
-      if (r) rv = *(const f16x8u*)r;
+        o[j] = (f16)(z[2 * j] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[2 * j] * -1.44269504088896341f)) * z[2 * j + 1]);
+      f16* d = out.y + m[u] * out.ldy + (n >> 1);
+      if (whole) {
+        *(f16x4u*)d = o;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = (f16)(r ? z[j] + (float)rv[j] : z[j]);
-      *(f16x8u*)d = o;
+        for (int j = 0; j < 4; ++j)
+          if (n + 2 * j < N) d[j] = o[j];
+      }
     } else {
+      f16* d = out.y + m[u] * out.ldy + n;
+      if (whole) {
+        f16x8 o;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (n + j < N) d[j] = (f16)(r ? z[j] + (float)r[j] : z[j]);
+        for (int j = 0; j < 8; ++j) o[j] = (f16)(out.res ? z[j] + (float)r[u][j] : z[j]);
+        *(f16x8u*)d = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + j < N) d[j] = (f16)(out.res ? z[j] + (float)out.res[m[u] * out.ldr + n + j] : z[j]);
+      }
     }
   }
 }
@@ -127,58 +137,49 @@ __device__ __forceinline__ void a8_scales(const f16* s, int n, int N, float (&sn
 }
 
 // ---- few rows: the weights stream once from memory into registers
-// One workgroup per 16 features and up to 16 RT rows; its WV waves take an equal share of K each and add their integer
-// sums in LDS.
-template <bool SILU, int RT, int WV>
-__global__ __launch_bounds__(64 * WV) void gemm_a8_few_kernel(const int8_t* __restrict__ c, long ldc,
-                                                              const int8_t* __restrict__ wp, A8Out out, int M, int N, int K) {
-  __shared__ __align__(16) int part[WV][RT * 16][20];
+// One workgroup per 16 features and 16 rows; its waves take an equal share of K each, eight 1 KB loads of the weights in
+// flight, and add their integer sums in LDS.  A chunk of packed weights (16 features x 64 k, 16 bytes a lane) is the A
+// operand of v_mfma_i32_16x16x64_i8 as it stands, a row's codes the B operand: both hold the k of a lane in the same order.
+// Bound by memory: 8 rows, (16384, 3072) 11.4 us (4.4 TB/s), (3072, 8192) 8.3 us; four waves 12.8 and 9.1, sixteen 9.2.
+constexpr int FEW_W = 8, FEW_U = 8;
+template <bool SILU>
+__global__ __launch_bounds__(64 * FEW_W) void gemm_a8_few_kernel(const int8_t* __restrict__ c, long ldc,
+                                                                 const int8_t* __restrict__ wp, A8Out out, int M, int N, int K) {
+  __shared__ __align__(16) int part[FEW_W][16][20];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * RT;
-  const int steps = K >> 6, s0 = steps * wv / WV, s1 = steps * (wv + 1) / WV;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+  const int steps = K >> 6, s1 = steps * (wv + 1) / FEW_W;
   const int8_t* w = wp + (long)blockIdx.x * 16 * K + 16 * lane;
-  const int8_t* x[RT];
-  i32x4 acc[RT];
+  const int8_t* x = c + (long)min(m0 + (lane & 15), M - 1) * ldc + 16 * (lane >> 4);
+  i32x4 acc = {0, 0, 0, 0};
+  int k = steps * wv / FEW_W;
+  for (; k + FEW_U <= s1; k += FEW_U) {
+    i32x4 a[FEW_U], b[FEW_U];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    x[i] = c + (long)min(m0 + 16 * i + (lane & 15), M - 1) * ldc + 16 * (lane >> 4);
-    acc[i] = (i32x4){0, 0, 0, 0};
-  }
-  constexpr int U = RT <= 2 ? 8 : 4;
-  int k = s0;
-  for (; k + U <= s1; k += U) {
-    i32x4 a[U], b[U][RT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < FEW_U; ++u) {
       a[u] = __builtin_nontemporal_load((const i32x4*)(w + 1024L * (k + u)));
-#pragma unroll
-      for (int i = 0; i < RT; ++i) b[u][i] = *(const i32x4*)(x[i] + 64 * (k + u));
+      b[u] = *(const i32x4*)(x + 64 * (k + u));
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][i], acc[i], 0, 0, 0);
+    for (int u = 0; u < FEW_U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u], acc, 0, 0, 0);
   }
-  for (; k < s1; ++k) {
-    const i32x4 a = __builtin_nontemporal_load((const i32x4*)(w + 1024L * k));
-#pragma unroll
-    for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const i32x4*)(x[i] + 64 * k), acc[i], 0, 0, 0);
-  }
-#pragma unroll
-  for (int i = 0; i < RT; ++i) *(i32x4*)&part[wv][16 * i + (lane & 15)][4 * (lane >> 4)] = acc[i];
+  for (; k < s1; ++k)
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_nontemporal_load((const i32x4*)(w + 1024L * k)),
+                                                *(const i32x4*)(x + 64 * k), acc, 0, 0, 0);
+  *(i32x4*)&part[wv][lane & 15][4 * (lane >> 4)] = acc;
   __syncthreads();
-  for (int t = threadIdx.x; t < 32 * RT; t += 64 * WV) {
-    const int r = t >> 1, h = 8 * (t & 1), m = m0 + r, n = n0 + h;
-    if (m >= M || n >= N) continue;
-    int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (threadIdx.x >= 32) return;
+  const int r = threadIdx.x >> 1, h = 8 * (threadIdx.x & 1), m[1] = {m0 + r}, n = n0 + h;
+  if (m[0] >= M || n >= N) return;
+  int v[1][8] = {{0, 0, 0, 0, 0, 0, 0, 0}};
 #pragma unroll
-    for (int i = 0; i < WV; ++i)
+  for (int i = 0; i < FEW_W; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += part[i][r][h + j];
-    float sn[8];
-    a8_scales(out.s, n, N, sn);
-    a8_finish<SILU>(out, v, out.sx[m], sn, m, n, N);
-  }
+    for (int j = 0; j < 8; ++j) v[0][j] += part[i][r][h + j];
+  float sn[8];
+  a8_scales(out.s, n, N, sn);
+  const float sm[1] = {out.sx[m[0]]};
+  a8_finish<SILU, 1>(out, v, sm, sn, m, n, M, N);
 }
 
 // ---- many rows: tiles of 32 WN FT features x 32 WM RT rows through an LDS ring of NS stages of 128 k
@@ -327,15 +328,16 @@ struct A8Tile {
     if (KG > 1 && nch < most) barrier();
   }
 
-  // f(row of the tile, 8 sums) for every row and this thread's piece of 8 features, rows in passes through LDS, where the
-  // groups' sums are added
+  // f(rows of the tile, their 8 sums) for U rows at a time of this thread's piece of 8 features, the rows in passes through
+  // LDS, where the groups' sums are added
+  static constexpr int PR = BN / 8, RS = THREADS / PR, ROWS = 32 * WM * RP;
+  static_assert(THREADS % PR == 0 && (ROWS % RS == 0 || RS > ROWS), "whole rows per step");
+  static constexpr int IT = ROWS > RS ? ROWS / RS : 1, U = IT % 4 == 0 ? 4 : IT % 2 == 0 ? 2 : 1;
   template <typename F>
   static __device__ __forceinline__ void sums(unsigned char* lds, const i32x16 (&acc)[FT][RT], F&& f) {
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wv = wid % NW, kg = wid / NW, wn = wv % WN, wm = wv / WN;
     int* buf = (int*)lds;
-    constexpr int PR = BN / 8, RS = THREADS / PR, ROWS = 32 * WM * RP;
-    static_assert(THREADS % PR == 0, "whole rows per step");
     const int p = threadIdx.x % PR;
     static_for<0, RT / RP>([&](auto P) {
       __syncthreads();
@@ -347,17 +349,29 @@ struct A8Tile {
           *(i32x4*)(d + 8 * g) = (i32x4){acc[ft][rt][4 * g], acc[ft][rt][4 * g + 1], acc[ft][rt][4 * g + 2], acc[ft][rt][4 * g + 3]};
       });
       __syncthreads();
-#pragma unroll 2
-      for (int r = threadIdx.x / PR; r < ROWS; r += RS) {
-        i32x4 a = *(const i32x4*)(buf + r * ROW + 8 * p), b = *(const i32x4*)(buf + r * ROW + 8 * p + 4);
+      const int first = threadIdx.x / PR;
+      if (first < ROWS) {
+#pragma unroll 1
+        for (int it = 0; it < IT; it += U) {
+          int v[U][8], row[U];
 #pragma unroll
-        for (int k = 1; k < KG; ++k) {
-          a += *(const i32x4*)(buf + k * PASS + r * ROW + 8 * p);
-          b += *(const i32x4*)(buf + k * PASS + r * ROW + 8 * p + 4);
+          for (int u = 0; u < U; ++u) {
+            const int r = first + RS * (it + u), w = r / (32 * RP);
+            row[u] = (w * RT + decltype(P)::value * RP) * 32 + r - w * 32 * RP;
+            i32x4 a = *(const i32x4*)(buf + r * ROW + 8 * p), b = *(const i32x4*)(buf + r * ROW + 8 * p + 4);
+#pragma unroll
+            for (int k = 1; k < KG; ++k) {
+              a += *(const i32x4*)(buf + k * PASS + r * ROW + 8 * p);
+              b += *(const i32x4*)(buf + k * PASS + r * ROW + 8 * p + 4);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              v[u][j] = a[j];
+              v[u][4 + j] = b[j];
+            }
+          }
+          f(row, v);
         }
-        const int v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        const int w = r / (32 * RP), q = r - w * 32 * RP;
-        f((w * RT + decltype(P)::value * RP) * 32 + q, v);
       }
     });
   }
@@ -387,18 +401,27 @@ __global__ __launch_bounds__(64 * WN * WM * KG, 1) void gemm_a8_kernel(const int
   int fb, mb;
   a8_block(blockIdx.x, nfb, nmb, fb, mb);
   const int n0 = fb * T::BN, m0 = mb * T::BM;
+  __shared__ float s_sx[T::BM];  // the rows' scales: here before the sums are (a load for each row cost 0.4 us a row)
+  for (int i = threadIdx.x; i < T::BM; i += T::THREADS) s_sx[i] = out.sx[min(m0 + i, M - 1)];
   i32x16 acc[FT][RT];
   T::run(lds, acc, c, ldc, wp, M, N, K, n0, m0);
-  const int nb = n0 + 8 * (threadIdx.x % (T::BN / 8));
+  const int nb = n0 + 8 * (threadIdx.x % T::PR);
   float sn[8];
   a8_scales(out.s, nb, N, sn);
-  T::sums(lds, acc, [&](int r, const int (&v)[8]) {
-    const int m = m0 + r;
-    if (m < M && nb < N) a8_finish<SILU>(out, v, out.sx[m], sn, m, nb, N);
+  T::sums(lds, acc, [&](const int (&row)[T::U], const int (&v)[T::U][8]) {
+    if (nb >= N) return;
+    int m[T::U];
+    float sm[T::U];
+#pragma unroll
+    for (int u = 0; u < T::U; ++u) {
+      m[u] = m0 + row[u];
+      sm[u] = s_sx[row[u]];
+    }
+    a8_finish<SILU, T::U>(out, v, sm, sn, m, nb, M, N);
   });
 }
 
-template <bool SILU, int WN, int WM, int FT, int RT, int NS, int KG = 1>
+template <bool SILU, int WN, int WM, int FT, int RT, int NS, int KG>
 static int launch_tile(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
   using T = A8Tile<WN, WM, FT, RT, NS, KG>;
   const int nfb = (N + T::BN - 1) / T::BN, nmb = (M + T::BM - 1) / T::BM;
@@ -408,53 +431,68 @@ static int launch_tile(const int8_t* c, long ldc, const int8_t* wp, const A8Out&
   return ecd_launch_status();
 }
 
-template <bool SILU, int RT, int WV>
+template <bool SILU>
 static int launch_few(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
-  if ((M + 16 * RT - 1) / (16 * RT) > 65535) return ECD_ENOTSUP;
-  hipLaunchKernelGGL((gemm_a8_few_kernel<SILU, RT, WV>), dim3((N + 15) / 16, (M + 16 * RT - 1) / (16 * RT)), dim3(64 * WV), 0, st, c, ldc,
-                     wp, out, M, N, K);
+  if ((M + 15) / 16 > 65535) return ECD_ENOTSUP;
+  hipLaunchKernelGGL(gemm_a8_few_kernel<SILU>, dim3((N + 15) / 16, (M + 15) / 16), dim3(64 * FEW_W), 0, st, c, ldc, wp, out, M, N, K);
   return ecd_launch_status();
+}
+
+// The tiles (features x rows), the ways that K is shared out in a workgroup, and measured times in ns: a chunk (of 128 KG k)
+// with at most 144 workgroups and with 256 (one per CU), what a launch and what each round of 256 add.
+struct A8Cfg {
+  int bn, bm, kg, light, full, edge, round;
+};
+constexpr A8Cfg A8_CFG[7] = {
+    {32, 64, 2, 207, 280, 3025, 461},     // 2: two workgroups per CU
+    {64, 64, 2, 267, 437, 2286, 1790},    // 3
+    {128, 64, 2, 426, 710, 2142, 2348},   // 4
+    {128, 64, 1, 242, 332, 3425, 1073},   // 5: two workgroups per CU
+    {128, 128, 1, 291, 595, 1622, 4469},  // 6
+    {256, 128, 1, 492, 892, 1028, 7892},  // 7
+    {256, 256, 1, 960, 1634, 14, 11186},  // 8
+};
+constexpr int A8_FEW = 1;
+
+// The kernel of a product: few rows stream the weights through registers (up to 8 rows, 16 where there are at most 4096
+// features; us at K = 3072, tiles -> it: 4 x 5120 6.5 -> 6.4, 16 x 3072 6.3 -> 6.3, 4 x 3072 x 8192 10.6 -> 8.2, and where
+// the rule keeps tiles: 16 x 5120 6.5 -> 8.0, 16 x 16384 11.6 -> 16.8), else the tile of the shortest estimate.  (Of 167
+// shapes of 24 to 3000 rows and 11 weight matrices measured with 14 tiles the rule's is 2.6% slower than the best on average,
+// 25% at worst.)
+static int a8_choice(int M, int N, int K) {
+  if (M <= 8 || (M <= 16 && N <= 4096)) return A8_FEW;
+  int best = 0;
+  long least = 0;
+  for (int i = 0; i < 7; ++i) {
+    const A8Cfg& t = A8_CFG[i];
+    const long b = (long)((N + t.bn - 1) / t.bn) * ((M + t.bm - 1) / t.bm), rest = b % 256;
+    const long nch = ((K + 127) / 128 + t.kg - 1) / t.kg;
+    long e = t.edge + b / 256 * (nch * t.full + t.round);
+    if (rest) e += nch * (t.light + (t.full - t.light) * (rest > 144 ? rest - 144 : 0) / 112) + t.round;
+    if (i == 0 || e < least) {
+      best = i;
+      least = e;
+    }
+  }
+  return 2 + best;
 }
 
 template <bool SILU>
 static int launch_a8(const void* cv, long ldc, const void* wv, const A8Out& out, int M, int N, int K, hipStream_t st, int cfg = 0) {
   const int8_t *c = (const int8_t*)cv, *wp = (const int8_t*)wv;
 #define A8_TILE(...) return launch_tile<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
-#define A8_FEW(...) return launch_few<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
-  if (!cfg) cfg = M <= 16 ? 4 : M <= 256 ? 14 : 11;
-  switch (cfg) {
-    case 1: A8_FEW(1, 4);
-    case 2: A8_FEW(2, 4);
-    case 3: A8_FEW(4, 4);
-    case 4: A8_FEW(1, 8);
-    case 5: A8_FEW(2, 8);
-    case 6: A8_FEW(4, 8);
-    case 7: A8_TILE(2, 2, 1, 1, 8);   // 64 x 64
-    case 8: A8_TILE(2, 2, 1, 2, 6);   // 64 x 128
-    case 9: A8_TILE(2, 2, 2, 2, 4);   // 128 x 128
-    case 10: A8_TILE(2, 2, 4, 4, 2);  // 256 x 256, 4 waves
-    case 11: A8_TILE(4, 2, 2, 4, 2);  // 256 x 256, 8 waves
-    case 12: A8_TILE(2, 2, 4, 2, 3);  // 256 x 128, 4 waves
-    case 13: A8_TILE(2, 2, 2, 4, 3);  // 128 x 256
-    case 14: A8_TILE(2, 2, 1, 1, 4);     // 64 x 64, two per CU
-    case 15: A8_TILE(2, 2, 1, 1, 3);     // 64 x 64, three per CU
-    case 16: A8_TILE(2, 2, 1, 2, 3);     // 64 x 128, two per CU
-    case 17: A8_TILE(2, 2, 2, 1, 3);     // 128 x 64
-    case 18: A8_TILE(2, 2, 2, 2, 2);     // 128 x 128, two per CU
-    case 20: A8_FEW(1, 16);
-    case 21: A8_TILE(2, 2, 1, 1, 4, 2);  // 64 x 64, K in two
-    case 22: A8_TILE(2, 2, 1, 1, 2, 4);  // 64 x 64, K in four
-    case 23: A8_TILE(1, 2, 1, 1, 3, 4);  // 32 x 64, K in four
-    case 24: A8_TILE(2, 1, 1, 1, 3, 4);  // 64 x 32, K in four
-    case 25: A8_TILE(2, 2, 1, 2, 3, 2);  // 64 x 128, K in two
-    case 26: A8_TILE(2, 2, 2, 1, 3, 2);  // 128 x 64, K in two
-    case 27: A8_TILE(2, 2, 1, 1, 2, 2);  // 64 x 64, K in two, two per CU
-    case 28: A8_TILE(1, 2, 1, 1, 3, 2);  // 32 x 64, K in two, two per CU
-    case 29: A8_TILE(2, 2, 2, 2, 2, 2);  // 128 x 128, K in two
+  switch (cfg ? cfg : a8_choice(M, N, K)) {
+    case A8_FEW: return launch_few<SILU>(c, ldc, wp, out, M, N, K, st);
+    case 2: A8_TILE(1, 2, 1, 1, 3, 2);
+    case 3: A8_TILE(2, 2, 1, 1, 4, 2);
+    case 4: A8_TILE(2, 2, 2, 1, 3, 2);
+    case 5: A8_TILE(2, 2, 2, 1, 3, 1);
+    case 6: A8_TILE(2, 2, 2, 2, 4, 1);
+    case 7: A8_TILE(2, 2, 4, 2, 3, 1);
+    case 8: A8_TILE(4, 2, 2, 4, 2, 1);
     default: return ECD_EINVAL;
   }
 #undef A8_TILE
-#undef A8_FEW
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -476,12 +514,19 @@ int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, lo
       !aligned16(x) || !aligned16(c) || (nw && !aligned16(nw)) || !(eps >= 0.f))
     return ECD_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
-  if (nw)
-    hipLaunchKernelGGL(quant_a8_kernel<true>, dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps,
-                       (int8_t*)c, ldc, sx, K);
-  else
-    hipLaunchKernelGGL(quant_a8_kernel<false>, dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nullptr, eps,
-                       (int8_t*)c, ldc, sx, K);
+#define QA(N_, V_)                                                                                                       \
+  hipLaunchKernelGGL((quant_a8_kernel<N_, V_>), dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps,      \
+                     (int8_t*)c, ldc, sx, K)
+  if (nw) {
+    if (K <= 2048) QA(true, 1);
+    else if (K <= 4096) QA(true, 2);
+    else QA(true, 4);
+  } else {
+    if (K <= 2048) QA(false, 1);
+    else if (K <= 4096) QA(false, 2);
+    else QA(false, 4);
+  }
+#undef QA
   return ecd_launch_status();
 }
 
@@ -494,7 +539,7 @@ int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const 
 
 int ecd_gemm_a8_tuned(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                       void* y, long ldy, int M, int N, int K, int cfg, void* stream) {
-  if (!a8_ok(c, ldc, sx, wp, s, y, M, N, K) || ldy < N || (res && ldr < N) || cfg < 0)
+  if (!a8_ok(c, ldc, sx, wp, s, y, M, N, K) || ldy < N || (res && ldr < N) || cfg < 0 || cfg > 8)
     return ECD_EINVAL;
   return launch_a8<false>(c, ldc, wp, A8Out{sx, (const f16*)s, (const f16*)res, ldr, (f16*)y, ldy}, M, N, K,
                           (hipStream_t)stream, cfg);

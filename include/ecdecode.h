@@ -620,7 +620,7 @@ int ecd_page_free(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length,
 
 /* Sequence dst[i] becomes a copy of src[i] (as it was before the call), i < n <= 1024: it shares the whole pages and
  * gets the slots of a last page that is not full copied, in every plane, into a page of its own.  Targets hold no slots.
- *   plan: [4 n] int32 workspace (any contents). */
+ *   plan: [4 n] int32 workspace (any contents), 16-byte aligned. */
 int ecd_page_fork(void* kv, int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B,
                   const int32_t* src, const int32_t* dst, int n, int32_t* plan, int32_t* err, int planes, int Hk,
                   int P, int HD, void* stream);
@@ -671,7 +671,7 @@ int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, lo
 int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                 void* y, long ldy, int M, int N, int K, void* stream);
 
-/* ecd_gemm_a8 with the kernel chosen by cfg (0: the library's choice); the results are the same bits. */
+/* ecd_gemm_a8 with the kernel chosen by cfg, 1 .. 8 (0: the library's choice); the results are the same bits. */
 int ecd_gemm_a8_tuned(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                       void* y, long ldy, int M, int N, int K, int cfg, void* stream);
 

@@ -188,3 +188,26 @@ def test_no_rows(dev):
     w, s = _weights(32, 64)
     c, sx = quant_a8(torch.empty(0, 64, dtype=torch.float16, device=dev))
     assert gemm_a8_packed(c, sx, pack_i8(_t(w, dev)), _t(s, dev), 32, 64).shape == (0, 32)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 16, 64), (9, 1001, 192), (40, 33, 128), (70, 300, 1344), (130, 260, 448), (300, 1030, 320)])
+def test_every_kernel_gives_the_same_bits(dev, M, N, K):
+    """All kernels that ecd_gemm_a8 chooses from, on shapes with fewer and more chunks of k than stages and K groups."""
+    import torch
+    from estudiocanciones_amd import _ffi
+    from estudiocanciones_amd.kernels import pack_i8, quant_a8, stream_ptr
+    w, s = _weights(N, K)
+    c, sx = quant_a8(_t(randn16(M, M, K), dev))
+    wp, sd, res = pack_i8(_t(w, dev)), _t(s, dev), _t(randn16(7, M, N), dev)
+    ys = []
+    for cfg in range(1, 9):
+        y = torch.full((M, N), float("nan"), dtype=torch.float16, device=dev)
+        _ffi.call("ecd_gemm_a8_tuned", c.data_ptr(), c.stride(0), sx.data_ptr(), wp.data_ptr(), sd.data_ptr(), res.data_ptr(), N,
+                  y.data_ptr(), N, M, N, K, cfg, stream_ptr(dev))
+        ys.append(y)
+    z = (c.cpu().numpy().astype(np.int64) @ w.T.astype(np.int64)) * sx.cpu().numpy().astype(np.float64)[:, None] * s.astype(np.float64)
+    want = z + res.cpu().numpy()
+    tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * (np.abs(z) + np.abs(want)) + 2.0 ** -25
+    assert (np.abs(ys[0].cpu().numpy() - want) <= tol).all()
+    for k, y in enumerate(ys):
+        assert torch.equal(y, ys[0]), k + 1
