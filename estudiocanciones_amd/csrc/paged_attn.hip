@@ -31,7 +31,7 @@ struct PagedArgs {
   const int* items;  // {first row, rows, lo, hi, part, kv head} of each shared part
   const int* rows;   // {shared slots, shared parts} of each row
   long ldq, ldt;
-  int MP, NP, S, Hq, Hk, G, PS, nitems, nown, parts;  // PS: log2 of the page size
+  int R, MP, NP, S, Hq, Hk, G, PS, nitems, nown, parts;  // PS: log2 of the page size
   float c2;          // scale log2(e)
 };
 
@@ -311,7 +311,8 @@ __global__ __launch_bounds__(64 * PQ_W, HD > 128 ? 1 : 2) void paged_attn_kernel
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < a.nitems) {
     const int* it = a.items + 6 * blockIdx.x;
-    const int row0 = it[0], n = it[1], lo = it[2], hi = it[3], kh = it[5];
+    const int row0 = it[0], n = it[1], lo = max(it[2], 0), hi = min(it[3], a.MP << a.PS), kh = it[5];
+    if (row0 < 0 || n < 1 || n * a.G > 16 * CT || row0 + n > a.R || kh < 0 || kh >= a.Hk || it[4] < 0 || it[4] >= a.parts) return;
     // the first row that attends the whole prefix leads: its pages hold every shared slot
     const int r = row0 + min(lane, n - 1);
     const uint64_t live = __ballot(lane < n && attended(a, r) >= a.rows[2 * r]);
@@ -321,6 +322,7 @@ __global__ __launch_bounds__(64 * PQ_W, HD > 128 ? 1 : 2) void paged_attn_kernel
   }
   const int x = blockIdx.x - a.nitems, u = x / a.Hk, kh = x - u * a.Hk, r = u / a.nown, k = u - r * a.nown;
   const int end = attended(a, r), shared = a.rows[2 * r], np = a.rows[2 * r + 1];
+  if (np < 0 || np + a.nown > a.parts) return;
   const int from = end >= shared ? shared : 0;
   const int per = (max(PQ_MIN, (end - from + a.nown - 1) / a.nown) + PQ_T - 1) & ~(PQ_T - 1);
   const int lo = min(from + k * per, end), hi = min(lo + per, end);
@@ -406,6 +408,7 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
   a.rows = rows;
   a.ldq = ldq;
   a.ldt = ldt;
+  a.R = R;
   a.MP = MP;
   a.NP = NP;
   a.S = S;

@@ -22,6 +22,9 @@ reference, all deliberate:
   with enough splits to cover the CUs (``attention_kb``), where the reference launches 16
   splits and a combine; the reference's launch pair is kept for the drop-in path
   (``decode_reference``);
+* ``generate(paged=True)`` computes the prompt once for all takes and keeps its keys and values in
+  pages that the takes share (paged.py); a frame's attention reads them once for all takes;
+  ``generate(a8=True)`` runs the prompt's linear layers on int8 activations (one scale per row);
 * the song loop keeps its bookkeeping on the device: the captured frame ends with a kernel
   that feeds the tokens back, stores the frame and records each take's first EOS frame, so
   the host only replays the graph and reads N integers every 25 frames.
@@ -37,13 +40,15 @@ import torch
 
 from . import _ffi
 from .kernels import (_attn, _attn_combine, _rope_cache, _silu_mul, cdiv, embed_gemv_packed,
-                      gemm_packed, gemm_rms_packed, gemm_silu_packed, gemv_packed_splitk, prefill_attn,
+                      gemm_a8_packed, gemm_a8_silu_packed, gemm_packed, gemm_rms_packed, gemm_silu_packed,
+                      gemv_packed_splitk, paged_attn, paged_attn_plan, paged_write, prefill_attn, quant_a8,
                       gemm_rope_packed, gemv_packed, int8_mm, layer_head, layer_stack,
                       layer_stack_plan, layer_stack_supported, layer_tail, layer_tail_supported,
                       layer_tail_ws_bytes, next_power_of_2,
                       pack_i8, rms as krms, rms_gemv_packed, rms_qkv_rope, rms_qkv_rope_rows,
                       rms_w13_silu,
                       sample_topk, stream_ptr)
+from .paged import PagedCache
 
 AUDIO_VOCAB = 8197
 PROMPT_GEMM_ROWS = 64  # prompt passes with more rows run the MFMA GEMM path
@@ -57,6 +62,7 @@ ATT_SHORT = 128      # caches of at most this many slots: one attention split pe
 ATT_WG = 256        # workgroups the merged attention grid aims at (one per CU of an MI355X)
 ATT_KB_MAX = 16     # workgroups per (row, kv head) pair at most (the last one merges them all)
 STACK_MAX = 64      # layers of one ecd_layer_stack launch at most
+PAGE = 64           # slots of a page of the backbone's paged cache
 DECODER_RESIDENT = 160 << 20  # weight bytes of a decoder pass kept in the 256 MB Infinity Cache
 
 
@@ -252,6 +258,8 @@ class Stack:
         self.tail_no_wait = False   # tests of the error path: every wait in the launches gives up
         self.tail_kv_nt = False     # the launches' attention reads every cache slot nontemporal
         self.use_stack = True       # all layer tails of a decode step as one launch where supported
+        self.prompt_a8 = False      # the prompt pass quantises its activations to int8, row by row
+        self.paged = self.paged_plan = None  # cache in pages and the plan of its rows (alloc_paged)
 
     def alloc(self, B, L, dev, dtype):
         self.rope = rope_cache(self.hd, max(L, 16), device=dev)
@@ -269,6 +277,16 @@ class Stack:
         self.tail = self._tail_buffers(B, dev, dtype, L)
         self.tail2 = None if self.tail is None else \
             self._tail_buffers(2 * B, dev, dtype, L, share=self.tail)
+
+    def alloc_paged(self, seqs, pages, max_pages, dev, groups, page=64):
+        """A cache in pages instead of the dense ones, for one row per sequence: ``groups`` lists (rows, shared slots) of
+        consecutive sequences that share a prompt (the plan of paged_attn)."""
+        if not self.blocks or any(lin.qp is None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2)):
+            raise NotImplementedError("Stack.alloc_paged: the paged path needs packed weights (widths in multiples of 64)")
+        b0, L = self.blocks[0], max_pages * page
+        self.rope = rope_cache(self.hd, max(L, 16), device=dev)
+        self.paged = PagedCache(len(self.blocks), seqs, pages, b0.kvh, self.hd, max_pages, page, dev)
+        self.paged_plan = paged_attn_plan(groups, b0.h, b0.kvh, self.hd, L, dev)
 
     def _tail_buffers(self, M, dev, dtype, L, share=None):
         """Static buffers of the one-launch layer tail (ecd_layer_tail) for M-row decode steps,
@@ -374,6 +392,7 @@ class Stack:
         for b in self.blocks:
             b.kc = b.vc = None
         self.tail = self.tail2 = self.att_ws = self.att_cnt = None
+        self.paged = self.paged_plan = None
 
     def __call__(self, x, pos, attn_len=None, mask=None):
         """Prompt pass (app/engine.py:174-178): x [B, S, D], pos [B, S] absolute positions
@@ -384,7 +403,7 @@ class Stack:
         B, S, D = x.shape
         x2 = x.reshape(B * S, D)
         p2 = pos.reshape(B * S).to(torch.int64).contiguous()
-        if B * S > PROMPT_GEMM_ROWS and all(b.qkv.qp is not None for b in self.blocks):
+        if (B * S > PROMPT_GEMM_ROWS or self.prompt_a8) and all(b.qkv.qp is not None for b in self.blocks):
             h = self._prompt_pass(x2.contiguous(), p2, S)
         else:
             h = self.decode(x2, p2, S)
@@ -394,6 +413,8 @@ class Stack:
         """Many rows (app/engine.py:123-153): every Linear runs the MFMA GEMM with the
         reference's dense numerics (M > 16); RMSNorm, RoPE + cache write and the causal
         attention (row r attends [0, pos[r]]) use the decode kernels."""
+        if self.prompt_a8:
+            return self._prompt_a8(x, pos, S)
         R = x.shape[0]
         norms = [b.n1 for b in self.blocks[1:]] + [self.norm]
         y = krms(x, self.blocks[0].n1 if self.blocks else self.norm)
@@ -419,6 +440,84 @@ class Stack:
             mm = gemm_silu_packed(y, b.w13.qp, b.w13.sp, b.w13.N // 2, b.w13.K)
             x, y = gemm_rms_packed(mm, b.w2.qp, b.w2.sp, b.w2.N, b.w2.K, x, next_norm)
         return y
+
+    def _prompt_attn(self, b, q, kc, vc, pos, S):
+        """Causal attention of prompt rows over dense caches."""
+        Hq, Hk, HD, L = b.h, b.kvh, b.hd, kc.shape[2]
+        if HD in (64, 128) and Hq // Hk <= 4:
+            return prefill_attn(q, kc, vc, pos, S, Hq, Hk)
+        o = torch.empty_like(q)
+        _ffi.call("ecd_decode_attn", q.data_ptr(), kc.data_ptr(), vc.data_ptr(), pos.data_ptr(), o.data_ptr(), None,
+                  None, None, q.shape[0], S, Hq, Hk, L, HD, 1, 1.0 / math.sqrt(HD), stream_ptr(q.device))
+        return o
+
+    @staticmethod
+    def _a8(x, lin, nw=None, res=None):
+        """lin(rms(x, nw)) (+ res) on int8 activations."""
+        c, s = quant_a8(x, nw)
+        return gemm_a8_packed(c, s, lin.qp, lin.s8, lin.N, lin.K, res)
+
+    def _prompt_a8(self, x, pos, S):
+        """_prompt_pass with int8 activations: each linear layer's input is quantised row by row (the norms in fp32
+        before it), the products are exact integer sums.  Not the reference's numerics: a row's codes are off by up to
+        half a step of max |row| / 127."""
+        for b in self.blocks:
+            q = torch.empty(x.shape[0], b.h * b.hd, device=x.device, dtype=x.dtype)
+            _rope_cache[(x.shape[0], b.h + b.kvh)](self._a8(x, b.qkv, b.n1), self.rope, pos, q, b.kc, b.vc, S, b.h, b.kvh,
+                                                   b.kc.shape[2], HD=b.hd)
+            x = self._a8(self._prompt_attn(b, q, b.kc, b.vc, pos, S), b.o, res=x)
+            c, s = quant_a8(x, b.n2)
+            x = self._a8(gemm_a8_silu_packed(c, s, b.w13.qp, b.w13.sp, b.w13.N // 2, b.w13.K), b.w2, res=x)
+        return krms(x, self.norm)
+
+    def prompt_paged(self, x, seqs):
+        """Prompt pass into the cache in pages: x [U, S, D], prompt u at slots 0 .. S - 1 of sequence seqs[u] (int64
+        tensor), which holds nothing yet.  Returns the last row's hidden state [U, D] (after the stack's norm)."""
+        U, S, D = x.shape
+        dev, cache = x.device, self.paged
+        last = torch.full_like(cache.length, -1)
+        last[seqs] = S - 1
+        cache.extend(last)
+        table = cache.table[seqs]
+        pos = torch.arange(S, device=dev).repeat(U)
+        x = x.reshape(U * S, D).contiguous()
+        b0 = self.blocks[0]
+        kc = torch.empty(U, b0.kvh, S, b0.hd, device=dev, dtype=x.dtype)  # one layer's keys and values in order
+        vc = torch.empty_like(kc)
+        for i, b in enumerate(self.blocks):
+            kp, vp = cache.layer(i)
+            if self.prompt_a8:
+                qkv = self._a8(x, b.qkv, b.n1)
+            else:
+                qkv = gemm_packed(krms(x, b.n1), b.qkv.qp, b.qkv.s8, b.qkv.N, b.qkv.K)
+            q = paged_write(qkv, kp, vp, table, pos, S, b.h, b.kvh, rope=self.rope)
+            _rope_cache[(U * S, b.h + b.kvh)](qkv, self.rope, pos, q, kc, vc, S, b.h, b.kvh, S, HD=b.hd)
+            o = self._prompt_attn(b, q, kc, vc, pos, S)
+            if self.prompt_a8:
+                x = self._a8(o, b.o, res=x)
+                c, s = quant_a8(x, b.n2)
+                x = self._a8(gemm_a8_silu_packed(c, s, b.w13.qp, b.w13.sp, b.w13.N // 2, b.w13.K), b.w2, res=x)
+            else:
+                x, y = gemm_rms_packed(o, b.o.qp, b.o.sp, b.o.N, b.o.K, x, b.n2)
+                x = gemm_packed(gemm_silu_packed(y, b.w13.qp, b.w13.sp, b.w13.N // 2, b.w13.K), b.w2.qp, b.w2.s8,
+                                b.w2.N, b.w2.K, x)
+        return krms(x.reshape(U, S, D)[:, -1].contiguous(), self.norm)
+
+    def decode_paged(self, x, pos, final_norm=True):
+        """A decode step over the cache in pages: x [R, D], row r at slot pos[r] of sequence r (R: all sequences).  The
+        slot's page is taken if it is not there yet, the step may be repeated (a capture's warm-up) and captured."""
+        cache = self.paged
+        cache.extend(pos)
+        for i, b in enumerate(self.blocks):
+            kp, vp = cache.layer(i)
+            qkv = torch.empty(x.shape[0], b.qkv.N, device=x.device, dtype=x.dtype)
+            rms_qkv_rope_rows(x, b.n1, b.qkv.qp, b.qkv.s8, self.rope, pos, qkv, b.h, b.kvh, b.hd, dense=x.shape[0] > 16)
+            paged_write(qkv, kp, vp, cache.table, pos, 1, b.h, b.kvh)
+            o = paged_attn(qkv[:, :b.h * b.hd], kp, vp, cache.table, pos, self.paged_plan)
+            x = b.o(o, res=x)
+            mm = rms_w13_silu(x, b.n2, b.w13.qp, b.w13.sp, b.w13.N // 2, stream=b.w13.stream)
+            x = b.w2(mm, res=x)
+        return krms(x, self.norm) if final_norm else x
 
     def decode(self, x, pos, S, final_norm=True, o0=None):
         """Fast path for few rows (app/engine.py:180-211): x [R, D] with R = B*S (row r -> batch
@@ -808,13 +907,16 @@ class HeartMuLaLite:
         h = self.audio_emb.sum_codebooks(tok, AUDIO_VOCAB)
         fused = kw.get("forced") is None and self._next_rows is not None and \
             self._c0proj is not None and all(b.qkv.qp is not None for b in self.backbone.blocks)
-        hb = self.backbone.decode(h, pos[:, 0].contiguous(), 1, final_norm=not fused)
+        p = pos[:, 0].contiguous()
+        hb = self.backbone.decode_paged(h, p, final_norm=not fused) if self.backbone.paged is not None else \
+            self.backbone.decode(h, p, 1, final_norm=not fused)
         return self._frame_fast(hb, cfg, topk, temp, pos=pos, normed=not fused, **kw)
 
     # -------------------------------------------------- caches
-    def alloc(self, n, L, cfg_scale=1.5, seed=None):
+    def alloc(self, n, L, cfg_scale=1.5, seed=None, paged=None):
         """Static caches for n takes and backbone capacity L (app/engine.py:380-388), and the
-        sampler's seed (drawn from torch's host generator when not given)."""
+        sampler's seed (drawn from torch's host generator when not given).  ``paged``: the slots of a
+        prompt that the takes share; the backbone's cache is then in pages of PAGE slots."""
         self.N = n
         self.B = 2 * n if cfg_scale != 1.0 else n
         if seed is None or seed < 0:
@@ -826,7 +928,14 @@ class HeartMuLaLite:
         self._pass0_pos = torch.arange(2 * self.B, device=self.dev) % 2
         self._pass_pos = torch.arange(2, N_CB, device=self.dev).repeat_interleave(self.B) \
             .view(N_CB - 2, self.B)
-        self.backbone.alloc(self.B, L, self.dev, self.dt)
+        if paged is None:
+            self.backbone.alloc(self.B, L, self.dev, self.dt)
+        else:
+            # whole pages of the prompt once per group, the rest of the capacity once per take
+            most, whole = -(-L // PAGE), paged // PAGE
+            groups = self.B // n
+            self.backbone.alloc_paged(self.B, groups * whole + self.B * (most - whole), most, self.dev,
+                                      [(n, paged)] * groups, PAGE)
         self.decoder.alloc(self.B, N_CB, self.dev, self.dt)
         # passes 1 .. 6 end in their codebook head inside the decoder's stack launch where the
         # stack supports it: one logits buffer per head
@@ -901,31 +1010,45 @@ class HeartMuLaLite:
     # -------------------------------------------------- generation
     @torch.inference_mode()
     def generate(self, text, muq_idx, *, max_ms=60_000, temperature=1.0, topk=50, cfg_scale=1.5,
-                 seed=None, use_graphs=True, progress=None, abort=None, n=1, forced=None):
+                 seed=None, use_graphs=True, progress=None, abort=None, n=1, forced=None, paged=False, a8=False):
         """A song of up to ``max_ms`` for n takes (app/engine.py:374-448) with the prompt given as
         token ids ``text`` [P] (int64) and the muq slot index.  Returns [8, T] if n == 1, else a
         list of n such tensors, each take cut before its first frame holding an EOS token.
         ``forced`` [max_ms // 80 + 1, B, 8] int64 on the device replaces the sampled tokens of
         every frame (teacher forcing a whole song).  Every 25 frames (and at the end) the host
         reads the takes' EOS frames together with the layer tails' error words, and raises
-        RuntimeError if a tail launch timed out at a gate."""
+        RuntimeError if a tail launch timed out at a gate.
+
+        ``paged``: the prompt is computed once for all takes (once more for the unconditional rows) and
+        its keys and values are stored once, in pages that the takes share; each frame's attention reads
+        them once for all takes.  The backbone then runs its kernels one by one instead of in layer
+        stacks: for many takes, whose rows a stack does not hold (more than 8), or whose caches take
+        the memory.  ``a8``: the prompt's linear layers run on int8 activations (not the reference's
+        numerics, about half the time)."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
         text = torch.as_tensor(text, dtype=torch.int64)
         P = int(text.numel())
         n_frames = max_ms // FRAME_MS
         cap = P + n_frames + 2 + 256
-        self.alloc(n, cap, cfg_scale)
+        self.alloc(n, cap, cfg_scale, paged=P if paged else None)
         N, B = self.N, self.B
         if forced is not None and tuple(forced.shape) != (n_frames + 1, B, N_CB):
             raise ValueError(f"generate: forced must be [{n_frames + 1}, {B}, {N_CB}]")
 
         # prompt pass (text rows, the muq slot's bias, unconditional rows for CFG)
-        h = self.text_emb(text.to(self.dev)).unsqueeze(0).repeat(B, 1, 1)
-        h[:N, muq_idx] = self.muq_b
-        if B == 2 * N:
-            h[N:] = self.uncond[0]
-        hb = self.backbone(h, torch.arange(P, device=self.dev).unsqueeze(0).expand(B, P), P, None)
+        self.backbone.prompt_a8 = bool(a8)
+        try:
+            if paged:
+                hb = self._prompt_shared(text, muq_idx)
+            else:
+                h = self.text_emb(text.to(self.dev)).unsqueeze(0).repeat(B, 1, 1)
+                h[:N, muq_idx] = self.muq_b
+                if B == 2 * N:
+                    h[N:] = self.uncond[0]
+                hb = self.backbone(h, torch.arange(P, device=self.dev).unsqueeze(0).expand(B, P), P, None)[:, -1]
+        finally:
+            self.backbone.prompt_a8 = False
 
         # song state on the device: next input tokens and position, the frames so far, and
         # each take's first EOS frame (-1 while it runs)
@@ -935,11 +1058,11 @@ class HeartMuLaLite:
                   eos=torch.full((N,), -1, dtype=torch.long, device=self.dev),
                   forced=None if forced is None else forced[0].clone())
         kw = {} if forced is None else {"forced": st["forced"]}
-        first = self._frame_fast(hb[:, -1].contiguous(), cfg_scale, topk, temperature,
+        first = self._frame_fast(hb.contiguous(), cfg_scale, topk, temperature,
                                  pos=st["pos"], **kw)
         self._advance(first, st, P, n_frames)
 
-        key = (B, cap, topk, float(temperature), float(cfg_scale))
+        key = (B, cap, topk, float(temperature), float(cfg_scale), P if paged else None)
         done = n_frames
         ends = None
         for i in range(n_frames):
@@ -971,17 +1094,37 @@ class HeartMuLaLite:
         self.release()
         return res[0] if n == 1 else res
 
+    def _prompt_shared(self, text, muq_idx):
+        """The prompt into sequence 0 of the paged cache and its unconditional rows into sequence N, forked for the
+        other takes -> the last hidden state of every row [B, D]."""
+        N, B = self.N, self.B
+        h = self.text_emb(text.to(self.dev)).unsqueeze(0).repeat(B // N, 1, 1)
+        h[0, muq_idx] = self.muq_b
+        if B == 2 * N:
+            h[1] = self.uncond[0]
+        first = torch.arange(0, B, N, device=self.dev)
+        hb = self.backbone.prompt_paged(h, first)
+        dst = [b for b in range(B) if b % N]
+        if dst:
+            self.backbone.paged.fork([b - b % N for b in dst], dst)
+        return hb.repeat_interleave(N, 0)
+
     def _song_status(self, eos):
         """Each take's first EOS frame (-1 while it runs) and the layer tails' error words, in
         one device -> host read (the song loop's only one).  A set error word means a gate wait
         of a persistent tail launch gave up (a workgroup of its grid was not resident, e.g.
         another process held CUs): the frames since the last read are undefined, so the gate
         state is cleared, the caches are released and the song stops with RuntimeError."""
-        errs = [s.tail["err"] for s in (self.backbone, self.decoder) if s.tail is not None]
+        cache = self.backbone.paged
+        tails = [(nm, s) for nm, s in (("backbone", self.backbone), ("decoder", self.decoder)) if s.tail is not None]
+        errs = [s.tail["err"] for _, s in tails] + ([] if cache is None else [cache.err])
         vals = torch.cat([eos, *[e.to(eos.dtype) for e in errs]]).tolist()
         n = eos.numel()
+        if cache is not None and vals[-1]:
+            self.release()
+            raise RuntimeError(f"the paged cache refused a step (error bits {vals[-1]:#x}); the song was stopped")
         if any(vals[n:]):
-            failed = [nm for nm, v in zip(("backbone", "decoder"), vals[n:]) if v]
+            failed = [nm for (nm, _), v in zip(tails, vals[n:]) if v]
             self.tail_reset()
             self.release()
             raise RuntimeError(f"layer-tail launch of the {' and '.join(failed)} timed out at a "

@@ -211,3 +211,27 @@ def test_every_kernel_gives_the_same_bits(dev, M, N, K):
     assert (np.abs(ys[0].cpu().numpy() - want) <= tol).all()
     for k, y in enumerate(ys):
         assert torch.equal(y, ys[0]), k + 1
+
+
+def test_refusals(dev):
+    import torch
+    from estudiocanciones_amd.kernels import gemm_a8_packed, gemm_a8_silu_packed, pack_i8, quant_a8
+    x = _t(randn16(1, 4, 128), dev)
+    for bad in (x[:, :96], x[:, ::2], x.reshape(-1)[4:4 + 64 * 7].reshape(7, 64), x[0]):
+        with pytest.raises(ValueError):
+            quant_a8(bad)
+    with pytest.raises(TypeError):
+        quant_a8(x.float())
+    with pytest.raises(ValueError):
+        quant_a8(x, _t(randn16(2, 64), dev))
+    w, s = _weights(32, 128)
+    wp, sd = pack_i8(_t(w, dev)), _t(s, dev)
+    c, sx = quant_a8(x)
+    for a in ((c, sx, wp, sd, 48, 128), (c, sx, wp, sd, 32, 64), (c[:, ::2], sx, wp, sd, 32, 64), (c, sx[:3], wp, sd, 32, 128),
+              (c, sx, wp[:100], sd, 32, 128), (c, sx, wp, sd[:16], 32, 128), (c.float(), sx, wp, sd, 32, 128)):
+        with pytest.raises(ValueError):
+            gemm_a8_packed(*a)
+    with pytest.raises(ValueError):
+        gemm_a8_packed(c, sx, wp, sd, 32, 128, res=x[:, :32].t())
+    with pytest.raises(ValueError):
+        gemm_a8_silu_packed(c, sx, wp, sd, 16, 128, out=torch.empty(4, 32, dtype=torch.float16, device=dev))

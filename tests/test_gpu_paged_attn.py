@@ -226,3 +226,27 @@ def test_on_another_stream(dev):
         other = b.run(dev)
     s.synchronize()
     assert torch.equal(first, other)
+
+
+def test_refusals(dev):
+    import torch
+    from estudiocanciones_amd.kernels import paged_attn, paged_attn_plan, paged_write
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16, device=dev)  # noqa: E731
+    plan = paged_attn_plan([(2, 16)], 4, 2, 64, 64, dev)
+    good = dict(q=h(2, 256), kp=h(9, 2, 16, 64), vp=h(9, 2, 16, 64), table=torch.zeros(2, 4, dtype=torch.int32, device=dev),
+                pos=torch.zeros(2, dtype=torch.long, device=dev), plan=plan)
+    assert paged_attn(**good).shape == (2, 256)
+    for bad in (dict(q=h(1, 256)), dict(q=h(2, 192)), dict(q=h(2, 512)[:, ::2]), dict(q=h(3, 264)[1:, 4:260]),
+                dict(kp=h(9, 2, 24, 64), vp=h(9, 2, 24, 64)), dict(kp=h(9, 1, 16, 64), vp=h(9, 1, 16, 64)),
+                dict(vp=h(8, 2, 16, 64)), dict(kp=h(9, 2, 64, 16).transpose(2, 3)), dict(table=good["table"][:1]),
+                dict(table=good["table"].t()), dict(table=good["table"].cpu()), dict(pos=good["pos"][:1]), dict(scale=0.0),
+                dict(scale=float("nan")), dict(out=h(2, 128)), dict(S=0)):
+        with pytest.raises(ValueError):
+            paged_attn(**{**good, **bad})
+    for bad in (dict(q=h(2, 256).float()), dict(pos=good["pos"].int()), dict(kp=h(9, 2, 16, 64).bfloat16())):
+        with pytest.raises(TypeError):
+            paged_attn(**{**good, **bad})
+    w = dict(qkv=h(2, 512), kp=good["kp"], vp=good["vp"], table=good["table"], pos=good["pos"], S=1, Hq=4, Hk=2)
+    for bad in (dict(S=0), dict(Hk=1), dict(qkv=h(3, 512)), dict(rope=torch.zeros(64, 30, 2, device=dev)), dict(table=good["table"][:1])):
+        with pytest.raises(ValueError):
+            paged_write(**{**w, **bad})
