@@ -124,7 +124,7 @@ SIGNATURES = {
     "ecd_paged_write": [_P, c_long, _P, c_int, _P, _P, _P, _P, _P, c_long, c_int, c_int, c_int, c_int, c_int, c_int,
                         c_int, c_int, _P],
     "ecd_paged_attn": [_P, c_long, _P, _P, _P, c_long, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
-                       c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
+                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "ecd_quant_a8": [_P, c_long, _P, c_float, _P, c_long, _P, c_int, c_int, _P],
     "ecd_gemm_a8": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, _P],
     "ecd_gemm_a8_tuned": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P],

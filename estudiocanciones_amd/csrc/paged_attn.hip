@@ -13,9 +13,7 @@
 
 namespace ecd {
 
-constexpr int PQ_W = 4;       // waves of a workgroup
-constexpr int PQ_T = 32;      // slots of a wave's tile
-constexpr int PQ_MIN = PQ_W * PQ_T;  // slots of a row's own share at least
+constexpr int PQ_T = 32;  // slots of a wave's tile
 
 // what does not change over a call
 struct PagedArgs {
@@ -202,7 +200,7 @@ __device__ __forceinline__ void begin(PState<HD, CT>& s, const PagedArgs& a, int
 
 // One part on one workgroup whose waves share out the slots: `cols` columns, slots [lo, hi) through `tab`.
 // `live`: bit i says whether row row0 + i takes this part.  Its result goes to place `part`, or with `whole` normalised to o.
-template <int HD, int CT>
+template <int HD, int CT, int W>
 __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0, int cols, int kh, const int* tab, int lo,
                                        int hi, int part, bool whole, uint64_t live) {
   constexpr int ST = HD + 4;  // floats of a column in LDS
@@ -211,33 +209,36 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
   PState<HD, CT> s;
   begin(s, a, row0, cols, 0, kh, lane);
   // K of the next tile is asked for once this one's scores are formed, V once this one's is used: one tile is always in
-  // flight, in the registers of the last one
+  // flight, in the registers of the last one.  (Two tiles ahead measured no faster: a CU gets about 45 GB/s of what its XCD's
+  // L2 does not hold, whatever is in flight.)
   PTile<HD> t;
+  constexpr int STEP = W * PQ_T;
   const int first = (lo & ~(PQ_T - 1)) + wv * PQ_T;
-  const int n = hi > first ? (hi - first + PQ_W * PQ_T - 1) / (PQ_W * PQ_T) : 0;
+  const int n = hi > first ? (hi - first + STEP - 1) / STEP : 0;
   Places at;
   if (n > 0) {
-    at = places(a, tab, kh, first, PQ_W * PQ_T, hi, lane);
+    at = places(a, tab, kh, first, STEP, hi, lane);
     load_k<HD>(t, a, at, 0, lane);
     load_v<HD>(t, a, at, 0, lane);
   }
   for (int i = 0; i < n; ++i) {
-    const bool more = i + 1 < n;
-    if (more && ((i + 1) & 63) == 0) at = places(a, tab, kh, first + (i + 1) * (PQ_W * PQ_T), PQ_W * PQ_T, hi, lane);
-    tile_attend<HD, CT>(s, t, a.c2, first + i * (PQ_W * PQ_T), lo, hi, lane, [&]() {
+    const int next = i + 1;
+    const bool more = next < n;
+    if (more && (next & 63) == 0) at = places(a, tab, kh, first + next * STEP, STEP, hi, lane);
+    tile_attend<HD, CT>(s, t, a.c2, first + i * STEP, lo, hi, lane, [&]() {
       asm volatile("" ::: "memory");
-      if (more) load_k<HD>(t, a, at, (i + 1) & 63, lane);
+      if (more) load_k<HD>(t, a, at, next & 63, lane);
       asm volatile("" ::: "memory");
     });
     asm volatile("" ::: "memory");
-    if (more) load_v<HD>(t, a, at, (i + 1) & 63, lane);
+    if (more) load_v<HD>(t, a, at, next & 63, lane);
     asm volatile("" ::: "memory");
   }
 
   // the waves' states to one: maxima and sums first, then the outputs on the common maximum
-  float* sm = lds;                    // [PQ_W][16 CT]
-  float* sl = lds + PQ_W * 16 * CT;
-  float* sa = lds + 2 * PQ_W * 16 * CT;  // [PQ_W][16 CT][ST]
+  float* sm = lds;                    // [W][16 CT]
+  float* sl = lds + W * 16 * CT;
+  float* sa = lds + 2 * W * 16 * CT;  // [W][16 CT][ST]
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     const float l = sum_groups(s.l[c]);
@@ -251,7 +252,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
   for (int c = 0; c < CT; ++c) {
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < PQ_W; ++w) M = fmaxf(M, sm[w * 16 * CT + 16 * c + col]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w * 16 * CT + 16 * c + col]);
     const float m = sm[wv * 16 * CT + 16 * c + col];
     const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * a.c2);
     float* d = sa + (wv * 16 * CT + 16 * c + col) * ST;
@@ -265,16 +266,16 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
               (f32x4){s.acc[c][x][b][i] * f, s.acc[c][x][b + 1][i] * f, s.acc[c][x][b + 2][i] * f, s.acc[c][x][b + 3][i] * f};
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < cols * (HD / 4); i += 64 * PQ_W) {
+  for (int i = threadIdx.x; i < cols * (HD / 4); i += 64 * W) {
     const int n = i / (HD / 4), d = 4 * (i - n * (HD / 4));
     const int row = row0 + n / a.G;
     const long head = (long)row * a.Hq + kh * a.G + n % a.G;
     float M = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < PQ_W; ++w) M = fmaxf(M, sm[w * 16 * CT + n]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w * 16 * CT + n]);
     f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < PQ_W; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float m = sm[w * 16 * CT + n];
       l += m == -INFINITY ? 0.f : sl[w * 16 * CT + n] * __builtin_amdgcn_exp2f((m - M) * a.c2);
       v = v + *(const f32x4*)(sa + (w * 16 * CT + n) * ST + d);
@@ -294,9 +295,9 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
   }
 }
 
-template <int HD, int CT>
+template <int HD, int CT, int W>
 constexpr int attend_lds() {
-  return PQ_W * 16 * CT * (2 + HD + 4);
+  return W * 16 * CT * (2 + HD + 4);
 }
 
 // slots that row r attends
@@ -305,9 +306,9 @@ __device__ __forceinline__ int attended(const PagedArgs& a, int r) {
   return (int)min(p < 0 ? 0l : p + 1, (long)a.MP << a.PS);
 }
 
-template <int HD, int CT>
-__global__ __launch_bounds__(64 * PQ_W, HD > 128 ? 1 : 2) void paged_attn_kernel(PagedArgs a) {
-  __shared__ __align__(16) float lds[attend_lds<HD, CT>()];
+template <int HD, int CT, int W>
+__global__ __launch_bounds__(64 * W, HD > 128 ? 1 : 2) void paged_attn_kernel(PagedArgs a) {
+  __shared__ __align__(16) float lds[attend_lds<HD, CT, W>()];
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < a.nitems) {
     const int* it = a.items + 6 * blockIdx.x;
@@ -317,16 +318,16 @@ __global__ __launch_bounds__(64 * PQ_W, HD > 128 ? 1 : 2) void paged_attn_kernel
     const int r = row0 + min(lane, n - 1);
     const uint64_t live = __ballot(lane < n && attended(a, r) >= a.rows[2 * r]);
     const int* tab = a.table + (long)((row0 + (live ? __builtin_ctzll(live) : 0)) / a.S) * a.ldt;
-    attend<HD, CT>(a, lds, row0, n * a.G, kh, tab, lo, live ? hi : lo, it[4], false, live);
+    attend<HD, CT, W>(a, lds, row0, n * a.G, kh, tab, lo, live ? hi : lo, it[4], false, live);
     return;
   }
   const int x = blockIdx.x - a.nitems, u = x / a.Hk, kh = x - u * a.Hk, r = u / a.nown, k = u - r * a.nown;
   const int end = attended(a, r), shared = a.rows[2 * r], np = a.rows[2 * r + 1];
   if (np < 0 || np + a.nown > a.parts) return;
   const int from = end >= shared ? shared : 0;
-  const int per = (max(PQ_MIN, (end - from + a.nown - 1) / a.nown) + PQ_T - 1) & ~(PQ_T - 1);
+  const int per = (max(W * PQ_T, (end - from + a.nown - 1) / a.nown) + PQ_T - 1) & ~(PQ_T - 1);
   const int lo = min(from + k * per, end), hi = min(lo + per, end);
-  attend<HD, 1>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1, ~0ull);
+  attend<HD, 1, W>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1, ~0ull);
 }
 
 // One thread per four dims of a head: JB parts at a time, all their loads at once, in the order of the parts.
@@ -371,9 +372,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int HD, in
   *(f16x4*)(a.o + (long)head * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
 }
 
-template <int HD, int CT>
+template <int HD, int CT, int W>
 static int launch_paged(const PagedArgs& a, int R, hipStream_t st) {
-  hipLaunchKernelGGL((paged_attn_kernel<HD, CT>), dim3(a.nitems + R * a.nown * a.Hk), dim3(64 * PQ_W), 0, st, a);
+  hipLaunchKernelGGL((paged_attn_kernel<HD, CT, W>), dim3(a.nitems + R * a.nown * a.Hk), dim3(64 * W), 0, st, a);
   return ecd_launch_status();
 }
 
@@ -383,7 +384,7 @@ using namespace ecd;
 
 extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const void* vp, const int32_t* table, long ldt,
                               const int64_t* pos, void* o, float* ws, const int32_t* items, const int32_t* rows,
-                              int nitems, int nown, int parts, int ctiles, int R, int S, int MP, int NP, int Hq, int Hk,
+                              int nitems, int nown, int parts, int ctiles, int waves, int R, int S, int MP, int NP, int Hq, int Hk,
                               int P, int HD, float scale, void* stream) {
   if (!q || !kp || !vp || !table || !pos || !o || !rows || (nitems > 0 && !items) || nitems < 0 || nown < 1 ||
       parts < nown || (parts > 1 && !ws) || R <= 0 || S <= 0 || MP <= 0 || NP <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
@@ -422,13 +423,15 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
   a.c2 = scale * 1.44269504088896341f;
   const hipStream_t st = (hipStream_t)stream;
   int rc = ECD_ENOTSUP;
-#define PQ(HD_, CT_)                     \
-  if (HD == HD_ && ctiles == CT_) rc = launch_paged<HD_, CT_>(a, R, st)
-  PQ(64, 1);
-  PQ(64, 2);
-  PQ(128, 1);
-  PQ(128, 2);
-  PQ(256, 1);
+#define PQ(HD_, CT_, W_)                     \
+  if (HD == HD_ && ctiles == CT_ && waves == W_) rc = launch_paged<HD_, CT_, W_>(a, R, st)
+  PQ(64, 1, 4);
+  PQ(64, 2, 4);
+  PQ(64, 1, 8);
+  PQ(128, 1, 4);
+  PQ(128, 2, 4);
+  PQ(128, 1, 8);
+  PQ(256, 1, 4);
 #undef PQ
   if (rc != ECD_OK || parts == 1) return rc;
   hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)((heads * (HD / 4) + 255) / 256)), dim3(256), 0, st, a, HD, (int)heads);

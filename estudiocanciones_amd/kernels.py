@@ -984,8 +984,9 @@ def paged_write(qkv, kp, vp, table, pos, S, Hq, Hk, rope=None, q=None):
 class PagedAttnPlan:
     """How paged_attn cuts a batch into parts (paged_attn_plan)."""
 
-    def __init__(self, items, rows, nown, parts, ctiles, Hq, Hk, HD, dev):
-        self.nitems, self.R, self.nown, self.parts, self.ctiles = len(items), len(rows), nown, parts, ctiles
+    def __init__(self, items, rows, nown, parts, ctiles, waves, Hq, Hk, HD, dev):
+        self.nitems, self.R, self.nown, self.parts = len(items), len(rows), nown, parts
+        self.ctiles, self.waves = ctiles, waves
         self.Hq, self.Hk, self.HD = Hq, Hk, HD
         flat = torch.tensor([v for x in rows for v in x] + [v for x in items for v in x], dtype=torch.int32, device=dev)
         self.flat = flat
@@ -995,16 +996,27 @@ class PagedAttnPlan:
         self.dev = flat.device
 
 
-PLAN_SHARED_WG = 256  # workgroups that the shared parts are cut for
-PLAN_OWN_WG = 128     # and the rows' own parts at least
-PLAN_OWN_SLOTS = 1024
-PLAN_CAP = 16
+# How a batch is cut, from times on an MI355X (24 query heads on 8 kv heads of 128; us):
+# sharing pays where it saves this many bytes of the other rows' reads, else the parts cost more than they save
+# (shared / not: 8 rows of 4096 + 64 slots, 117 MB saved, 16.0 / 22.7; 2 x 4 of 1500 + 500, 37 MB, 14.5 / 14.0; 2 x 16 of
+# 256 + 500, 31 MB, 18.0 / 15.1; 2 x 4 of 256 + 494, 6 MB, 10.3 / 10.4)
+PLAN_SAVED = 48 << 20
+# workgroups that the shared parts are cut for (2 x 16 rows of 4096: 128 28.1, 256 29.1, 384 32.2; 2 x 32 of 7000: 42.1 with
+# 256, 46.0 with 384)
+PLAN_SHARED_WG = 256
+# a row's own slots: parts so that all rows together have this many workgroups, none of more than PLAN_OWN_SLOTS (8 rows of
+# 256 + 3000: 4 parts 22.4, 7 parts 23.1; 2 x 16 of 1000 + 4000: 2 parts 71, 4 parts 64), at most PLAN_OWN_MOST parts
+PLAN_OWN_WG, PLAN_OWN_SLOTS, PLAN_OWN_MOST = 256, 1280, 16
+# one workgroup (of eight waves; head_dim 256 of four) for a row and kv head, nothing to join: rows of few slots (8 rows of 160: 5.7, in parts
+# 7.5; of 750: 11.7 and 10.4), or as many pairs as CUs (2 x 16 rows of 100 + 2000, ragged: 32.6 and 35.6)
+PLAN_SOLO_BYTES, PLAN_SOLO_WG = 512 * 512, 256
 
 
-def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda"):
+def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda", share=None):
     """The plan of paged_attn for rows in ``groups``: a list of (rows, prefix), consecutive rows whose first ``prefix``
     slots are the same (0: nothing shared).  ``max_len``: the most slots that a row may come to hold.  Made once for all
-    layers and steps in which the groups stay the same (it copies to the device: not under graph capture)."""
+    layers and steps in which the groups stay the same (it copies to the device: not under graph capture).  ``share``:
+    whether prefixes are read once per group (None: where that saves more than joining the parts costs)."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise RuntimeError("paged_attn_plan: the decode path runs only on a ROCm GPU")
@@ -1013,13 +1025,19 @@ def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda"):
         raise ValueError("paged_attn_plan: groups must be (rows >= 1, 0 <= prefix <= max_len) pairs")
     if Hk < 1 or Hq % Hk or Hq // Hk > 16 or HD not in (64, 128, 256):
         raise ValueError("paged_attn_plan: head_dim 64, 128 or 256 and at most 16 query heads per kv head")
-    return _make_plan(groups, Hq, Hk, HD, int(max_len), dev)
+    return _make_plan(groups, Hq, Hk, HD, int(max_len), dev, share)
 
 
-def _make_plan(groups, Hq, Hk, HD, max_len, dev):
+def _make_plan(groups, Hq, Hk, HD, max_len, dev, share=None):
     G = Hq // Hk
     R = sum(n for n, _ in groups)
-    shared = [n > 1 and p > 0 for n, p in groups]
+    slot = 4 * HD  # bytes of a slot's key and value
+    if share is None:
+        share = sum((n - 1) * p for n, p in groups) * Hk * slot > PLAN_SAVED
+    if not share and (R * Hk >= PLAN_SOLO_WG or max_len * slot <= PLAN_SOLO_BYTES):
+        # one workgroup per row and kv head, which writes the output itself
+        return PagedAttnPlan([], [(0, 0)] * R, 1, 1, 1, 8 if HD <= 128 else 4, Hq, Hk, HD, dev)
+    shared = [share and n > 1 and p > 0 for n, p in groups]
     cols = max([n * G for (n, p), s in zip(groups, shared) if s], default=0)
     ct = 2 if cols > 16 and HD <= 128 else 1
     fit = 16 * ct // G  # rows of a shared part
@@ -1042,8 +1060,8 @@ def _make_plan(groups, Hq, Hk, HD, max_len, dev):
         for c in range(max(len(x) for x in eight)):
             items += [x[c] for x in eight if c < len(x)]
     longest = max(max_len - (p if s else 0) for (n, p), s in zip(groups, shared))
-    nown = max(1, min(PLAN_CAP, max(-(-PLAN_OWN_WG // (R * Hk)), -(-longest // PLAN_OWN_SLOTS)), -(-longest // 128)))
-    return PagedAttnPlan(items, rows, nown, most + nown, ct, Hq, Hk, HD, dev)
+    nown = max(1, min(PLAN_OWN_MOST, max(-(-PLAN_OWN_WG // (R * Hk)), -(-longest // PLAN_OWN_SLOTS)), -(-longest // 128)))
+    return PagedAttnPlan(items, rows, nown, most + nown, ct, 4, Hq, Hk, HD, dev)
 
 
 def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
@@ -1078,7 +1096,7 @@ def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
     ws = torch.empty(plan.ws, device=dev, dtype=torch.float32).data_ptr() if plan.ws else None
     _call_on(dev, "ecd_paged_attn", q.data_ptr(), ldq, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), ldt,
              pos.data_ptr(), o.data_ptr(), ws, plan.items_ptr, plan.rows_ptr, plan.nitems, plan.nown, plan.parts,
-             plan.ctiles, R, int(S), MP, NP, Hq, Hk, P, HD, scale)
+             plan.ctiles, plan.waves, R, int(S), MP, NP, Hq, Hk, P, HD, scale)
     return o
 
 

@@ -80,24 +80,26 @@ class Batch:
                 tol[r, at] = 2.0 ** -11 * np.abs(out) + rel * avg + 2.0 ** -25 * (1 + m * np.abs(v[:, h // G]).max() / l)
         return o, tol
 
-    def run(self, dev, max_len=None, scale=None, plan=None, out=None):
+    def run(self, dev, max_len=None, scale=None, plan=None, out=None, share=True):
         import torch
         from estudiocanciones_amd.kernels import paged_attn, paged_attn_plan
         Hq, Hk, HD, P = self.H
         T = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
         kv = T(self.pool)
-        plan = plan or paged_attn_plan(self.groups, Hq, Hk, HD, max_len or self.table.shape[1] * P, dev)
+        plan = plan or paged_attn_plan(self.groups, Hq, Hk, HD, max_len or self.table.shape[1] * P, dev, share)
         pos = T(np.array(self.lens, np.int64) - 1)
         return paged_attn(T(self.q), kv[0], kv[1], T(self.table), pos, plan, S=self.S, scale=scale, out=out)
 
     def check(self, dev, **kw):
+        """With shared parts, without them (split and joined, or a workgroup per row), and as the rule has it."""
         want, tol = self.want(kw.get("scale") or 1 / math.sqrt(self.H[2]))
-        got = self.run(dev, **kw).float().cpu().numpy()
-        bad = ~(np.abs(got - want) <= tol)
-        assert not bad.any(), (int(bad.sum()), np.abs(got - want).max(), np.argwhere(bad)[:4])
-        for r, m in enumerate(self.lens):
-            if not m:
-                assert (got[r] == 0).all()
+        for share in (True, False, None):
+            got = self.run(dev, share=share, **kw).float().cpu().numpy()
+            bad = ~(np.abs(got - want) <= tol)
+            assert not bad.any(), (share, int(bad.sum()), np.abs(got - want).max(), np.argwhere(bad)[:4])
+            for r, m in enumerate(self.lens):
+                if not m:
+                    assert (got[r] == 0).all()
 
 
 HEADS = [(24, 8, 128), (8, 2, 128), (12, 2, 64), (5, 5, 64), (16, 1, 128), (8, 2, 256), (32, 2, 64), (6, 2, 256)]
@@ -136,6 +138,13 @@ def test_many_parts_and_a_long_table(dev):
 def test_what_is_not_attended_does_not_matter(dev, poison):
     groups, lens = [(4, 100), (2, 0)], [101, 0, 100, 150, 7, 33]
     Batch(groups, lens, 12, 4, 128, 64, seed=9, poison=poison).check(dev)
+
+
+@pytest.mark.parametrize("long", [False, True])
+def test_split_rows_without_sharing(dev, long):
+    """Rows too few or too long for a workgroup each: split over their slots and joined."""
+    lens = [4100, 1, 3000, 0] if long else [900, 700, 31, 32]
+    Batch([(2, 500), (2, 0)] if not long else [(4, 0)], lens, 6, 2, 128, 64, seed=3).check(dev, max_len=16384)
 
 
 def test_a_short_row_does_not_see_its_groups_slots(dev):
@@ -196,7 +205,7 @@ def test_the_same_bits_each_time_and_in_graphs(dev):
     T = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
     kv, table, q = T(b.pool), T(b.table), T(b.q)
     pos = T(np.array(b.lens, np.int64) - 1)
-    plan = paged_attn_plan(b.groups, 24, 8, 128, 1536, dev)
+    plan = paged_attn_plan(b.groups, 24, 8, 128, 1536, dev, share=True)
     first = paged_attn(q, kv[0], kv[1], table, pos, plan).clone()
     graphs, outs = [], []
     for _ in range(2):

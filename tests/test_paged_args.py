@@ -22,16 +22,16 @@ I, N = -22, -95
     (I, lambda L: L.ecd_paged_write(16, 504, None, 0, 8, None, 16, 16, 8, 4, 4, 4, 1, 1, 4, 2, 16, 64, None)),   # ld short
     (I, lambda L: L.ecd_paged_write(16, 512, 16, 9, 8, None, 16, 16, 8, 4, 4, 4, 1, 1, 4, 2, 16, 64, None)),     # rope, no q
     (I, lambda L: L.ecd_paged_write(16, 512, None, 0, 8, None, 16, 16, 8, 3, 4, 4, 1, 1, 4, 2, 16, 64, None)),   # table rows
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, None, 8, 1, 1, 2, 1, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, None, 8, 8, 0, 2, 2, 1, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 2, 1, 4, 9, 4, 2, 24, 128, 0.1, None)),
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 2, 1, 4, 9, 4, 2, 8, 128, 0.1, None)),
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 2, 1, 4, 9, 4, 3, 16, 128, 0.1, None)),
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 2, 1, 4, 9, 4, 2, 16, 128, 0.0, None)),
-    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 1 << 27, 8, 8, 16, 8, 8, 0, 1, 1, 1, 2, 1, 1 << 27, 9, 4, 2, 16, 128, 0.1, None)),
-    (N, lambda L: L.ecd_paged_attn(16, 768, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 2, 1, 4, 9, 4, 2, 16, 192, 0.1, None)),
-    (N, lambda L: L.ecd_paged_attn(16, 1024, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 2, 2, 1, 4, 9, 4, 2, 16, 256, 0.1, None)),
-    (N, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 513, 513, 1, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, None, 8, 1, 1, 2, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, None, 8, 8, 0, 2, 2, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 24, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 8, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 3, 16, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, 0.0, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 1 << 27, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 1 << 27, 9, 4, 2, 16, 128, 0.1, None)),
+    (N, lambda L: L.ecd_paged_attn(16, 768, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 16, 192, 0.1, None)),
+    (N, lambda L: L.ecd_paged_attn(16, 1024, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 2, 4, 2, 1, 4, 9, 4, 2, 16, 256, 0.1, None)),
+    (N, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 513, 513, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
     (I, lambda L: L.ecd_quant_a8(16, 96, None, 0.0, 16, 128, 16, 1, 96, None)),         # K % 64
     (I, lambda L: L.ecd_quant_a8(16, 64, None, 0.0, 16, 64, 16, 1, 64, None)),          # ldc % 128
     (I, lambda L: L.ecd_quant_a8(16, 64, None, -1.0, 16, 128, 16, 1, 64, None)),        # eps
@@ -89,7 +89,7 @@ def test_parts_of_a_plan(groups, Hq, Hk, HD):
     """Every shared slot of every row and kv head lies in exactly one part, and no two parts of a row have one number."""
     from estudiocanciones_amd.kernels import _make_plan
     G = Hq // Hk
-    plan = _make_plan(groups, Hq, Hk, HD, 8192, torch.device("cpu"))
+    plan = _make_plan(groups, Hq, Hk, HD, 8192, torch.device("cpu"), share=True)
     rows = plan.flat[:2 * plan.R].view(-1, 2).tolist()
     items = plan.flat[2 * plan.R:].view(-1, 6).tolist()
     assert plan.R == sum(n for n, _ in groups) and len(items) == plan.nitems
@@ -111,3 +111,16 @@ def test_parts_of_a_plan(groups, Hq, Hk, HD):
             r += 1
     heads = plan.R * Hq
     assert plan.ws == (0 if plan.parts == 1 else 2 * (-(-heads * plan.parts // 4) * 4) + heads * plan.parts * HD)
+
+
+def test_plans_by_the_rule():
+    """Little to share: a workgroup per row and kv head and nothing to join; much to share, or too few pairs for long rows: parts."""
+    from estudiocanciones_amd.kernels import _make_plan
+    cpu = torch.device("cpu")
+    solo = _make_plan([(4, 100), (4, 100)], 24, 8, 128, 512, cpu)
+    assert (solo.nitems, solo.parts, solo.ws, solo.waves) == (0, 1, 0, 8)
+    assert _make_plan([(2, 100)], 8, 2, 64, 1024, cpu).parts == 1
+    assert _make_plan([(2, 100)], 8, 2, 64, 1025, cpu).parts > 1
+    assert _make_plan([(32, 100)], 24, 8, 128, 8192, cpu).waves == 8
+    assert _make_plan([(16, 4096)], 24, 8, 128, 8192, cpu).nitems > 0
+    assert _make_plan([(16, 4096)], 24, 8, 128, 8192, cpu, share=False).nitems == 0
