@@ -24,7 +24,7 @@ class Batch:
         for rows, pre in groups:
             first = None
             for k in range(rows):
-                m = lens[r]
+                m = max(lens[r - r % S:r - r % S + S])  # what the sequence holds
                 if r % S == 0:
                     full = pre // P if m >= pre and first is not None else 0
                     own = -(-max(lens[r:r + S]) // P) - full
@@ -259,3 +259,37 @@ def test_refusals(dev):
     for bad in (dict(S=0), dict(Hk=1), dict(qkv=h(3, 512)), dict(rope=torch.zeros(64, 30, 2, device=dev)), dict(table=good["table"][:1])):
         with pytest.raises(ValueError):
             paged_write(**{**w, **bad})
+
+
+def test_rows_of_one_sequence_share_a_prefix(dev):
+    """S = 2: a group of three sequences with two rows each, one of them behind the prefix's end and one before it."""
+    Batch([(6, 100)], [130, 131, 101, 102, 99, 100], 6, 2, 128, 32, seed=12, S=2).check(dev)
+
+
+def test_pool_offsets_past_32_bits(dev):
+    """Pages at the end of a pool of more than 2^32 values a plane: the write, the attention and a fork reach them."""
+    import torch
+    from estudiocanciones_amd.kernels import page_fork, paged_attn, paged_attn_plan, paged_write
+    NP, P, HD, n = 263000, 128, 128, 300
+    kv = torch.empty(1, 2, NP, 1, P, HD, dtype=torch.float16, device=dev)
+    assert kv[0, 0].numel() > 1 << 32
+    ref = torch.ones(NP, dtype=torch.int32, device=dev)
+    ref[[NP - 9, NP - 5]] = 0
+    table = torch.full((3, 3), -1, dtype=torch.int32, device=dev)
+    table[0] = torch.tensor([NP - 1, 7, NP - 2], device=dev)
+    length = torch.tensor([n, 0, 0], device=dev)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    x = torch.from_numpy(randn16(1, n, 5 * HD)).to(dev)
+    paged_write(x, kv[0, 0], kv[0, 1], table[:1], torch.arange(n, device=dev), n, 3, 1)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    page_fork(kv, ref, table, length, i32(0, 0), i32(1, 2), err)
+    assert err.item() == 0 and table[1:, 2].tolist() == [NP - 9, NP - 5]
+    q = torch.from_numpy(randn16(2, 3, 3 * HD)).to(dev)
+    plan = paged_attn_plan([(3, n)], 3, 1, HD, 3 * P, dev, share=True)
+    o = paged_attn(q, kv[0, 0], kv[0, 1], table, torch.full((3,), n - 1, device=dev), plan).cpu().double().reshape(3, 3, HD)
+    k, v = (x[:, i * HD:(i + 1) * HD].cpu().double() for i in (3, 4))
+    s = q.cpu().double().reshape(3, 3, HD) @ k.T / HD ** 0.5
+    want = s.softmax(-1) @ v
+    ds = (HD + 8) * 2.0 ** -24 * float((q.cpu().double().abs().reshape(9, HD) @ k.abs().T).max()) / HD ** 0.5 + 2.0 ** -20
+    tol = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2 * ds) * (s.softmax(-1) @ v.abs()) + 2.0 ** -20
+    assert ((o - want).abs() <= tol).all()
