@@ -6,7 +6,7 @@
 // depend on the tile, the split of K or the other rows.  fp32 behind the sum, one rounding to fp16 at the end.
 //
 // Of fp16 x (no norm) the codes are the nearest integers to the exact quotients: 127 x has 18 bits, so a quotient that is
-// no tie is further from one than the correctly rounded division moves it.
+// no tie is further from one than the rounding of the quotient to fp32 moves it, and a tie is a value of fp32.
 #include "gemm_core.h"
 
 namespace ecd {
@@ -15,7 +15,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // One workgroup per row, its values in registers (NV pieces of 8 per thread; rows of more than 2048 NV values are read
-// again).  A row that holds an infinity or a NaN gets the scale NaN (and codes 0).
+// again).  A row that holds an infinity or a NaN gets the scale NaN (and codes 0).  Bound by vector instructions, then by the
+// row's two reductions: 2048 x 3072 with the norm 9.4 us with a division for each value, 7.8 us as written (18.9 MB).
 template <bool NORM, int NV>
 __global__ __launch_bounds__(256) void quant_a8_kernel(const f16* __restrict__ x, long ldx, const f16* __restrict__ w,
                                                        float eps, int8_t* __restrict__ c, long ldc,
@@ -60,17 +61,25 @@ __global__ __launch_bounds__(256) void quant_a8_kernel(const f16* __restrict__ x
   __syncthreads();
   top = max(max(__float_as_uint(red[4]), __float_as_uint(red[5])), max(__float_as_uint(red[6]), __float_as_uint(red[7])));
   const bool bad = top >= 0x7F800000u, none = bad || top == 0;
-  const float big = __uint_as_float(top);
+  const float big = __uint_as_float(top), inv = 1.f / big;
   if (t == 0) sx[m] = bad ? NAN : big / 127.f;
   int8_t* cr = c + m * ldc;
   each([&](int k, const f16x8& a, const f16x8& b) {
     if (k >= ldc) return;
-    uint32_t o[2] = {0u, 0u};
+    uint32_t o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
     if (!none) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j >> 2] |= (uint32_t)((int)rintf(value(a[j], b[j]) * 127.f / big) & 255) << (8 * (j & 3));
+      for (int j = 0; j < 8; ++j) {
+        const float t = value(a[j], b[j]) * 127.f, q = t * inv;
+        // one step from the quotient by the rounded reciprocal gives the rounded quotient; adding 1.5 2^23 leaves the nearest
+        // integer (ties to even) in the low bits
+        o[j] = __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, big, t), inv, q) + 12582912.f);
+      }
     }
-    *(u32x2*)(cr + k) = (u32x2){o[0], o[1]};
+    auto pack = [](uint32_t x, uint32_t y, uint32_t z, uint32_t w) {  // the low bytes
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0C0C0400u), __builtin_amdgcn_perm(y, x, 0x0C0C0400u), 0x05040100u);
+    };
+    *(u32x2*)(cr + k) = (u32x2){pack(o[0], o[1], o[2], o[3]), pack(o[4], o[5], o[6], o[7])};
   });
   // the columns behind K that lie behind the last piece (K is a multiple of 64, ldc of 128)
   for (int k = max(K, 2048 * NV) + 8 * t; k < ldc; k += 2048) *(u32x2*)(cr + k) = (u32x2){0u, 0u};

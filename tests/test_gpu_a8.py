@@ -36,6 +36,20 @@ def test_codes_are_the_nearest(dev, M, K):
     assert (pad == 0).all() and c.stride(0) % 128 == 0
 
 
+def test_codes_of_every_value(dev):
+    """Rows of all positive fp16 values up to a largest one, and their negatives: every code is the nearest integer."""
+    from estudiocanciones_amd.kernels import quant_a8
+    every = np.arange(0, 0x7C00, dtype=np.uint16).view(np.float16)
+    tops = [1, 2, 3, 1023, 1024, 2047, 0x3C00, 0x3BFF, 0x3F80, 0x57F0, 0x57F1, 0x7BFF] + rng(1).integers(1, 0x7C00, 100).tolist()
+    K = -(-len(every) // 64) * 64
+    x = np.zeros((len(tops), K), np.float16)
+    for r, t in enumerate(tops):
+        x[r, :t + 1] = every[:t + 1] * np.float16(-1 if r % 2 else 1)
+    c, _ = quant_a8(_t(x, dev))
+    want, _ = _codes_np(x.astype(np.float64))
+    assert np.array_equal(c.cpu().numpy(), want)
+
+
 def test_rows_of_zeros_tiny_and_no_numbers(dev):
     from estudiocanciones_amd.kernels import gemm_a8_packed, pack_i8, quant_a8
     x = randn16(1, 6, 128)
