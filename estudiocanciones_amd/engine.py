@@ -262,6 +262,7 @@ class Stack:
         self.paged = self.paged_plan = None  # cache in pages and the plan of its rows (alloc_paged)
 
     def alloc(self, B, L, dev, dtype):
+        self.paged = self.paged_plan = None
         self.rope = rope_cache(self.hd, max(L, 16), device=dev)
         for b in self.blocks:
             b.alloc(B, L, dev, dtype)
@@ -278,11 +279,16 @@ class Stack:
         self.tail2 = None if self.tail is None else \
             self._tail_buffers(2 * B, dev, dtype, L, share=self.tail)
 
+    def packed(self):
+        """Whether every layer's weights are packed (what the paged cache and int8 activations need)."""
+        return bool(self.blocks) and all(lin.qp is not None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2))
+
     def alloc_paged(self, seqs, pages, max_pages, dev, groups, page=64):
         """A cache in pages instead of the dense ones, for one row per sequence: ``groups`` lists (rows, shared slots) of
         consecutive sequences that share a prompt (the plan of paged_attn)."""
-        if not self.blocks or any(lin.qp is None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2)):
+        if not self.packed():
             raise NotImplementedError("Stack.alloc_paged: the paged path needs packed weights (widths in multiples of 64)")
+        self.free()
         b0, L = self.blocks[0], max_pages * page
         self.rope = rope_cache(self.hd, max(L, 16), device=dev)
         self.paged = PagedCache(len(self.blocks), seqs, pages, b0.kvh, self.hd, max_pages, page, dev)
@@ -1027,6 +1033,8 @@ class HeartMuLaLite:
         numerics, about half the time)."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
+        if a8 and not self.backbone.packed():
+            raise NotImplementedError("generate: int8 activations need packed weights (widths in multiples of 64)")
         text = torch.as_tensor(text, dtype=torch.int64)
         P = int(text.numel())
         n_frames = max_ms // FRAME_MS

@@ -112,6 +112,31 @@ def test_generate_shared_graph_equals_eager(dev):
     assert one.shape[0] == N_CB
 
 
+def test_caches_of_the_two_kinds_replace_each_other(dev):
+    """A model that is allocated anew, without release, runs on the new cache."""
+    import torch
+    gm, _ = _model(dev)
+    text = torch.from_numpy(rng(9).integers(0, 64, 20).astype(np.int64))
+    dense = _frames(gm, dev, text, 2, 2, False)
+    assert gm.backbone.paged is None
+    paged = _frames(gm, dev, text, 2, 2, True)
+    assert gm.backbone.blocks[0].kc is None and gm.backbone.tail is None
+    again = _frames(gm, dev, text, 2, 2, False)
+    assert gm.backbone.paged is None
+    for a, b, c in zip(dense, paged, again):
+        assert np.array_equal(a, c)
+        assert_close16(b, a, what="paged")
+
+
+def test_int8_activations_need_packed_weights(dev):
+    gm, _ = _model(dev)
+    gm.backbone.blocks[1].w2.qp = None
+    with pytest.raises(NotImplementedError, match="packed"):
+        gm.generate([1, 2, 3], 1, max_ms=160, a8=True)
+    with pytest.raises(NotImplementedError, match="packed"):
+        gm.generate([1, 2, 3], 1, max_ms=160, paged=True)
+
+
 def test_generate_stops_when_the_cache_refuses(dev):
     """A pool with too few pages: the song stops with RuntimeError, and the next one runs."""
     import torch
