@@ -522,6 +522,7 @@ int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, lo
   if (!x || !c || !sx || M <= 0 || K <= 0 || K % 64 || K > 1 << 17 || ldx < K || ldx % 8 || ldc < K || ldc % 128 ||
       !aligned16(x) || !aligned16(c) || (nw && !aligned16(nw)) || !(eps >= 0.f))
     return ECD_EINVAL;
+  if (M > 0xFFFFFF) return ECD_ENOTSUP;  // (a launch has fewer than 2^32 threads)
   const hipStream_t st = (hipStream_t)stream;
 #define QA(N_, V_)                                                                                                       \
   hipLaunchKernelGGL((quant_a8_kernel<N_, V_>), dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps,      \

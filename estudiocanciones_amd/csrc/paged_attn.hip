@@ -336,8 +336,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int HD, in
   const int i = blockIdx.x * 256 + threadIdx.x, per = HD / 4;
   const int head = i / per, d = 4 * (i - head * per);
   if (head >= heads) return;
-  const int r = head / a.Hq, n = a.rows[2 * r + 1] + a.nown;
-  if (n == 1) return;
+  const int r = head / a.Hq, np = a.rows[2 * r + 1], n = np + a.nown;
+  if (np < 0 || n > a.parts || n == 1) return;
   const float *pm = a.pm + (long)head * a.parts, *pl = a.pl + (long)head * a.parts, *pa = a.pa + (long)head * a.parts * HD + d;
   float M = -INFINITY, l = 0.f;
   f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -390,7 +390,7 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
       parts < nown || (parts > 1 && !ws) || R <= 0 || S <= 0 || MP <= 0 || NP <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
       Hq / Hk > 16 || P < 16 || (P & (P - 1)) || ldt < MP || ldq < (long)Hq * HD || (ldq % 8) ||
       ((uintptr_t)q & 15) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)o & 7) || ((uintptr_t)ws & 15) ||
-      !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown * Hk + nitems > 0x7FFFFFFFL || (long)R * Hq > 0x7FFFFFFFL / 64 ||
+      !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown * Hk + nitems > 0x7FFFFFL || (long)R * Hq > 0x7FFFFFFFL / 64 ||
       (long)NP * Hk * P > 0xFFFFFFFFL)
     return ECD_EINVAL;
   if ((HD != 64 && HD != 128 && HD != 256) || parts > 512) return ECD_ENOTSUP;

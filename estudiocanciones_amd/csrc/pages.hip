@@ -128,7 +128,7 @@ __global__ __launch_bounds__(PG_T) void page_fork_plan_kernel(const int* __restr
 // and writes it to every child of its source, so the slots of a prompt are read once for all of them (as long as its
 // children follow one another); the last block of a row writes the children's tables and counts their pages.
 // Bound by the writes.  32 children of 2 prompts, 40 slots of 28 layers (147 MB written): 51.1 us with a block per child
-// and run, FORK_NOW us now.
+// and run, 30 us now.
 constexpr int FORKS = 8, FORK_V = 2;  // children of a block, 16-byte pieces of a thread
 __global__ __launch_bounds__(256) void page_fork_kernel(f16* __restrict__ kv, int* __restrict__ ref, int NP,
                                                         int* __restrict__ table, int MP, const int* __restrict__ src,
@@ -322,6 +322,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const f16* __restrict_
 static bool pool_ok(int planes, int NP, int Hk, int P, int HD) {
   return planes > 0 && NP > 0 && Hk > 0 && P > 0 && HD > 0 && HD % 8 == 0;
 }
+constexpr long GRID_MOST = 0xFFFFFF;  // workgroups of 256 along x: a launch has fewer than 2^32 threads there
 static bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace ecd
@@ -333,6 +334,7 @@ extern "C" {
 int ecd_page_free(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B, int P, const int32_t* seqs,
                   int n, int32_t* err, void* stream) {
   if (!ref || !table || !length || !seqs || !err || NP <= 0 || MP <= 0 || B <= 0 || P <= 0 || n <= 0) return ECD_EINVAL;
+  if (n > GRID_MOST) return ECD_ENOTSUP;
   hipLaunchKernelGGL(page_free_kernel, dim3(n), dim3(256), 0, (hipStream_t)stream, ref, NP, table, MP, length, B, P,
                      seqs, err);
   return ecd_launch_status();
@@ -345,10 +347,10 @@ int ecd_page_fork(void* kv, int32_t* ref, int NP, int32_t* table, int MP, int64_
       !pool_ok(planes, NP, Hk, P, HD) || !a16(kv) || !a16(plan))
     return ECD_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
+  const long pieces = ((long)P * HD / 8 + 256 * FORK_V - 1) / (256 * FORK_V), x = pieces * planes * Hk + 1;
+  if (x > GRID_MOST) return ECD_ENOTSUP;
   hipLaunchKernelGGL(page_fork_plan_kernel, dim3(1), dim3(PG_T), 0, st, ref, NP, table, MP, length, B, P, src, dst, n,
                      plan, err);
-  const long pieces = ((long)P * HD / 8 + 256 * FORK_V - 1) / (256 * FORK_V), x = pieces * planes * Hk + 1;
-  if (x > 0x7FFFFFFFL) return ECD_ENOTSUP;
   hipLaunchKernelGGL(page_fork_kernel, dim3((unsigned)x, (n + FORKS - 1) / FORKS), dim3(256), 0, st, (f16*)kv, ref, NP,
                      table, MP, src, dst, plan, n, (int)pieces, Hk, P, HD);
   return ecd_launch_status();
@@ -357,6 +359,7 @@ int ecd_page_fork(void* kv, int32_t* ref, int NP, int32_t* table, int MP, int64_
 int ecd_page_extend(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B, int P, const int64_t* pos,
                     int32_t* err, void* stream) {
   if (!ref || !table || !length || !pos || !err || NP <= 0 || MP <= 0 || B <= 0 || B > PG_T || P <= 0) return ECD_EINVAL;
+  if ((long)B * MP > 0xFFFFFFFFL) return ECD_ENOTSUP;  // (new pages are counted in 32 bits)
   hipLaunchKernelGGL(page_extend_kernel, dim3(1), dim3(PG_T), 0, (hipStream_t)stream, ref, NP, table, MP, length, B, P,
                      pos, err);
   return ecd_launch_status();
@@ -383,7 +386,7 @@ int ecd_paged_write(const void* qkv, long ld, const float* rope, int LR, const i
       !a16(vp) || (q && !a16(q)) || ((uintptr_t)rope & 15))
     return ECD_EINVAL;
   const long W = (long)(rope ? Hq + 2 * Hk : 2 * Hk) * (HD / 8), blocks = (M * W + 255) / 256;
-  if (W > 0x7FFFFFFFL || blocks > 0x7FFFFFFFL) return ECD_ENOTSUP;
+  if (W > 0x7FFFFFFFL || blocks > GRID_MOST) return ECD_ENOTSUP;
   const hipStream_t st = (hipStream_t)stream;
 #define PW(R_)                                                                                                        \
   hipLaunchKernelGGL((paged_write_kernel<R_>), dim3((unsigned)blocks), dim3(256), 0, st, (const f16*)qkv, ld, rope,    \

@@ -28,7 +28,8 @@ class PagedCache:
         dev = torch.device(device)
         if dev.type != "cuda":
             raise RuntimeError("PagedCache needs a ROCm GPU device")
-        if min(layers, seqs, pages, kv_heads, page) < 1 or head_dim < 8 or head_dim % 8 or page < 16 or page & (page - 1):
+        max_pages = pages if max_pages is None else int(max_pages)
+        if min(layers, seqs, pages, kv_heads, page, max_pages) < 1 or head_dim < 8 or head_dim % 8 or page < 16 or page & (page - 1):
             raise ValueError("PagedCache: positive sizes, a head_dim in multiples of 8 and a page of 16, 32, 64, .. slots")
         if seqs > 1024:
             raise ValueError("PagedCache: at most 1024 sequences")
@@ -36,7 +37,7 @@ class PagedCache:
         self.kv = torch.zeros(layers, 2, pages, kv_heads, page, head_dim, device=dev, dtype=torch.float16)
         self.dev = self.kv.device
         self.ref = torch.zeros(pages, device=dev, dtype=torch.int32)
-        self.table = torch.full((seqs, pages if max_pages is None else int(max_pages)), -1, device=dev, dtype=torch.int32)
+        self.table = torch.full((seqs, max_pages), -1, device=dev, dtype=torch.int32)
         self.length = torch.zeros(seqs, device=dev, dtype=torch.int64)
         self.err = torch.zeros(1, device=dev, dtype=torch.int32)
 

@@ -16,6 +16,11 @@ I, N = -22, -95
     (I, lambda L: L.ecd_page_fork(16, 8, 4, 8, 4, 8, 2, 8, 8, 1, 16, 8, 2, 1, 16, 60, None)),     # HD % 8
     (I, lambda L: L.ecd_page_extend(8, 4, 8, 4, 8, 1025, 16, 8, 8, None)),
     (I, lambda L: L.ecd_page_extend(8, 4, 8, 4, 8, 2, 16, None, 8, None)),
+    (N, lambda L: L.ecd_page_extend(8, 4, 8, 1 << 30, 8, 4, 16, 8, 8, None)),           # 2^32 pages of a table
+    (N, lambda L: L.ecd_page_free(8, 4, 8, 4, 8, 2, 16, 8, 1 << 24, 8, None)),          # 2^32 threads
+    (N, lambda L: L.ecd_page_fork(16, 8, 4, 8, 4, 8, 2, 8, 8, 1, 16, 8, 1 << 20, 16, 16, 64, None)),
+    (N, lambda L: L.ecd_paged_write(16, 512, None, 0, 8, None, 16, 16, 8, 4, 4, 4, 1 << 28, 1, 4, 2, 16, 64, None)),
+    (N, lambda L: L.ecd_quant_a8(16, 64, None, 0.0, 16, 128, 16, 1 << 24, 64, None)),
     (I, lambda L: L.ecd_page_compact(16, 8, 4, 8, 8, 16, 8, 4, 8, 8, 2, 4, 8, 8, 2, 1, 16, 64, None)),  # kv2 is kv
     (I, lambda L: L.ecd_page_compact(16, 8, 4, 8, 8, 32, 8, 0, 8, 8, 2, 4, 8, 8, 2, 1, 16, 64, None)),  # empty pool
     (I, lambda L: L.ecd_paged_write(16, 512, None, 0, 8, None, 16, 16, 8, 4, 4, 4, 1, 1, 4, 2, 16, 60, None)),   # HD % 8
@@ -29,6 +34,7 @@ I, N = -22, -95
     (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 3, 16, 128, 0.1, None)),
     (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, 0.0, None)),
     (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 1 << 27, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 1 << 27, 9, 4, 2, 16, 128, 0.1, None)),
+    (I, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 1 << 22, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
     (N, lambda L: L.ecd_paged_attn(16, 768, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 16, 192, 0.1, None)),
     (N, lambda L: L.ecd_paged_attn(16, 1024, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 1, 1, 2, 4, 2, 1, 4, 9, 4, 2, 16, 256, 0.1, None)),
     (N, lambda L: L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, 16, 8, 8, 0, 513, 513, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, 0.1, None)),
@@ -74,7 +80,8 @@ def test_plan_refuses(kw):
         paged_attn_plan(**{**a, **kw})
 
 
-@pytest.mark.parametrize("kw", [dict(layers=0), dict(page=8), dict(page=48), dict(head_dim=20), dict(seqs=1025), dict(pages=0)])
+@pytest.mark.parametrize("kw", [dict(layers=0), dict(page=8), dict(page=48), dict(head_dim=20), dict(seqs=1025), dict(pages=0),
+                                dict(max_pages=0)])
 def test_cache_refuses(kw):
     from estudiocanciones_amd.paged import PagedCache
     a = dict(layers=1, seqs=1, pages=1, kv_heads=1, head_dim=64)
