@@ -217,7 +217,7 @@ struct A8Tile {
 
   // The sums of this wave's group: KG groups of NW waves take an equal share of K each, from a ring of their own (a CU
   // with one workgroup then has KG times the loads in flight, where there are too few tiles for all CUs).  A chunk of 128 k
-  // that K ends in: the second half of the weights re-reads the first, the codes behind K are 0.
+  // that K ends in: its second half re-reads the first and its products are left out, so nothing behind K is read.
   static __device__ __forceinline__ void run(unsigned char* all, i32x16 (&acc)[FT][RT], const int8_t* __restrict__ c, long ldc,
                                              const int8_t* __restrict__ wp, int M, int N, int K, int n0, int m0) {
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -250,7 +250,7 @@ struct A8Tile {
       if constexpr (j < WI)
         lds_dma16_at<NW * j * 1024>(wb, odd && left == 1 ? woff[j] - back : woff[j], sa);
       else
-        lds_dma16_at<LW + NW * (j - WI) * 1024>(xb, xoff[j - WI], sa);
+        lds_dma16_at<LW + NW * (j - WI) * 1024>(xb, odd && left == 1 ? xoff[j - WI] & ~64u : xoff[j - WI], sa);  // (ldc % 128 == 0)
     };
     auto next_chunk = [&]() {
       wb += 2048;
@@ -333,7 +333,7 @@ struct A8Tile {
       half(fa, IC<1>{}, base, fc, IC<0>{}, IC<0>{}, 0);
       st = sn;
     }
-    half(fc, IC<0>{}, lds, fa, IC<0>{}, IC<0>{}, 0);  // (its reads are never used)
+    if (!odd) half(fc, IC<0>{}, lds, fa, IC<0>{}, IC<0>{}, 0);  // (its reads are never used)
     if (KG > 1 && nch < most) barrier();
   }
 

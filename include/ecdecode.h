@@ -668,7 +668,7 @@ int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, lo
                  void* stream);
 
 /* y[m, n] = f16(sx[m] s[n] sum_k c[m, k] q[n, k] (+ res[m, n])) with weights packed by ecd_pack_i8: the sum is an
- * integer, one rounding at the end.  c from ecd_quant_a8 (zero columns behind K). */
+ * integer, one rounding at the end.  c as from ecd_quant_a8: ldc % 128 == 0, at most 2^23; columns from K on are not read. */
 int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                 void* y, long ldy, int M, int N, int K, void* stream);
 

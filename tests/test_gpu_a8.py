@@ -196,6 +196,30 @@ def test_strides_and_destinations(dev):
     assert (mm[:, 0] == 5).all() and (mm[:, 1 + N // 2:] == 5).all()
 
 
+@pytest.mark.parametrize("M", [5, 40, 300, 600])
+def test_a_part_of_the_columns(dev, M):
+    """Codes of a longer row, from one column to another: the columns behind K do not count, whatever they hold."""
+    from estudiocanciones_amd._ffi import call
+    from estudiocanciones_amd.kernels import gemm_a8_packed, pack_i8, stream_ptr
+    import torch
+    g = rng(31)
+    whole = _t(g.integers(-127, 128, (M, 512)).astype(np.int8), dev)
+    N = 300
+    s, sx = _t((0.01 * (1 + g.random(N))).astype(np.float16), dev), _t((0.01 * (1 + g.random(M))).astype(np.float32), dev)
+    for a, b in ((0, 192), (64, 512), (320, 384), (192, 512)):
+        w = _t(g.integers(-127, 128, (N, b - a)).astype(np.int8), dev)
+        wp, c = pack_i8(w), whole[:, a:b]
+        got = gemm_a8_packed(c, sx, wp, s, N, b - a)
+        want = (c.double() @ w.double().T) * sx.double()[:, None] * s.double()
+        # |sum| < 2^24 is a value of fp32; two products in fp32, one rounding to fp16 (2^-24 absolute where it is subnormal)
+        assert ((got.double() - want).abs() <= (2.0 ** -11 + 2.0 ** -22) * want.abs() + 2.0 ** -25).all()
+        for cfg in range(2, 9):
+            y = torch.empty_like(got)
+            call("ecd_gemm_a8_tuned", c.data_ptr(), 512, sx.data_ptr(), wp.data_ptr(), s.data_ptr(), None, 0, y.data_ptr(), N,
+                 M, N, b - a, cfg, stream_ptr(y.device))
+            assert torch.equal(y, got)
+
+
 def test_no_rows(dev):
     import torch
     from estudiocanciones_amd.kernels import gemm_a8_packed, pack_i8, quant_a8
