@@ -194,6 +194,10 @@ __global__ __launch_bounds__(64 * FEW_W) void gemm_a8_few_kernel(const int8_t* _
 // ---- many rows: tiles of 32 WN FT features x 32 WM RT rows through an LDS ring of NS stages of 128 k
 // The loads, the stages and the order of a loop pass are those of GemmTile (gemm_core.h) on bytes: 16 bytes of a row or a
 // feature are 16 k of v_mfma_i32_32x32x32_i8 instead of 8 of the fp16 product.
+// The largest tile (256 x 256, 8 waves) is bound by the products and their LDS reads: 2048 rows, (16384, 3072) 97 us, of which
+// 11 are the sums' way out (2.1 POPS; matrix pipes busy 54%); 8192^3 2.35 POPS.  Four waves of 128 x 128 took 110 us.  The
+// small tiles are bound by what a CU gets from its L2 and by latency: 187 rows, (3072, 8192), 64 x 64 with K in two shares,
+// 14.1 to 15.2 us (25 MB of weights); 128 x 64 with K whole 15.7.
 template <int FT, int RT>
 struct A8Frags {
   i32x4 w[2][FT], x[2][RT];

@@ -9,6 +9,14 @@
 //
 // A row takes the shared parts only if it attends the whole prefix; else its own part covers [0, pos].  The shared slots
 // are read through the first such row's pages.
+//
+// Both products run on v_mfma_f32_16x16x32_f16 with the slots of a tile as its rows (scores) and its k (output): a column's
+// probabilities then lie in the lane that needs them, and a tile goes from memory to registers to the products without LDS.
+// Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 for the second product (2^-11 each).
+// Bound by the reads of K and V: of 24 query heads on 8 kv heads of 128, 2 x 32 rows on prompts of 7000 slots (126 MB, each
+// slot read from memory once) take 38.5 us and 4.7 us for the join, 2 x 16 on 4096 (98 MB) 25.7 and 3.9: about 5.5 us until the
+// first tile is there, then 2 us for each of 14 tiles of a wave (8 waves a CU), 3 us to add the waves up.  A few short
+// rows are bound by those first and last steps: 8 rows of 750 slots 7.4 to 8.3 us and 3.7 for the join.
 #include "common.h"
 
 namespace ecd {
@@ -330,7 +338,9 @@ __global__ __launch_bounds__(64 * W, HD > 128 ? 1 : 2) void paged_attn_kernel(Pa
   attend<HD, 1, W>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1, ~0ull);
 }
 
-// One thread per four dims of a head: JB parts at a time, all their loads at once, in the order of the parts.
+// The parts of a head to one output: one thread per four dims, JB parts at a time, all their loads at once (one after the other
+// cost a memory latency each), in the order of the parts, so the result does not depend on timing.  Bound by latency: 3.7 us
+// for 8 rows of 4 parts, 4.7 us for 64 rows of 5.
 constexpr int JB = 8;
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int HD, int heads) {
   const int i = blockIdx.x * 256 + threadIdx.x, per = HD / 4;
