@@ -206,7 +206,7 @@ def test_a_part_of_the_columns(dev, M):
     whole = _t(g.integers(-127, 128, (M, 512)).astype(np.int8), dev)
     N = 300
     s, sx = _t((0.01 * (1 + g.random(N))).astype(np.float16), dev), _t((0.01 * (1 + g.random(M))).astype(np.float32), dev)
-    for a, b in ((0, 192), (64, 512), (320, 384), (192, 512)):
+    for a, b in ((0, 192), (64, 512), (320, 384), (192, 512), (16, 208), (432, 496)):
         w = _t(g.integers(-127, 128, (N, b - a)).astype(np.int8), dev)
         wp, c = pack_i8(w), whole[:, a:b]
         got = gemm_a8_packed(c, sx, wp, s, N, b - a)
@@ -218,6 +218,25 @@ def test_a_part_of_the_columns(dev, M):
             call("ecd_gemm_a8_tuned", c.data_ptr(), 512, sx.data_ptr(), wp.data_ptr(), s.data_ptr(), None, 0, y.data_ptr(), N,
                  M, N, b - a, cfg, stream_ptr(y.device))
             assert torch.equal(y, got)
+
+
+@pytest.mark.parametrize("M,N", [(3, 40), (12, 300), (90, 1001), (600, 520)])
+def test_residual_in_place(dev, M, N):
+    """The residual's rows may be the result's."""
+    from estudiocanciones_amd.kernels import gemm_a8_packed, pack_i8, quant_a8
+    import torch
+    g = rng(32)
+    K = 320
+    c, sx = quant_a8(_t(g.standard_normal((M, K)).astype(np.float16), dev))
+    wp = pack_i8(_t(g.integers(-127, 128, (N, K)).astype(np.int8), dev))
+    s = _t((0.001 * (1 + g.random(N))).astype(np.float16), dev)
+    wide = _t(g.standard_normal((M, N + 13)).astype(np.float16), dev)
+    y = wide[:, 3:3 + N]
+    keep = wide.clone()
+    want = gemm_a8_packed(c, sx, wp, s, N, K, res=y.clone())
+    gemm_a8_packed(c, sx, wp, s, N, K, res=y, out=y)
+    assert torch.equal(y, want)
+    assert torch.equal(wide[:, :3], keep[:, :3]) and torch.equal(wide[:, 3 + N:], keep[:, 3 + N:])
 
 
 def test_no_rows(dev):
