@@ -1014,15 +1014,16 @@ PLAN_SOLO_BYTES, PLAN_SOLO_WG = 512 * 512, 256
 
 def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda", share=None):
     """The plan of paged_attn for rows in ``groups``: a list of (rows, prefix), consecutive rows whose first ``prefix``
-    slots are the same (0: nothing shared).  ``max_len``: the most slots that a row may come to hold.  Made once for all
-    layers and steps in which the groups stay the same (it copies to the device: not under graph capture).  ``share``:
-    whether prefixes are read once per group (None: where that saves more than joining the parts costs)."""
+    slots are the same (0: nothing shared).  ``max_len``: the most slots that a row may come to hold (a prefix of more is
+    not shared: no row attends all of it).  Made once for all layers and steps in which the groups stay the same (it
+    copies to the device: not under graph capture).  ``share``: whether prefixes are read once per group (None: where
+    that saves more than joining the parts costs)."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise RuntimeError("paged_attn_plan: the decode path runs only on a ROCm GPU")
     groups = [(int(n), int(p)) for n, p in groups]
-    if not groups or any(n < 1 or p < 0 or p > max_len for n, p in groups):
-        raise ValueError("paged_attn_plan: groups must be (rows >= 1, 0 <= prefix <= max_len) pairs")
+    if not groups or max_len < 0 or any(n < 1 or p < 0 for n, p in groups):
+        raise ValueError("paged_attn_plan: groups must be (rows >= 1, prefix >= 0) pairs and max_len >= 0")
     if Hk < 1 or Hq % Hk or Hq // Hk > 16 or HD not in (64, 128, 256):
         raise ValueError("paged_attn_plan: head_dim 64, 128 or 256 and at most 16 query heads per kv head")
     return _make_plan(groups, Hq, Hk, HD, int(max_len), dev, share)
@@ -1030,6 +1031,7 @@ def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda", share=None):
 
 def _make_plan(groups, Hq, Hk, HD, max_len, dev, share=None):
     G = Hq // Hk
+    groups = [(n, p if p <= max_len else 0) for n, p in groups]
     R = sum(n for n, _ in groups)
     slot = 4 * HD  # bytes of a slot's key and value
     if share is None:

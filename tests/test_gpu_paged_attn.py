@@ -293,3 +293,9 @@ def test_pool_offsets_past_32_bits(dev):
     ds = (HD + 8) * 2.0 ** -24 * float((q.cpu().double().abs().reshape(9, HD) @ k.abs().T).max()) / HD ** 0.5 + 2.0 ** -20
     tol = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2 * ds) * (s.softmax(-1) @ v.abs()) + 2.0 ** -20
     assert ((o - want).abs() <= tol).all()
+
+
+def test_prefixes_and_rows_past_the_plans_length(dev):
+    """A prefix longer than any row can hold (nobody attends all of it), rows that hold more than the plan was made for."""
+    Batch([(1, 500), (3, 400)], [0, 20, 0, 33], 6, 2, 128, 16, seed=21).check(dev)
+    Batch([(2, 50), (2, 0)], [61, 300, 1000, 52], 6, 2, 64, 32, seed=22).check(dev, max_len=60)

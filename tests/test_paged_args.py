@@ -71,7 +71,7 @@ def test_calls_refuse_tensors_that_are_not_on_a_gpu():
         PagedCache(1, 1, 1, 1, 64, device="cpu")
 
 
-@pytest.mark.parametrize("kw", [dict(groups=[]), dict(groups=[(0, 4)]), dict(groups=[(2, 65)]), dict(groups=[(2, -1)]),
+@pytest.mark.parametrize("kw", [dict(groups=[]), dict(groups=[(0, 4)]), dict(max_len=-1), dict(groups=[(2, -1)]),
                                 dict(Hq=5), dict(Hq=34), dict(HD=96), dict(HD=384)])
 def test_plan_refuses(kw):
     from estudiocanciones_amd.kernels import paged_attn_plan
@@ -118,6 +118,15 @@ def test_parts_of_a_plan(groups, Hq, Hk, HD):
             r += 1
     heads = plan.R * Hq
     assert plan.ws == (0 if plan.parts == 1 else 2 * (-(-heads * plan.parts // 4) * 4) + heads * plan.parts * HD)
+
+
+@pytest.mark.parametrize("share", [None, True, False])
+def test_a_prefix_that_no_row_can_hold_is_not_shared(share):
+    from estudiocanciones_amd.kernels import _make_plan
+    a = _make_plan([(3, 100), (2, 65), (4, 64)], 4, 2, 64, 64, torch.device("cpu"), share=share)
+    b = _make_plan([(3, 0), (2, 0), (4, 64)], 4, 2, 64, 64, torch.device("cpu"), share=share)
+    assert (a.nitems, a.nown, a.parts, a.ws) == (b.nitems, b.nown, b.parts, b.ws) and torch.equal(a.flat, b.flat)
+    assert _make_plan([(1, 5)], 4, 2, 64, 0, torch.device("cpu"), share=share).parts == 1
 
 
 def test_plans_by_the_rule():
