@@ -237,6 +237,28 @@ def test_on_another_stream(dev):
     assert torch.equal(first, other)
 
 
+def test_two_calls_at_once(dev):
+    """One plan on two streams, each with queries of its own."""
+    import torch
+    from estudiocanciones_amd.kernels import paged_attn, paged_attn_plan
+    b = Batch([(8, 2000), (4, 300)], [2000 + 40 * r for r in range(8)] + [300, 301, 420, 777], 24, 8, 128, 64, seed=8)
+    T = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    kv, table, pos = T(b.pool), T(b.table), T(np.array(b.lens, np.int64) - 1)
+    qs = [T(b.q), T(b.q[::-1])]
+    plan = paged_attn_plan(b.groups, 24, 8, 128, 4096, dev, share=True)
+    want = [paged_attn(q, kv[0], kv[1], table, pos, plan) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged_attn(qs[i], kv[0], kv[1], table, pos, plan))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in (0, 1) for g in got[i])
+
+
 def test_refusals(dev):
     import torch
     from estudiocanciones_amd.kernels import paged_attn, paged_attn_plan, paged_write

@@ -40,7 +40,7 @@ def _frames(gm, dev, text, n, steps, paged, cfg=1.5):
     return [o.float().cpu().numpy() for o in out]
 
 
-@pytest.mark.parametrize("n,cfg,P,steps", [(1, 1.0, 5, 3), (3, 1.5, 70, 61), (2, 1.5, 128, 3), (10, 1.5, 100, 4)])
+@pytest.mark.parametrize("n,cfg,P,steps", [(1, 1.0, 5, 3), (3, 1.5, 70, 61), (2, 1.5, 128, 3), (10, 1.5, 100, 4), (70, 1.5, 40, 2)])
 def test_logits_of_shared_and_dense_caches(dev, n, cfg, P, steps):
     """Prompts within a page, that end in one and on a border; a step that takes a new page; more than 16 rows."""
     import torch
