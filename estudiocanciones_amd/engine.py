@@ -923,6 +923,7 @@ class HeartMuLaLite:
         """Static caches for n takes and backbone capacity L (app/engine.py:380-388), and the
         sampler's seed (drawn from torch's host generator when not given).  ``paged``: the slots of a
         prompt that the takes share; the backbone's cache is then in pages of PAGE slots."""
+        self.graphs.clear()  # (a frame captured over earlier caches, whose song did not end, is not replayed)
         self.N = n
         self.B = 2 * n if cfg_scale != 1.0 else n
         if seed is None or seed < 0:

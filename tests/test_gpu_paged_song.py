@@ -112,6 +112,27 @@ def test_generate_shared_graph_equals_eager(dev):
     assert one.shape[0] == N_CB
 
 
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_song_after_one_that_broke_off(dev, paged):
+    """A callback that raises leaves a captured frame and caches behind: the next song does not run on them."""
+    import torch
+    gm, _ = _model(dev)
+    text = rng(9).integers(0, 64, 40)
+    forced = torch.from_numpy(rng(12).integers(0, 8193, (61, 4, N_CB)).astype(np.int64)).to(dev)
+    kw = dict(max_ms=80 * 60, seed=5, n=2, paged=paged)
+    want = gm.generate(text, 3, **kw)
+
+    def stop(*_):
+        raise KeyboardInterrupt
+
+    with pytest.raises(KeyboardInterrupt):
+        gm.generate(text, 3, progress=stop, forced=forced, **kw)
+    kept = torch.zeros(64 << 20, dtype=torch.uint8, device=dev)  # what may lie where the old caches were
+    for x, y in zip(gm.generate(text, 3, **kw), want):
+        assert torch.equal(x, y)
+    assert not kept.any()
+
+
 def test_caches_of_the_two_kinds_replace_each_other(dev):
     """A model that is allocated anew, without release, runs on the new cache."""
     import torch
