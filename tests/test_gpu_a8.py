@@ -239,6 +239,26 @@ def test_residual_in_place(dev, M, N):
     assert torch.equal(wide[:, :3], keep[:, :3]) and torch.equal(wide[:, 3 + N:], keep[:, 3 + N:])
 
 
+@pytest.mark.parametrize("M,N,K", [(262200, 8200, 64), (33000, 40, 131072)])
+def test_offsets_past_32_bits(dev, M, N, K):
+    """More than 2^31 results, more than 2^32 bytes of codes: the last rows have the bits that they have by themselves."""
+    from estudiocanciones_amd.kernels import gemm_a8_packed, gemm_a8_silu_packed, pack_i8, quant_a8
+    import torch
+    g = rng(33)
+    x = _t(g.standard_normal((64, K)).astype(np.float16), dev).repeat(-(-M // 64), 1)[:M]
+    wp = pack_i8(_t(g.integers(-127, 128, (N, K)).astype(np.int8), dev))
+    s = _t((0.001 * (1 + g.random(N))).astype(np.float16), dev)
+    c, sx = quant_a8(x)
+    y = gemm_a8_packed(c, sx, wp, s, N, K, res=None)
+    z = gemm_a8_silu_packed(c, sx, wp, s, N // 2, K)
+    for r in (0, M // 2 // 64 * 64, M - 70):
+        c1, sx1 = quant_a8(x[r:r + 70])
+        assert torch.equal(c1, c[r:r + 70]) and torch.equal(sx1, sx[r:r + 70])
+        assert torch.equal(gemm_a8_packed(c1, sx1, wp, s, N, K), y[r:r + 70])
+        assert torch.equal(gemm_a8_silu_packed(c1, sx1, wp, s, N // 2, K), z[r:r + 70])
+    assert torch.equal(y[:64], y[(M // 64 - 1) * 64:M // 64 * 64])
+
+
 def test_no_rows(dev):
     import torch
     from estudiocanciones_amd.kernels import gemm_a8_packed, pack_i8, quant_a8
