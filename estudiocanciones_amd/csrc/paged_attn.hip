@@ -12,7 +12,12 @@
 //
 // Both products run on v_mfma_f32_16x16x32_f16 with the slots of a tile as its rows (scores) and its k (output): a column's
 // probabilities then lie in the lane that needs them, and a tile goes from memory to registers to the products without LDS.
-// Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 for the second product (2^-11 each).
+// Scores, maxima, sums and outputs are fp32.  A weight is exp(s - m) 2^14 and goes into the second product as the sum of two
+// fp16 values, the upper one rounded towards zero and the lower one what that leaves: 2^-20 of the weight, or 2^-38 of the
+// largest, where one fp16 value would lose 2^-12 of each and every weight below 2^-25 of the largest (of thousands of
+// slots beside a few large ones they are a part of the result that counts).  The matrix pipes wait for the tiles, so the second
+// product's other half costs little: 2 x 32 rows on prompts of 7000 slots 42.1 us against 41.4 with its join, 2 x 16 on 4096
+// 29.2 against 28.9, short rows the same.
 // Bound by the reads of K and V: of 24 query heads on 8 kv heads of 128, 2 x 32 rows on prompts of 7000 slots (126 MB, each
 // slot read from memory once) take 38.5 us and 4.7 us for the join, 2 x 16 on 4096 (98 MB) 25.7 and 3.9: about 5.5 us until the
 // first tile is there, then 2 us for each of 14 tiles of a wave (8 waves a CU), 3 us to add the waves up.  A few short
@@ -108,6 +113,16 @@ struct PState {
   float m[CT], l[CT];
 };
 
+// w0 and w1 (not negative) as sums of two fp16 values each.  The lower one is never 0 beside an upper one that is not, since
+// a value of infinity times 0 would be no number.
+__device__ __forceinline__ void two_halves(float w0, float w1, f16x2& hi, f16x2& lo) {
+  const f16 least = __builtin_bit_cast(f16, (uint16_t)1);
+  hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+  lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w0 - (float)hi.x, w1 - (float)hi.y));
+  lo = __builtin_elementwise_max(lo, __builtin_elementwise_min(hi, (f16x2){least, least}));
+}
+constexpr float W_LOG2 = 14.f;  // weights are scaled by 2^14
+
 // Slots outside [lo, hi) of the tile at t0 do not count, whatever they hold.  `after_scores` runs once K is used.
 template <int HD, int CT, typename F>
 __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, float c2, int t0, int lo, int hi, int lane, F&& after_scores) {
@@ -124,7 +139,7 @@ __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, flo
       for (int i = 0; i < T::KC; ++i) sc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[j][i], s.q[c][i], sc[c][j], 0, 0, 0);
     }
   after_scores();
-  f16x8 p[CT];
+  f16x8 p[CT], pr[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     if (edge) {
@@ -142,18 +157,23 @@ __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, flo
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[c][j][e]);
     const float mn = fmaxf(s.m[c], max_groups(mx));
-    const float mb = mn == -INFINITY ? 0.f : mn * c2;
+    // the difference first: m c2 rounded by itself would be a factor of its own in each tile's weights where scores are large
+    const float mb = mn == -INFINITY ? 0.f : mn;
     float ps = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][j][e], c2, -mb));
-        ps += w;
-        p[c][4 * j + e] = (f16)w;
+      for (int e = 0; e < 4; e += 2) {
+        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][j][e] - mb, c2, W_LOG2));
+        const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][j][e + 1] - mb, c2, W_LOG2));
+        ps += w0 + w1;
+        f16x2 h, r;
+        two_halves(w0, w1, h, r);
+        p[c][4 * j + e] = h.x, p[c][4 * j + e + 1] = h.y;
+        pr[c][4 * j + e] = r.x, pr[c][4 * j + e + 1] = r.y;
       }
     if (__any(mn != s.m[c])) {
-      const float alpha = __builtin_amdgcn_exp2f(s.m[c] * c2 - mb);
+      const float alpha = __builtin_amdgcn_exp2f((s.m[c] - mb) * c2);
       s.l[c] *= alpha;
 #pragma unroll
       for (int x = 0; x < T::ND; ++x)
@@ -183,6 +203,8 @@ __device__ __forceinline__ void tile_attend(PState<HD, CT>& s, PTile<HD>& t, flo
       const f16x8 va = {v0[b], v1[b], v2[b], v3[b], v4[b], v5[b], v6[b], v7[b]};
 #pragma unroll
       for (int c = 0; c < CT; ++c) s.acc[c][x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[c], s.acc[c][x][b], 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) s.acc[c][x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pr[c], s.acc[c][x][b], 0, 0, 0);
     }
   }
 }
