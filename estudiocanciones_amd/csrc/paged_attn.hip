@@ -229,10 +229,11 @@ __device__ __forceinline__ void begin(PState<HD, CT>& s, const PagedArgs& a, int
 }
 
 // One part on one workgroup whose waves share out the slots: `cols` columns, slots [lo, hi) through `tab`.
-// `live`: bit i says whether row row0 + i takes this part.  Its result goes to place `part`, or with `whole` normalised to o.
+// `live`: bit i says whether row row0 + i takes this part.  Its result goes to place `part` of the rows of `mine`, or with
+// `whole` normalised to o.
 template <int HD, int CT, int W>
 __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0, int cols, int kh, const int* tab, int lo,
-                                       int hi, int part, bool whole, uint64_t live) {
+                                       int hi, int part, bool whole, uint64_t mine, uint64_t live) {
   constexpr int ST = HD + 4;  // floats of a column in LDS
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = lane >> 4, col = lane & 15;
@@ -313,7 +314,7 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
     if (whole) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a sum that is no number stays none)
       *(f16x4*)(a.o + head * HD + d) = (f16x4){(f16)(v[0] * inv), (f16)(v[1] * inv), (f16)(v[2] * inv), (f16)(v[3] * inv)};
-    } else {
+    } else if (mine >> (row - row0) & 1) {
       const long pi = head * a.parts + part;
       M = !(live >> (row - row0) & 1) ? -INFINITY : l == l ? M : l;
       if (d == 0) {
@@ -343,12 +344,14 @@ __global__ __launch_bounds__(64 * W, HD > 128 ? 1 : 2) void paged_attn_kernel(Pa
   if ((int)blockIdx.x < a.nitems) {
     const int* it = a.items + 6 * blockIdx.x;
     const int row0 = it[0], n = it[1], lo = max(it[2], 0), hi = min(it[3], a.MP << a.PS), kh = it[5];
-    if (row0 < 0 || n < 1 || n * a.G > 16 * CT || row0 + n > a.R || kh < 0 || kh >= a.Hk || it[4] < 0 || it[4] >= a.parts) return;
-    // the first row that attends the whole prefix leads: its pages hold every shared slot
+    if (row0 < 0 || n < 1 || n > 16 * CT / a.G || row0 > a.R - n || kh < 0 || kh >= a.Hk || it[4] < 0 || it[4] >= a.parts - a.nown) return;
+    // the first row that attends the whole prefix leads: its pages hold every shared slot.  The places of a row behind its
+    // shared parts are those of its own slots: a part number that is not below the row's count is not for it.
     const int r = row0 + min(lane, n - 1);
-    const uint64_t live = __ballot(lane < n && attended(a, r) >= a.rows[2 * r]);
+    const uint64_t mine = __ballot(lane < n && it[4] < a.rows[2 * r + 1]);
+    const uint64_t live = mine & __ballot(lane < n && attended(a, r) >= a.rows[2 * r]);
     const int* tab = a.table + (long)((row0 + (live ? __builtin_ctzll(live) : 0)) / a.S) * a.ldt;
-    attend<HD, CT, W>(a, lds, row0, n * a.G, kh, tab, lo, live ? hi : lo, it[4], false, live);
+    attend<HD, CT, W>(a, lds, row0, n * a.G, kh, tab, lo, live ? hi : lo, it[4], false, mine, live);
     return;
   }
   const int x = blockIdx.x - a.nitems, u = x / a.Hk, kh = x - u * a.Hk, r = u / a.nown, k = u - r * a.nown;
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(64 * W, HD > 128 ? 1 : 2) void paged_attn_kernel(Pa
   const int from = end >= shared ? shared : 0;
   const int per = (max(W * PQ_T, (end - from + a.nown - 1) / a.nown) + PQ_T - 1) & ~(PQ_T - 1);
   const int lo = min(from + k * per, end), hi = min(lo + per, end);
-  attend<HD, 1, W>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1, ~0ull);
+  attend<HD, 1, W>(a, lds, r, a.G, kh, a.table + (long)(r / a.S) * a.ldt, lo, hi, np + k, np + a.nown == 1, ~0ull, ~0ull);
 }
 
 // The parts of a head to one output: one thread per four dims, JB parts at a time, all their loads at once (one after the other
@@ -418,7 +421,7 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
                               const int64_t* pos, void* o, float* ws, const int32_t* items, const int32_t* rows,
                               int nitems, int nown, int parts, int ctiles, int waves, int R, int S, int MP, int NP, int Hq, int Hk,
                               int P, int HD, float scale, void* stream) {
-  if (!q || !kp || !vp || !table || !pos || !o || !rows || (nitems > 0 && !items) || nitems < 0 || nown < 1 ||
+  if (!q || !kp || !vp || !table || !pos || !o || !rows || (nitems > 0 && (!items || parts <= nown)) || nitems < 0 || nown < 1 ||
       parts < nown || (parts > 1 && !ws) || R <= 0 || S <= 0 || MP <= 0 || NP <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
       Hq / Hk > 16 || P < 16 || (P & (P - 1)) || ldt < MP || ldq < (long)Hq * HD || (ldq % 8) ||
       ((uintptr_t)q & 15) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)o & 7) || ((uintptr_t)ws & 15) ||

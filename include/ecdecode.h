@@ -652,9 +652,10 @@ int ecd_paged_write(const void* qkv, long ld, const float* rope, int LR, const i
  *   Hq / Hk <= 16; MP P <= 2^30.
  *   rows [R, 2] int32: shared slots and number of shared parts of each row; items [nitems, 6] int32: first row, rows (at
  *   most 16 ctiles / (Hq / Hk)), first slot, last slot + 1, part number and kv head of each shared part; nown: parts of
- *   each row's own slots; parts: the most parts of any row (<= 512); ctiles 1 or 2 with waves 4, or 1 with
- *   waves 8, of a workgroup (HD 256: 1 with 4).  A row that does not
- *   attend all shared slots takes none of the shared parts and attends its own slots from 0.
+ *   each row's own slots; parts: the most parts of any row (<= 512; more than nown where there are items); ctiles 1 or 2
+ *   with waves 4, or 1 with waves 8, of a workgroup (HD 256: 1 with 4).  A row that does not attend all shared slots takes
+ *   none of the shared parts and attends its own slots from 0.  An item whose rows, head or part number is out of range is
+ *   skipped, and so is a row of an item whose part number is not below the row's number of shared parts.
  *   ws: fp32 workspace of 2 ceil4(R Hq parts) + R Hq parts HD values (any contents; NULL where parts is 1). */
 int ecd_paged_attn(const void* q, long ldq, const void* kp, const void* vp, const int32_t* table, long ldt,
                    const int64_t* pos, void* o, float* ws, const int32_t* items, const int32_t* rows, int nitems,
