@@ -434,11 +434,13 @@ __global__ __launch_bounds__(64 * WN * WM * KG, 1) void gemm_a8_kernel(const int
   });
 }
 
+constexpr long THREADS_MOST = 0xFFFFFFFFL;  // of a launch along x
+
 template <bool SILU, int WN, int WM, int FT, int RT, int NS, int KG>
 static int launch_tile(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
   using T = A8Tile<WN, WM, FT, RT, NS, KG>;
   const int nfb = (N + T::BN - 1) / T::BN, nmb = (M + T::BM - 1) / T::BM;
-  if ((long)nfb * nmb > 0x7FFFFFFFL) return ECD_ENOTSUP;
+  if ((long)nfb * nmb > THREADS_MOST / T::THREADS) return ECD_ENOTSUP;
   hipLaunchKernelGGL((gemm_a8_kernel<SILU, WN, WM, FT, RT, NS, KG>), dim3((unsigned)(nfb * nmb)), dim3(T::THREADS), 0, st, c, ldc, wp, out,
                      M, N, K, nfb, nmb);
   return ecd_launch_status();
@@ -446,7 +448,7 @@ static int launch_tile(const int8_t* c, long ldc, const int8_t* wp, const A8Out&
 
 template <bool SILU>
 static int launch_few(const int8_t* c, long ldc, const int8_t* wp, const A8Out& out, int M, int N, int K, hipStream_t st) {
-  if ((M + 15) / 16 > 65535) return ECD_ENOTSUP;
+  if ((M + 15) / 16 > 65535 || (N + 15) / 16 > THREADS_MOST / (64 * FEW_W)) return ECD_ENOTSUP;
   hipLaunchKernelGGL(gemm_a8_few_kernel<SILU>, dim3((N + 15) / 16, (M + 15) / 16), dim3(64 * FEW_W), 0, st, c, ldc, wp, out, M, N, K);
   return ecd_launch_status();
 }
@@ -492,6 +494,7 @@ static int a8_choice(int M, int N, int K) {
 
 template <bool SILU>
 static int launch_a8(const void* cv, long ldc, const void* wv, const A8Out& out, int M, int N, int K, hipStream_t st, int cfg = 0) {
+  if (M > 1 << 30 || N > 1 << 30) return ECD_ENOTSUP;  // (row and feature numbers of a tile are 32-bit)
   const int8_t *c = (const int8_t*)cv, *wp = (const int8_t*)wv;
 #define A8_TILE(...) return launch_tile<SILU, __VA_ARGS__>(c, ldc, wp, out, M, N, K, st)
   switch (cfg ? cfg : a8_choice(M, N, K)) {

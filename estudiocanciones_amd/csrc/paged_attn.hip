@@ -426,7 +426,7 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
       Hq / Hk > 16 || P < 16 || (P & (P - 1)) || ldt < MP || ldq < (long)Hq * HD || (ldq % 8) ||
       ((uintptr_t)q & 15) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)o & 7) || ((uintptr_t)ws & 15) ||
       !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown * Hk + nitems > 0x7FFFFFL || (long)R * Hq > 0x7FFFFFFFL / 64 ||
-      (long)NP * Hk * P > 0xFFFFFFFFL)
+      (long)NP * P > 0xFFFFFFFFL || (long)NP * P * Hk > 0xFFFFFFFFL)
     return ECD_EINVAL;
   if ((HD != 64 && HD != 128 && HD != 256) || parts > 512) return ECD_ENOTSUP;
   const long heads = (long)R * Hq, n2 = (heads * parts + 3) & ~3l;

@@ -329,6 +329,7 @@ static bool pool_ok(int planes, int NP, int Hk, int P, int HD) {
   return planes > 0 && NP > 0 && Hk > 0 && P > 0 && HD > 0 && HD % 8 == 0;
 }
 constexpr long GRID_MOST = 0xFFFFFF;  // workgroups of 256 along x: a launch has fewer than 2^32 threads there
+constexpr int COUNT_MOST = 1 << 30;   // pages of a pool or a sequence: loops count them in 32 bits, PG_T at a time
 static bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace ecd
@@ -340,7 +341,7 @@ extern "C" {
 int ecd_page_free(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B, int P, const int32_t* seqs,
                   int n, int32_t* err, void* stream) {
   if (!ref || !table || !length || !seqs || !err || NP <= 0 || MP <= 0 || B <= 0 || P <= 0 || n <= 0) return ECD_EINVAL;
-  if (n > GRID_MOST) return ECD_ENOTSUP;
+  if (n > GRID_MOST || NP > COUNT_MOST || MP > COUNT_MOST) return ECD_ENOTSUP;
   hipLaunchKernelGGL(page_free_kernel, dim3(n), dim3(256), 0, (hipStream_t)stream, ref, NP, table, MP, length, B, P,
                      seqs, err);
   return ecd_launch_status();
@@ -353,7 +354,10 @@ int ecd_page_fork(void* kv, int32_t* ref, int NP, int32_t* table, int MP, int64_
       !pool_ok(planes, NP, Hk, P, HD) || !a16(kv) || !a16(plan))
     return ECD_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
-  const long pieces = ((long)P * HD / 8 + 256 * FORK_V - 1) / (256 * FORK_V), x = pieces * planes * Hk + 1;
+  const long pieces = ((long)P * HD / 8 + 256 * FORK_V - 1) / (256 * FORK_V), runs = (long)planes * Hk;
+  if (runs >= GRID_MOST || pieces > GRID_MOST / runs || (long)P * HD > 8L * COUNT_MOST || NP > COUNT_MOST || MP > COUNT_MOST)
+    return ECD_ENOTSUP;
+  const long x = pieces * runs + 1;
   if (x > GRID_MOST) return ECD_ENOTSUP;
   hipLaunchKernelGGL(page_fork_plan_kernel, dim3(1), dim3(PG_T), 0, st, ref, NP, table, MP, length, B, P, src, dst, n,
                      plan, err);
@@ -365,7 +369,8 @@ int ecd_page_fork(void* kv, int32_t* ref, int NP, int32_t* table, int MP, int64_
 int ecd_page_extend(int32_t* ref, int NP, int32_t* table, int MP, int64_t* length, int B, int P, const int64_t* pos,
                     int32_t* err, void* stream) {
   if (!ref || !table || !length || !pos || !err || NP <= 0 || MP <= 0 || B <= 0 || B > PG_T || P <= 0) return ECD_EINVAL;
-  if ((long)B * MP > 0xFFFFFFFFL) return ECD_ENOTSUP;  // (new pages are counted in 32 bits)
+  // (new pages are counted in 32 bits)
+  if ((long)B * MP > 0xFFFFFFFFL || NP > COUNT_MOST || MP > COUNT_MOST) return ECD_ENOTSUP;
   hipLaunchKernelGGL(page_extend_kernel, dim3(1), dim3(PG_T), 0, (hipStream_t)stream, ref, NP, table, MP, length, B, P,
                      pos, err);
   return ecd_launch_status();
@@ -377,6 +382,7 @@ int ecd_page_compact(const void* kv, const int32_t* ref, int NP, const int32_t* 
   if (!kv || !ref || !table || !length || !kv2 || !ref2 || !table2 || !length2 || !ws || !err || B <= 0 || MP <= 0 ||
       NP2 <= 0 || !pool_ok(planes, NP, Hk, P, HD) || !a16(kv) || !a16(kv2) || kv == kv2)
     return ECD_EINVAL;
+  if (NP > COUNT_MOST || NP2 > COUNT_MOST || MP > COUNT_MOST) return ECD_ENOTSUP;
   const hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(page_compact_plan_kernel, dim3(1), dim3(PG_T), 0, st, ref, NP, ref2, NP2, ws, err);
   hipLaunchKernelGGL(page_compact_kernel, dim3(4096), dim3(256), 0, st, (const f16*)kv, NP, (f16*)kv2, NP2, table,
@@ -388,11 +394,12 @@ int ecd_paged_write(const void* qkv, long ld, const float* rope, int LR, const i
                     void* vp, const int32_t* table, long ldt, int MP, int NP, int M, int S, int Hq, int Hk, int P,
                     int HD, void* stream) {
   if (!qkv || !pos || !kp || !vp || !table || (rope && (!q || LR <= 0)) || M <= 0 || S <= 0 || Hq <= 0 || MP <= 0 ||
-      ldt < MP || !pool_ok(1, NP, Hk, P, HD) || ld < (long)(Hq + 2 * Hk) * HD || (ld % 8) || !a16(qkv) || !a16(kp) ||
+      ldt < MP || !pool_ok(1, NP, Hk, P, HD) || ld < (Hq + 2L * Hk) * HD || (ld % 8) || !a16(qkv) || !a16(kp) ||
       !a16(vp) || (q && !a16(q)) || ((uintptr_t)rope & 15))
     return ECD_EINVAL;
-  const long W = (long)(rope ? Hq + 2 * Hk : 2 * Hk) * (HD / 8), blocks = (M * W + 255) / 256;
-  if (W > 0x7FFFFFFFL || blocks > GRID_MOST) return ECD_ENOTSUP;
+  const long W = (rope ? Hq + 2L * Hk : 2L * Hk) * (HD / 8);
+  if (W > 0x7FFFFFFFL || (M * W + 255) / 256 > GRID_MOST) return ECD_ENOTSUP;
+  const long blocks = (M * W + 255) / 256;
   const hipStream_t st = (hipStream_t)stream;
 #define PW(R_)                                                                                                        \
   hipLaunchKernelGGL((paged_write_kernel<R_>), dim3((unsigned)blocks), dim3(256), 0, st, (const f16*)qkv, ld, rope,    \

@@ -611,7 +611,8 @@ int ecd_copy_bytes(const void* src, void* dst, long nbytes, void* stream);
  *     1 a sequence or page number out of range, 2 the target of a fork holds slots or is named twice,
  *     4 no free page, 8 a slot or length beyond the table, 16 the other pool is too small.
  * Such a call changes nothing but err (ecd_page_free skips the numbers out of range).  Free pages are taken lowest number
- * first, in the order of the call's sequences.  Calls on one state have to be ordered (one stream, or events). */
+ * first, in the order of the call's sequences.  Calls on one state have to be ordered (one stream, or events).  At most
+ * 2^30 pages of a pool or a sequence. */
 
 /* The n sequences of seqs give their pages back (a page is free once its last owner has); a sequence named twice is
  * freed once.  Their table rows become -1, their lengths 0. */
@@ -669,7 +670,8 @@ int ecd_quant_a8(const void* x, long ldx, const void* nw, float eps, void* c, lo
                  void* stream);
 
 /* y[m, n] = f16(sx[m] s[n] sum_k c[m, k] q[n, k] (+ res[m, n])) with weights packed by ecd_pack_i8: the sum is an
- * integer, one rounding at the end.  c as from ecd_quant_a8: ldc % 128 == 0, at most 2^23; columns from K on are not read. */
+ * integer, one rounding at the end.  c as from ecd_quant_a8: ldc % 128 == 0, at most 2^23; columns from K on are not read.
+ * M and N at most 2^30. */
 int ecd_gemm_a8(const void* c, long ldc, const float* sx, const void* wp, const void* s, const void* res, long ldr,
                 void* y, long ldy, int M, int N, int K, void* stream);
 

@@ -15,3 +15,50 @@ def test_shared_parts_need_places_of_their_own(nitems, nown, parts, ws):
     workspace that is not there."""
     from estudiocanciones_amd import _ffi
     assert _attn(_ffi.lib(), nitems, nown, parts, ws) == I
+
+
+BIG = 2 ** 31 - 1
+
+
+def _a8(L, M, N, cfg=0):
+    return L.ecd_gemm_a8_tuned(16, 128, 16, 16, 16, None, 0, 16, N, M, N, 64, cfg, None)
+
+
+@pytest.mark.parametrize("call", [
+    # 2^32 threads of a launch: 16 features of 512 threads, tiles of 256 and 512 threads
+    lambda L: L.ecd_gemm_a8(16, 128, 16, 16, 16, None, 0, 16, 1 << 27, 1, 1 << 27, 64, None),
+    lambda L: L.ecd_gemm_a8_silu(16, 128, 16, 16, 16, 16, 1 << 26, 1, 1 << 26, 64, None),
+    lambda L: _a8(L, 1 << 30, 32, 2), lambda L: _a8(L, 1 << 29, 64, 3), lambda L: _a8(L, 64, 1 << 30, 4),
+    lambda L: _a8(L, 1 << 29, 256, 5), lambda L: _a8(L, 1 << 28, 1024, 6), lambda L: _a8(L, 1 << 28, 4096, 7),
+    lambda L: _a8(L, 1 << 28, 2048, 8), lambda L: _a8(L, 1, 1 << 27, 1),
+    # row and feature numbers that pass 32 bits within a tile
+    lambda L: _a8(L, BIG, 256, 8), lambda L: _a8(L, 256, BIG, 8), lambda L: _a8(L, 1, BIG, 1), lambda L: _a8(L, BIG, 16),
+    # page numbers and table columns that are counted in 32 bits, a workgroup's step at a time
+    lambda L: L.ecd_page_free(8, BIG, 8, 4, 8, 2, 16, 8, 1, 8, None),
+    lambda L: L.ecd_page_free(8, 4, 8, BIG, 8, 2, 16, 8, 1, 8, None),
+    lambda L: L.ecd_page_extend(8, BIG, 8, 4, 8, 2, 16, 8, 8, None),
+    lambda L: L.ecd_page_extend(8, 4, 8, BIG, 8, 1, 16, 8, 8, None),
+    lambda L: L.ecd_page_fork(16, 8, BIG, 8, 4, 8, 2, 8, 8, 1, 16, 8, 2, 1, 16, 64, None),
+    lambda L: L.ecd_page_fork(16, 8, 4, 8, BIG, 8, 2, 8, 8, 1, 16, 8, 2, 1, 16, 64, None),
+    lambda L: L.ecd_page_compact(16, 8, BIG, 8, 8, 32, 8, 9, 8, 8, 2, 4, 8, 8, 2, 1, 16, 64, None),
+    lambda L: L.ecd_page_compact(16, 8, 4, 8, 8, 32, 8, BIG, 8, 8, 2, 4, 8, 8, 2, 1, 16, 64, None),
+    lambda L: L.ecd_page_compact(16, 8, 4, 8, 8, 32, 8, 9, 8, 8, 2, BIG, 8, 8, 2, 1, 16, 64, None),
+    # pages of 2^34 values: their pieces pass 32 bits
+    lambda L: L.ecd_page_fork(16, 8, 4, 8, 4, 8, 2, 8, 8, 1, 16, 8, 2, 1, 1 << 28, 64, None),
+    # products of sizes that pass 64 bits
+    lambda L: L.ecd_page_fork(16, 8, 4, 8, 4, 8, 2, 8, 8, 1, 16, 8, 1 << 30, 1 << 30, 16, 2048, None),
+])
+def test_sizes_that_the_kernels_do_not_count(call):
+    from estudiocanciones_amd import _ffi
+    assert call(_ffi.lib()) == N
+
+
+@pytest.mark.parametrize("call", [
+    # 2^30 + 2 2^30 heads are not -2^30
+    lambda L: L.ecd_paged_write(16, 512, None, 0, 8, None, 16, 16, 8, 4, 4, 4, 1, 1, 1 << 30, 1 << 30, 16, 64, None),
+    # 2^31 pages of 2^30 slots and 8 heads are not 0 rows of the pool
+    lambda L: L.ecd_paged_attn(16, 2048, 16, 16, 8, 1, 8, 8, None, 8, 8, 0, 1, 1, 1, 4, 1, 1, 1, 1 << 30, 16, 16, 1 << 30, 128, 0.1, None),
+])
+def test_sizes_whose_products_pass_64_bits(call):
+    from estudiocanciones_amd import _ffi
+    assert call(_ffi.lib()) in (I, N)
