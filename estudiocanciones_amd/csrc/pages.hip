@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void page_free_kernel(int* __restrict__ ref, i
 }
 
 // One workgroup, which sees every refusal before anything is changed: a thread per child finds what it needs, then all look
-// for free pages, PG_T at a time.  Bound by latency (3.8 us for 2 children, 4.4 for 32 of 3540 pages).
+// at the sources' pages and for free ones, PG_T at a time.  Bound by latency (3.8 us for 2 children, 4.4 for 32 of 3540 pages).
 // plan[i] = {page of the source's partial slots, page for them, their number, whole pages shared (-1: nothing to do)}
 __global__ __launch_bounds__(PG_T) void page_fork_plan_kernel(const int* __restrict__ ref, int NP,
                                                               const int* __restrict__ table, int MP,
@@ -81,16 +81,17 @@ __global__ __launch_bounds__(PG_T) void page_fork_plan_kernel(const int* __restr
                                                               const int* __restrict__ src, const int* __restrict__ dst,
                                                               int n, int* __restrict__ plan, int* __restrict__ err) {
   __shared__ uint32_t wsum[PG_W];
-  __shared__ int s_dst[PG_T], s_page[PG_T];
+  __shared__ int s_dst[PG_T], s_page[PG_T], s_src[PG_T], s_full[PG_T];
   __shared__ int s_err;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, lane = t & 63;
   if (t == 0) s_err = 0;
   s_dst[t] = t < n ? dst[t] : -1;
+  s_src[t] = t < n ? src[t] : -1;
   __syncthreads();
   int bad = 0, full = 0, tail = 0, from = 0;
   long len = 0;
   if (t < n) {
-    const int s = src[t], d = s_dst[t];
+    const int s = s_src[t], d = s_dst[t];
     if (s < 0 || s >= B || d < 0 || d >= B) {
       bad = PAGE_E_INDEX;
     } else {
@@ -111,8 +112,16 @@ __global__ __launch_bounds__(PG_T) void page_fork_plan_kernel(const int* __restr
     }
     if (bad) atomicOr(&s_err, bad);
   }
+  s_full[t] = full;
   uint32_t want;
-  const uint32_t k = block_excl_add(tail > 0, wsum, want);
+  const uint32_t k = block_excl_add(tail > 0, wsum, want);  // (its barriers: s_full whole)
+  // the whole pages of each source, a wave per child; children that follow one another share the look at theirs
+  for (int i = t >> 6; i < n; i += PG_W)
+    if (i == 0 || s_src[i] != s_src[i - 1])
+      for (int j = lane; j < s_full[i]; j += 64) {
+        const int p = table[(long)s_src[i] * MP + j];
+        if (p < 0 || p >= NP) atomicOr(&s_err, PAGE_E_INDEX);
+      }
   const uint32_t got = free_pages(ref, NP, want, wsum, [&](uint32_t r, int p) { s_page[r] = p; });
   __syncthreads();  // s_page and s_err whole
   const int e = s_err | (got < want ? PAGE_E_FULL : 0);

@@ -608,9 +608,10 @@ int ecd_copy_bytes(const void* src, void* dst, long nbytes, void* stream);
  *   kv [planes, NP, Hk, P, HD] f16: NP pages of P slots in each plane (layer by layer, keys then values);
  *   ref [NP] int32 owners of each page (0: free); table [B, MP] int32: page of slots j P .. of each sequence, -1 behind
  *   its last one; length [B] int64 slots held; err [1] int32, bits set by a call that cannot be done:
- *     1 a sequence or page number out of range, 2 the target of a fork holds slots or is named twice,
- *     4 no free page, 8 a slot or length beyond the table, 16 the other pool is too small.
- * Such a call changes nothing but err (ecd_page_free skips the numbers out of range).  Free pages are taken lowest number
+ *     1 a sequence number out of range, or the number of a page that a fork shares or copies, 2 the target of a fork
+ *     holds slots or is named twice, 4 no free page, 8 a slot or length beyond the table, 16 the other pool is too small.
+ * Such a call changes nothing but err (ecd_page_free skips the numbers out of range; a table entry that is no page in use is
+ * skipped by it and becomes -1 in a compaction).  Free pages are taken lowest number
  * first, in the order of the call's sequences.  Calls on one state have to be ordered (one stream, or events).  At most
  * 2^30 pages of a pool or a sequence. */
 

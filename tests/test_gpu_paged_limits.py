@@ -34,3 +34,63 @@ def test_shared_parts_out_of_range_are_skipped(dev):
     want = paged_attn(q, kv[0], kv[1], table, pos, plan)
     for _ in range(3):
         assert torch.equal(paged_attn(q, kv[0], kv[1], table, pos, more), want)
+
+
+def _pool(dev, pages=9, B=6, MP=4, P=16):
+    from test_gpu_pages import Model, State
+    st = State(dev, 2, pages, 1, P, 8, B, MP)
+    m = Model(st.np.view(np.uint16), B, MP)
+    pos = [40, 31] + [-1] * (B - 2)  # three pages, the last one partial; two whole pages
+    m.extend(pos)
+    st.extend(pos)
+    return st, m
+
+
+@pytest.mark.parametrize("bad", [-1, -7, 9, 2 ** 31 - 1])
+@pytest.mark.parametrize("seq,col", [(0, 0), (0, 1), (0, 2), (1, 0), (1, 1)])
+def test_fork_reports_a_page_number_out_of_range(dev, bad, seq, col):
+    """Among the whole pages as well as the partial one: bit 1, and nothing else changes, for the good source's child neither."""
+    st, m = _pool(dev)
+    st.table[seq, col] = bad
+    m.table[seq][col] = bad
+    st.fork([1 - seq, seq], [2, 3])
+    st.same(m, "two sources", 1)
+    st.err.zero_()
+    st.fork([seq] * 3, [4, 2, 5])
+    st.same(m, "one source", 1)
+    st.err.zero_()
+    st.fork([1 - seq], [3])  # the other one is as good as before
+    m.fork([1 - seq], [3])
+    st.same(m, "the good one")
+
+
+def test_fork_looks_at_all_pages_of_many_children(dev):
+    """A bad page behind 200 good ones, of the last of 1000 children, whose sources do not repeat in a row."""
+    st, m = _pool(dev, pages=1600, B=1024, MP=260, P=16)
+    pos = [-1, -1] + [16 * 203 - 1] * 3 + [-1] * 1019  # whole pages only
+    m.extend(pos)
+    st.extend(pos)
+    src, dst = [2 + i % 2 for i in range(1000)], list(range(24, 1024))
+    src[-1] = 4
+    st.table[4, 202] = 1600
+    m.table[4][202] = 1600
+    st.fork(src, dst)
+    st.same(m, "bad", 1)
+    st.err.zero_()
+    src[-1] = 3
+    m.fork(src, dst)
+    st.fork(src, dst)
+    st.same(m, "good")
+
+
+def test_fork_without_enough_pages_changes_nothing(dev):
+    """Four pages are free: five children with a partial page each get bit 4 alone, four of them are made."""
+    st, m = _pool(dev, B=8)
+    st.fork([0, 1, 0, 0, 0, 0], [2, 3, 4, 5, 6, 7])
+    st.same(m, "five partial pages", 4)
+    st.err.zero_()
+    m.fork([0, 1, 0, 0, 0], [2, 3, 4, 5, 6])
+    st.fork([0, 1, 0, 0, 0], [2, 3, 4, 5, 6])
+    st.same(m, "four partial pages")
+    st.fork([0], [7])
+    st.same(m, "none is left", 4)
