@@ -61,6 +61,7 @@ FRAME_MS = 80
 ATT_SHORT = 128      # caches of at most this many slots: one attention split per (row, kv head)
 ATT_WG = 256        # workgroups the merged attention grid aims at (one per CU of an MI355X)
 ATT_KB_MAX = 16     # workgroups per (row, kv head) pair at most (the last one merges them all)
+GRID_Z = 65535      # workgroups of a launch along its third dimension
 STACK_MAX = 64      # layers of one ecd_layer_stack launch at most
 PAGE = 64           # slots of a page of the backbone's paged cache
 DECODER_RESIDENT = 160 << 20  # weight bytes of a decoder pass kept in the 256 MB Infinity Cache
@@ -453,8 +454,14 @@ class Stack:
         if HD in (64, 128) and Hq // Hk <= 4:
             return prefill_attn(q, kc, vc, pos, S, Hq, Hk)
         o = torch.empty_like(q)
-        _ffi.call("ecd_decode_attn", q.data_ptr(), kc.data_ptr(), vc.data_ptr(), pos.data_ptr(), o.data_ptr(), None,
-                  None, None, q.shape[0], S, Hq, Hk, L, HD, 1, 1.0 / math.sqrt(HD), stream_ptr(q.device))
+        # a row per workgroup along the third grid dimension: whole sequences of up to GRID_Z rows, or parts of a longer one
+        R, per = q.shape[0], S if S > GRID_Z else GRID_Z // S * S
+        for a in range(0, R, per):
+            k, v = kc[a // S:].data_ptr(), vc[a // S:].data_ptr()
+            for r in range(a, min(a + per, R), GRID_Z):
+                n = min(GRID_Z, a + per - r, R - r)
+                _ffi.call("ecd_decode_attn", q[r:].data_ptr(), k, v, pos[r:].data_ptr(), o[r:].data_ptr(), None, None, None,
+                          n, min(S, GRID_Z), Hq, Hk, L, HD, 1, 1.0 / math.sqrt(HD), stream_ptr(q.device))
         return o
 
     @staticmethod

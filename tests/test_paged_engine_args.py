@@ -1,0 +1,61 @@
+"""What the engine's paged and int8-activation paths refuse before they touch a cache: host logic, no GPU."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from estudiocanciones_amd import engine
+
+
+def _stack(heads=2, kv=1, dim=256, packed=True):
+    """A stack of one layer whose weights are names only."""
+    lin = lambda: SimpleNamespace(qp=object() if packed else None)  # noqa: E731
+    st = object.__new__(engine.Stack)
+    b = SimpleNamespace(qkv=lin(), o=lin(), w13=lin(), w2=lin(), h=heads, kvh=kv, hd=dim // heads, kc=None, vc=None)
+    st.blocks, st.dim, st.hd, st.rope, st.prompt_a8 = [b], dim, dim // heads, None, False
+    st.tail = st.tail2 = st.att_ws = st.att_cnt = st.paged = st.paged_plan = None
+    return st
+
+
+def _no_gpu(monkeypatch):
+    def call(name, *_):
+        raise AssertionError(f"{name} was launched")
+    monkeypatch.setattr(engine._ffi, "call", call)
+
+
+@pytest.mark.parametrize("B,S", [(3, 7), (66000, 1), (700, 100), (2, 40000), (1, 70000), (65535, 1), (65536, 1), (3, 65536)])
+def test_prompt_attention_by_rows_stays_within_a_launch(monkeypatch, B, S):
+    """Head shapes without a prompt kernel take a row per workgroup along the third grid dimension, which ends at 65536:
+    every row exactly once, with its own sequence's cache."""
+    Hq, Hk, HD, L = 6, 1, 128, 4
+    rows, seen = B * S, torch.zeros(B * S, dtype=torch.long)
+    st, calls = _stack(6, 1, 768), []
+
+    class At:  # (its pointers are fictions: only offsets are looked at)
+        def __init__(self, base, step, shape, i0=0):
+            self.base, self.step, self.shape, self.i0, self.device, self.dtype = base, step, shape, i0, "cpu", torch.float16
+
+        def data_ptr(self):
+            return self.base + self.step * self.i0
+
+        def __getitem__(self, s):
+            a, b, _ = s.indices(self.shape[0])
+            return At(self.base, self.step, (b - a,) + tuple(self.shape[1:]), self.i0 + a)
+
+    monkeypatch.setattr(engine._ffi, "call", lambda name, *a: calls.append((name, a)))
+    monkeypatch.setattr(engine, "stream_ptr", lambda d: 0)
+    out = At(3 << 40, Hq * HD * 2, (rows, Hq * HD))
+    monkeypatch.setattr(engine.torch, "empty_like", lambda t: out)
+    q, pos = At(1 << 40, Hq * HD * 2, (rows, Hq * HD)), At(2 << 40, 8, (rows,))
+    kc, vc = At(4 << 40, Hk * L * HD * 2, (B, Hk, L, HD)), At(5 << 40, Hk * L * HD * 2, (B, Hk, L, HD))
+    assert st._prompt_attn(st.blocks[0], q, kc, vc, pos, S) is out
+    for name, a in calls:
+        assert name == "ecd_decode_attn"
+        qp, kp, vp, pp, op, _, _, _, R, s, hq, hk, l, hd, ns, scale, _ = a
+        assert 0 < R <= 65535 and (hq, hk, l, hd, ns) == (Hq, Hk, L, HD, 1) and scale == pytest.approx(HD ** -0.5)
+        r0, b0 = (qp - (1 << 40)) // (Hq * HD * 2), (kp - (4 << 40)) // (Hk * L * HD * 2)
+        assert (pp - (2 << 40)) // 8 == r0 == (op - (3 << 40)) // (Hq * HD * 2) and (vp - (5 << 40)) // (Hk * L * HD * 2) == b0
+        for r in (0, R // 2, R - 1):  # (the kernel's own sequence number of a row)
+            assert b0 + r // s == (r0 + r) // S
+        seen[r0:r0 + R] += 1
+    assert (seen == 1).all()
