@@ -284,6 +284,15 @@ class Stack:
         """Whether every layer's weights are packed (what the paged cache and int8 activations need)."""
         return bool(self.blocks) and all(lin.qp is not None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2))
 
+    def _dense(self, call):
+        if self.paged is not None:
+            raise RuntimeError(f"Stack.{call}: the cache is in pages (alloc_paged): prompt_paged and decode_paged run on it")
+
+    def _pages(self, call):
+        if self.paged is None:
+            raise RuntimeError(f"Stack.{call}: there is no cache in pages (alloc_paged)")
+        return self.paged
+
     def alloc_paged(self, seqs, pages, max_pages, dev, groups, page=64):
         """A cache in pages instead of the dense ones, for one row per sequence: ``groups`` lists (rows, shared slots) of
         consecutive sequences that share a prompt (the plan of paged_attn)."""
@@ -407,6 +416,7 @@ class Stack:
         [0, pos[b, s]], which is the causal mask of the reference's SDPA call."""
         if mask is not None:
             raise NotImplementedError("explicit attention masks are not part of the fast path")
+        self._dense("__call__")
         B, S, D = x.shape
         x2 = x.reshape(B * S, D)
         p2 = pos.reshape(B * S).to(torch.int64).contiguous()
@@ -487,7 +497,9 @@ class Stack:
         """Prompt pass into the cache in pages: x [U, S, D], prompt u at slots 0 .. S - 1 of sequence seqs[u] (int64
         tensor), which holds nothing yet.  Returns the last row's hidden state [U, D] (after the stack's norm)."""
         U, S, D = x.shape
-        dev, cache = x.device, self.paged
+        dev, cache = x.device, self._pages("prompt_paged")
+        if S > cache.table.shape[1] * cache.page:
+            raise ValueError(f"Stack.prompt_paged: a sequence holds {cache.table.shape[1] * cache.page} slots, the prompt {S}")
         last = torch.full_like(cache.length, -1)
         last[seqs] = S - 1
         cache.extend(last)
@@ -519,7 +531,7 @@ class Stack:
     def decode_paged(self, x, pos, final_norm=True):
         """A decode step over the cache in pages: x [R, D], row r at slot pos[r] of sequence r (R: all sequences).  The
         slot's page is taken if it is not there yet, the step may be repeated (a capture's warm-up) and captured."""
-        cache = self.paged
+        cache = self._pages("decode_paged")
         cache.extend(pos)
         for i, b in enumerate(self.blocks):
             kp, vp = cache.layer(i)
@@ -542,6 +554,7 @@ class Stack:
         consumer that fuses that norm into its own GEMV (the codebook heads).  ``o0``: layer 0's
         attention output, its q|k|v, RoPE and cache slot already done (by the depth decoder's
         sampler); the step then starts at layer 0's O projection."""
+        self._dense("decode")
         if any(b.qkv.qp is None for b in self.blocks):
             h = self.decode_reference(x, pos, S)
             return h if final_norm else None
@@ -650,6 +663,7 @@ class Stack:
         """The reference's launch sequence (app/engine.py:180-211) through the drop-in kernel
         entry points of kernels.py (unpacked weights, one launch per reference kernel, the
         reference's attention grid and split count)."""
+        self._dense("decode_reference")
         R = x.shape[0]
         for b in self.blocks:
             Hq, Hk, HD, L = b.h, b.kvh, b.hd, b.kc.shape[2]

@@ -23,6 +23,34 @@ def _no_gpu(monkeypatch):
     monkeypatch.setattr(engine._ffi, "call", call)
 
 
+@pytest.mark.parametrize("call", ["__call__", "decode", "decode_reference"])
+@pytest.mark.parametrize("packed", [True, False])
+def test_a_stack_in_pages_refuses_the_dense_calls(monkeypatch, call, packed):
+    _no_gpu(monkeypatch)
+    st = _stack(packed=packed)
+    st.paged = SimpleNamespace()
+    x, pos = torch.zeros(1, 3, 256, dtype=torch.float16), torch.arange(3)[None]
+    with pytest.raises(RuntimeError, match="in pages"):
+        st(x, pos) if call == "__call__" else getattr(st, call)(x[0], pos[0], 3)
+
+
+def test_a_stack_without_pages_refuses_the_paged_calls(monkeypatch):
+    _no_gpu(monkeypatch)
+    st = _stack()
+    with pytest.raises(RuntimeError, match="alloc_paged"):
+        st.decode_paged(torch.zeros(3, 256, dtype=torch.float16), torch.arange(3))
+    with pytest.raises(RuntimeError, match="alloc_paged"):
+        st.prompt_paged(torch.zeros(1, 3, 256, dtype=torch.float16), torch.tensor([0]))
+
+
+def test_a_prompt_longer_than_the_table_is_refused_before_it_takes_pages(monkeypatch):
+    _no_gpu(monkeypatch)
+    st = _stack()
+    st.paged = SimpleNamespace(table=torch.zeros(2, 3, dtype=torch.int32), page=16, length=torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError, match="48 slots"):
+        st.prompt_paged(torch.zeros(1, 49, 256, dtype=torch.float16), torch.tensor([0]))
+
+
 @pytest.mark.parametrize("B,S", [(3, 7), (66000, 1), (700, 100), (2, 40000), (1, 70000), (65535, 1), (65536, 1), (3, 65536)])
 def test_prompt_attention_by_rows_stays_within_a_launch(monkeypatch, B, S):
     """Head shapes without a prompt kernel take a row per workgroup along the third grid dimension, which ends at 65536:
