@@ -293,16 +293,26 @@ class Stack:
             raise RuntimeError(f"Stack.{call}: there is no cache in pages (alloc_paged)")
         return self.paged
 
+    def prompt_heads(self, paged=False):
+        """Whether there is a prompt attention (_prompt_attn) for the heads of this stack and, with ``paged``, a decode attention
+        over pages."""
+        return all((b.hd in (64, 128) and b.h // b.kvh <= 4) or
+                   (b.hd in (64, 128, 256, 384) and b.h // b.kvh in (1, 2, 3, 4, 6, 8)) for b in self.blocks) and \
+            not (paged and any(b.hd not in (64, 128, 256) for b in self.blocks))
+
     def alloc_paged(self, seqs, pages, max_pages, dev, groups, page=64):
         """A cache in pages instead of the dense ones, for one row per sequence: ``groups`` lists (rows, shared slots) of
         consecutive sequences that share a prompt (the plan of paged_attn)."""
         if not self.packed():
             raise NotImplementedError("Stack.alloc_paged: the paged path needs packed weights (widths in multiples of 64)")
+        if not self.prompt_heads(paged=True):
+            raise NotImplementedError("Stack.alloc_paged: the paged path runs head_dim 64, 128 or 256 and 1, 2, 3, 4, 6 or 8 "
+                                      "query heads per kv head")
         self.free()
         b0, L = self.blocks[0], max_pages * page
+        plan = paged_attn_plan(groups, b0.h, b0.kvh, self.hd, L, dev)
         self.rope = rope_cache(self.hd, max(L, 16), device=dev)
-        self.paged = PagedCache(len(self.blocks), seqs, pages, b0.kvh, self.hd, max_pages, page, dev)
-        self.paged_plan = paged_attn_plan(groups, b0.h, b0.kvh, self.hd, L, dev)
+        self.paged, self.paged_plan = PagedCache(len(self.blocks), seqs, pages, b0.kvh, self.hd, max_pages, page, dev), plan
 
     def _tail_buffers(self, M, dev, dtype, L, share=None):
         """Static buffers of the one-launch layer tail (ecd_layer_tail) for M-row decode steps,
@@ -944,6 +954,8 @@ class HeartMuLaLite:
         """Static caches for n takes and backbone capacity L (app/engine.py:380-388), and the
         sampler's seed (drawn from torch's host generator when not given).  ``paged``: the slots of a
         prompt that the takes share; the backbone's cache is then in pages of PAGE slots."""
+        if paged is not None and not 0 <= paged <= L:
+            raise ValueError(f"alloc: a prompt of {paged} slots and a capacity of {L}")
         self.graphs.clear()  # (a frame captured over earlier caches, whose song did not end, is not replayed)
         self.N = n
         self.B = 2 * n if cfg_scale != 1.0 else n
@@ -1057,6 +1069,9 @@ class HeartMuLaLite:
             torch.manual_seed(seed)
         if a8 and not self.backbone.packed():
             raise NotImplementedError("generate: int8 activations need packed weights (widths in multiples of 64)")
+        if a8 and not self.backbone.prompt_heads():
+            raise NotImplementedError("generate: int8 activations need a head_dim of 64, 128, 256 or 384 and 1, 2, 3, 4, 6 or 8 "
+                                      "query heads per kv head")
         text = torch.as_tensor(text, dtype=torch.int64)
         P = int(text.numel())
         n_frames = max_ms // FRAME_MS

@@ -51,6 +51,43 @@ def test_a_prompt_longer_than_the_table_is_refused_before_it_takes_pages(monkeyp
         st.prompt_paged(torch.zeros(1, 49, 256, dtype=torch.float16), torch.tensor([0]))
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 1536),    # head_dim 384: no paged attention
+                                          (4, 2, 384),     # 96
+                                          (5, 1, 640),     # five query heads on one: no prompt attention
+                                          (16, 1, 2048)])
+def test_heads_that_the_paged_path_does_not_run(monkeypatch, heads, kv, dim):
+    """Refused before the old caches go."""
+    _no_gpu(monkeypatch)
+    st = _stack(heads, kv, dim)
+    st.blocks[0].kc = st.blocks[0].vc = kept = object()
+    with pytest.raises(NotImplementedError, match="head"):
+        st.alloc_paged(2, 9, 4, torch.device("cuda"), [(2, 16)], 16)
+    assert st.paged is None and st.paged_plan is None and st.blocks[0].kc is kept
+
+
+def _model(**kw):
+    gm = object.__new__(engine.HeartMuLaLite)
+    gm.backbone, gm.graphs = _stack(**kw), {}
+    return gm
+
+
+@pytest.mark.parametrize("paged", [-1, 11, 200])
+def test_a_prompt_longer_than_the_capacity_is_refused(monkeypatch, paged):
+    _no_gpu(monkeypatch)
+    with pytest.raises(ValueError, match="capacity"):
+        _model().alloc(2, 10, 1.5, seed=1, paged=paged)
+
+
+@pytest.mark.parametrize("kw", [dict(a8=True), dict(paged=True), dict(a8=True, paged=True)])
+def test_generate_refuses_heads_without_a_prompt_attention(monkeypatch, kw):
+    _no_gpu(monkeypatch)
+    gm = _model(heads=5, kv=1, dim=640)
+    gm.alloc = lambda *a, **k: gm.backbone.alloc_paged(2, 9, 4, torch.device("cuda"), [(2, 16)], 16) if k.get("paged") else \
+        pytest.fail("allocated")
+    with pytest.raises(NotImplementedError, match="head"):
+        gm.generate([1, 2, 3], 1, max_ms=160, **kw)
+
+
 @pytest.mark.parametrize("B,S", [(3, 7), (66000, 1), (700, 100), (2, 40000), (1, 70000), (65535, 1), (65536, 1), (3, 65536)])
 def test_prompt_attention_by_rows_stays_within_a_launch(monkeypatch, B, S):
     """Head shapes without a prompt kernel take a row per workgroup along the third grid dimension, which ends at 65536:
