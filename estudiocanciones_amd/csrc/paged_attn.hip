@@ -331,10 +331,10 @@ constexpr int attend_lds() {
   return W * 16 * CT * (2 + HD + 4);
 }
 
-// slots that row r attends
+// slots that row r attends: all that the table has where its position lies behind them
 __device__ __forceinline__ int attended(const PagedArgs& a, int r) {
   const long p = a.pos[r];
-  return (int)min(p < 0 ? 0l : p + 1, (long)a.MP << a.PS);
+  return p < 0 ? 0 : (int)min(p, ((long)a.MP << a.PS) - 1) + 1;
 }
 
 template <int HD, int CT, int W>

@@ -208,7 +208,7 @@ __global__ __launch_bounds__(PG_T) void page_extend_kernel(int* __restrict__ ref
     bad = len < 0 || p >= (long)MP * P;
     have = bad ? 0 : pages_of(len, P);
     more = bad || p < len ? 0 : pages_of(p + 1, P) - have;
-    if (p >= len) len = p + 1;
+    if (!bad && p >= len) len = p + 1;
   }
   s_have[t] = (int)have;
   uint32_t want;

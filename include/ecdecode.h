@@ -648,8 +648,8 @@ int ecd_paged_write(const void* qkv, long ld, const float* rope, int LR, const i
                     void* vp, const int32_t* table, long ldt, int MP, int NP, int M, int S, int Hq, int Hk, int P,
                     int HD, void* stream);
 
-/* Decode attention over pages: row r (sequence r / S) attends slots [0, pos[r]] (pos -1: nothing, its output is 0); the
- * slots that a group of rows shares are read once for all of them.
+/* Decode attention over pages: row r (sequence r / S) attends slots [0, pos[r]] (pos -1: nothing, its output is 0; a pos
+ * behind the table's last slot: all of them); the slots that a group of rows shares are read once for all of them.
  *   q row stride ldq; o [R, Hq * HD]; table row stride ldt; P a power of two from 16; HD in {64, 128, 256};
  *   Hq / Hk <= 16; MP P <= 2^30.
  *   rows [R, 2] int32: shared slots and number of shared parts of each row; items [nitems, 6] int32: first row, rows (at

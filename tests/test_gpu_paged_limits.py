@@ -94,3 +94,27 @@ def test_fork_without_enough_pages_changes_nothing(dev):
     st.same(m, "four partial pages")
     st.fork([0], [7])
     st.same(m, "none is left", 4)
+
+
+@pytest.mark.parametrize("far", [2 ** 63 - 1, 2 ** 62, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5])
+def test_positions_behind_the_table_attend_all_of_it(dev, far):
+    """A position past the table's last slot counts as that slot, whatever its size; one far below 0 as none."""
+    import torch
+    from estudiocanciones_amd.kernels import page_extend, paged_attn, paged_attn_plan, paged_write
+    b = Batch([(2, 64), (1, 0), (1, 0)], [127, 128, 128, 1], 6, 2, 64, 32, seed=2)
+    MP = 4
+    table = b.table[:, :MP]
+    assert (table[:3] >= 0).all()
+    T = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    kv, q, tab = T(b.pool), T(b.q), T(table)
+    for share in (True, False):
+        plan = paged_attn_plan(b.groups, 6, 2, 64, 4096, dev, share)
+        want = paged_attn(q, kv[0], kv[1], tab, torch.tensor([126, 127, 127, -1], device=dev), plan)
+        got = paged_attn(q, kv[0], kv[1], tab, torch.tensor([126, far, far, -far], device=dev), plan)
+        assert torch.equal(got, want) and (got[3] == 0).all() and got[2].any()
+    before = kv.clone()
+    paged_write(torch.ones(4, 10 * 64, dtype=torch.float16, device=dev), kv[0], kv[1], tab, torch.full((4,), far, device=dev), 1, 6, 2)
+    assert torch.equal(kv, before)
+    st, m = _pool(dev)
+    page_extend(st.ref, st.table, st.length, torch.tensor([-1, far, -far, -1, -1, -1], device=dev), 16, st.err)
+    st.same(m, "extend", 8)
