@@ -308,6 +308,8 @@ class Stack:
         if not self.prompt_heads(paged=True):
             raise NotImplementedError("Stack.alloc_paged: the paged path runs head_dim 64, 128 or 256 and 1, 2, 3, 4, 6 or 8 "
                                       "query heads per kv head")
+        if sum(n for n, _ in groups) != seqs:
+            raise ValueError(f"Stack.alloc_paged: groups of {sum(n for n, _ in groups)} rows for {seqs} sequences")
         self.free()
         b0, L = self.blocks[0], max_pages * page
         plan = paged_attn_plan(groups, b0.h, b0.kvh, self.hd, L, dev)

@@ -1070,7 +1070,7 @@ def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
     """Decode attention over pages: row r of ``q`` [>= R, Hq HD] (R: the plan's rows) attends slots [0, pos[r]] of
     sequence r // S through ``table`` [B, MP] int32, and the slots that a group shares are read once for the group.
     ``kp`` / ``vp`` [NP, Hk, P, HD], P a power of two from 16; ``pos`` int64 [>= R], -1: the row attends nothing and its
-    output is 0.  Rows of ``out`` behind the plan's are left as they are.  The result of a row does not depend on what
+    output is 0.  Rows of ``out`` behind the plan's are left as they are (whatever the memory holds where out is None).  The result of a row does not depend on what
     lies in slots that it does not attend."""
     dev, ldq = _rows16(q, "paged_attn q")
     NP, hk, P, hd, MP, ldt = _paged("paged_attn", kp, vp, table, dev)

@@ -124,3 +124,14 @@ def test_prompt_attention_by_rows_stays_within_a_launch(monkeypatch, B, S):
             assert b0 + r // s == (r0 + r) // S
         seen[r0:r0 + R] += 1
     assert (seen == 1).all()
+
+
+@pytest.mark.parametrize("groups", [[(1, 16)], [(3, 0)], [(2, 16), (1, 0)], []])
+def test_groups_that_are_not_the_sequences(monkeypatch, groups):
+    """A row per sequence: rows that the plan does not know would come out as whatever lay in the memory."""
+    _no_gpu(monkeypatch)
+    st = _stack()
+    st.blocks[0].kc = kept = object()
+    with pytest.raises(ValueError, match="2 sequences"):
+        st.alloc_paged(2, 9, 4, torch.device("cuda"), groups, 16)
+    assert st.paged is None and st.blocks[0].kc is kept
