@@ -1095,9 +1095,9 @@ def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
     else:
         o = out
         _on(o, dev, "paged_attn", "out", torch.float16, (rows, wide))
-    ws = torch.empty(plan.ws, device=dev, dtype=torch.float32).data_ptr() if plan.ws else None
+    ws = torch.empty(plan.ws, device=dev, dtype=torch.float32) if plan.ws else None  # (held until the launch)
     _call_on(dev, "ecd_paged_attn", q.data_ptr(), ldq, kp.data_ptr(), vp.data_ptr(), table.data_ptr(), ldt,
-             pos.data_ptr(), o.data_ptr(), ws, plan.items_ptr, plan.rows_ptr, plan.nitems, plan.nown, plan.parts,
+             pos.data_ptr(), o.data_ptr(), _ptr(ws), plan.items_ptr, plan.rows_ptr, plan.nitems, plan.nown, plan.parts,
              plan.ctiles, plan.waves, R, int(S), MP, NP, Hq, Hk, P, HD, scale)
     return o
 

@@ -118,3 +118,25 @@ def test_positions_behind_the_table_attend_all_of_it(dev, far):
     st, m = _pool(dev)
     page_extend(st.ref, st.table, st.length, torch.tensor([-1, far, -far, -1, -1, -1], device=dev), 16, st.err)
     st.same(m, "extend", 8)
+
+
+def test_the_workspace_is_held_until_the_launch(dev, monkeypatch):
+    """What another thread allocates while a call is on its way to its launch does not lie in the call's workspace."""
+    import torch
+    from estudiocanciones_amd import kernels as K
+    b = Batch([(4, 700), (2, 0)], [701, 830, 900, 700, 151, 400], 6, 2, 128, 32, seed=4)
+    kv, table, q = (torch.from_numpy(np.ascontiguousarray(a)).to(dev) for a in (b.pool, b.table, b.q))
+    pos = torch.tensor(b.lens, device=dev) - 1
+    plan = K.paged_attn_plan(b.groups, 6, 2, 128, 1024, dev, share=True)
+    assert plan.ws
+    want = K.paged_attn(q, kv[0], kv[1], table, pos, plan)
+    launch, met = K._call_on, []
+
+    def later(d, name, *args):
+        other = torch.empty(plan.ws, device=d, dtype=torch.float32)  # on the same stream, as another thread's would be
+        met.append(other.data_ptr() in args)
+        launch(d, name, *args)
+    monkeypatch.setattr(K, "_call_on", later)
+    for _ in range(3):
+        assert torch.equal(K.paged_attn(q, kv[0], kv[1], table, pos, plan), want)
+    assert met == [False] * 3
