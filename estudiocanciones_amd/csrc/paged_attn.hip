@@ -417,6 +417,8 @@ static int launch_paged(const PagedArgs& a, int R, hipStream_t st) {
 
 using namespace ecd;
 
+static constexpr float LOG2E = 1.44269504088896341f;
+
 extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const void* vp, const int32_t* table, long ldt,
                               const int64_t* pos, void* o, float* ws, const int32_t* items, const int32_t* rows,
                               int nitems, int nown, int parts, int ctiles, int waves, int R, int S, int MP, int NP, int Hq, int Hk,
@@ -425,7 +427,7 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
       parts < nown || (parts > 1 && !ws) || R <= 0 || S <= 0 || MP <= 0 || NP <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
       Hq / Hk > 16 || P < 16 || (P & (P - 1)) || ldt < MP || ldq < (long)Hq * HD || (ldq % 8) ||
       ((uintptr_t)q & 15) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)o & 7) || ((uintptr_t)ws & 15) ||
-      !(scale > 0.f) || (long)MP * P > 1 << 30 || (long)R * nown * Hk + nitems > 0x7FFFFFL || (long)R * Hq > 0x7FFFFFFFL / 64 ||
+      !(scale > 0.f && scale * LOG2E < INFINITY) || (long)MP * P > 1 << 30 || (long)R * nown * Hk + nitems > 0x7FFFFFL || (long)R * Hq > 0x7FFFFFFFL / 64 ||
       (long)NP * P > 0xFFFFFFFFL || (long)NP * P * Hk > 0xFFFFFFFFL)
     return ECD_EINVAL;
   if ((HD != 64 && HD != 128 && HD != 256) || parts > 512) return ECD_ENOTSUP;
@@ -455,7 +457,7 @@ extern "C" int ecd_paged_attn(const void* q, long ldq, const void* kp, const voi
   a.nitems = nitems;
   a.nown = nown;
   a.parts = parts;
-  a.c2 = scale * 1.44269504088896341f;
+  a.c2 = scale * LOG2E;
   const hipStream_t st = (hipStream_t)stream;
   int rc = ECD_ENOTSUP;
 #define PQ(HD_, CT_, W_)                     \

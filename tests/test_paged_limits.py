@@ -62,3 +62,10 @@ def test_sizes_that_the_kernels_do_not_count(call):
 def test_sizes_whose_products_pass_64_bits(call):
     from estudiocanciones_amd import _ffi
     assert call(_ffi.lib()) in (I, N)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), 3e38, 1e300])
+def test_a_scale_that_no_number_of_32_bits_holds_times_log2_e(scale):
+    from estudiocanciones_amd import _ffi
+    L = _ffi.lib()
+    assert L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, None, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, scale, None) == I
