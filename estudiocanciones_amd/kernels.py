@@ -852,8 +852,13 @@ def _call_on(dev, name, *args):
             _ffi.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
 
 
-def _page_state(name, ref, table, length, err):
+INT_MOST = 0x7FFFFFFF  # (the library takes counts as 32-bit numbers: a larger one would wrap)
+
+
+def _page_state(name, ref, table, length, err, page=1):
     dev = _dev(ref, name)
+    if not 1 <= page <= INT_MOST:
+        raise ValueError(f"{name}: {page} slots of a page")
     if table.dim() != 2:
         raise ValueError(f"{name}: table must be [B, MP]")
     B, MP = table.shape
@@ -878,7 +883,7 @@ def page_free(ref, table, length, seqs, page, err):
     """The sequences ``seqs`` [n] int32 give their pages back: a page whose last owner goes is free.  ``ref`` [NP] int32
     owners of each page, ``table`` [B, MP] int32 page numbers (-1 behind a sequence's last), ``length`` [B] int64 slots
     held, ``page`` slots of a page; ``err`` [1] int32 collects what was refused (include/ecdecode.h lists its bits)."""
-    dev, NP, B, MP = _page_state("page_free", ref, table, length, err)
+    dev, NP, B, MP = _page_state("page_free", ref, table, length, err, page)
     n = seqs.numel()
     _on(seqs, dev, "page_free", "seqs", torch.int32, (n,))
     if n:
@@ -902,7 +907,7 @@ def page_fork(kv, ref, table, length, src, dst, err):
 
 def page_extend(ref, table, length, pos, page, err):
     """Every sequence b holds slot pos[b] (int64 [B], B <= 1024) afterwards; -1, or a slot it holds, leaves it alone."""
-    dev, NP, B, MP = _page_state("page_extend", ref, table, length, err)
+    dev, NP, B, MP = _page_state("page_extend", ref, table, length, err, page)
     _on(pos, dev, "page_extend", "pos", torch.int64, (B,))
     _call_on(dev, "ecd_page_extend", ref.data_ptr(), NP, table.data_ptr(), MP, length.data_ptr(), B, int(page),
              pos.data_ptr(), err.data_ptr())
@@ -963,7 +968,7 @@ def paged_write(qkv, kp, vp, table, pos, S, Hq, Hk, rope=None, q=None):
     dev, ld = _rows16(qkv, "paged_write qkv")
     NP, hk, P, HD, MP, ldt = _paged("paged_write", kp, vp, table, dev)
     M, W = qkv.shape
-    if hk != Hk or W != (Hq + 2 * Hk) * HD or HD % 8 or S < 1 or table.shape[0] * S < M:
+    if hk != Hk or W != (Hq + 2 * Hk) * HD or HD % 8 or not 1 <= S <= INT_MOST or table.shape[0] * S < M:
         raise ValueError("paged_write: qkv must be [M, (Hq + 2 Hk) HD], kp / vp [NP, Hk, P, HD], table [B, MP] with "
                          "B * S >= M")
     _on(pos, dev, "paged_write", "pos", torch.int64, (M,))
@@ -1078,7 +1083,7 @@ def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
     rows, wide = q.shape
     if plan.dev != dev:
         raise ValueError(f"paged_attn: the plan is on {plan.dev}, the tensors on {dev}")
-    if hk != Hk or hd != HD or wide != Hq * HD or rows < R or S < 1 or table.shape[0] * S < R:
+    if hk != Hk or hd != HD or wide != Hq * HD or rows < R or not 1 <= S <= INT_MOST or table.shape[0] * S < R:
         raise ValueError("paged_attn: q [>= R, Hq HD], kp / vp [NP, Hk, P, HD] and table [B, MP] (B * S >= R) must fit "
                          "the plan")
     if P < 16 or P & (P - 1):

@@ -69,3 +69,55 @@ def test_a_scale_that_no_number_of_32_bits_holds_times_log2_e(scale):
     from estudiocanciones_amd import _ffi
     L = _ffi.lib()
     assert L.ecd_paged_attn(16, 512, 16, 16, 8, 4, 8, 8, None, 8, 8, 0, 1, 1, 1, 4, 2, 1, 4, 9, 4, 2, 16, 128, scale, None) == I
+
+
+class _Made:
+    """A tensor as the calls' checks look at it, of sizes that need no memory."""
+
+    def __init__(self, dtype, *shape):
+        import torch
+        self.dtype, self.shape, self.device, self.is_cuda = dtype, torch.Size(shape), torch.device("cuda", 0), True
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def stride(self, i=None):
+        s = [1]
+        for n in reversed(self.shape[1:]):
+            s.insert(0, s[0] * n)
+        return tuple(s) if i is None else s[i]
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 4096
+
+
+@pytest.mark.parametrize("far", [2 ** 32 + 1, 2 ** 31, 2 ** 33 + 16, 2 ** 40])
+def test_counts_that_would_wrap_in_the_entry(monkeypatch, far):
+    """Rows per sequence and slots per page go to the library as 32-bit numbers: 2^32 + 1 rows would be 1 there, and each row
+    would have a row of the table of its own, also where the table has not."""
+    import ctypes
+    import torch
+    from types import SimpleNamespace
+    from estudiocanciones_amd import kernels as K
+    assert ctypes.c_int(2 ** 32 + 1).value == 1
+    monkeypatch.setattr(K, "_call_on", lambda *a: pytest.fail("launched"))
+    monkeypatch.setattr(K.torch, "empty", lambda *a, **k: _Made(torch.float16, 3, 256))
+    h, i32, i64 = torch.float16, torch.int32, torch.int64
+    kp, table, pos = _Made(h, 9, 2, 16, 64), _Made(i32, 1, 4), _Made(i64, 3)
+    plan = SimpleNamespace(R=3, Hq=4, Hk=2, HD=64, dev=kp.device, ws=0, items_ptr=0, rows_ptr=0, nitems=0, nown=1, parts=1,
+                           ctiles=1, waves=4)
+    with pytest.raises(ValueError):
+        K.paged_attn(_Made(h, 3, 256), kp, kp, table, pos, plan, S=far)
+    with pytest.raises(ValueError):
+        K.paged_write(_Made(h, 3, 512), kp, kp, table, pos, far, 4, 2)
+    state = (_Made(i32, 9), _Made(i32, 2, 4), _Made(i64, 2))
+    with pytest.raises(ValueError):
+        K.page_free(*state, _Made(i32, 1), far, _Made(i32, 1))
+    with pytest.raises(ValueError):
+        K.page_extend(*state, _Made(i64, 2), far, _Made(i32, 1))
