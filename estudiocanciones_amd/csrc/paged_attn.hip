@@ -19,9 +19,9 @@
 // product's other half costs little: 2 x 32 rows on prompts of 7000 slots 42.1 us against 41.4 with its join, 2 x 16 on 4096
 // 29.2 against 28.9, short rows the same.
 // Bound by the reads of K and V: of 24 query heads on 8 kv heads of 128, 2 x 32 rows on prompts of 7000 slots (126 MB, each
-// slot read from memory once) take 38.5 us and 4.7 us for the join, 2 x 16 on 4096 (98 MB) 25.7 and 3.9: about 5.5 us until the
+// slot read from memory once) take 40.1 us and 4.8 us for the join, 2 x 16 on 4096 (98 MB) 25.0 and 4.1: about 5.5 us until the
 // first tile is there, then 2 us for each of 14 tiles of a wave (8 waves a CU), 3 us to add the waves up.  A few short
-// rows are bound by those first and last steps: 8 rows of 750 slots 7.4 to 8.3 us and 3.7 for the join.
+// rows are bound by those first and last steps: 8 rows of 750 slots 7.6 us and 3.6 for the join.
 #include "common.h"
 
 namespace ecd {
@@ -240,8 +240,8 @@ __device__ __forceinline__ void attend(const PagedArgs& a, float* lds, int row0,
   PState<HD, CT> s;
   begin(s, a, row0, cols, 0, kh, lane);
   // K of the next tile is asked for once this one's scores are formed, V once this one's is used: one tile is always in
-  // flight, in the registers of the last one.  (Two tiles ahead measured no faster: a CU gets about 45 GB/s of what its XCD's
-  // L2 does not hold, whatever is in flight.)
+  // flight, in the registers of the last one.  (Two tiles ahead measured no faster: what the L2s do not hold comes at 4 to
+  // 6 TB/s, about 20 GB/s for each CU, whatever is in flight.)
   PTile<HD> t;
   constexpr int STEP = W * PQ_T;
   const int first = (lo & ~(PQ_T - 1)) + wv * PQ_T;

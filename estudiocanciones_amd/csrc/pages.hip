@@ -51,8 +51,8 @@ __device__ __forceinline__ uint32_t free_pages(const int* ref, int NP, uint32_t 
   return seen < want ? seen : want;
 }
 
-// One workgroup per entry of seqs: its pages lose an owner (2.7 us for 4 sequences, of which a launch is about 2).  The length is taken by an exchange, so a sequence that is
-// named twice is freed once.
+// One workgroup per entry of seqs: its pages lose an owner (2.4 us for 2 sequences of 5 pages, 3.6 for 32 of 16; a launch is
+// about 2).  The length is taken by an exchange, so a sequence that is named twice is freed once.
 __global__ __launch_bounds__(256) void page_free_kernel(int* __restrict__ ref, int NP, int* __restrict__ table, int MP,
                                                         int64_t* __restrict__ length, int B, int P,
                                                         const int* __restrict__ seqs, int* __restrict__ err) {
@@ -73,7 +73,8 @@ __global__ __launch_bounds__(256) void page_free_kernel(int* __restrict__ ref, i
 }
 
 // One workgroup, which sees every refusal before anything is changed: a thread per child finds what it needs, then all look
-// at the sources' pages and for free ones, PG_T at a time.  Bound by latency (3.8 us for 2 children, 4.4 for 32 of 3540 pages).
+// at the sources' pages and for free ones, PG_T at a time.  Bound by latency (4.2 us for 2 children, 5.4 for 32 of 2
+// prompts of 16 pages; 3.8 and 4.4 without the look at the whole pages).
 // plan[i] = {page of the source's partial slots, page for them, their number, whole pages shared (-1: nothing to do)}
 __global__ __launch_bounds__(PG_T) void page_fork_plan_kernel(const int* __restrict__ ref, int NP,
                                                               const int* __restrict__ table, int MP,
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(256) void page_fork_kernel(f16* __restrict__ kv, in
   }
 }
 
-// Every sequence b holds slot pos[b] afterwards (pos[b] < length[b]: nothing to do, 1.9 us).  The first pass over ref counts, the
-// second one takes, so a call that does not fit takes nothing.
+// Every sequence b holds slot pos[b] afterwards.  The first pass over ref counts, the second one takes, so a call that does not
+// fit takes nothing.  Slots in pages that are held: 1.9 us for 6 sequences, 3.9 for 36.
 __global__ __launch_bounds__(PG_T) void page_extend_kernel(int* __restrict__ ref, int NP, int* __restrict__ table,
                                                            int MP, int64_t* __restrict__ length, int B, int P,
                                                            const int64_t* __restrict__ pos, int* __restrict__ err) {

@@ -964,7 +964,8 @@ def paged_write(qkv, kp, vp, table, pos, S, Hq, Hk, rope=None, q=None):
     """K and V of the rows of ``qkv`` [M, (Hq + 2 Hk) HD] into pages: row m belongs to sequence m // S at slot pos[m]
     (int64 [M]); ``kp`` / ``vp`` [NP, Hk, P, HD], ``table`` [B, MP] int32 with B S >= M.  With ``rope`` [L, HD/2, 2]
     float32, q and k are rotated first (the numerics of _rope_cache) and q [M, Hq HD] is returned (``q``: its
-    destination); without it nothing is.  A row whose slot has no page writes nothing into the cache."""
+    destination); without it nothing is.  A row whose slot has no page writes nothing into the cache; the others of a call
+    name different slots."""
     dev, ld = _rows16(qkv, "paged_write qkv")
     NP, hk, P, HD, MP, ldt = _paged("paged_write", kp, vp, table, dev)
     M, W = qkv.shape
@@ -1001,19 +1002,22 @@ class PagedAttnPlan:
         self.dev = flat.device
 
 
-# How a batch is cut, from times on an MI355X (24 query heads on 8 kv heads of 128; us):
-# sharing pays where it saves this many bytes of the other rows' reads, else the parts cost more than they save
+# How a batch is cut, from times on an MI355X (24 query heads on 8 kv heads of 128; other heads follow the same rules, by their
+# bytes and slots, not measured one by one; us):
+# sharing pays where it saves this many bytes of the other rows' reads, else the parts cost more than they save; taken for the
+# whole batch, since one group's parts already bring the join: then every prefix is shared, a short one too
 # (shared / not: 8 rows of 4096 + 64 slots, 117 MB saved, 16.0 / 22.7; 2 x 4 of 1500 + 500, 37 MB, 14.5 / 14.0; 2 x 16 of
 # 256 + 500, 31 MB, 18.0 / 15.1; 2 x 4 of 256 + 494, 6 MB, 10.3 / 10.4)
 PLAN_SAVED = 48 << 20
 # workgroups that the shared parts are cut for (2 x 16 rows of 4096: 128 28.1, 256 29.1, 384 32.2; 2 x 32 of 7000: 42.1 with
 # 256, 46.0 with 384)
 PLAN_SHARED_WG = 256
-# a row's own slots: parts so that all rows together have this many workgroups, none of more than PLAN_OWN_SLOTS (8 rows of
-# 256 + 3000: 4 parts 22.4, 7 parts 23.1; 2 x 16 of 1000 + 4000: 2 parts 71, 4 parts 64), at most PLAN_OWN_MOST parts
+# a row's own slots: parts so that all rows together have this many workgroups and, as far as PLAN_OWN_MOST parts go, none has
+# more than PLAN_OWN_SLOTS of the longest row that max_len allows (8 rows of 256 + 3000: 4 parts 22.4, 7 parts 23.1; 2 x 16 of
+# 1000 + 4000: 2 parts 71, 4 parts 64)
 PLAN_OWN_WG, PLAN_OWN_SLOTS, PLAN_OWN_MOST = 256, 1280, 16
-# one workgroup (of eight waves; head_dim 256 of four) for a row and kv head, nothing to join: rows of few slots (8 rows of 160: 5.7, in parts
-# 7.5; of 750: 11.7 and 10.4), or as many pairs as CUs (2 x 16 rows of 100 + 2000, ragged: 32.6 and 35.6)
+# one workgroup (of eight waves; head_dim 256 of four) for a row and kv head, nothing to join: rows of few slots (8 rows of
+# 160: 5.7, in parts 7.5; of 750: 11.7 and 10.4), or as many pairs as CUs (2 x 16 rows of 100 + 2000, ragged: 32.6 and 35.6)
 PLAN_SOLO_BYTES, PLAN_SOLO_WG = 512 * 512, 256
 
 
@@ -1021,8 +1025,8 @@ def paged_attn_plan(groups, Hq, Hk, HD, max_len, device="cuda", share=None):
     """The plan of paged_attn for rows in ``groups``: a list of (rows, prefix), consecutive rows whose first ``prefix``
     slots are the same (0: nothing shared).  ``max_len``: the most slots that a row may come to hold (a prefix of more is
     not shared: no row attends all of it).  Made once for all layers and steps in which the groups stay the same (it
-    copies to the device: not under graph capture).  ``share``: whether prefixes are read once per group (None: where
-    that saves more than joining the parts costs)."""
+    copies to the device: not under graph capture), and kept until the work that uses it is done.  ``share``: whether
+    prefixes are read once per group (None: where that saves more than joining the parts costs, for the whole batch)."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise RuntimeError("paged_attn_plan: the decode path runs only on a ROCm GPU")
@@ -1075,8 +1079,9 @@ def paged_attn(q, kp, vp, table, pos, plan, S=1, scale=None, out=None):
     """Decode attention over pages: row r of ``q`` [>= R, Hq HD] (R: the plan's rows) attends slots [0, pos[r]] of
     sequence r // S through ``table`` [B, MP] int32, and the slots that a group shares are read once for the group.
     ``kp`` / ``vp`` [NP, Hk, P, HD], P a power of two from 16; ``pos`` int64 [>= R], -1: the row attends nothing and its
-    output is 0.  Rows of ``out`` behind the plan's are left as they are (whatever the memory holds where out is None).  The result of a row does not depend on what
-    lies in slots that it does not attend."""
+    output is 0; a position behind the table's last slot: all of them.  Rows of ``out`` behind the plan's are left as they
+    are (whatever the memory holds where out is None).  The result of a row does not depend on what lies in slots that it
+    does not attend."""
     dev, ldq = _rows16(q, "paged_attn q")
     NP, hk, P, hd, MP, ldt = _paged("paged_attn", kp, vp, table, dev)
     R, Hq, Hk, HD = plan.R, plan.Hq, plan.Hk, plan.HD
