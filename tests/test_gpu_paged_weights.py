@@ -102,14 +102,15 @@ def test_an_infinite_value_that_is_attended(dev, Hq, Hk, HD):
     k = (np.arange(n) % 7)[:, None] * 1.5
     v = np.random.default_rng(8).standard_normal((n, HD)).astype(np.float16)
     clean = v.copy()
-    v[21, 3], v[260, HD - 1] = np.inf, -np.inf  # scores 0 (e^-9 of the largest) and 1.5
+    # scores 0 (e^-9 of the largest), 1.5, and the largest, whose weight is one fp16 value exactly
+    v[21, 3], v[260, HD - 1], v[6, 5], v[13, 7] = np.inf, -np.inf, np.inf, -np.inf
     b = Batch([(2, 0), (3, 280)], [n, 300, 280, 300, 290], Hq, Hk, HD, 32, seed=6)
     _fill(b, n, np.array([1.0]), k.astype(np.float16), v)
     for share in SHARES:
         got = b.run(dev, scale=1.0, share=share).double().cpu().numpy().reshape(b.R, Hq, HD)
-        assert (got[:, :, 3] == np.inf).all() and (got[:, :, HD - 1] == -np.inf).all()
+        assert (got[:, :, [3, 5]] == np.inf).all() and (got[:, :, [7, HD - 1]] == -np.inf).all()
         for r, m in enumerate(b.lens):
             p = np.exp(k[:m, 0] - 9.0)
             want = p @ clean[:m].astype(np.float64) / p.sum()
-            rest = [d for d in range(HD) if d not in (3, HD - 1)]
+            rest = [d for d in range(HD) if d not in (3, 5, 7, HD - 1)]
             assert (np.abs(got[r] - want)[:, rest] <= 2.0 ** -10).all()
