@@ -129,6 +129,12 @@ SIGNATURES = {
     "ecd_gemm_a8": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, _P],
     "ecd_gemm_a8_tuned": [_P, c_long, _P, _P, _P, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P],
     "ecd_gemm_a8_silu": [_P, c_long, _P, _P, _P, _P, c_long, c_int, c_int, c_int, _P],
+    "ecd_quantize_rows_q4": [_P, c_int, _P, _P, _P, c_int, c_int, c_int, _P],
+    "ecd_packed_bytes_q4": [c_int, c_int],
+    "ecd_pack_q4": [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P],
+    "ecd_mm_q4": [_P, c_long, _P, c_float, _P, _P, c_int, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P],
+    "ecd_process_logits": [_P, c_long, c_int, c_float, _P, c_long, c_long, c_int, _P, c_int, _P, _P, _P, c_int, _P, c_long, _P,
+                           c_long, c_int, _P, _P, c_long, c_int, c_int, _P],
 }
 
 _lib = None

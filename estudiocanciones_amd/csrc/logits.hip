@@ -1,0 +1,150 @@
+// Logits from a model's heads to those a sampler draws from (gfx950): guidance, penalties for tokens of a history, biases,
+// masks of allowed tokens.
+//
+// Per row r and token v, in fp32, one rounding to fp16 at the end:
+//   l = u + (c - u) cfg                        with guidance (c row r, u row N + r), else the row itself
+//   if v occurs n > 0 times in the row's history:
+//     l = l > 0 ? l / rep[r] : l rep[r];  l = l - (presence[r] + frequency[r] n)
+//   l = l + bias[v]
+//   l = -inf                                   where the row's mask does not allow v
+// The history of a row are the last `window` (0: all) of its first length[r] tokens; tokens outside [0, V) count for nothing.
+//
+// A workgroup takes a segment of a row: its logits, biases and mask bits are loaded first; while they are in flight the row's
+// history is counted for the segment with integer atomics in LDS (the order of their arrival cannot change a count), then
+// each thread finishes its 8 tokens.  Nothing is written in between, so one launch is one pass over the data.
+#include "gemm_core.h"
+
+namespace ecd {
+
+typedef f32x4 f32x4u __attribute__((aligned(4)));
+
+struct LogitsArgs {
+  const f16* logits;
+  long ld;
+  float cfg;
+  int guided;
+  const int64_t* hist;
+  long hrow, htok;
+  int T;
+  const int64_t* length;
+  int window;
+  const float *rep, *pres, *freq;
+  int per_row;  // bit 0 / 1 / 2: rep / pres / freq has an element per row (else one for all)
+  const float* bias;
+  long ldb;
+  const uint32_t* allowed;
+  long lda;
+  int A;
+  const int32_t* state;
+  f16* out;
+  long ldo;
+  int N, V, seg;
+};
+
+template <int TH>
+__global__ __launch_bounds__(TH) void process_logits_kernel(const LogitsArgs a) {
+  __shared__ __align__(16) uint32_t count[8 * TH];
+  const int r = blockIdx.y, v0 = blockIdx.x * a.seg, v1 = min(v0 + a.seg, a.V), i = v0 + 8 * threadIdx.x;
+  const bool on = i < v1, full = i + 8 <= v1;
+  const f16* lc = a.logits + (long)r * a.ld;
+  const f16* lu = a.logits + (long)(r + a.N) * a.ld;
+  f16x8 c = {0, 0, 0, 0, 0, 0, 0, 0}, u = c;
+  float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float* bp = a.bias ? a.bias + (long)r * a.ldb : nullptr;
+  if (full) {
+    c = *(const f16x8u*)(lc + i);
+    if (a.guided) u = *(const f16x8u*)(lu + i);
+    if (bp) {
+      const f32x4 b0 = *(const f32x4u*)(bp + i), b1 = *(const f32x4u*)(bp + i + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[j] = b0[j];
+        b[4 + j] = b1[j];
+      }
+    }
+  } else if (on) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < v1) {
+        c[j] = lc[i + j];
+        if (a.guided) u[j] = lu[i + j];
+        if (bp) b[j] = bp[i + j];
+      }
+  }
+  // a state outside the masks allows nothing, -1 everything
+  uint32_t keep = 0xFFu;
+  if (a.allowed) {
+    const int s = a.state ? a.state[r] : a.A == 1 ? 0 : r;
+    if (s >= a.A || s < -1)
+      keep = 0u;
+    else if (s >= 0 && on)
+      keep = a.allowed[(long)s * a.lda + (i >> 5)] >> (i & 31);
+  }
+  uint32_t n[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+  float rep = 1.f, pres = 0.f, freq = 0.f;
+  if (a.hist) {
+    const int64_t len = a.length ? a.length[r] : a.T;
+    const int t1 = (int)(len < 0 ? 0 : len > a.T ? a.T : len);
+    const int t0 = a.window > 0 && t1 > a.window ? t1 - a.window : 0;
+    if (a.rep) rep = a.rep[a.per_row & 1 ? r : 0];
+    if (a.pres) pres = a.pres[a.per_row & 2 ? r : 0];
+    if (a.freq) freq = a.freq[a.per_row & 4 ? r : 0];
+    u32x4* const mine = (u32x4*)(count + 8 * threadIdx.x);
+    mine[0] = mine[1] = (u32x4){0u, 0u, 0u, 0u};
+    __syncthreads();
+    const int64_t* hp = a.hist + (long)r * a.hrow;
+    for (int t = t0 + (int)threadIdx.x; t < t1; t += TH) {
+      const int64_t v = hp[(long)t * a.htok];
+      if (v >= v0 && v < v1) atomicAdd(&count[(int)(v - v0)], 1u);
+    }
+    __syncthreads();
+    const u32x4 n0 = mine[0], n1 = mine[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      n[j] = n0[j];
+      n[4 + j] = n1[j];
+    }
+  }
+  if (!on) return;
+  f16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float l = (float)c[j];
+    if (a.guided) {
+      const float w = (float)u[j];
+      l = w + (l - w) * a.cfg;
+    }
+    if (n[j]) {
+      l = l > 0.f ? l / rep : l * rep;
+      l -= pres + freq * (float)n[j];
+    }
+    l += b[j];
+    o[j] = keep >> j & 1u ? (f16)l : (f16)-INFINITY;
+  }
+  f16* op = a.out + (long)r * a.ldo + i;
+  if (full)
+    *(f16x8u*)op = o;
+  else
+    store_tail(op, nullptr, o, v1 - i);
+}
+
+}  // namespace ecd
+
+using namespace ecd;
+
+extern "C" int ecd_process_logits(const void* logits, long ld, int guided, float cfg, const int64_t* hist, long hrow, long htok,
+                                  int T, const int64_t* length, int window, const float* rep, const float* pres,
+                                  const float* freq, int per_row, const float* bias, long ldb, const uint32_t* allowed, long lda,
+                                  int A, const int32_t* state, void* out, long ldo, int N, int V, void* stream) {
+  if (!logits || !out || N <= 0 || V <= 0 || ld < V || ldo < V || T < 0 || window < 0 || (hist && (hrow < 0 || htok < 0)) ||
+      ((rep || pres || freq) && !hist) || (bias && ldb != 0 && ldb < V) ||
+      (allowed && (A <= 0 || lda < (V + 31L) / 32 || (!state && A != 1 && A != N))))
+    return ECD_EINVAL;
+  if (N > 65535 || V > 0x7FFFFFFF - 8192) return ECD_ENOTSUP;
+  constexpr int TH = 256, SEG = 8 * TH;
+  const int parts = (V + SEG - 1) / SEG, seg = ((V + parts - 1) / parts + 7) / 8 * 8;
+  const LogitsArgs a{(const f16*)logits, ld, cfg, guided, hist, hrow, htok, T, length, window, rep, pres, freq, per_row, bias, ldb,
+                     allowed, lda, A, state, (f16*)out, ldo, N, V, seg};
+  hipLaunchKernelGGL(process_logits_kernel<TH>, dim3((V + seg - 1) / seg, N), dim3(TH), 0, (hipStream_t)stream, a);
+  return ecd_launch_status();
+}

@@ -1174,3 +1174,189 @@ def gemm_a8_silu_packed(c, sx, wp, s, F, K, out=None):
         _call_on(dev, "ecd_gemm_a8_silu", c.data_ptr(), c.stride(0), sx.data_ptr(), wp.data_ptr(), s.data_ptr(),
                  mm.data_ptr(), mm.stride(0), M, F, K)
     return mm
+
+
+# ---------------------------------------------------------------- 4-bit weights
+class PackedQ4:
+    """An [N, K] matrix of 4-bit weights laid out for mm_q4 and mm_q4_silu (pack_q4)."""
+
+    def __init__(self, codes, scales, N, K, group, zeros, interleave):
+        self.codes, self.scales = codes, scales
+        self.N, self.K, self.group, self.zeros, self.interleave = N, K, group, zeros, interleave
+        self.dev = codes.device
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel() * 2
+
+
+def pack_q4(q4, s4, z4=None, interleave=False):
+    """4-bit weights in groups (quant.q4_rows) -> PackedQ4: q4 uint8 [N, K / 2] (element 2 i in the low half of byte i), s4
+    fp16 [N, groups], z4 uint8 [N, groups] or None (zero point 8), groups = K / 32, 64 or 128 rounded up.  With
+    ``interleave`` the two halves of the rows are interleaved (w1 | w3 -> pairs, for mm_q4_silu)."""
+    dev = _dev(q4, "pack_q4")
+    if q4.dim() != 2 or s4.dim() != 2:
+        raise ValueError("pack_q4: q4 must be [N, K / 2] and s4 [N, groups]")
+    N, K = q4.shape[0], 2 * q4.shape[1]
+    if K % 64 or not 0 < K <= INT_MOST or not 0 < N <= INT_MOST - 32 or (interleave and N % 2):
+        raise ValueError("pack_q4: K must be a multiple of 64 (and N even to interleave)")
+    ng = s4.shape[1]
+    group = next((g for g in (128, 64, 32) if -(-K // g) == ng), 0)
+    if not group:
+        raise ValueError(f"pack_q4: {ng} groups of {K} weights are none of 32, 64 or 128")
+    _on(q4, dev, "pack_q4", "q4", torch.uint8, (N, K // 2))
+    _on(s4, dev, "pack_q4", "s4", torch.float16, (N, ng))
+    if z4 is not None:
+        _on(z4, dev, "pack_q4", "z4", torch.uint8, (N, ng))
+    if q4.data_ptr() % 4:
+        q4 = q4.clone()
+    codes = torch.empty(_ffi.lib().ecd_packed_bytes_q4(N, K), device=dev, dtype=torch.uint8)
+    scales = torch.empty(ng * (-(-N // 32) * 32) * (1 if z4 is None else 2), device=dev, dtype=torch.float16)
+    _call_on(dev, "ecd_pack_q4", q4.data_ptr(), s4.data_ptr(), _ptr(z4), N, K, group, int(interleave), codes.data_ptr(),
+             scales.data_ptr())
+    return PackedQ4(codes, scales, N, K, group, z4 is not None, bool(interleave))
+
+
+def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
+    dev, ldx = _rows16(x, name)
+    M, K = x.shape
+    if K != w.K or dev != w.dev or w.interleave is not silu or M > INT_MOST:
+        if w.interleave is not silu:
+            raise ValueError(f"{name}: the weights were packed {'with' if w.interleave else 'without'} interleave")
+        if dev != w.dev:
+            raise ValueError(f"{name}: the weights are on {w.dev}, x on {dev}")
+        raise ValueError(f"{name}: x must be [M, {w.K}]")
+    if nw is not None:
+        _on(nw, dev, name, "nw", torch.float16, (K,))
+        if nw.data_ptr() % 16:
+            raise ValueError(f"{name}: nw must be 16-byte aligned")
+    y = torch.empty(M, cols, device=dev, dtype=torch.float16) if out is None else out
+    ldr = 0
+    if res is not None:
+        ldr = _rows_of(res, M, cols, dev, name, "res")
+    ldy = cols
+    if out is not None:
+        ldy = _rows_of(out, M, cols, dev, name, "out")
+        if _ends(out)[0] < _ends(x)[1] and _ends(x)[0] < _ends(out)[1]:
+            raise ValueError(f"{name}: out must not overlap x")
+    if M:
+        _call_on(dev, "ecd_mm_q4", x.data_ptr(), ldx, _ptr(nw), eps, w.codes_ptr, w.scales_ptr, w.zeros, w.group, _ptr(res), ldr,
+                 y.data_ptr(), ldy, M, w.N, K, silu)
+    return y
+
+
+def _ends(t):
+    """First byte of a tensor with positive strides, and the one behind its last."""
+    a = t.data_ptr()
+    return a, a + (1 + sum((n - 1) * d for n, d in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else a
+
+
+def _rows_of(t, M, N, dev, call, name):
+    """Row stride of an fp16 [M, N] tensor on dev with unit inner stride and rows that do not overlap."""
+    if t.dtype is torch.float16 and t.device == dev and t.shape == (M, N):
+        ld, one = t.stride()
+        if (one == 1 or N == 1) and (ld >= N or M == 1):
+            return max(ld, N)
+    raise ValueError(f"{call}: {name} must be fp16 [{M}, {N}] on {dev} with unit inner stride")
+
+
+def mm_q4(x, w, res=None, nw=None, eps=1e-5, out=None):
+    """y = x @ w^T (+ res) -> [M, N] for 4-bit weights ``w`` (pack_q4) and x [M, K] fp16, or with ``nw`` [K] the RMS norm of
+    x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end.  Any number of rows.
+    ``out`` may be ``res``, not x."""
+    return _mm_q4("mm_q4", x, w, w.N, res, nw, eps, out, False)
+
+
+def mm_q4_silu(x, w, nw=None, eps=1e-5, out=None):
+    """silu(a) * b -> [M, N / 2] for the products a, b of mm_q4 on interleaved w1 | w3 (pack_q4(..., interleave=True)), in fp32
+    with one rounding at the end."""
+    return _mm_q4("mm_q4_silu", x, w, w.N // 2, None, nw, eps, out, True)
+
+
+# ---------------------------------------------------------------- logits before the sampler
+def _per_row(t, N, dev, name):
+    if t.dtype is not torch.float32 or t.device != dev or t.dim() != 1 or t.shape[0] not in (1, N) or not t.is_contiguous():
+        raise ValueError(f"process_logits: {name} must be float32 [{N}] or [1] on {dev}")
+    return t.data_ptr(), t.shape[0] == N
+
+
+def process_logits(logits, hist=None, length=None, window=0, repetition=None, presence=None, frequency=None, bias=None,
+                   allowed=None, state=None, cfg=None, out=None):
+    """Logits [B, V] fp16 -> those that sample_topk draws from [N, V], in fp32 with one rounding to fp16:
+
+    guidance (``cfg`` given: B = 2N, cond rows then uncond rows): l = uncond + (cond - uncond) cfg; else N = B;
+    a token that occurs n > 0 times in the row's history: l / ``repetition`` if l > 0, else l * ``repetition``; then
+    l - (``presence`` + ``frequency`` * n) (each float32 [N] or [1], read on the device);
+    l + ``bias`` (float32 [V], or [N, V]);
+    -inf for tokens that the row's mask does not allow, whatever their logits hold (a row that may draw nothing is all -inf).
+
+    ``hist`` int64 [N, T] with any strides: the row's tokens, of which the first ``length`` (int64 [N] on the device; None: T)
+    are there and the last ``window`` of those count (0: all); tokens outside [0, V) count for nothing.  ``allowed`` int32
+    [A, ceil(V / 32)]: masks of allowed tokens, bit v % 32 of word v // 32; ``state`` int32 [N] gives each row its mask (-1:
+    none; any other number outside [0, A): nothing is allowed), without it A is 1 or N.  ``out``: the destination; it may be
+    the first N rows of ``logits``."""
+    dev = _dev(logits, "process_logits")
+    _f16(logits, "process_logits logits")
+    if logits.dim() != 2:
+        raise ValueError("process_logits: logits must be [B, V]")
+    B, V = logits.shape
+    ld, one = logits.stride()
+    guided = cfg is not None
+    N = B // 2 if guided else B
+    if (one != 1 and V != 1) or (ld < V and B != 1) or V < 1 or V > INT_MOST - 8192 or (guided and B % 2):
+        raise ValueError("process_logits: logits must be [B, V] with contiguous rows (B even with cfg)")
+    ld = max(ld, V)
+    hp = hrow = htok = T = lp = rp = pp = fp = bp = ldb = ap = lda = A = sp = 0
+    flags = 0
+    if hist is not None:
+        if hist.dtype is not torch.int64 or hist.device != dev or hist.dim() != 2 or hist.shape[0] != N or \
+                hist.shape[1] > INT_MOST:
+            raise ValueError(f"process_logits: hist must be int64 [{N}, T] on {dev}")
+        hp, T = hist.data_ptr(), hist.shape[1]
+        hrow, htok = hist.stride()
+        if length is not None:
+            _on(length, dev, "process_logits", "length", torch.int64, (N,))
+            lp = length.data_ptr()
+        if not 0 <= window <= INT_MOST:
+            raise ValueError("process_logits: window must be 0 (all tokens) or a number of tokens")
+        if repetition is not None:
+            rp, f = _per_row(repetition, N, dev, "repetition")
+            flags |= f
+        if presence is not None:
+            pp, f = _per_row(presence, N, dev, "presence")
+            flags |= f << 1
+        if frequency is not None:
+            fp, f = _per_row(frequency, N, dev, "frequency")
+            flags |= f << 2
+        if T == 0 or not (rp or pp or fp):  # nothing to count, or nothing that depends on it
+            hp = rp = pp = fp = 0
+    elif length is not None or window or repetition is not None or presence is not None or frequency is not None:
+        raise ValueError("process_logits: penalties need a history (hist)")
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.device != dev or bias.shape not in ((V,), (N, V)) or \
+                (bias.stride(-1) != 1 and V != 1) or (bias.dim() == 2 and bias.stride(0) < V and N != 1):
+            raise ValueError(f"process_logits: bias must be float32 [{V}] or [{N}, {V}] on {dev} with contiguous rows")
+        bp, ldb = bias.data_ptr(), max(bias.stride(0), V) if bias.dim() == 2 else 0
+    if allowed is not None:
+        A = allowed.shape[0] if allowed.dim() == 2 else 0
+        lda = -(-V // 32)
+        if A < 1 or A > INT_MOST or (state is None and A != 1 and A != N):
+            raise ValueError(f"process_logits: allowed must be [A, {lda}] (A 1 or {N} without state)")
+        _on(allowed, dev, "process_logits", "allowed", torch.int32, (A, lda))
+        ap = allowed.data_ptr()
+        if state is not None:
+            _on(state, dev, "process_logits", "state", torch.int32, (N,))
+            sp = state.data_ptr()
+    elif state is not None:
+        raise ValueError("process_logits: state needs masks (allowed)")
+    if out is None:
+        out = torch.empty(N, -(-V // 64) * 64, device=dev, dtype=torch.float16)[:, :V]  # rows start aligned for the sampler
+        ldo = out.stride(0)
+    else:
+        ldo = _rows_of(out, N, V, dev, "process_logits", "out")
+    if N:
+        _call_on(dev, "ecd_process_logits", logits.data_ptr(), ld, guided, cfg if guided else 1.0, hp or None, hrow, htok, T,
+                 lp or None, window, rp or None, pp or None, fp or None, flags, bp or None, ldb, ap or None, lda, A, sp or None,
+                 out.data_ptr(), ldo, N, V)
+    return out

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _ffi
-from .kernels import stream_ptr
+from .kernels import INT_MOST, _call_on, stream_ptr
 
 AUDIO_VOCAB = 8197
 N_CB = 8
@@ -28,6 +28,34 @@ def q8_rows(t: torch.Tensor):
     _ffi.call("ecd_quantize_rows_i8", tf.data_ptr(), q.data_ptr(), s.data_ptr(), None, N, K,
               stream_ptr(tf.device))
     return q, s
+
+
+_Q4_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def q4_rows(t: torch.Tensor, group: int = 128, zeros: bool = False):
+    """t [N, K] (float32, float16 or bfloat16, ROCm device) -> (q4 uint8 [N, K / 2], s4 float16 [N, K / group rounded up],
+    z4 uint8 of the same shape or None): weights of 4 bits with a scale, and with ``zeros`` a zero point, for each ``group``
+    (32, 64 or 128) of a row.  Element 2 i is in the low half of byte i and stands for s4 (code - z4), z4 = 8 without
+    zeros; include/ecdecode.h gives the rounding.  K is a multiple of 64."""
+    if not t.is_cuda:
+        raise RuntimeError("q4_rows runs on a ROCm GPU tensor")
+    if t.dtype not in _Q4_TYPES:
+        raise TypeError(f"q4_rows: expected float32, float16 or bfloat16, got {t.dtype}")
+    if t.dim() != 2 or t.shape[1] % 64 or not 0 < t.shape[1] <= INT_MOST or not 0 < t.shape[0] <= INT_MOST:
+        raise ValueError("q4_rows: t must be [N, K] with K a multiple of 64")
+    if group not in (32, 64, 128):
+        raise ValueError("q4_rows: the group must be 32, 64 or 128")
+    t = t.contiguous()
+    if t.data_ptr() % 16:
+        t = t.clone()
+    N, K = t.shape
+    q = torch.empty(N, K // 2, device=t.device, dtype=torch.uint8)
+    s = torch.empty(N, -(-K // group), device=t.device, dtype=torch.float16)
+    z = torch.empty_like(s, dtype=torch.uint8) if zeros else None
+    _call_on(t.device, "ecd_quantize_rows_q4", t.data_ptr(), _Q4_TYPES[t.dtype], q.data_ptr(), s.data_ptr(),
+             None if z is None else z.data_ptr(), N, K, int(group))
+    return q, s, z
 
 
 def _stack_shapes(prefix, cfg):

@@ -684,6 +684,41 @@ int ecd_gemm_a8_tuned(const void* c, long ldc, const float* sx, const void* wp, 
 int ecd_gemm_a8_silu(const void* c, long ldc, const float* sx, const void* wp, const void* s, void* mm, long ldm,
                      int M, int F, int K, void* stream);
 
+/* Weights of 4 bits in groups: w[n, k] = s[n, g] (u[n, k] - z[n, g]), u in 0 .. 15, g = k / group, group 32, 64 or 128,
+ * K % 64 == 0 (the last group of a row may be short); ng = ceil(K / group) groups.
+ *   q [N, K / 2] uint8, element 2 i in the low half of byte i; s [N, ng] f16; z [N, ng] uint8, or NULL: z = 8 everywhere.
+ * The quantiser takes w [N, K] of f32, f16 or bf16 (type 0, 1, 2), 16-byte aligned.  Without z: s = f16(max |w| / 7),
+ * u = 8 + rint(w / s).  With z: lo = min(0, min w), hi = max(0, max w), s = f16((hi - lo) / 15), z = rint(-lo / s),
+ * u = z + rint(w / s).  u and z are kept in 0 .. 15; the codes are those of the stored scale, exact ties go to the even
+ * integer; a group with an infinity, a NaN or a scale past f16 gets the scale NaN. */
+int ecd_quantize_rows_q4(const void* w, int type, void* q, void* s, void* z, int N, int K, int group, void* stream);
+
+/* The layout that ecd_mm_q4 reads: codes of ecd_packed_bytes_q4(N, K) bytes; scales of ng * 32 ceil(N / 32) f16, twice as many
+ * with zero points; both 16-byte aligned.  interleave: rows n and N / 2 + n become rows 2 n and 2 n + 1 (N even). */
+long ecd_packed_bytes_q4(int N, int K);
+int ecd_pack_q4(const void* q, const void* s, const void* z, int N, int K, int group, int interleave, void* codes, void* scales,
+                void* stream);
+
+/* y[m, n] = f16(sum_k x'[m, k] w[n, k] (+ res[m, n])) with x' = x, or with nw [K] the RMS norm of its rows; sums, scales and the
+ * residual in fp32.  silu: N is 2 F interleaved rows, y [M, F] = f16(silu(a) b) of the pairs (a, b), no res.
+ *   x rows and nw 16-byte aligned; zeros: whether the weights were packed with zero points. */
+int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* codes, const void* scales, int zeros, int group,
+              const void* res, long ldr, void* y, long ldy, int M, int N, int K, int silu, void* stream);
+
+/* Logits for the sampler: out[r, v], in fp32 with one rounding, of l = logits[r, v], or guided:
+ * l = u + (logits[r, v] - u) cfg with u = logits[N + r, v];
+ * where v occurs n > 0 times in the row's history: l = l > 0 ? l / rep : l * rep, l = l - (pres + freq n);
+ * l = l + bias[r * ldb + v] (ldb 0: one bias for all rows); -inf where a mask does not allow v, whatever the logit is.
+ *   hist: token t of row r at hist[r hrow + t htok], t < T; the last `window` (0: all) of its first length[r] (NULL: T) tokens
+ *   count, those outside [0, V) for nothing; rep, pres, freq: f32, bit 0, 1, 2 of per_row: an element per row (else one; NULL: 1, 0, 0);
+ *   allowed [A] rows of ceil(V / 32) words (row stride lda), bit v & 31 of word v >> 5: v is allowed; state [N]: each row's mask,
+ *   -1: none, any other outside [0, A): nothing is allowed; without state A is 1 (all rows) or N (row r's mask is r).
+ *   out may be the rows of logits themselves (same address and stride).  N <= 65535. */
+int ecd_process_logits(const void* logits, long ld, int guided, float cfg, const int64_t* hist, long hrow, long htok, int T,
+                       const int64_t* length, int window, const float* rep, const float* pres, const float* freq, int per_row,
+                       const float* bias, long ldb, const uint32_t* allowed, long lda, int A, const int32_t* state, void* out,
+                       long ldo, int N, int V, void* stream);
+
 /* Library version string (static storage). */
 const char* ecd_version(void);
 

@@ -1,0 +1,64 @@
+"""What the entries of 4-bit weights and of logits refuse, and what the calls refuse without a GPU: host logic."""
+import pytest
+import torch
+
+I, N = -22, -95
+
+
+def mm(**kw):
+    d = dict(x=16, ldx=64, nw=None, eps=1e-5, codes=16, scales=16, zeros=0, group=64, res=None, ldr=0, y=16, ldy=32, M=1, N=32,
+             K=64, silu=0)
+    d.update(kw)
+    return lambda L: L.ecd_mm_q4(*d.values(), None)
+
+
+def lg(**kw):
+    d = dict(logits=8, ld=100, guided=0, cfg=1.0, hist=None, hrow=0, htok=0, T=0, length=None, window=0, rep=None, pres=None,
+             freq=None, per_row=0, bias=None, ldb=0, allowed=None, lda=0, A=0, state=None, out=8, ldo=100, N=4, V=100)
+    d.update(kw)
+    return lambda L: L.ecd_process_logits(*d.values(), None)
+
+
+@pytest.mark.parametrize("want,call", [
+    (I, lambda L: L.ecd_quantize_rows_q4(None, 0, 16, 16, None, 1, 64, 64, None)),
+    (I, lambda L: L.ecd_quantize_rows_q4(16, 3, 16, 16, None, 1, 64, 64, None)),        # no such type
+    (I, lambda L: L.ecd_quantize_rows_q4(16, 0, 16, 16, None, 1, 96, 32, None)),        # K % 64
+    (I, lambda L: L.ecd_quantize_rows_q4(16, 0, 16, 16, None, 1, 64, 16, None)),        # group
+    (I, lambda L: L.ecd_quantize_rows_q4(24, 0, 16, 16, None, 1, 64, 64, None)),        # alignment
+    (I, lambda L: L.ecd_quantize_rows_q4(16, 0, 16, 16, None, 0, 64, 64, None)),
+    (N, lambda L: L.ecd_quantize_rows_q4(16, 0, 16, 16, None, 0x7FFFFFFF, 1 << 20, 64, None)),
+    (I, lambda L: L.ecd_pack_q4(16, None, None, 32, 64, 64, 0, 16, 16, None)),
+    (I, lambda L: L.ecd_pack_q4(16, 16, None, 31, 64, 64, 1, 16, 16, None)),            # odd rows to interleave
+    (I, lambda L: L.ecd_pack_q4(16, 16, None, 32, 64, 48, 0, 16, 16, None)),
+    (I, lambda L: L.ecd_pack_q4(16, 16, None, 32, 64, 64, 0, 24, 16, None)),
+    (N, lambda L: L.ecd_pack_q4(16, 16, None, 0x7FFFFFF0, 64, 64, 0, 16, 16, None)),
+    (I, mm(x=None)), (I, mm(codes=None)), (I, mm(scales=None)), (I, mm(y=None)), (I, mm(M=0)), (I, mm(N=0)), (I, mm(K=0)),
+    (I, mm(K=96, ldx=96)), (I, mm(ldx=56)), (I, mm(ldx=68)), (I, mm(x=24)), (I, mm(nw=24)), (I, mm(codes=24)),
+    (I, mm(scales=24)), (I, mm(group=256)), (I, mm(ldy=31)), (I, mm(res=16, ldr=31)), (I, mm(silu=1, N=31)),
+    (I, mm(silu=1, res=16, ldr=32)), (I, mm(nw=16, eps=-1.0)), (I, mm(nw=16, eps=float("nan"))),
+    (I, lg(logits=None)), (I, lg(out=None)), (I, lg(N=0)), (I, lg(V=0)), (I, lg(ld=99)), (I, lg(ldo=99)), (I, lg(window=-1)),
+    (I, lg(T=-1)), (I, lg(rep=8)), (I, lg(pres=8)), (I, lg(freq=8)), (I, lg(hist=8, hrow=-1)), (I, lg(bias=8, ldb=99)),
+    (I, lg(allowed=8, lda=3, A=1)), (I, lg(allowed=8, lda=4, A=0)), (I, lg(allowed=8, lda=4, A=3)),
+    (N, lg(N=65536)),
+])
+def test_entries_refuse_on_the_host(want, call):
+    from estudiocanciones_amd import _ffi
+    assert call(_ffi.lib()) == want
+
+
+def test_packed_bytes():
+    from estudiocanciones_amd import _ffi
+    L = _ffi.lib()
+    assert [L.ecd_packed_bytes_q4(n, k) for n, k in ((1, 64), (32, 64), (33, 64), (8197, 3072), (1, 65), (0, 64))] == \
+        [1024, 1024, 2048, 257 * 48 * 1024, 0, 0]
+    assert L.ecd_packed_bytes_q4(1 << 20, 1 << 16) == 1 << 35  # (past 32 bits)
+
+
+def test_calls_refuse_tensors_that_are_not_on_a_gpu():
+    from estudiocanciones_amd import kernels as K
+    from estudiocanciones_amd.quant import q4_rows
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    for call in (lambda: q4_rows(x), lambda: K.pack_q4(torch.zeros(4, 32, dtype=torch.uint8), x[:, :1]),
+                 lambda: K.process_logits(x)):
+        with pytest.raises(RuntimeError):
+            call()
