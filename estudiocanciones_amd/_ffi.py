@@ -132,7 +132,10 @@ SIGNATURES = {
     "ecd_quantize_rows_q4": [_P, c_int, _P, _P, _P, c_int, c_int, c_int, _P],
     "ecd_packed_bytes_q4": [c_int, c_int],
     "ecd_pack_q4": [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P],
-    "ecd_mm_q4": [_P, c_long, _P, c_float, _P, _P, c_int, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P],
+    "ecd_mm_q4": [_P, c_long, _P, c_float, _P, _P, c_int, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int,
+                  c_int, _P, _P],
+    "ecd_mm_q4_plan": [c_int, c_int, c_int],
+    "ecd_mm_q4_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
     "ecd_process_logits": [_P, c_long, c_int, c_float, _P, c_long, c_long, c_int, _P, c_int, _P, _P, _P, c_int, _P, c_long, _P,
                            c_long, c_int, _P, _P, c_long, c_int, c_int, _P],
 }
@@ -157,7 +160,8 @@ def lib() -> ctypes.CDLL:
             fn = getattr(handle, name)
             fn.argtypes = argtypes
             fn.restype = c_long if name.startswith("ecd_packed_bytes") or \
-                name in ("ecd_layer_tail_ws_bytes", "ecd_layer_stack_plan_bytes") else c_int
+                name in ("ecd_layer_tail_ws_bytes", "ecd_layer_stack_plan_bytes",
+                                                        "ecd_mm_q4_ws_bytes") else c_int
         handle.ecd_version.argtypes = []
         handle.ecd_version.restype = ctypes.c_char_p
         _lib = handle

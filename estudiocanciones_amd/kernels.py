@@ -1185,6 +1185,16 @@ class PackedQ4:
         self.N, self.K, self.group, self.zeros, self.interleave = N, K, group, zeros, interleave
         self.dev = codes.device
         self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+        self._plans = {}
+
+    def plan(self, M):
+        """(kernel choice, workspace bytes without and with a norm) of a product of M rows."""
+        p = self._plans.get(M)
+        if p is None:
+            lib = _ffi.lib()
+            n = lib.ecd_mm_q4_plan(M, self.N, self.K)
+            p = self._plans[M] = (n, *(lib.ecd_mm_q4_ws_bytes(M, self.N, self.K, n, f) for f in (0, 1)))
+        return p
 
     @property
     def nbytes(self):
@@ -1241,8 +1251,11 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         if _ends(out)[0] < _ends(x)[1] and _ends(x)[0] < _ends(out)[1]:
             raise ValueError(f"{name}: out must not overlap x")
     if M:
+        plan, *nb = w.plan(M)
+        nb = nb[nw is not None]
+        ws = torch.empty(nb, device=dev, dtype=torch.uint8) if nb else None  # (held until the launch)
         _call_on(dev, "ecd_mm_q4", x.data_ptr(), ldx, _ptr(nw), eps, w.codes_ptr, w.scales_ptr, w.zeros, w.group, _ptr(res), ldr,
-                 y.data_ptr(), ldy, M, w.N, K, silu)
+                 y.data_ptr(), ldy, M, w.N, K, silu, plan, _ptr(ws))
     return y
 
 

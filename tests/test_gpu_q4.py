@@ -49,7 +49,7 @@ def sums_tol(x, w, norm):
 def check(got, want, tol, what="", floor=0.0):
     got = got.double().cpu().numpy()
     err = np.abs(got - want)
-    bad = err > tol + H * (np.abs(want) + tol) + 2.0 ** -25
+    bad = ~(err <= tol + H * (np.abs(want) + tol) + 2.0 ** -25)
     assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, worst {np.nanmax(err)} at {np.argwhere(bad)[0]}"
     if want.size >= 2000:
         # at most four independent roundings of H / sqrt(3) each on the average value; among the subnormal numbers a rounding is
@@ -145,7 +145,9 @@ def test_quantiser_takes_views(dev):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M", [5, 13, 40, 192])
 def test_single_weights_come_out_exactly(dev, M, group, zeros):
-    """Rows that hold one 1 give single weights: fp16(s (u - z)), the nearest fp16."""
+    """Rows that hold one 1 give single weights s (u - z), rounded to fp16 once: the nearest fp16, or with many rows its other
+    neighbour where the weight (of 16 bits) lies so near the middle that the quotients of scales (K / 32 at most, each off by
+    2^-22 with its reciprocal, and a product each) pass it."""
     from estudiocanciones_amd.kernels import mm_q4
     N, K = 75, 192
     q, s, z, w = make(M + group, N, K, group, zeros)
@@ -155,9 +157,14 @@ def test_single_weights_come_out_exactly(dev, M, group, zeros):
         ks = np.arange(k0, min(k0 + M, K))
         x[np.arange(len(ks)), ks] = 1
         y = mm_q4(_t(x, dev), wp).cpu().numpy()
-        want = np.zeros((M, N), np.float16)
-        want[:len(ks)] = w[:, ks].T.astype(np.float16)
-        assert np.array_equal(y, want)
+        want = np.zeros((M, N))
+        want[:len(ks)] = w[:, ks].T
+        if M <= 16:
+            assert np.array_equal(y, want.astype(np.float16))
+        else:
+            # half a step at the magnitude of the weight (2^-11 of its power of two), widened by the quotients' 6 (2^-22 + 2^-24)
+            step = 2.0 ** np.floor(np.log2(np.maximum(np.abs(want), 2.0 ** -14))) * H
+            assert (np.abs(y.astype(np.float64) - want) <= step + 2.0 ** -19 * np.abs(want)).all()
 
 
 SHAPES = [(1, 1, 64), (1, 33, 64), (2, 1001, 192), (7, 31, 320), (8, 512, 1024), (9, 77, 8192), (16, 1024, 448), (17, 40, 64),
@@ -181,6 +188,38 @@ def test_products(dev, M, N, K, group, zeros):
     check(mm_q4(_t(x * np.float16(3), dev), wp, nw=_t(nw, dev)), xn @ w.T, sums_tol(xn, w, True), "norm")
 
 
+@pytest.mark.parametrize("tile", range(1, 7))
+@pytest.mark.parametrize("M,N,K,ks", [(5, 40, 64, 1), (37, 300, 320, 1), (37, 300, 320, 3), (150, 129, 1088, 1), (150, 129, 1088, 5),
+                                      (300, 520, 192, 2), (8, 64, 832, 13)])
+@pytest.mark.parametrize("group,zeros,silu", [(32, True, False), (64, False, True), (128, True, True), (128, False, False)])
+def test_every_tile(dev, tile, M, N, K, ks, group, zeros, silu):
+    """The kernels of many rows that the sizes' own plan need not choose: K of an odd number of chunks, split in uneven parts."""
+    import torch
+    from estudiocanciones_amd import _ffi
+    q, s, z, w = make(M + N + K, N, K, group, zeros)
+    wp = packed(dev, q, s, z, silu and N % 2 == 0)
+    silu = wp.interleave
+    x, nw = randn16(M, M, K), (1 + 0.1 * rng(K).standard_normal(K)).astype(np.float16)
+    cols = N // 2 if silu else N
+    xt, nt, st = _t(x, dev), _t(nw, dev), torch.cuda.current_stream().cuda_stream
+    plan = tile + 256 * ks
+    ws = torch.full((_ffi.lib().ecd_mm_q4_ws_bytes(M, N, K, plan, 1) // 4,), float("nan"), device=dev)
+    for norm in (False, True):
+        y = torch.full((M + 1, cols), 7.0, device=dev, dtype=torch.float16)
+        _ffi.call("ecd_mm_q4", xt.data_ptr(), K, nt.data_ptr() if norm else None, 1e-5, wp.codes_ptr, wp.scales_ptr, zeros, group,
+                  None, 0, y.data_ptr(), cols, M, N, K, silu, plan, ws.data_ptr(), st)
+        xn = norm64(x, nw) if norm else x.astype(np.float64)
+        want, tol = xn @ w.T, sums_tol(xn, w, norm)
+        if silu:
+            a, b, ta, tb = want[:, :cols], want[:, cols:], tol[:, :cols], tol[:, cols:]
+            f = a / (1 + np.exp(-a))
+            want, tol = f * b, (1.1 * ta + 2.0 ** -20 * np.abs(f)) * (np.abs(b) + tb) + np.abs(f) * tb
+        got = y[:M].double().cpu().numpy()
+        bad = ~(np.abs(got - want) <= tol + H * (np.abs(want) + tol) + 2.0 ** -25)
+        assert not bad.any(), (norm, bad.sum(), np.argwhere(bad)[0])
+        assert (y[M] == 7.0).all()
+
+
 @pytest.mark.parametrize("M,F,K", [(1, 1, 64), (1, 4099, 192), (3, 17, 192), (8, 512, 1024), (16, 40, 320), (30, 33, 64), (33, 500, 192),
                                    (64, 64, 128), (70, 65, 1024), (187, 1001, 320), (300, 256, 512)])
 @pytest.mark.parametrize("group,zeros,norm", [(32, True, True), (64, False, False), (128, False, True), (128, True, False)])
@@ -201,7 +240,7 @@ def test_silu(dev, M, F, K, group, zeros, norm):
     if M > 64:
         tol += H * np.abs(f) * np.abs(b)
     got = mm_q4_silu(_t(x, dev), packed(dev, q, s, z, True), nw=None if nw is None else _t(nw, dev)).double().cpu().numpy()
-    bad = np.abs(got - f * b) > tol + H * (np.abs(f * b) + tol) + 2.0 ** -25
+    bad = ~(np.abs(got - f * b) <= tol + H * (np.abs(f * b) + tol) + 2.0 ** -25)
     assert not bad.any(), (bad.sum(), np.argwhere(bad)[0])
 
 

@@ -7,7 +7,7 @@ I, N = -22, -95
 
 def mm(**kw):
     d = dict(x=16, ldx=64, nw=None, eps=1e-5, codes=16, scales=16, zeros=0, group=64, res=None, ldr=0, y=16, ldy=32, M=1, N=32,
-             K=64, silu=0)
+             K=64, silu=0, plan=0, ws=None)
     d.update(kw)
     return lambda L: L.ecd_mm_q4(*d.values(), None)
 
@@ -36,6 +36,9 @@ def lg(**kw):
     (I, mm(K=96, ldx=96)), (I, mm(ldx=56)), (I, mm(ldx=68)), (I, mm(x=24)), (I, mm(nw=24)), (I, mm(codes=24)),
     (I, mm(scales=24)), (I, mm(group=256)), (I, mm(ldy=31)), (I, mm(res=16, ldr=31)), (I, mm(silu=1, N=31)),
     (I, mm(silu=1, res=16, ldr=32)), (I, mm(nw=16, eps=-1.0)), (I, mm(nw=16, eps=float("nan"))),
+    (I, mm(M=17)), (I, mm(plan=7 + 256)), (I, mm(plan=1)), (I, mm(plan=1 + 512)), (I, mm(plan=-1)),  # plans: K / 64 ways at most
+    (I, mm(plan=1 + 512, K=128, ldx=128)), (I, mm(plan=1 + 512, K=128, ldx=128, ws=24)), (I, mm(plan=1 + 256, nw=16)),  # no workspace
+    (N, mm(ldx=1 << 27)), (N, mm(plan=1 + 256, ldx=1 << 27, M=99)), (N, mm(plan=1 + 256, K=1 << 24, ldx=1 << 24)),
     (I, lg(logits=None)), (I, lg(out=None)), (I, lg(N=0)), (I, lg(V=0)), (I, lg(ld=99)), (I, lg(ldo=99)), (I, lg(window=-1)),
     (I, lg(T=-1)), (I, lg(rep=8)), (I, lg(pres=8)), (I, lg(freq=8)), (I, lg(hist=8, hrow=-1)), (I, lg(bias=8, ldb=99)),
     (I, lg(allowed=8, lda=3, A=1)), (I, lg(allowed=8, lda=4, A=0)), (I, lg(allowed=8, lda=4, A=3)),
@@ -52,6 +55,27 @@ def test_packed_bytes():
     assert [L.ecd_packed_bytes_q4(n, k) for n, k in ((1, 64), (32, 64), (33, 64), (8197, 3072), (1, 65), (0, 64))] == \
         [1024, 1024, 2048, 257 * 48 * 1024, 0, 0]
     assert L.ecd_packed_bytes_q4(1 << 20, 1 << 16) == 1 << 35  # (past 32 bits)
+
+
+def test_plans():
+    """Few rows run without a plan of tiles; every plan names a tile and a split that the product takes; the workspace holds the
+    parts and the normed rows."""
+    from estudiocanciones_amd import _ffi
+    L = _ffi.lib()
+    for M, N, K in [(1, 1, 64), (8, 16384, 3072), (16, 1024, 4096), (16, 1024, 8192), (17, 33, 64), (48, 3072, 3072),
+                    (187, 3072, 8192), (2048, 16384, 3072), (100000, 8197, 1024), (30, 2000000, 128)]:
+        p = L.ecd_mm_q4_plan(M, N, K)
+        if M <= 8:
+            assert p == 0
+        if M > 16:
+            assert p > 0
+        if p:
+            tile, ks = p & 255, p >> 8
+            assert 1 <= tile <= 6 and 1 <= ks <= K // 64
+            part = ks * M * (-(-N // 8) * 8) * 4 if ks > 1 else 0
+            assert L.ecd_mm_q4_ws_bytes(M, N, K, p, 0) == part and L.ecd_mm_q4_ws_bytes(M, N, K, p, 1) == part + 2 * M * K
+    assert L.ecd_mm_q4_ws_bytes(8, 64, 64, 0, 1) == 0
+    assert [L.ecd_mm_q4_plan(*a) for a in ((0, 1, 64), (1, 0, 64), (1, 1, 65), (1, 1, 0))] == [-22] * 4
 
 
 def test_calls_refuse_tensors_that_are_not_on_a_gpu():
