@@ -11,18 +11,23 @@ kept in bf16, and with ``--keep-emb-bf16`` the ``text_embeddings`` / ``audio_emb
 too (app/convert_final.py:43, :66).  The file metadata carries
 ``{"lite": "{\\"mode\\": \\"int8\\"}"}``.
 
+With ``--int4`` the backbone's linear layers (most of the weights, read once per frame) become 4-bit codes
+``<name>.q4`` [N, K / 2] with fp16 scales ``<name>.s4`` per group of 128 (``--group``: 32 or 64) and, with ``--zeros``, zero
+points ``<name>.z4`` (``quant.q4_rows``); embeddings, heads and the depth decoder stay as they are.  The
+metadata's mode is then "int4".
+
     python -m estudiocanciones_amd.convert <HeartMuLa dir | model.safetensors> <out.safetensors>
-        [--keep-emb-bf16]
+        [--keep-emb-bf16] [--int4 [--group 128] [--zeros]]
 """
 from __future__ import annotations
 
+import argparse
 import json
-import sys
 from pathlib import Path
 
 import torch
 
-from .quant import q8_rows
+from .quant import q4_rows, q8_rows
 
 DROPPED = ("muq_linear.weight",)
 KEPT_DENSE = ("unconditional_text_embedding.weight",)
@@ -37,9 +42,16 @@ def _quantise(t: torch.Tensor, device) -> tuple[torch.Tensor, torch.Tensor]:
     return q.cpu(), s.cpu()
 
 
-def convert_tensors(items, device="cuda", keep_emb=False) -> dict:
+def _four(name: str) -> bool:
+    """The layers that --int4 stores in 4 bits."""
+    return name.startswith("backbone.layers.") and name.endswith("_proj.weight") or \
+        name.startswith("backbone.layers.") and ".mlp.w" in name
+
+
+def convert_tensors(items, device="cuda", keep_emb=False, group=None, zeros=False) -> dict:
     """(name, tensor) pairs of the official checkpoint -> {name: tensor} of the int8 format;
-    ``keep_emb`` keeps the embedding tables in bf16."""
+    ``keep_emb`` keeps the embedding tables in bf16; ``group``: the backbone's linear layers in 4 bits with a
+    scale (and with ``zeros`` a zero point) per group of so many weights."""
     dev = torch.device(device)
     out = {}
     for name, t in items:
@@ -48,6 +60,11 @@ def convert_tensors(items, device="cuda", keep_emb=False) -> dict:
         if name == "audio_head":
             for i in range(t.shape[0]):
                 out[f"audio_head.{i}.q8"], out[f"audio_head.{i}.s8"] = _quantise(t[i].t(), dev)
+        elif group is not None and t.dim() == 2 and _four(name):
+            q, s, z = q4_rows(t.to(device=dev, dtype=torch.float32), group, zeros)
+            out[name + ".q4"], out[name + ".s4"] = q.cpu(), s.cpu()
+            if zeros:
+                out[name + ".z4"] = z.cpu()
         elif t.dim() == 2 and name not in KEPT_DENSE and not (keep_emb and "embeddings" in name):
             out[name + ".q8"], out[name + ".s8"] = _quantise(t, dev)
         else:
@@ -67,7 +84,7 @@ def checkpoint_files(src) -> list[Path]:
     return [src / "model.safetensors"]
 
 
-def convert_file(src, dst, device="cuda", keep_emb=False) -> Path:
+def convert_file(src, dst, device="cuda", keep_emb=False, group=None, zeros=False) -> Path:
     """Convert an official checkpoint (directory or file) into ``dst``."""
     from safetensors import safe_open
     from safetensors.torch import save_file
@@ -78,15 +95,20 @@ def convert_file(src, dst, device="cuda", keep_emb=False) -> Path:
                 for k in f.keys():
                     yield k, f.get_tensor(k)
 
-    out = convert_tensors(items(), device, keep_emb)
+    out = convert_tensors(items(), device, keep_emb, group, zeros)
     dst = Path(dst)
-    save_file(out, str(dst), metadata={"lite": json.dumps({"mode": "int8"})})
+    save_file(out, str(dst), metadata={"lite": json.dumps({"mode": "int8" if group is None else "int4"})})
     return dst
 
 
 if __name__ == "__main__":
-    args = [a for a in sys.argv[1:] if a != "--keep-emb-bf16"]
-    if len(args) != 2:
-        raise SystemExit(__doc__)
-    path = convert_file(args[0], args[1], keep_emb="--keep-emb-bf16" in sys.argv)
+    ap = argparse.ArgumentParser(usage=__doc__, add_help=False)
+    ap.add_argument("src")
+    ap.add_argument("dst")
+    ap.add_argument("--keep-emb-bf16", action="store_true")
+    ap.add_argument("--int4", action="store_true")
+    ap.add_argument("--group", type=int, choices=(32, 64, 128), default=128)
+    ap.add_argument("--zeros", action="store_true")
+    a = ap.parse_args()
+    path = convert_file(a.src, a.dst, keep_emb=a.keep_emb_bf16, group=a.group if a.int4 else None, zeros=a.zeros)
     print(path.name, round(path.stat().st_size / 1e9, 3), "GB")

@@ -44,13 +44,24 @@ struct LogitsArgs {
 template <int TH>
 __global__ __launch_bounds__(TH) void process_logits_kernel(const LogitsArgs a) {
   __shared__ __align__(16) uint32_t count[8 * TH];
-  const int r = blockIdx.y, v0 = blockIdx.x * a.seg, v1 = min(v0 + a.seg, a.V), i = v0 + 8 * threadIdx.x;
-  const bool on = i < v1, full = i + 8 <= v1;
+  const int r = blockIdx.y, v0 = blockIdx.x * a.seg, v1 = min(v0 + a.seg, a.V);
   const f16* lc = a.logits + (long)r * a.ld;
   const f16* lu = a.logits + (long)(r + a.N) * a.ld;
+  const float* bp = a.bias ? a.bias + (long)r * a.ldb : nullptr;
+  // a state outside the masks allows nothing, -1 everything
+  uint32_t keep = 0xFFu;
+  const uint32_t* mask = nullptr;
+  if (a.allowed) {
+    const int s = a.state ? a.state[r] : a.A == 1 ? 0 : r;
+    if (s >= a.A || s < -1)
+      keep = 0u;
+    else if (s >= 0)
+      mask = a.allowed + (long)s * a.lda;
+  }
+  const int i = v0 + 8 * (int)threadIdx.x;
+  const bool on = i < v1, full = i + 8 <= v1;
   f16x8 c = {0, 0, 0, 0, 0, 0, 0, 0}, u = c;
   float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const float* bp = a.bias ? a.bias + (long)r * a.ldb : nullptr;
   if (full) {
     c = *(const f16x8u*)(lc + i);
     if (a.guided) u = *(const f16x8u*)(lu + i);
@@ -71,16 +82,7 @@ __global__ __launch_bounds__(TH) void process_logits_kernel(const LogitsArgs a) 
         if (bp) b[j] = bp[i + j];
       }
   }
-  // a state outside the masks allows nothing, -1 everything
-  uint32_t keep = 0xFFu;
-  if (a.allowed) {
-    const int s = a.state ? a.state[r] : a.A == 1 ? 0 : r;
-    if (s >= a.A || s < -1)
-      keep = 0u;
-    else if (s >= 0 && on)
-      keep = a.allowed[(long)s * a.lda + (i >> 5)] >> (i & 31);
-  }
-  uint32_t n[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+  if (mask && on) keep = mask[i >> 5] >> (i & 31);
   float rep = 1.f, pres = 0.f, freq = 0.f;
   if (a.hist) {
     const int64_t len = a.length ? a.length[r] : a.T;
@@ -92,20 +94,29 @@ __global__ __launch_bounds__(TH) void process_logits_kernel(const LogitsArgs a) 
     u32x4* const mine = (u32x4*)(count + 8 * threadIdx.x);
     mine[0] = mine[1] = (u32x4){0u, 0u, 0u, 0u};
     __syncthreads();
+    // HB loads of a thread in flight: tokens of a song's frames lie in lines of their own
+    constexpr int HB = 4;
     const int64_t* hp = a.hist + (long)r * a.hrow;
-    for (int t = t0 + (int)threadIdx.x; t < t1; t += TH) {
-      const int64_t v = hp[(long)t * a.htok];
-      if (v >= v0 && v < v1) atomicAdd(&count[(int)(v - v0)], 1u);
+    for (int t = t0 + (int)threadIdx.x; t < t1; t += HB * TH) {
+      int64_t v[HB];
+#pragma unroll
+      for (int k = 0; k < HB; ++k) v[k] = hp[(long)min(t + k * TH, t1 - 1) * a.htok];
+#pragma unroll
+      for (int k = 0; k < HB; ++k)
+        if (t + k * TH < t1 && v[k] >= v0 && v[k] < v1) atomicAdd(&count[(int)(v[k] - v0)], 1u);
     }
     __syncthreads();
-    const u32x4 n0 = mine[0], n1 = mine[1];
+  }
+  if (!on) return;
+  uint32_t n[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+  if (a.hist) {
+    const u32x4 n0 = *(const u32x4*)(count + 8 * threadIdx.x), n1 = *(const u32x4*)(count + 8 * threadIdx.x + 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       n[j] = n0[j];
       n[4 + j] = n1[j];
     }
   }
-  if (!on) return;
   f16x8 o;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -128,6 +139,15 @@ __global__ __launch_bounds__(TH) void process_logits_kernel(const LogitsArgs a) 
     store_tail(op, nullptr, o, v1 - i);
 }
 
+template <int TH>
+static int launch_logits(LogitsArgs a, hipStream_t st) {
+  constexpr int SEG = 8 * TH;
+  const int parts = (a.V + SEG - 1) / SEG;
+  a.seg = ((a.V + parts - 1) / parts + 7) / 8 * 8;
+  hipLaunchKernelGGL((process_logits_kernel<TH>), dim3((a.V + a.seg - 1) / a.seg, a.N), dim3(TH), 0, st, a);
+  return ecd_launch_status();
+}
+
 }  // namespace ecd
 
 using namespace ecd;
@@ -140,11 +160,14 @@ extern "C" int ecd_process_logits(const void* logits, long ld, int guided, float
       ((rep || pres || freq) && !hist) || (bias && ldb != 0 && ldb < V) ||
       (allowed && (A <= 0 || lda < (V + 31L) / 32 || (!state && A != 1 && A != N))))
     return ECD_EINVAL;
-  if (N > 65535 || V > 0x7FFFFFFF - 8192) return ECD_ENOTSUP;
-  constexpr int TH = 256, SEG = 8 * TH;
-  const int parts = (V + SEG - 1) / SEG, seg = ((V + parts - 1) / parts + 7) / 8 * 8;
+  if (N > 65535 || V > 0x7FFFFFFF - 8192 || T > 1 << 30) return ECD_ENOTSUP;
   const LogitsArgs a{(const f16*)logits, ld, cfg, guided, hist, hrow, htok, T, length, window, rep, pres, freq, per_row, bias, ldb,
-                     allowed, lda, A, state, (f16*)out, ldo, N, V, seg};
-  hipLaunchKernelGGL(process_logits_kernel<TH>, dim3((V + seg - 1) / seg, N), dim3(TH), 0, (hipStream_t)stream, a);
-  return ecd_launch_status();
+                     allowed, lda, A, state, (f16*)out, ldo, N, V, 0};
+  const hipStream_t st = (hipStream_t)stream;
+  // A workgroup's history costs a line of memory per token, or a 16th of one where tokens are neighbours.  Segments of 2048 tokens
+  // by 256 threads give short histories the most parallelism; for long ones, and for many rows of them, segments of 8192
+  // by 1024 threads read them fewer times (us: 4 rows of 3000 frames 8.0 and 5.7, 128 of 750 12.0 and 8.8, 32 rows of 4096
+  // neighbours over 100003 tokens 10.7 and 9.4; 1 row of 750 frames 3.7 and 4.4, 8 of 2000 neighbours over 40000 3.9 and 5.1).
+  const long lines = hist ? (window && window < T ? window : T) / (htok == 1 ? 16 : 1) : 0;
+  return lines > 1500 || lines * N * ((V + 2047) / 2048) > 300000 ? launch_logits<1024>(a, st) : launch_logits<256>(a, st);
 }

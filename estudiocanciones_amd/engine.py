@@ -25,6 +25,10 @@ reference, all deliberate:
 * ``generate(paged=True)`` computes the prompt once for all takes and keeps its keys and values in
   pages that the takes share (paged.py); a frame's attention reads them once for all takes;
   ``generate(a8=True)`` runs the prompt's linear layers on int8 activations (one scale per row);
+* layers may hold weights of 4 bits with a scale per group (``<name>.q4`` / ``.s4`` / ``.z4`` in the weights,
+  convert.py ``--int4``): a stack of such layers runs mm_q4 and mm_q4_silu, prompt and frames alike;
+* ``generate`` takes penalties for codes that came before, biases, masks of allowed codes and a shortest
+  length; process_logits then works on each codebook's logits before the sampler;
 * the song loop keeps its bookkeeping on the device: the captured frame ends with a kernel
   that feeds the tokens back, stores the frame and records each take's first EOS frame, so
   the host only replays the graph and reads N integers every 25 frames.
@@ -39,13 +43,13 @@ from pathlib import Path
 import torch
 
 from . import _ffi
-from .kernels import (_attn, _attn_combine, _rope_cache, _silu_mul, cdiv, embed_gemv_packed,
+from .kernels import (INT_MOST, _attn, _attn_combine, _rope_cache, _silu_mul, cdiv, embed_gemv_packed,
                       gemm_a8_packed, gemm_a8_silu_packed, gemm_packed, gemm_rms_packed, gemm_silu_packed,
                       gemv_packed_splitk, paged_attn, paged_attn_plan, paged_write, prefill_attn, quant_a8,
                       gemm_rope_packed, gemv_packed, int8_mm, layer_head, layer_stack,
                       layer_stack_plan, layer_stack_supported, layer_tail, layer_tail_supported,
-                      layer_tail_ws_bytes, next_power_of_2,
-                      pack_i8, rms as krms, rms_gemv_packed, rms_qkv_rope, rms_qkv_rope_rows,
+                      layer_tail_ws_bytes, mm_q4, mm_q4_silu, next_power_of_2,
+                      pack_i8, pack_mask, pack_q4, process_logits, rms as krms, rms_gemv_packed, rms_qkv_rope, rms_qkv_rope_rows,
                       rms_w13_silu,
                       sample_topk, stream_ptr)
 from .paged import PagedCache
@@ -104,21 +108,29 @@ def rope_cache(head_dim: int, max_seq: int, base=500_000, scale=32, low=1, high=
 
 # ---------------------------------------------------------------- linear layers
 class Linear:
-    """int8 per-output-channel linear layer (app/engine.py:62-79)."""
+    """int8 per-output-channel linear layer (app/engine.py:62-79), or one of 4-bit weights with a scale (and with ``z4`` a zero
+    point) per group: q4 uint8 [N, K / 2], s4 fp16 [N, groups], z4 uint8 [N, groups] (quant.q4_rows)."""
 
-    def __init__(self, w=None, q8=None, s8=None):
-        if q8 is None:
-            raise NotImplementedError("the gfx950 decode path runs int8 per-channel weights only")
+    def __init__(self, w=None, q8=None, s8=None, q4=None, s4=None, z4=None):
+        if q8 is None and q4 is None:
+            raise NotImplementedError("the gfx950 decode path runs int8 per-channel or 4-bit group weights only")
         self.w, self.q8, self.s8 = None, q8, s8
-        self.qp = self.sp = None
-        self.N, self.K = q8.shape
+        self.q4, self.s4, self.z4 = q4, s4, z4
+        self.qp = self.sp = self.w4 = None
+        self.N, self.K = q8.shape if q8 is not None else (q4.shape[0], 2 * q4.shape[1])
         self.stream = False
         self.ks = 1
 
     def pack(self, interleave=False, stream=False):
         """Add the lane-ordered tile copy used by the fused GEMVs (K % 64 == 0).  With
         ``interleave`` the w1 | w3 halves become (a_j, b_j) row pairs (scales likewise).
-        ``stream``: the layer is read once per frame, so its loads bypass cache allocation."""
+        ``stream``: the layer is read once per frame, so its loads bypass cache allocation.
+        4-bit weights are laid out for mm_q4 and not kept in the given form."""
+        if self.q4 is not None:
+            self.w4 = pack_q4(self.q4, self.s4, self.z4, interleave)
+            self.q4 = self.s4 = self.z4 = None
+        if self.q8 is None:
+            return self
         self.stream = stream
         if self.K % 64:
             return self
@@ -134,6 +146,10 @@ class Linear:
         return self
 
     def __call__(self, x, res=None):
+        if self.q8 is None:
+            if self.w4 is None:
+                self.pack()
+            return mm_q4(x, self.w4, res=res)
         if self.qp is not None and self.sp is self.s8 and x.dim() == 2 and x.stride(1) == 1 \
                 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
             if self.ks > 1:
@@ -144,11 +160,19 @@ class Linear:
 
     @property
     def nbytes(self):
-        return self.q8.numel() + self.s8.numel() * 2
+        if self.w4 is not None:
+            return self.w4.nbytes
+        ts = (self.q8, self.s8, self.q4, self.s4, self.z4)
+        return sum(t.numel() * t.element_size() for t in ts if t is not None)
 
 
 def fuse(parts):
     """Row-concatenate layers that read the same input (q|k|v, w1|w3), app/engine.py:82-86."""
+    if any(p.q8 is None for p in parts):
+        if any(p.q4 is None for p in parts) or len({(p.s4.shape[1], p.z4 is None) for p in parts}) > 1:
+            raise ValueError("fuse: 4-bit layers that read the same input must have the same groups, all with zero points or none")
+        cat = lambda n: torch.cat([getattr(p, n) for p in parts]).contiguous()  # noqa: E731
+        return Linear(q4=cat("q4"), s4=cat("s4"), z4=None if parts[0].z4 is None else cat("z4"))
     return Linear(q8=torch.cat([p.q8 for p in parts]).contiguous(),
                   s8=torch.cat([p.s8 for p in parts]).contiguous())
 
@@ -281,8 +305,37 @@ class Stack:
             self._tail_buffers(2 * B, dev, dtype, L, share=self.tail)
 
     def packed(self):
-        """Whether every layer's weights are packed (what the paged cache and int8 activations need)."""
+        """Whether every layer's weights are packed (what the paged cache needs)."""
+        return self.eight() or self.four()
+
+    def eight(self):
+        """Whether every layer's weights are packed in 8 bits (what int8 activations need)."""
         return bool(self.blocks) and all(lin.qp is not None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2))
+
+    def four(self):
+        """Whether every layer's weights are packed in 4 bits."""
+        return bool(self.blocks) and all(getattr(lin, "w4", None) is not None for b in self.blocks
+                                         for lin in (b.qkv, b.o, b.w13, b.w2))
+
+    def _layer_q4(self, b, x, attend):
+        """A layer on 4-bit weights; attend: rows of q | k | v -> rows of the attention's output."""
+        o = attend(mm_q4(x, b.qkv.w4, nw=b.n1))
+        x = mm_q4(o, b.o.w4, res=x)
+        return mm_q4(mm_q4_silu(x, b.w13.w4, nw=b.n2), b.w2.w4, res=x)
+
+    def _dense_q4(self, x, pos, S, prompt):
+        """The layers on 4-bit weights over dense caches; ``prompt``: of many rows, whose attention is not split."""
+        tiles = prompt and self.prompt_heads()
+        for b in self.blocks:
+            def attend(qkv):
+                q = torch.empty(x.shape[0], b.h * b.hd, device=x.device, dtype=x.dtype)
+                _rope_cache[(x.shape[0], b.h + b.kvh)](qkv, self.rope, pos, q, b.kc, b.vc, S, b.h, b.kvh, b.kc.shape[2], HD=b.hd)
+                if tiles:
+                    return self._prompt_attn(b, q, b.kc, b.vc, pos, S)
+                return self._attention(b, q, pos, S, splits=1 if prompt else None)
+
+            x = self._layer_q4(b, x, attend)
+        return x
 
     def _dense(self, call):
         if self.paged is not None:
@@ -432,7 +485,9 @@ class Stack:
         B, S, D = x.shape
         x2 = x.reshape(B * S, D)
         p2 = pos.reshape(B * S).to(torch.int64).contiguous()
-        if (B * S > PROMPT_GEMM_ROWS or self.prompt_a8) and all(b.qkv.qp is not None for b in self.blocks):
+        if B * S > PROMPT_GEMM_ROWS and self.four():
+            h = krms(self._dense_q4(x2.contiguous(), p2, S, True), self.norm)
+        elif (B * S > PROMPT_GEMM_ROWS or self.prompt_a8) and all(b.qkv.qp is not None for b in self.blocks):
             h = self._prompt_pass(x2.contiguous(), p2, S)
         else:
             h = self.decode(x2, p2, S)
@@ -521,15 +576,23 @@ class Stack:
         b0 = self.blocks[0]
         kc = torch.empty(U, b0.kvh, S, b0.hd, device=dev, dtype=x.dtype)  # one layer's keys and values in order
         vc = torch.empty_like(kc)
+        four = self.four()
         for i, b in enumerate(self.blocks):
             kp, vp = cache.layer(i)
+
+            def attend(qkv):
+                q = paged_write(qkv, kp, vp, table, pos, S, b.h, b.kvh, rope=self.rope)
+                _rope_cache[(U * S, b.h + b.kvh)](qkv, self.rope, pos, q, kc, vc, S, b.h, b.kvh, S, HD=b.hd)
+                return self._prompt_attn(b, q, kc, vc, pos, S)
+
+            if four:
+                x = self._layer_q4(b, x, attend)
+                continue
             if self.prompt_a8:
                 qkv = self._a8(x, b.qkv, b.n1)
             else:
                 qkv = gemm_packed(krms(x, b.n1), b.qkv.qp, b.qkv.s8, b.qkv.N, b.qkv.K)
-            q = paged_write(qkv, kp, vp, table, pos, S, b.h, b.kvh, rope=self.rope)
-            _rope_cache[(U * S, b.h + b.kvh)](qkv, self.rope, pos, q, kc, vc, S, b.h, b.kvh, S, HD=b.hd)
-            o = self._prompt_attn(b, q, kc, vc, pos, S)
+            o = attend(qkv)
             if self.prompt_a8:
                 x = self._a8(o, b.o, res=x)
                 c, s = quant_a8(x, b.n2)
@@ -545,8 +608,14 @@ class Stack:
         slot's page is taken if it is not there yet, the step may be repeated (a capture's warm-up) and captured."""
         cache = self._pages("decode_paged")
         cache.extend(pos)
+        four = self.four()
         for i, b in enumerate(self.blocks):
             kp, vp = cache.layer(i)
+            if four:
+                x = self._layer_q4(b, x, lambda qkv: paged_attn(
+                    paged_write(qkv, kp, vp, cache.table, pos, 1, b.h, b.kvh, rope=self.rope), kp, vp, cache.table, pos,
+                    self.paged_plan))
+                continue
             qkv = torch.empty(x.shape[0], b.qkv.N, device=x.device, dtype=x.dtype)
             rms_qkv_rope_rows(x, b.n1, b.qkv.qp, b.qkv.s8, self.rope, pos, qkv, b.h, b.kvh, b.hd, dense=x.shape[0] > 16)
             paged_write(qkv, kp, vp, cache.table, pos, 1, b.h, b.kvh)
@@ -567,6 +636,11 @@ class Stack:
         attention output, its q|k|v, RoPE and cache slot already done (by the depth decoder's
         sampler); the step then starts at layer 0's O projection."""
         self._dense("decode")
+        if self.four():
+            if o0 is not None:
+                raise NotImplementedError("Stack.decode: layers of 4-bit weights start at their own q|k|v")
+            x = self._dense_q4(x, pos, S, False)
+            return krms(x, self.norm) if final_norm else x
         if any(b.qkv.qp is None for b in self.blocks):
             h = self.decode_reference(x, pos, S)
             return h if final_norm else None
@@ -676,6 +750,8 @@ class Stack:
         entry points of kernels.py (unpacked weights, one launch per reference kernel, the
         reference's attention grid and split count)."""
         self._dense("decode_reference")
+        if any(lin.q8 is None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2)):
+            raise NotImplementedError("Stack.decode_reference: the reference's launches take int8 weights")
         R = x.shape[0]
         for b in self.blocks:
             Hq, Hk, HD, L = b.h, b.kvh, b.hd, b.kc.shape[2]
@@ -730,7 +806,8 @@ class HeartMuLaLite:
     """Backbone + depth decoder of HeartMuLa on the gfx950 decode kernels (app/engine.py:215-477).
 
     ``weights`` is a ``mula_int8.safetensors``-format file or a dict of tensors with the same
-    names (``<name>.q8`` int8, ``<name>.s8`` bf16, norm ``.scale`` bf16)."""
+    names (``<name>.q8`` int8, ``<name>.s8`` bf16, norm ``.scale`` bf16; 4-bit layers as
+    ``<name>.q4``, ``.s4`` and, with zero points, ``.z4``: all linear layers of a stack or none)."""
 
     def __init__(self, weights, device="cuda", dtype=None, backbone=BACKBONE, decoder=DECODER):
         self.dev = torch.device(device)
@@ -749,6 +826,9 @@ class HeartMuLaLite:
             if name in f:
                 t = f.get(name).to(dtype)
                 return t if norm else Linear(w=t)
+            if name + ".q4" in f:
+                return Linear(q4=f.get(name + ".q4").contiguous(), s4=f.get(name + ".s4").to(dtype).contiguous(),
+                              z4=f.get(name + ".z4").contiguous() if name + ".z4" in f else None)
             q8, s8 = f.get(name + ".q8"), f.get(name + ".s8")
             return Linear(q8=q8.contiguous(), s8=s8.to(dtype).contiguous())
 
@@ -812,15 +892,18 @@ class HeartMuLaLite:
 
     # -------------------------------------------------- one frame (backbone + 7 decoder passes)
     def _frame_fast(self, last_h, cfg, topk, temp, pos=None, forced=None, logits_out=None,
-                    noise=None, normed=True):
+                    noise=None, normed=True, rules=None):
         """app/engine.py:328-343.  Sampling is one fused kernel per codebook (CFG, temperature,
         top-k, Exponential race) writing straight into the [B, 8] token tensor; its draws are
         keyed by the seed and the frame position ``pos`` (int64 device tensor, first element).
         ``forced`` [B, 8] replaces the samples (teacher forcing), ``logits_out`` collects the
         8 logit tensors, ``noise`` [8, N, V] fixes the Exponential draws (tests).
         ``normed=False``: last_h is the backbone's residual stream before its final RMSNorm,
-        which the first GEMV then applies itself."""
+        which the first GEMV then applies itself.  ``rules``: what process_logits does to each codebook's
+        logits before the sampler (_song_rules)."""
         B = self.B
+        if rules is not None and forced is None:
+            self._rules_at(rules, pos)
         if forced is None:
             samples = torch.empty(B, N_CB, dtype=torch.long, device=self.dev)
             if pos is None:
@@ -843,7 +926,10 @@ class HeartMuLaLite:
                                                   o=self._onext)
                 if rows is not None and x is None:
                     x = self._xnext
-                sample_topk(lg, self.N, cfg, temp, topk, samples[:, i], seed=self._seed, pos=pos,
+                c = cfg
+                if rules is not None:
+                    lg, c = self._ruled(rules, i, lg, cfg)
+                sample_topk(lg, self.N, c, temp, topk, samples[:, i], seed=self._seed, pos=pos,
                             salt=i, noise=None if noise is None else noise[i], rows=rows,
                             x=x, ev=ev, xe=xe, **att)
             return samples[:, i:i + 1]
@@ -877,6 +963,59 @@ class HeartMuLaLite:
                 lg = self._decode_head(x, self._pass_pos[i - 1], i,
                                        o0=None if qkv is None else self._onext)
         return samples
+
+    # -------------------------------------------------- logits before the sampler
+    @staticmethod
+    def _check_rules(repetition, presence, frequency, window, bias, allowed):
+        for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            if not math.isfinite(v) or (name == "repetition" and v <= 0):
+                raise ValueError(f"generate: {name} must be a finite number" + (" above 0" if name == "repetition" else ""))
+        if not 0 <= window <= INT_MOST:
+            raise ValueError("generate: window must be 0 (the whole song) or a number of frames")
+        for name, t, dt in (("bias", bias, torch.float32), ("allowed", allowed, torch.bool)):
+            if t is not None and (t.dtype != dt or tuple(t.shape) != (N_CB, AUDIO_VOCAB)):
+                raise ValueError(f"generate: {name} must be {dt} [{N_CB}, {AUDIO_VOCAB}]")
+
+    def _song_rules(self, out, P, repetition, presence, frequency, window, bias, allowed, min_frames):
+        """The arguments of process_logits for a song whose frames go to ``out`` [F, N, 8] (the history of codebook i is
+        out[:, :, i]), or None where they change nothing.  Before frame ``min_frames`` no end code (>= AUDIO_EOS) is allowed."""
+        counts = repetition != 1.0 or presence != 0.0 or frequency != 0.0
+        if not counts and bias is None and allowed is None and min_frames <= 0:
+            return None
+        N, dev = self.N, self.dev
+        r = dict(P=P, hist=[out[:, :, i].t() for i in range(N_CB)] if counts else None, window=int(window),
+                 length=torch.zeros(N, device=dev, dtype=torch.int64), state=None, masks=None,
+                 bias=None if bias is None else bias.to(dev).contiguous(), min_frames=min_frames,
+                 # the sampler's rows: the processed logits and zeros as the unconditional half, which it then mixes with weight 1
+                 logits=torch.zeros(self.B, -(-AUDIO_VOCAB // 64) * 64, device=dev, dtype=torch.float16)[:, :AUDIO_VOCAB])
+        if counts:
+            r.update({k: torch.tensor([v], device=dev, dtype=torch.float32)
+                      for k, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency))})
+        if allowed is not None or min_frames > 0:
+            keep = torch.ones(N_CB, AUDIO_VOCAB, device=dev, dtype=torch.bool) if allowed is None else allowed.to(dev)
+            if min_frames > 0:  # two masks per codebook: before min_frames, and from there on
+                early = keep.clone()
+                early[:, AUDIO_EOS:] = False
+                r["masks"] = [pack_mask(torch.stack([early[i], keep[i]])) for i in range(N_CB)]
+                r["state"] = torch.zeros(N, device=dev, dtype=torch.int32)
+            else:
+                r["masks"] = [pack_mask(keep[i]) for i in range(N_CB)]
+        return r
+
+    def _rules_at(self, r, pos):
+        """The song's length so far, and each row's mask, for the frame at position ``pos`` (on the device)."""
+        torch.sub(pos.reshape(-1)[:self.N], r["P"] - 1, out=r["length"])
+        if r["state"] is not None:
+            r["state"].copy_(r["length"] >= r["min_frames"])
+
+    def _ruled(self, r, i, lg, cfg):
+        """Codebook i's logits after the rules, as rows for the sampler, and the guidance that it still has to apply."""
+        N = self.N
+        h = {} if r["hist"] is None else dict(hist=r["hist"][i], length=r["length"], window=r["window"], repetition=r["repetition"],
+                                              presence=r["presence"], frequency=r["frequency"])
+        process_logits(lg, bias=None if r["bias"] is None else r["bias"][i], allowed=None if r["masks"] is None else r["masks"][i],
+                       state=r["state"], cfg=cfg if self.B == 2 * N else None, out=r["logits"][:N], **h)
+        return r["logits"], 1.0
 
     def _packed_decoder(self):
         return self.audio_head[0].qp is not None and bool(self.decoder.blocks) and \
@@ -944,8 +1083,8 @@ class HeartMuLaLite:
         first GEMV takes the backbone's final RMSNorm as its prologue, the backbone step returns
         its residual stream."""
         h = self.audio_emb.sum_codebooks(tok, AUDIO_VOCAB)
-        fused = kw.get("forced") is None and self._next_rows is not None and \
-            self._c0proj is not None and all(b.qkv.qp is not None for b in self.backbone.blocks)
+        fused = kw.get("forced") is None and self._next_rows is not None and self._c0proj is not None and \
+            (self.backbone.four() or all(b.qkv.qp is not None for b in self.backbone.blocks))
         p = pos[:, 0].contiguous()
         hb = self.backbone.decode_paged(h, p, final_norm=not fused) if self.backbone.paged is not None else \
             self.backbone.decode(h, p, 1, final_norm=not fused)
@@ -1052,7 +1191,8 @@ class HeartMuLaLite:
     # -------------------------------------------------- generation
     @torch.inference_mode()
     def generate(self, text, muq_idx, *, max_ms=60_000, temperature=1.0, topk=50, cfg_scale=1.5,
-                 seed=None, use_graphs=True, progress=None, abort=None, n=1, forced=None, paged=False, a8=False):
+                 seed=None, use_graphs=True, progress=None, abort=None, n=1, forced=None, paged=False, a8=False,
+                 repetition=1.0, presence=0.0, frequency=0.0, window=0, bias=None, allowed=None, min_ms=0):
         """A song of up to ``max_ms`` for n takes (app/engine.py:374-448) with the prompt given as
         token ids ``text`` [P] (int64) and the muq slot index.  Returns [8, T] if n == 1, else a
         list of n such tensors, each take cut before its first frame holding an EOS token.
@@ -1066,14 +1206,21 @@ class HeartMuLaLite:
         them once for all takes.  The backbone then runs its kernels one by one instead of in layer
         stacks: for many takes, whose rows a stack does not hold (more than 8), or whose caches take
         the memory.  ``a8``: the prompt's linear layers run on int8 activations (not the reference's
-        numerics; 0.61 to 0.66 of the prompt's time over dense caches, 0.69 to 0.76 over pages)."""
+        numerics; 0.61 to 0.66 of the prompt's time over dense caches, 0.69 to 0.76 over pages).
+
+        ``repetition``, ``presence``, ``frequency``: penalties for codes that a take's codebook has had in the last
+        ``window`` frames (0: in the song so far): logits l > 0 become l / repetition, others l * repetition, then
+        l - (presence + frequency * count).  ``bias`` float32 [8, V] is added; ``allowed`` bool [8, V] forbids codes;
+        before ``min_ms`` no frame ends the song (process_logits, on the guided logits in fp32; teacher forcing ignores them)."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
-        if a8 and not self.backbone.packed():
+        if a8 and not self.backbone.eight():
             raise NotImplementedError("generate: int8 activations need packed weights (widths in multiples of 64)")
         if a8 and not self.backbone.prompt_heads():
             raise NotImplementedError("generate: int8 activations need a head_dim of 64, 128, 256 or 384 and 1, 2, 3, 4, 6 or 8 "
                                       "query heads per kv head")
+        rules = float(repetition), float(presence), float(frequency), int(window)
+        self._check_rules(*rules, bias, allowed)
         text = torch.as_tensor(text, dtype=torch.int64)
         P = int(text.numel())
         n_frames = max_ms // FRAME_MS
@@ -1104,7 +1251,11 @@ class HeartMuLaLite:
                   out=torch.empty(n_frames + 1, N, N_CB, dtype=torch.long, device=self.dev),
                   eos=torch.full((N,), -1, dtype=torch.long, device=self.dev),
                   forced=None if forced is None else forced[0].clone())
-        kw = {} if forced is None else {"forced": st["forced"]}
+        kw = {}
+        if forced is not None:
+            kw["forced"] = st["forced"]
+        else:
+            kw["rules"] = st["rules"] = self._song_rules(st["out"], P, *rules, bias, allowed, -(-int(min_ms) // FRAME_MS))
         first = self._frame_fast(hb.contiguous(), cfg_scale, topk, temperature,
                                  pos=st["pos"], **kw)
         self._advance(first, st, P, n_frames)
@@ -1201,6 +1352,8 @@ class HeartMuLaLite:
         With ``song`` = (P, n_frames) the graph ends with the frame bookkeeping (``_advance``),
         so consecutive replays make consecutive frames with no host work in between."""
         kw = {"forced": static["forced"]} if static.get("forced") is not None else {}
+        if static.get("rules") is not None:
+            kw["rules"] = static["rules"]
         s = torch.cuda.Stream(device=self.dev)
         s.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(s):
@@ -1240,7 +1393,8 @@ class HeartMuLaLite:
         lins += [self.projection, self.c0_head, *self.audio_head]
         if self._c0proj is not None:
             lins.append(self._c0proj)
-        ts = [t for lin in lins for t in (lin.q8, lin.s8, lin.qp, lin.sp)]
+        ts = [t for lin in lins for t in (lin.q8, lin.s8, lin.qp, lin.sp, lin.q4, lin.s4, lin.z4)]
+        ts += [t for lin in lins if lin.w4 is not None for t in (lin.w4.codes, lin.w4.scales)]
         ts += [t for e in (self.text_emb, self.audio_emb) for t in (e.w, e.q8, e.s8)]
         ts += [t for st in (self.backbone, self.decoder) for b in st.blocks for t in (b.n1, b.n2)]
         ts += [self.backbone.norm, self.decoder.norm, self.uncond, self.muq_b, self._next_rows,

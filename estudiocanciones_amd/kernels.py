@@ -1185,15 +1185,13 @@ class PackedQ4:
         self.N, self.K, self.group, self.zeros, self.interleave = N, K, group, zeros, interleave
         self.dev = codes.device
         self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
-        self._plans = {}
+        self.plans = {}  # rows -> plan(rows): they depend on sizes alone
 
     def plan(self, M):
         """(kernel choice, workspace bytes without and with a norm) of a product of M rows."""
-        p = self._plans.get(M)
-        if p is None:
-            lib = _ffi.lib()
-            n = lib.ecd_mm_q4_plan(M, self.N, self.K)
-            p = self._plans[M] = (n, *(lib.ecd_mm_q4_ws_bytes(M, self.N, self.K, n, f) for f in (0, 1)))
+        lib = _ffi.lib()
+        n = lib.ecd_mm_q4_plan(M, self.N, self.K)
+        p = self.plans[M] = (n, *(lib.ecd_mm_q4_ws_bytes(M, self.N, self.K, n, f) for f in (0, 1)))
         return p
 
     @property
@@ -1237,26 +1235,31 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         if dev != w.dev:
             raise ValueError(f"{name}: the weights are on {w.dev}, x on {dev}")
         raise ValueError(f"{name}: x must be [M, {w.K}]")
+    np = rp = wp = None
+    ldr = 0
     if nw is not None:
         _on(nw, dev, name, "nw", torch.float16, (K,))
-        if nw.data_ptr() % 16:
+        np = nw.data_ptr()
+        if np % 16:
             raise ValueError(f"{name}: nw must be 16-byte aligned")
-    y = torch.empty(M, cols, device=dev, dtype=torch.float16) if out is None else out
-    ldr = 0
     if res is not None:
         ldr = _rows_of(res, M, cols, dev, name, "res")
-    ldy = cols
-    if out is not None:
+        rp = res.data_ptr()
+    if out is None:
+        out, ldy = torch.empty(M, cols, device=dev, dtype=torch.float16), cols
+    else:
         ldy = _rows_of(out, M, cols, dev, name, "out")
         if _ends(out)[0] < _ends(x)[1] and _ends(x)[0] < _ends(out)[1]:
             raise ValueError(f"{name}: out must not overlap x")
     if M:
-        plan, *nb = w.plan(M)
-        nb = nb[nw is not None]
-        ws = torch.empty(nb, device=dev, dtype=torch.uint8) if nb else None  # (held until the launch)
-        _call_on(dev, "ecd_mm_q4", x.data_ptr(), ldx, _ptr(nw), eps, w.codes_ptr, w.scales_ptr, w.zeros, w.group, _ptr(res), ldr,
-                 y.data_ptr(), ldy, M, w.N, K, silu, plan, _ptr(ws))
-    return y
+        plan = w.plans.get(M) or w.plan(M)
+        nb = plan[1 if np is None else 2]
+        if nb:
+            ws = torch.empty(nb, device=dev, dtype=torch.uint8)  # (held until the launch)
+            wp = ws.data_ptr()
+        _call_on(dev, "ecd_mm_q4", x.data_ptr(), ldx, np, eps, w.codes_ptr, w.scales_ptr, w.zeros, w.group, rp, ldr,
+                 out.data_ptr(), ldy, M, w.N, K, silu, plan[0], wp)
+    return out
 
 
 def _ends(t):
@@ -1289,9 +1292,27 @@ def mm_q4_silu(x, w, nw=None, eps=1e-5, out=None):
 
 # ---------------------------------------------------------------- logits before the sampler
 def _per_row(t, N, dev, name):
-    if t.dtype is not torch.float32 or t.device != dev or t.dim() != 1 or t.shape[0] not in (1, N) or not t.is_contiguous():
-        raise ValueError(f"process_logits: {name} must be float32 [{N}] or [1] on {dev}")
-    return t.data_ptr(), t.shape[0] == N
+    """(address, whether there is an element per row) of a penalty."""
+    if t.dtype is torch.float32 and t.device == dev and t.dim() == 1 and t.is_contiguous():
+        n = t.numel()
+        if n == N:
+            return t.data_ptr(), N != 1
+        if n == 1:
+            return t.data_ptr(), False
+    raise ValueError(f"process_logits: {name} must be float32 [{N}] or [1] on {dev}")
+
+
+def pack_mask(keep):
+    """bool [A, V] (or [V]) of allowed tokens -> the int32 [A, ceil(V / 32)] masks of process_logits, bit v % 32 of word
+    v // 32.  Set-up work: elementary torch operations."""
+    if keep.dtype is not torch.bool or keep.dim() not in (1, 2):
+        raise TypeError("pack_mask: keep must be bool [A, V] or [V]")
+    keep = keep if keep.dim() == 2 else keep[None]
+    A, V = keep.shape
+    bits = torch.zeros(A, -(-V // 32) * 32, device=keep.device, dtype=torch.int64)
+    bits[:, :V] = keep
+    w = (bits.view(A, -1, 32) << torch.arange(32, device=keep.device)).sum(2)
+    return torch.where(w < 1 << 31, w, w - (1 << 32)).to(torch.int32)
 
 
 def process_logits(logits, hist=None, length=None, window=0, repetition=None, presence=None, frequency=None, bias=None,
@@ -1309,52 +1330,56 @@ def process_logits(logits, hist=None, length=None, window=0, repetition=None, pr
     [A, ceil(V / 32)]: masks of allowed tokens, bit v % 32 of word v // 32; ``state`` int32 [N] gives each row its mask (-1:
     none; any other number outside [0, A): nothing is allowed), without it A is 1 or N.  ``out``: the destination; it may be
     the first N rows of ``logits``."""
-    dev = _dev(logits, "process_logits")
-    _f16(logits, "process_logits logits")
+    dev = logits.device
+    if logits.dtype is not torch.float16 or not logits.is_cuda:
+        _dev(logits, "process_logits")
+        _f16(logits, "process_logits logits")
     if logits.dim() != 2:
         raise ValueError("process_logits: logits must be [B, V]")
-    B, V = logits.shape
-    ld, one = logits.stride()
+    (B, V), (ld, one) = logits.shape, logits.stride()
     guided = cfg is not None
     N = B // 2 if guided else B
-    if (one != 1 and V != 1) or (ld < V and B != 1) or V < 1 or V > INT_MOST - 8192 or (guided and B % 2):
+    if (one != 1 and V != 1) or (ld < V and B != 1) or not 1 <= V <= INT_MOST - 8192 or (guided and B % 2):
         raise ValueError("process_logits: logits must be [B, V] with contiguous rows (B even with cfg)")
-    ld = max(ld, V)
-    hp = hrow = htok = T = lp = rp = pp = fp = bp = ldb = ap = lda = A = sp = 0
-    flags = 0
+    hp = lp = rp = pp = fp = bp = ap = sp = None
+    hrow = htok = T = ldb = lda = A = flags = 0
     if hist is not None:
-        if hist.dtype is not torch.int64 or hist.device != dev or hist.dim() != 2 or hist.shape[0] != N or \
-                hist.shape[1] > INT_MOST:
+        if hist.dtype is not torch.int64 or hist.device != dev or hist.dim() != 2:
             raise ValueError(f"process_logits: hist must be int64 [{N}, T] on {dev}")
-        hp, T = hist.data_ptr(), hist.shape[1]
-        hrow, htok = hist.stride()
+        (rows, T), (hrow, htok) = hist.shape, hist.stride()
+        if rows != N or T > INT_MOST:
+            raise ValueError(f"process_logits: hist must be int64 [{N}, T] on {dev}")
         if length is not None:
             _on(length, dev, "process_logits", "length", torch.int64, (N,))
             lp = length.data_ptr()
         if not 0 <= window <= INT_MOST:
             raise ValueError("process_logits: window must be 0 (all tokens) or a number of tokens")
         if repetition is not None:
-            rp, f = _per_row(repetition, N, dev, "repetition")
-            flags |= f
+            rp, flags = _per_row(repetition, N, dev, "repetition")
         if presence is not None:
             pp, f = _per_row(presence, N, dev, "presence")
             flags |= f << 1
         if frequency is not None:
             fp, f = _per_row(frequency, N, dev, "frequency")
             flags |= f << 2
-        if T == 0 or not (rp or pp or fp):  # nothing to count, or nothing that depends on it
-            hp = rp = pp = fp = 0
+        if T and (rp or pp or fp):
+            hp = hist.data_ptr()
+        else:  # nothing to count, or nothing that depends on it
+            rp = pp = fp = None
     elif length is not None or window or repetition is not None or presence is not None or frequency is not None:
         raise ValueError("process_logits: penalties need a history (hist)")
     if bias is not None:
-        if bias.dtype is not torch.float32 or bias.device != dev or bias.shape not in ((V,), (N, V)) or \
-                (bias.stride(-1) != 1 and V != 1) or (bias.dim() == 2 and bias.stride(0) < V and N != 1):
+        shape, step = bias.shape, bias.stride()
+        if len(shape) == 2:
+            ldb = step[0] if N > 1 else V
+        if bias.dtype is not torch.float32 or bias.device != dev or shape not in ((V,), (N, V)) or \
+                (step[-1] != 1 and V != 1) or (len(shape) == 2 and ldb < V):
             raise ValueError(f"process_logits: bias must be float32 [{V}] or [{N}, {V}] on {dev} with contiguous rows")
-        bp, ldb = bias.data_ptr(), max(bias.stride(0), V) if bias.dim() == 2 else 0
+        bp = bias.data_ptr()
     if allowed is not None:
-        A = allowed.shape[0] if allowed.dim() == 2 else 0
         lda = -(-V // 32)
-        if A < 1 or A > INT_MOST or (state is None and A != 1 and A != N):
+        A = allowed.shape[0] if allowed.dim() == 2 else 0
+        if not 1 <= A <= INT_MOST or (state is None and A != 1 and A != N):
             raise ValueError(f"process_logits: allowed must be [A, {lda}] (A 1 or {N} without state)")
         _on(allowed, dev, "process_logits", "allowed", torch.int32, (A, lda))
         ap = allowed.data_ptr()
@@ -1363,13 +1388,16 @@ def process_logits(logits, hist=None, length=None, window=0, repetition=None, pr
             sp = state.data_ptr()
     elif state is not None:
         raise ValueError("process_logits: state needs masks (allowed)")
-    if out is None:
-        out = torch.empty(N, -(-V // 64) * 64, device=dev, dtype=torch.float16)[:, :V]  # rows start aligned for the sampler
-        ldo = out.stride(0)
+    if out is None:  # rows start aligned for the sampler
+        ldo = -(-V // 64) * 64
+        out = torch.empty_strided((N, V), (ldo, 1), device=dev, dtype=torch.float16)
     else:
         ldo = _rows_of(out, N, V, dev, "process_logits", "out")
+        lo, hi = _ends(out)
+        a, b = _ends(logits)
+        if lo < b and a < hi and not (lo == a and (ldo == ld or N == 1)):
+            raise ValueError("process_logits: out must be apart from logits or their first rows")
     if N:
-        _call_on(dev, "ecd_process_logits", logits.data_ptr(), ld, guided, cfg if guided else 1.0, hp or None, hrow, htok, T,
-                 lp or None, window, rp or None, pp or None, fp or None, flags, bp or None, ldb, ap or None, lda, A, sp or None,
-                 out.data_ptr(), ldo, N, V)
+        _call_on(dev, "ecd_process_logits", logits.data_ptr(), max(ld, V), guided, cfg if guided else 1.0, hp, hrow, htok, T, lp,
+                 window, rp, pp, fp, flags, bp, ldb, ap, lda, A, sp, out.data_ptr(), ldo, N, V)
     return out

@@ -98,6 +98,23 @@ def weight_shapes(backbone: dict, decoder: dict, text_vocab: int = 1024):
     return lin, dense
 
 
+def to_q4(weights: dict, group: int = 128, zeros: bool = False, device="cuda", stack: str = "backbone") -> dict:
+    """A model's int8 weights with the linear layers of ``stack`` in 4 bits (their values requantised group by group): the
+    names ``<name>.q8`` / ``.s8`` become ``<name>.q4`` / ``.s4`` (/ ``.z4``)."""
+    out = {}
+    for k, v in weights.items():
+        name, kind = k.rsplit(".", 1)
+        if not name.startswith(f"{stack}.layers.") or kind not in ("q8", "s8"):
+            out[k] = v
+        elif kind == "q8":
+            w = v.to(device).float() * weights[name + ".s8"].to(device).float()[:, None]
+            q, s, z = q4_rows(w, group, zeros)
+            out[name + ".q4"], out[name + ".s4"] = q, s
+            if zeros:
+                out[name + ".z4"] = z
+    return out
+
+
 @torch.no_grad()
 def synthetic_weights(backbone: dict, decoder: dict, device="cuda", seed: int = 0,
                       std: float = 0.02, emb_std: float = 1.0, text_vocab: int = 1024):

@@ -718,7 +718,7 @@ int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* co
  *   count, those outside [0, V) for nothing; rep, pres, freq: f32, bit 0, 1, 2 of per_row: an element per row (else one; NULL: 1, 0, 0);
  *   allowed [A] rows of ceil(V / 32) words (row stride lda), bit v & 31 of word v >> 5: v is allowed; state [N]: each row's mask,
  *   -1: none, any other outside [0, A): nothing is allowed; without state A is 1 (all rows) or N (row r's mask is r).
- *   out may be the rows of logits themselves (same address and stride).  N <= 65535. */
+ *   out may be the rows of logits themselves (same address and stride).  N <= 65535, T <= 2^30. */
 int ecd_process_logits(const void* logits, long ld, int guided, float cfg, const int64_t* hist, long hrow, long htok, int T,
                        const int64_t* length, int window, const float* rep, const float* pres, const float* freq, int per_row,
                        const float* bias, long ldb, const uint32_t* allowed, long lda, int A, const int32_t* state, void* out,

@@ -42,7 +42,7 @@ def lg(**kw):
     (I, lg(logits=None)), (I, lg(out=None)), (I, lg(N=0)), (I, lg(V=0)), (I, lg(ld=99)), (I, lg(ldo=99)), (I, lg(window=-1)),
     (I, lg(T=-1)), (I, lg(rep=8)), (I, lg(pres=8)), (I, lg(freq=8)), (I, lg(hist=8, hrow=-1)), (I, lg(bias=8, ldb=99)),
     (I, lg(allowed=8, lda=3, A=1)), (I, lg(allowed=8, lda=4, A=0)), (I, lg(allowed=8, lda=4, A=3)),
-    (N, lg(N=65536)),
+    (N, lg(N=65536)), (N, lg(hist=8, hrow=0, htok=0, T=(1 << 30) + 1)), (N, lg(V=0x7FFFFFFF, ld=0x7FFFFFFF, ldo=0x7FFFFFFF)),
 ])
 def test_entries_refuse_on_the_host(want, call):
     from estudiocanciones_amd import _ffi
