@@ -38,8 +38,11 @@ def hipcc() -> str:
 
 
 # per-file additions: the layer-stack launch keeps constants and addresses inside its layer loop
-# (hoisted out of it, they would hold registers across every layer)
-FILE_FLAGS = {"layer_stack.hip": ["-mllvm", "-disable-machine-licm"]}
+# (hoisted out of it, they would hold registers across every layer); the products with 4-bit weights find their first 14
+# words of arguments in scalar registers at the start, where a load of them is a good part of so short a kernel
+# (5120 x 3072, 8 rows: 0.27 of 5.4 us)
+FILE_FLAGS = {"layer_stack.hip": ["-mllvm", "-disable-machine-licm"],
+              "q4.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"]}
 
 
 def _compile(src: Path) -> Path:

@@ -356,26 +356,30 @@ int gemm_q4(const Q4Args& a, bool zp, int tile, float* ws, int ks, hipStream_t s
 
 // The tiles: features x rows, chunks of a step (WK), workgroups that a CU holds, and measured times in ns: a step of a workgroup
 // alone on its CU and of a full CU, and the rest of a workgroup's time.  Fitted to 2400 timings (12 to 3000 rows, 1001 to 16384
-// features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.
+// features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.  The last three are the
+// few-row kernel's forms, whose 8 waves take a pair of chunks each in a step (360 timings of 16 to 256 rows, 7 to 9% rms): they
+// read the codes again for every 16 rows, but a CU starts on them with all loads in flight and ends without a split's join
+// (48 rows of 3072 x 3072: 5.8 us, the best tile 8.8; 192 rows of 5120 x 3072: 15.5 and 11.7).
 struct Q4Cost {
   int bn, bm, wk, fit, step, full, rest;
 };
-constexpr Q4Cost Q4_COST[Q4_TILES] = {
+constexpr Q4Cost Q4_COST[Q4_TILES + Q4_ROWS] = {
     {256, 128, 1, 2, 874, 1372, 3509}, {128, 128, 2, 1, 882, 882, 2404}, {128, 64, 2, 2, 551, 1142, 1853},
     {128, 32, 2, 2, 413, 741, 1582},   {64, 32, 4, 1, 484, 484, 1462},   {64, 64, 4, 1, 677, 677, 1732},
+    {16, 16, 16, 1, 438, 363, 619},    {32, 16, 16, 1, 596, 516, 693},  {64, 16, 16, 1, 994, 961, 717},
 };
 
 // The choice of the shortest estimate.  Over the 96 shapes that the times were taken at it is 0.8% behind the fastest of all on
-// average, 11% at most.  A split's join costs a launch and the passage of its sums through memory.
-int gemm_q4_plan(int M, int N, int K) {
+// average, 11% at most; over 120 shapes with few rows as much, and 12%.  A split's join costs a launch and the passage of its sums through memory.
+int gemm_q4_plan(int M, int N, int K, bool rows) {
   const int nch = K >> 6;
   long best = 0x7FFFFFFFFFFFFFFFL;
   int plan = 1 + 256;
-  for (int t = 0; t < Q4_TILES; ++t) {
+  for (int t = 0; t < Q4_TILES + (rows ? Q4_ROWS : 0); ++t) {
     const Q4Cost& c = Q4_COST[t];
     const long tiles = ((long)N + c.bn - 1) / c.bn * (((long)M + c.bm - 1) / c.bm);
     for (int ks = 1; ks <= 12; ++ks) {
-      if (ks > 1 && (tiles * ks > 1100 || nch < 4 * ks)) break;
+      if (ks > 1 && (t >= Q4_TILES || tiles * ks > 1100 || nch < 4 * ks)) break;
       const long blocks = tiles * ks, steps = ((nch + ks - 1) / ks + c.wk - 1) / c.wk, per = 256L * c.fit, rem = blocks % per;
       long e = blocks / per * (steps * c.full + c.rest);
       // a last round of more than one workgroup per CU: 30% of the way to a full one at once, the rest with their number
@@ -383,7 +387,7 @@ int gemm_q4_plan(int M, int N, int K) {
       if (ks > 1) e += 2700 + 12L * (ks + 1) * M * N / 10000;
       if (e < best) {
         best = e;
-        plan = t + 1 + 256 * ks;
+        plan = (t < Q4_TILES ? t + 1 : t + 1 - Q4_TILES + Q4_ROWS_AT) + 256 * ks;
       }
     }
   }

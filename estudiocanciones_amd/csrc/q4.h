@@ -57,10 +57,11 @@ struct Q4Args {
 };
 
 // The product by a tile (1 .. Q4_TILES) of gemm_q4.hip, K split ks ways (ws: ks M ceil8(N) floats where ks > 1); no norm.
-// go false: only whether the sizes fit.  And the choice for given sizes: tile + 256 ks.
-constexpr int Q4_TILES = 6;
+// go false: only whether the sizes fit.  And the choice for given sizes: tile + 256 ks; with rows also of the few-row
+// kernel's forms of 16, 32 and 64 features, which count as tiles Q4_ROWS_AT + 1 ..
+constexpr int Q4_TILES = 6, Q4_ROWS_AT = 16, Q4_ROWS = 3;
 int gemm_q4(const Q4Args& a, bool zp, int tile, float* ws, int ks, hipStream_t st, bool go);
-int gemm_q4_plan(int M, int N, int K);
+int gemm_q4_plan(int M, int N, int K, bool rows);
 
 // silu(a) * b in fp32
 // (the exponential and the reciprocal by their instructions, 1 ulp of fp32 each)

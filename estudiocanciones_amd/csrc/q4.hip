@@ -128,181 +128,248 @@ __global__ __launch_bounds__(256) void pack_q4_scales_kernel(const f16* __restri
 }
 
 // ---------------------------------------------------------------- products of few rows
-// A workgroup of KW waves computes 16 NT features of up to 8 MR rows with v_mfma_f32_16x16x32_f16; the waves share out the
-// 64-wide chunks of K, and a wave keeps the loads of CW chunks in flight (a ring of registers).  GS: scales of a chunk (2 for
-// groups of 32).
+// A workgroup of KW waves computes 16 NT features of up to R = 4 XO rows with v_mfma_f32_16x16x32_f16; the waves share out the
+// pairs of 64-wide chunks of K, and a wave keeps the loads of CW pairs in flight (a ring of registers).
 //
-// A wave loads its chunk of x as whole lines, 8 MR rows by 8 / MR octets an instruction, works on it there (the norm), and passes
-// it through its own part of LDS into the operand's lane order.
+// What such a kernel runs into first is the address path: a load instruction takes a CU 16 cycles at least, whatever it
+// brings, and longer if neighbouring lanes are in different lines.  So every load has 16 bytes a lane where there is as
+// much: a lane takes the 16 bytes of its feature in one chunk of the pair (half the lanes each), and the matrix instruction's k
+// are numbered to match; x comes as whole lines, 4 rows an instruction, is worked on in that order (the norm) and passes through
+// the wave's own part of LDS into the operand's; scales of up to four (feature tile, group) slots come with one load and are
+// spread by lane swaps.  Groups under 128 split the pair: x is zeroed outside the group at hand (GS = 128 / group).
 //
 // The norm: x 2^e with 2^e a power of two near 1 / rms of the row's part at hand (exact), times nw in two fp16 parts, the product
 // and what its rounding left (exact by the fused multiply-add), both multiplied by the codes.  Sums take 2^-e back in fp32, and
 // 1 / rms of the whole row at the end, when the waves' sums meet: nothing waits for the statistics.  Up to 8 rows the second
 // part takes the matrix instruction's rows 8 .. 15, which are idle otherwise.
-template <int NT, int MR, int GS, bool ZP, bool NORM>
-struct Q4Chunk {
-  f16x8 x[MR], nw[NORM ? MR : 1];  // octets lane / (8 MR) + 8 / MR i of row lane % (8 MR)
-  u32x2 code[NT];                  // octet lane / 16 of both halves
-  f16 s[NT][GS];
-  f16x2 sz[NT][GS];  // with zero points: (s, 1024 + z)
+template <int NT, int XO, int GS, bool ZP, bool NORM>
+struct Q4Pair {
+  static constexpr int SLOTS = NT * GS, SL = (SLOTS + 3) / 4;  // scales of 16 features each, and loads for them
+  f16x8 x[XO], nw;   // octet lane % 16 of rows lane / 16 + 4 i
+  u32x4 code[NT];    // chunk lane / 32, half (lane / 16) % 2
+  f16 s[SL];         // slot 4 i + lane / 16
+  f16x2 sz[SL];      // with zero points: (s, 1024 + z)
 };
 
-template <int KW, int CW, int NT, int MR, bool ZP, int GS, bool NORM>
-__global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const Q4Args a) {
-  constexpr bool PAIR = NORM && MR == 1;           // both parts in one instruction
-  constexpr int MT = MR == 1 ? 1 : MR / 2;         // instructions' rows: tiles of 16
-  constexpr int R = 8 * MR, P = 16 * MT;           // rows, and 16-byte pieces of an octet in LDS
-  constexpr int LO = NORM && !PAIR ? 8 * P : 0;    // where the second parts start
-  using Chunk = Q4Chunk<NT, MR, GS, ZP, NORM>;
-  const int lane = threadIdx.x & 63, f = lane & 15, g4 = lane >> 4;
+// v of lanes 16 i .. 16 i + 15 for all lanes, i < n
+template <int n>
+__device__ __forceinline__ void spread16(uint32_t v, uint32_t* to) {
+  if constexpr (n == 1) {
+    to[0] = v;
+  } else if constexpr (n == 2) {  // (the upper half of the lanes holds the lower's again)
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    to[0] = p[0], to[1] = p[1];
+  } else {
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    spread16<2>(h[0], to);
+    spread16<2>(h[1], to + 2);
+  }
+}
+
+// the sum over 16 neighbouring lanes, for all of them
+__device__ __forceinline__ float row_sum16(float v) {
+  auto ror = [&](auto n) { return __builtin_bit_cast(float, dpp_u32<0x120 + decltype(n)::value, 0xF>(__builtin_bit_cast(uint32_t, v), 0)); };
+  v += ror(std::integral_constant<int, 8>());
+  v += ror(std::integral_constant<int, 4>());
+  v += ror(std::integral_constant<int, 2>());
+  v += ror(std::integral_constant<int, 1>());
+  return v;
+}
+
+template <int KW, int CW, int NT, int XO, bool ZP, int GS, bool NORM>
+__global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const f16* __restrict__ x, const uint8_t* __restrict__ codes,
+                                                             const f16* __restrict__ scales, const f16* __restrict__ nw, int N,
+                                                             int K, int M, int lg, long ldx, float eps, const f16* res, long ldr,
+                                                             f16* y, long ldy, int silu) {
+  constexpr bool PAIR = NORM && XO < 4;            // both parts in one instruction
+  constexpr int R = 4 * XO, P = 16;                // rows, and those of an instruction
+  constexpr int PP = P + 1;                        // 16-byte pieces of an octet in LDS (odd: a line's octets fall on all banks)
+  constexpr int LO = NORM && !PAIR ? 16 * PP : 0;  // where the second parts start
+  using Pair = Q4Pair<NT, XO, GS, ZP, NORM>;
+  const int lane = threadIdx.x & 63, f = lane & 15, g4 = lane >> 4, h = g4 & 1, cc = g4 >> 1;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nch = a.K >> 6, m0 = blockIdx.y * R, n0 = blockIdx.x * (16 * NT);
-  const int xr = lane & (R - 1), xj = lane / R, tile0 = n0 >> 5, last = (a.N - 1) >> 5;
-  const auto xbuf = q4_buffer(a.x + (long)m0 * a.ldx), nbuf = q4_buffer(a.nw);
-  const auto cbuf = q4_buffer(a.codes + (long)tile0 * nch * 1024);
-  const int tstep = ((a.K - 1) >> a.lg) + 1;  // scales of a tile's row
-  const auto sbuf = q4_buffer(a.scales + (long)tile0 * tstep * (ZP ? 64 : 32));
-  const int xoff = m0 + xr < a.M ? (int)(xr * a.ldx * 2) + 16 * xj : Q4_NONE;
-  int coff[NT], soff[NT];
+  const int nch = K >> 6, npr = (nch + 1) >> 1, m0 = blockIdx.y * R, n0 = blockIdx.x * (16 * NT);
+  const int xr = lane >> 4, xj = lane & 15, tile0 = n0 >> 5, last = (N - 1) >> 5;
+  const int ng = ((K - 1) >> lg) + 1;
+  const auto xbuf = q4_buffer(x + (long)m0 * ldx), nbuf = q4_buffer(nw);
+  const auto cbuf = q4_buffer(codes + (long)tile0 * nch * 1024);
+  const auto sbuf = q4_buffer(scales + (long)tile0 * ng * (ZP ? 64 : 32));
+  int xoff[XO];
+#pragma unroll
+  for (int o = 0; o < XO; ++o) {
+    const int r = xr + 4 * o;
+    xoff[o] = m0 + r < M ? (int)(r * ldx * 2) + 16 * xj : Q4_NONE;
+  }
+  const int coff = 16 * (f + 32 * h);
+  int ctile[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int n = n0 + 16 * t, tile = min(n >> 5, last) - tile0;  // (past the last: again, and not stored)
-    coff[t] = tile * nch * 1024 + 16 * ((n & 16) + f + 32 * (g4 >> 1)) + 8 * (g4 & 1);
-    soff[t] = (tile * tstep * 32 + (n & 16) + f) * (ZP ? 4 : 2);
+    const int n = n0 + 16 * t;  // (a tile past the last: the last again, and not stored)
+    ctile[t] = (min(n >> 5, last) - tile0) * nch * 1024 + 16 * (n & 16);
   }
-  constexpr int PW = 16 * NT + 1;
-  constexpr int OPS = 8 * P + LO;  // operand pieces of a chunk
-  constexpr int PART = KW * P * PW * 4, OPB = KW * OPS * 16;
+  int soff[Pair::SL], sg[Pair::SL];
+#pragma unroll
+  for (int i = 0; i < Pair::SL; ++i) {
+    const int slot = (4 * i + g4) % Pair::SLOTS, n = n0 + 16 * (slot / GS);
+    soff[i] = ((min(n >> 5, last) - tile0) * ng * 32 + (n & 16) + f) * (ZP ? 4 : 2);
+    sg[i] = slot % GS;
+  }
+  constexpr int PW = 16 * NT + 4;    // (rows of 4 lanes' sums fall on different banks)
+  constexpr int OPS = 16 * PP + LO;  // operand pieces of a pair
+  constexpr int PR = PAIR ? 8 : P;   // rows of sums in LDS
+  constexpr int PART = KW * PR * PW * 4, OPB = KW * OPS * 16;
   __shared__ __align__(16) char lds[PART > OPB ? PART : OPB];
   __shared__ __align__(16) float us[NORM ? KW * P : 1];
   __shared__ float rs[NORM ? KW * R : 1];
-  f16x8* const ops = (f16x8*)lds + wv * OPS;  // the wave's operands; afterwards part [KW][P][PW] of sums
+  f16x8* const ops = (f16x8*)lds + wv * OPS;  // the wave's operands; afterwards part [KW][PR][PW] of sums
   float* const part = (float*)lds;
 
-  const int cnt = wv < nch ? (nch - 1 - wv) / KW + 1 : 0;  // chunks wv, wv + KW, ..
-  Chunk ring[CW];
-  auto load_x = [&](Chunk& k, int i) {
-    const int c = min(wv + KW * i, nch - 1);
+  const int cnt = wv < npr ? (npr - 1 - wv) / KW + 1 : 0;  // pairs wv, wv + KW, ..
+  Pair ring[CW];
+  auto load_x = [&](Pair& k, int i) {
+    const int p = min(wv + KW * i, npr - 1);
+    const bool in = 2 * p + (xj >> 3) < nch;  // (an odd number of chunks: zeros in place of the last)
 #pragma unroll
-    for (int o = 0; o < MR; ++o)
-      k.x[o] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(xbuf, xoff + 128 / MR * o, 128 * c, 0));
-  };
-  auto load_w = [&](Chunk& k, int i) {
-    const int c = min(wv + KW * i, nch - 1);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      k.code[t] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(cbuf, coff[t], 1024 * c, 0));
-#pragma unroll
-      for (int H = 0; H < GS; ++H) {
-        const int g = (64 * c + 32 * H) >> a.lg;
-        if constexpr (ZP)
-          k.sz[t][H] = __builtin_bit_cast(f16x2, __builtin_amdgcn_raw_buffer_load_b32(sbuf, soff[t], 128 * g, 0));
-        else
-          k.s[t][H] = __builtin_bit_cast(f16, __builtin_amdgcn_raw_buffer_load_b16(sbuf, soff[t], 64 * g, 0));
-      }
-    }
+    for (int o = 0; o < XO; ++o)
+      k.x[o] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(xbuf, in ? xoff[o] : Q4_NONE, 256 * p, 0));
     if constexpr (NORM)
+      k.nw = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(nbuf, in ? 16 * xj : Q4_NONE, 256 * p, 0));
+  };
+  auto load_w = [&](Pair& k, int i) {
+    const int p = min(wv + KW * i, npr - 1);
+    const int c = coff + 1024 * min(2 * p + cc, nch - 1);
 #pragma unroll
-      for (int o = 0; o < MR; ++o)
-        k.nw[o] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(nbuf, 16 * xj + 128 / MR * o, 128 * c, 0));
+    for (int t = 0; t < NT; ++t)
+      k.code[t] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(cbuf, c, ctile[t], 0));
+#pragma unroll
+    for (int q = 0; q < Pair::SL; ++q) {
+      const int g = GS == 1 ? p : min(GS * p + sg[q], ng - 1);
+      if constexpr (ZP)
+        k.sz[q] = __builtin_bit_cast(f16x2, __builtin_amdgcn_raw_buffer_load_b32(sbuf, soff[q] + 128 * g, 0, 0));
+      else
+        k.s[q] = __builtin_bit_cast(f16, __builtin_amdgcn_raw_buffer_load_b16(sbuf, soff[q] + 64 * g, 0, 0));
+    }
   };
 #pragma unroll
   for (int j = 0; j < CW; ++j) load_x(ring[j], j);
 #pragma unroll
   for (int j = 0; j < CW; ++j) load_w(ring[j], j);
+  // the thread's outputs and their residuals, in time for the end (where there are none, of the codes, and not used)
+  constexpr int PER = (R * 16 * NT + 64 * KW - 1) / (64 * KW);
+  const int lw = __builtin_ctz(16 * NT) - (silu ? 1 : 0), nout = silu ? N / 2 : N;
+  f16 rv[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = threadIdx.x + i * 64 * KW, m = m0 + (at >> lw), n = (blockIdx.x << lw) + (at & ((1 << lw) - 1));
+    rv[i] = *(res && (at >> lw) < R && m < M && n < nout ? res + (long)m * ldr + n : (const f16*)codes);
+  }
+  __builtin_amdgcn_sched_barrier(0);
 
-  f32x4 tot[NT][MT];  // with a norm scaled by 2^e of their rows
+  f32x4 tot[NT];  // with a norm scaled by 2^e of their rows
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) tot[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  f16 p2[XO];
+  float ss[XO];
+  int e[XO];
 #pragma unroll
-    for (int q = 0; q < MT; ++q) tot[t][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  f16 p2 = (f16)1.f;
-  float ss = 0.f;
+  for (int o = 0; o < XO; ++o) p2[o] = (f16)1.f, ss[o] = 0.f, e[o] = 0;
 
   // every row's sums times its factor in us
   auto times_us = [&]() {
+    const f32x4 u = *(const f32x4*)(us + P * wv + 4 * g4);
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const f32x4 u = *(const f32x4*)(us + P * wv + 16 * q + 4 * g4);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) tot[t][q][r] *= u[r];
+      for (int r = 0; r < 4; ++r) tot[t][r] *= u[r];
+  };
+  auto set_us = [&](int o, float u) {
+    if (xj == 0) {
+      us[P * wv + 4 * o + xr] = u;
+      if constexpr (PAIR) us[P * wv + 8 + 4 * o + xr] = u;
     }
   };
-  auto set_us = [&](float u) {
-    if (lane < R) {
-      us[P * wv + lane] = u;
-      if constexpr (PAIR) us[P * wv + 8 + lane] = u;
-    }
-  };
-  // 2^e of the rows' n chunks in the ring, and their sums of squares
-  int e = 0;
+  // 2^e of the rows' n pairs in the ring, and their sums of squares
   auto scale_rows = [&](int n, bool first) {
-    float v = 0.f;
 #pragma unroll
-    for (int j = 0; j < CW; ++j)
-      if (j < n)
+    for (int o = 0; o < XO; ++o) {
+      float v = 0.f;
 #pragma unroll
-        for (int o = 0; o < MR; ++o)
+      for (int j = 0; j < CW; ++j)
+        if (j < n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const f16x2 p = {ring[j].x[o][2 * i], ring[j].x[o][2 * i + 1]};
             v = __builtin_amdgcn_fdot2(p, p, v, false);
           }
-#pragma unroll
-    for (int o = R; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    ss += v;
-    const float inv = __builtin_amdgcn_rsqf(v * (1.f / (64 * CW)));
-    const int was = e;
-    e = min(max((int)(__builtin_bit_cast(uint32_t, inv) >> 23) - 127, -14), 15);
-    p2 = __builtin_bit_cast(f16, (uint16_t)((e + 15) << 10));
-    if (!first) {
-      set_us(__builtin_bit_cast(float, (uint32_t)(127 + e - was) << 23));
-      times_us();
+      v = row_sum16(v);
+      ss[o] += v;
+      const float inv = __builtin_amdgcn_rsqf(v * (1.f / (128 * CW)));
+      const int was = e[o];
+      e[o] = min(max((int)(__builtin_bit_cast(uint32_t, inv) >> 23) - 127, -14), 15);
+      p2[o] = __builtin_bit_cast(f16, (uint16_t)((e[o] + 15) << 10));
+      if (!first) set_us(o, __builtin_bit_cast(float, (uint32_t)(127 + e[o] - was) << 23));
     }
+    if (!first) times_us();
   };
 
-  f16x8* const put = ops + xj * P + xr;
-  const f16x8* const get = ops + g4 * P + f;
-  auto compute = [&](const Chunk& k) {
+  f16x8* const put = ops + xj * PP + xr;
+  const f16x8* const get = ops + (8 * cc + 2 * h) * PP + f;
+  auto compute = [&](const Pair& k) {
 #pragma unroll
-    for (int o = 0; o < MR; ++o) {
+    for (int o = 0; o < XO; ++o) {
       f16x8 v = k.x[o];
       if constexpr (NORM) {
-        const f16x8 xv = v * p2;
-        v = xv * k.nw[o];
-        put[8 / MR * o * P + (PAIR ? 8 : LO)] = __builtin_elementwise_fma(xv, k.nw[o], -v);
+        const f16x8 xv = v * p2[o];
+        v = xv * k.nw;
+        put[4 * o + (PAIR ? 8 : LO)] = __builtin_elementwise_fma(xv, k.nw, -v);
       }
-      put[8 / MR * o * P] = v;
+      put[4 * o] = v;
     }
-    f32x4 acc[NT][MT];
+    uint32_t sc[Pair::SL * 4];
 #pragma unroll
-    for (int H = 0; H < 2; ++H) {
+    for (int q = 0; q < Pair::SL; ++q) {
+      uint32_t v;
+      if constexpr (ZP)
+        v = __builtin_bit_cast(uint32_t, k.sz[q]);
+      else
+        v = __builtin_bit_cast(uint16_t, k.s[q]);
+      spread16<(Pair::SLOTS < 4 ? Pair::SLOTS : 4)>(v, sc + 4 * q);
+    }
+    f16x8 xa[4], xb[LO > 0 ? 4 : 1];  // operands for dword 2 S + H of the lanes' codes
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float s;
+    for (int j = 0; j < 4; ++j) {
+      xa[j] = get[(4 * (j & 1) + (j >> 1)) * PP];
+      if constexpr (LO > 0) xb[j] = get[(4 * (j & 1) + (j >> 1)) * PP + LO];
+    }
+    const f16x8 none = {};
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      f16x8 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
         f16x2 c0 = {(f16)-1032.f, (f16)-1032.f}, c1 = {(f16)-72.f, (f16)-72.f};
         if constexpr (ZP) {
-          const f16x2 sz = k.sz[t][H & (GS - 1)];
-          s = (float)sz.x;
-          c0 = (f16x2){-sz.y, -sz.y};
+          const uint32_t* st = sc + t * GS;
+          const uint32_t v = GS == 1 ? st[0] : GS == 2 ? (cc ? st[GS / 2] : st[0]) : (cc ? st[GS / 2 + (j & 1) * (GS / 4)] : st[(j & 1) * (GS / 4)]);
+          const f16 z = __builtin_bit_cast(f16x2, v).y;
+          c0 = (f16x2){-z, -z};
           c1 = c0 + (f16x2){(f16)960.f, (f16)960.f};
-        } else {
-          s = (float)k.s[t][H & (GS - 1)];
         }
-        const f16x8 w = q4_halves(k.code[t][H], c0, c1);
+        w[j] = q4_halves(k.code[t][j], c0, c1);
+      }
 #pragma unroll
-        for (int q = 0; q < MT; ++q) {
-          if (H == 0 || GS == 2) acc[t][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
-          acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(get[4 * H * P + 16 * q], w, acc[t][q], 0, 0, 0);
-          if constexpr (LO > 0)
-            acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(get[4 * H * P + 16 * q + LO], w, acc[t][q], 0, 0, 0);
-          if (H == 1 || GS == 2) {
+      for (int g = 0; g < GS; ++g) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) tot[t][q][r] += s * acc[t][q][r];
-          }
+        for (int j = 0; j < 4; ++j) {
+          if (GS == 4 && (j & 1) != (g & 1)) continue;
+          const bool mine = GS == 1 || cc == g / (GS / 2 + (GS == 1));
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(mine ? xa[j] : none, w[j], acc, 0, 0, 0);
+          if constexpr (LO > 0) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(mine ? xb[j] : none, w[j], acc, 0, 0, 0);
         }
+        const float s = (float)__builtin_bit_cast(f16x2, sc[t * GS + g]).x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tot[t][r] += s * acc[r];
       }
     }
   };
@@ -326,85 +393,96 @@ __global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const Q4Args a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   if constexpr (NORM) {
-    set_us(__builtin_bit_cast(float, (uint32_t)(127 - e) << 23));
+#pragma unroll
+    for (int o = 0; o < XO; ++o) {
+      set_us(o, __builtin_bit_cast(float, (uint32_t)(127 - e[o]) << 23));
+      if (xj == 0) rs[R * wv + 4 * o + xr] = ss[o];
+    }
     times_us();
-    if (lane < R) rs[R * wv + lane] = ss;
   }
   __syncthreads();  // every wave is done with its operands
-  // a lane's sums: rows 16 q + 4 (lane / 16) .. + 3 of feature lane % 16
+  // a lane's sums: rows 4 (lane / 16) .. + 3 of feature lane % 16
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int q = 0; q < MT; ++q)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) part[(wv * P + 16 * q + 4 * g4 + r) * PW + 16 * t + f] = tot[t][q][r];
+    for (int r = 0; r < 4; ++r) {
+      float v = tot[t][r];
+      if constexpr (PAIR) {  // the second parts' sums are in the upper lanes
+        const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+        v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+      }
+      if (!PAIR || lane < 32) part[(wv * PR + 4 * g4 + r) * PW + 16 * t + f] = v;
+    }
   __syncthreads();
-  const int W = a.silu ? 8 * NT : 16 * NT;
-  for (int i = threadIdx.x; i < R * W; i += 64 * KW) {
-    const int r = i / W, j = i - r * W, m = m0 + r;
-    const int n = (a.silu ? n0 / 2 : n0) + j;
-    if (m >= a.M || n >= (a.silu ? a.N / 2 : a.N)) continue;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = threadIdx.x + i * 64 * KW, r = at >> lw, j = at & ((1 << lw) - 1), m = m0 + r, n = (blockIdx.x << lw) + j;
+    if (r >= R || m >= M || n >= nout) continue;
     float inv = 1.f;
     if constexpr (NORM) {
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < KW; ++w) v += rs[R * w + r];
-      inv = 1.0f / sqrtf(v / (float)a.K + a.eps);
+      inv = 1.0f / sqrtf(v / (float)K + eps);
     }
     auto add = [&](int c) {
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        v += part[(w * P + r) * PW + c];
-        if constexpr (PAIR) v += part[(w * P + 8 + r) * PW + c];
-      }
+      for (int w = 0; w < KW; ++w) v += part[(w * PR + r) * PW + c];
       return NORM ? v * inv : v;
     };
     float v;
-    if (a.silu) {
+    if (silu) {
       v = silu_mul(add(2 * j), add(2 * j + 1));
     } else {
       v = add(j);
-      if (a.res) v += (float)a.res[(long)m * a.ldr + n];
+      if (res) v += (float)rv[i];
     }
-    a.y[(long)m * a.ldy + n] = (f16)v;
+    y[(long)m * ldy + n] = (f16)v;
   }
 }
 
-template <int KW, int CW, int NT, int MR, bool ZP, int GS, bool NORM>
+template <int KW, int CW, int NT, int XO, bool ZP, int GS, bool NORM>
 static int launch_rows(const Q4Args& a, hipStream_t st) {
-  hipLaunchKernelGGL((mm_q4_rows_kernel<KW, CW, NT, MR, ZP, GS, NORM>),
-                     dim3((a.N + 16 * NT - 1) / (16 * NT), (a.M + 8 * MR - 1) / (8 * MR)), dim3(64 * KW), 0, st, a);
+  hipLaunchKernelGGL((mm_q4_rows_kernel<KW, CW, NT, XO, ZP, GS, NORM>),
+                     dim3((a.N + 16 * NT - 1) / (16 * NT), (a.M + 4 * XO - 1) / (4 * XO)), dim3(64 * KW), 0, st, a.x, a.codes,
+                     a.scales, a.nw, a.N, a.K, a.M, a.lg, a.ldx, a.eps, a.res, a.ldr, a.y, a.ldy, a.silu);
   return ecd_launch_status();
 }
-
 template <int KW, int CW, int NT, bool ZP, int GS, bool NORM>
 static int rows_by_m(const Q4Args& a, hipStream_t st) {
-  if (a.M <= 8) return launch_rows<KW, CW, NT, 1, ZP, GS, NORM>(a, st);
-  return launch_rows<KW, CW, NT, 2, ZP, GS, NORM>(a, st);
+  if (a.M <= 4) return launch_rows<KW, CW, NT, 1, ZP, GS, NORM>(a, st);
+  if (a.M <= 8) return launch_rows<KW, CW, NT, 2, ZP, GS, NORM>(a, st);
+  return launch_rows<KW, CW, NT, 4, ZP, GS, NORM>(a, st);
 }
-
+template <int KW, int CW, int NT, bool ZP, int GS>
+static int rows_by_norm(const Q4Args& a, hipStream_t st) {
+  return a.nw ? rows_by_m<KW, CW, NT, ZP, GS, true>(a, st) : rows_by_m<KW, CW, NT, ZP, GS, false>(a, st);
+}
+template <int KW, int CW, int NT, bool ZP>
+static int rows_by_group(const Q4Args& a, hipStream_t st) {
+  if (a.lg == 7) return rows_by_norm<KW, CW, NT, ZP, 1>(a, st);
+  if (a.lg == 6) return rows_by_norm<KW, CW, NT, ZP, 2>(a, st);
+  return rows_by_norm<KW, CW, NT, ZP, 4>(a, st);
+}
 template <int KW, int CW, int NT>
 static int rows_by_weights(const Q4Args& a, bool zp, hipStream_t st) {
-#define Q4_ROWS(Z, G) return a.nw ? rows_by_m<KW, CW, NT, Z, G, true>(a, st) : rows_by_m<KW, CW, NT, Z, G, false>(a, st)
-  if (zp) {
-    if (a.lg == 5) Q4_ROWS(true, 2);
-    Q4_ROWS(true, 1);
-  }
-  if (a.lg == 5) Q4_ROWS(false, 2);
-  Q4_ROWS(false, 1);
-#undef Q4_ROWS
+  return zp ? rows_by_group<KW, CW, NT, true>(a, st) : rows_by_group<KW, CW, NT, false>(a, st);
 }
 
-// One workgroup per CU where the features give as many: 16, 32 or 64 features each.  Over a long K, where 16 features leave CUs
-// idle anyway, twice the waves (3072 x 8192: 1 row 5.7 -> 5.1 us, 8 rows 7.7 -> 7.4; 3072 x 3072 with 8 rows 4.2 and 5.0).
-// us of 16 / 32 / 64 features: 8 rows of 3072 x 3072 4.2 / 4.7 / 6.4, 5120 x 3072 6.1 / 4.9 / 6.6, 16384 x 3072 9.9 / 7.4 / 7.2;
-// with the norm 5.5 / 6.1 / 7.8, 7.7 / 6.2 / 7.9, 12.2 / 9.4 / 8.4.  Four waves instead of eight: 5.2 (32 features), 5.3, 8.2.
-static int mm_rows(const Q4Args& a, bool zp, hipStream_t st) {
-  const int n16 = (a.N + 15) / 16;
-  if (n16 <= 256) return a.K >= 6144 ? rows_by_weights<16, 4, 1>(a, zp, st) : rows_by_weights<8, 3, 1>(a, zp, st);
-  if (n16 <= 512) return rows_by_weights<8, 3, 2>(a, zp, st);
-  return rows_by_weights<8, 3, 4>(a, zp, st);
+// form: features of a workgroup, 16 << (form - 1)
+static int mm_rows(const Q4Args& a, bool zp, int form, hipStream_t st) {
+  if (32L * a.ldx > 0x7FFFFFFFL || (a.M + 15) / 16 > 65535) return ECD_ENOTSUP;
+  if (form == 1) return rows_by_weights<8, 3, 1>(a, zp, st);
+  if (form == 2) return rows_by_weights<8, 3, 2>(a, zp, st);
+  return rows_by_weights<8, 2, 4>(a, zp, st);
+}
+// One workgroup per CU where the features give as many.  us of 16 / 32 / 64 features: 8 rows of 3072 x 3072 3.6 / 4.1 / 5.2,
+// 5120 x 3072 5.1 / 4.7 / 5.8, 16384 x 3072 with a norm 11.5 / 9.0 / 8.8 (and SiLU), 1 row of 8197 x 3072 with a norm
+// 7.2 / 7.0 / 6.9.  Sixteen waves instead of eight: 3.5, 4.6, 8.9, 7.0 with half the pairs in flight, and more rows spill.
+static int rows_form(int N) {
+  const int n16 = (N + 15) / 16;
+  return n16 <= 256 ? 1 : n16 <= 512 ? 2 : 3;
 }
 
 // ---------------------------------------------------------------- norm of many rows
@@ -481,12 +559,14 @@ int ecd_pack_q4(const void* q, const void* s, const void* z, int N, int K, int g
   return ecd_launch_status();
 }
 
-// Up to 16 rows the few-row kernel (plan 0), but for 9 .. 16 rows of a long K the matrix tiles, which split K over more
-// workgroups (16 rows, 1024 x 8192: 10.7 and 8.6 us; 3072 x 3072: 5.7 and 7.4).
-int ecd_mm_q4_plan(int M, int N, int K) {
+// Up to 16 rows the few-row kernel with the norm inside (plan 0): 9 .. 16 rows of 3072 x 3072 4.0 us and with a norm 5.7, of
+// 1024 x 8192 5.9 and 10.0, where the matrix tiles take 7.7, 10.1, 8.2 and 11.4.
+static int mm_q4_plan(int M, int N, int K, bool rows) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 64) return ECD_EINVAL;
-  return M <= 8 || (M <= 16 && K < 6144) ? 0 : gemm_q4_plan(M, N, K);
+  return M <= 16 ? 0 : gemm_q4_plan(M, N, K, rows);
 }
+int ecd_mm_q4_plan(int M, int N, int K) { return mm_q4_plan(M, N, K, false); }
+int ecd_mm_q4_choice(int M, int N, int K) { return mm_q4_plan(M, N, K, true); }
 
 long ecd_mm_q4_ws_bytes(int M, int N, int K, int plan, int norm) {
   if (M <= 0 || N <= 0 || K <= 0 || plan <= 0) return 0;
@@ -498,25 +578,32 @@ int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* co
               const void* res, long ldr, void* y, long ldy, int M, int N, int K, int silu, int plan, void* ws, void* stream) {
   const int cols = silu ? N / 2 : N;
   const int tile = plan & 255, ks = plan >> 8;
+  const bool rows = tile > Q4_ROWS_AT && tile <= Q4_ROWS_AT + Q4_ROWS;
   if (!x || !codes || !scales || !y || M <= 0 || N <= 0 || K <= 0 || K % 64 || !group_ok(group) || ldx < K || ldx % 8 ||
       !al16(x) || (nw && !al16(nw)) || !al16(codes) || !al16(scales) || ldy < cols || (res && ldr < cols) ||
-      (silu && (N % 2 || res)) || (nw && !(eps >= 0.f)) || (plan ? tile < 1 || tile > Q4_TILES || ks < 1 || ks > K / 64 : M > 16) ||
+      (silu && (N % 2 || res)) || (nw && !(eps >= 0.f)) || (plan ? !(rows ? ks == 1 : tile >= 1 && tile <= Q4_TILES && ks >= 1 && ks <= K / 64) : M > 16) ||
       (ecd_mm_q4_ws_bytes(M, N, K, plan, nw != nullptr) && (!ws || !al16(ws))))
     return ECD_EINVAL;
   if (N > 0x7FFFFFFF - 255 || K > 1 << 24 || ks > 65535) return ECD_ENOTSUP;
   Q4Args a{(const f16*)x, ldx, (const f16*)nw, eps, (const uint8_t*)codes, (const f16*)scales, log2_group(group),
            (const f16*)res, ldr, (f16*)y, ldy, M, N, K, silu};
   const hipStream_t st = (hipStream_t)stream;
-  if (!plan) return 16 * ldx * 2 > 0x7FFFFFFFL ? ECD_ENOTSUP : mm_rows(a, zeros, st);
+  if (!plan) return mm_rows(a, zeros, rows_form(N), st);
   if (nw) {
     a.x = (const f16*)((char*)ws + ecd_mm_q4_ws_bytes(M, N, K, plan, 0));
     a.ldx = K;
-    const int rc = gemm_q4(a, zeros, tile, (float*)ws, ks, nullptr, false);  // (refused sizes before the norm is launched)
-    if (rc != ECD_OK) return rc;
+    if (!rows) {  // (refused sizes before the norm is launched)
+      const int rc = gemm_q4(a, zeros, tile, (float*)ws, ks, nullptr, false);
+      if (rc != ECD_OK) return rc;
+    } else if ((M + 15) / 16 > 65535) {
+      return ECD_ENOTSUP;
+    }
     hipLaunchKernelGGL(q4_norm_kernel, dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps, (f16*)a.x, K);
     const int err = ecd_launch_status();
     if (err != ECD_OK) return err;
+    a.nw = nullptr;
   }
+  if (rows) return mm_rows(a, zeros, tile - Q4_ROWS_AT, st);
   return gemm_q4(a, zeros, tile, (float*)ws, ks, st, true);
 }
 

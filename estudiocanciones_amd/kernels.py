@@ -1190,7 +1190,7 @@ class PackedQ4:
     def plan(self, M):
         """(kernel choice, workspace bytes without and with a norm) of a product of M rows."""
         lib = _ffi.lib()
-        n = lib.ecd_mm_q4_plan(M, self.N, self.K)
+        n = lib.ecd_mm_q4_choice(M, self.N, self.K)
         p = self.plans[M] = (n, *(lib.ecd_mm_q4_ws_bytes(M, self.N, self.K, n, f) for f in (0, 1)))
         return p
 

@@ -220,6 +220,42 @@ def test_every_tile(dev, tile, M, N, K, ks, group, zeros, silu):
         assert (y[M] == 7.0).all()
 
 
+@pytest.mark.parametrize("form", [1, 2, 3])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 64), (4, 129, 192), (17, 300, 320), (40, 66, 1088), (150, 129, 2176), (33, 520, 128)])
+@pytest.mark.parametrize("group,zeros,silu", [(32, True, False), (32, False, True), (64, True, True), (64, False, False),
+                                              (128, True, True), (128, False, False)])
+def test_few_rows_at_a_time(dev, form, M, N, K, group, zeros, silu):
+    """The few-row kernel over blocks of rows, 16, 32 or 64 features a workgroup, with residual, norm and SiLU, into rows of a
+    larger matrix: the same values as without a plan, of which it changes nothing else."""
+    import torch
+    from estudiocanciones_amd import _ffi
+    q, s, z, w = make(M + N + K, N, K, group, zeros)
+    wp = packed(dev, q, s, z, silu and N % 2 == 0)
+    silu = wp.interleave
+    x, nw = randn16(M, M, K), (1 + 0.1 * rng(K).standard_normal(K)).astype(np.float16)
+    cols = N // 2 if silu else N
+    res = None if silu else randn16(M + 1, M, cols)
+    xt, nt, rt, st = _t(x, dev), _t(nw, dev), None if silu else _t(res, dev), torch.cuda.current_stream().cuda_stream
+    ws = torch.full((M * K,), float("nan"), device=dev, dtype=torch.float16)
+    for norm in (False, True):
+        y = torch.full((M + 1, cols + 8), 7.0, device=dev, dtype=torch.float16)
+        _ffi.call("ecd_mm_q4", xt.data_ptr(), K, nt.data_ptr() if norm else None, 1e-5, wp.codes_ptr, wp.scales_ptr, zeros, group,
+                  None if silu else rt.data_ptr(), cols, y.data_ptr(), cols + 8, M, N, K, silu, 16 + form + 256,
+                  ws.data_ptr() if norm else None, st)
+        xn = norm64(x, nw) if norm else x.astype(np.float64)
+        want, tol = xn @ w.T, sums_tol(xn, w, norm)
+        if silu:
+            a, b, ta, tb = want[:, :cols], want[:, cols:], tol[:, :cols], tol[:, cols:]
+            f = a / (1 + np.exp(-a))
+            want, tol = f * b, (1.1 * ta + 2.0 ** -20 * np.abs(f)) * (np.abs(b) + tb) + np.abs(f) * tb
+        else:
+            want = want + res
+        got = y[:M, :cols].double().cpu().numpy()
+        bad = ~(np.abs(got - want) <= tol + H * (np.abs(want) + tol) + 2.0 ** -25)
+        assert not bad.any(), (norm, bad.sum(), np.argwhere(bad)[0])
+        assert (y[M] == 7.0).all() and (y[:, cols:] == 7.0).all()
+
+
 @pytest.mark.parametrize("M,F,K", [(1, 1, 64), (1, 4099, 192), (3, 17, 192), (8, 512, 1024), (16, 40, 320), (30, 33, 64), (33, 500, 192),
                                    (64, 64, 128), (70, 65, 1024), (187, 1001, 320), (300, 256, 512)])
 @pytest.mark.parametrize("group,zeros,norm", [(32, True, True), (64, False, False), (128, False, True), (128, True, False)])

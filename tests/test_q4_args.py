@@ -86,3 +86,31 @@ def test_calls_refuse_tensors_that_are_not_on_a_gpu():
                  lambda: K.process_logits(x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_choices():
+    """Up to 16 rows no plan; more run by a tile or by the few-row kernel over blocks of rows, whose workspace is the normed rows'."""
+    from estudiocanciones_amd import _ffi
+    L = _ffi.lib()
+    seen = set()
+    for M, N, K in [(1, 1, 64), (16, 1024, 8192), (17, 33, 64), (48, 3072, 3072), (20, 5120, 3072), (187, 3072, 8192),
+                    (2048, 16384, 3072), (1 << 24, 64, 64), (30, 2000000, 128)]:
+        p = L.ecd_mm_q4_choice(M, N, K)
+        seen.add(p & 255)
+        assert (p == 0) == (M <= 16)
+        if p:
+            tile, ks = p & 255, p >> 8
+            assert 1 <= ks <= K // 64 and (1 <= tile <= 6 or (17 <= tile <= 19 and ks == 1 and M <= 16 * 65535))
+            if tile > 6:
+                assert L.ecd_mm_q4_ws_bytes(M, N, K, p, 0) == 0 and L.ecd_mm_q4_ws_bytes(M, N, K, p, 1) == 2 * M * K
+    assert seen & {17, 18, 19} and seen & set(range(1, 7))
+    assert [L.ecd_mm_q4_choice(*a) for a in ((0, 1, 64), (1, 0, 64), (1, 1, 65), (1, 1, 0))] == [-22] * 4
+
+
+@pytest.mark.parametrize("code,call", [
+    (I, mm(plan=16 + 256)), (I, mm(plan=17)), (I, mm(plan=17 + 512)), (I, mm(plan=20 + 256)), (I, mm(plan=18 + 256, nw=16)),
+    (N, mm(plan=17 + 256, ldx=1 << 27)), (N, mm(plan=19 + 256, M=16 * 65535 + 1)),
+    (N, mm(plan=19 + 256, M=16 * 65535 + 1, nw=16, ws=16))])
+def test_refused_few_row_plans(code, call):
+    from estudiocanciones_amd import _ffi
+    assert call(_ffi.lib()) == code
