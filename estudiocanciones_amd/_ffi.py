@@ -136,6 +136,7 @@ SIGNATURES = {
                   c_int, _P, _P],
     "ecd_mm_q4_plan": [c_int, c_int, c_int],
     "ecd_mm_q4_choice": [c_int, c_int, c_int],
+    "ecd_mm_q4_norm_choice": [c_int, c_int, c_int, c_int],
     "ecd_mm_q4_ws_bytes": [c_int, c_int, c_int, c_int, c_int],
     "ecd_process_logits": [_P, c_long, c_int, c_float, _P, c_long, c_long, c_int, _P, c_int, _P, _P, _P, c_int, _P, c_long, _P,
                            c_long, c_int, _P, _P, c_long, c_int, c_int, _P],

@@ -35,7 +35,7 @@ struct Q4Tile {
   static constexpr int EP = WK * ER * 4;
   static constexpr int LDS = NS * STG > EP ? NS * STG : EP;
 
-  // The sums of features n0 .., rows m0 .. over chunks c0 .. c1 - 1, in acc: lane l holds feature 32 (wn FT + ft) + (l & 31) of
+  // The sums of features n0 .., rows m0 .. over chunks c0 .. c1 - 1 (of x: with two parts twice those of the codes), in acc: lane l holds feature 32 (wn FT + ft) + (l & 31) of
   // rows 32 (wm RT + rt) + 8 (i / 4) + 4 (l / 32) + i % 4, i the register.
   static __device__ __forceinline__ void run(char* lds, const Q4Args& a, int n0, int m0, int c0, int c1, f32x16 (&acc)[FT][RT]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -45,7 +45,7 @@ struct Q4Tile {
     const int nch = a.K >> 6, ng = ((a.K - 1) >> a.lg) + 1, last = (a.N - 1) >> 5, t0 = n0 >> 5;
     // sources: uniform bases that advance with the chunk, and each lane's offset
     const char* xb = (const char*)(a.x + (long)m0 * a.ldx) + 128L * c0;
-    const char* cb = (const char*)a.codes + ((long)t0 * nch + c0) * 1024;
+    const char* cb = (const char*)a.codes + (long)t0 * nch * 1024;
     const char* sb = (const char*)a.scales + (long)t0 * ng * (ZP ? 128 : 64);
     uint32_t xoff[XI], coff[CI], soff;
 #pragma unroll
@@ -67,10 +67,9 @@ struct Q4Tile {
     auto load = [&](int st) {
       static_for<0, XI>([&](auto J) { lds_dma16_at<NW * J.value * 1024>(xb, xoff[J.value], lx + st * STG); });
       if (CB >= 1024 || 16 * lane < CB)
-        static_for<0, CI>([&](auto J) { lds_dma16_at<J.value * 1024>(cb, coff[J.value], lc + st * STG); });
-      if (16 * lane < SW) lds_dma16_at<0>(sb + (long)((64 * cl) >> a.lg) * (ZP ? 128 : 64), soff, ls + st * STG);
+        static_for<0, CI>([&](auto J) { lds_dma16_at<J.value * 1024>(cb + 1024L * (cl >> a.two), coff[J.value], lc + st * STG); });
+      if (16 * lane < SW) lds_dma16_at<0>(sb + (long)((64 * (cl >> a.two)) >> a.lg) * (ZP ? 128 : 64), soff, ls + st * STG);
       xb += WK * 128;
-      cb += WK * 1024;
       cl += WK;
     };
     static_for<0, FT * RT>([&](auto I) { acc[I.value / RT][I.value % RT] = (f32x16)(0.f); });
@@ -162,7 +161,7 @@ struct Q4Tile {
     static_for<0, 2 * FT>([&](auto I) { dequant(I, IC<0>{}, fa); });
     // what the sums are multiplied by before the products of half H of chunk c, whose scales are in sz
     auto turn = [&](int c, int H) {
-      if (GS == 2 ? (c == 0 && H == 0) : (H != 0 || c == 0 || (WK == 1 && ((c0 + c) << 6 & ((1 << a.lg) - 1))))) return false;
+      if (GS == 2 ? (c == 0 && H == 0) : (H != 0 || c == 0 || (WK == 1 && ((c0 + c) << 6 & ((1 << (a.lg + a.two)) - 1))))) return false;
       static_for<0, FT>([&](auto F) {
         const float s = scale(F.value, H & (GS - 1));
         q[F.value] = was[F.value] * __builtin_amdgcn_rcpf(s);
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK, 2) void gemm_q4_kernel(const Q4A
   GemmTile<true, false, 1, 1, 1, 1, 2>::block(nfb, nmb, fb, mb);
   const int n0 = fb * T::BN, m0 = mb * T::BM;
   f32x16 acc[FT][RT];
-  T::run(lds, a, n0, m0, 0, a.K >> 6, acc);
+  T::run(lds, a, n0, m0, 0, a.K >> 6 << a.two, acc);
   T::rows(lds, acc, [&](int r, int p, f32x4 u, f32x4 v) { q4_finish(a, m0 + r, n0 + 8 * p, u, v); });
 }
 
@@ -288,7 +287,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK, 2) void gemm_q4_partial_kernel(c
   __shared__ __align__(16) char lds[T::LDS];
   int fb, mb;
   GemmTile<true, false, 1, 1, 1, 1, 2>::block(nfb, nmb, fb, mb);
-  const int n0 = fb * T::BN, m0 = mb * T::BM, nch = a.K >> 6, z = blockIdx.y, ks = gridDim.y;
+  const int n0 = fb * T::BN, m0 = mb * T::BM, nch = a.K >> 6 << a.two, z = blockIdx.y, ks = gridDim.y;
   f32x16 acc[FT][RT];
   T::run(lds, a, n0, m0, (int)((long)nch * z / ks), (int)((long)nch * (z + 1) / ks), acc);
   const long ld = (a.N + 7) & ~7L;
@@ -356,38 +355,44 @@ int gemm_q4(const Q4Args& a, bool zp, int tile, float* ws, int ks, hipStream_t s
 
 // The tiles: features x rows, chunks of a step (WK), workgroups that a CU holds, and measured times in ns: a step of a workgroup
 // alone on its CU and of a full CU, and the rest of a workgroup's time.  Fitted to 2400 timings (12 to 3000 rows, 1001 to 16384
-// features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.  The last three are the
+// features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.  Then the
 // few-row kernel's forms, whose 8 waves take a pair of chunks each in a step (360 timings of 16 to 256 rows, 7 to 9% rms): they
 // read the codes again for every 16 rows, but a CU starts on them with all loads in flight and ends without a split's join
-// (48 rows of 3072 x 3072: 5.8 us, the best tile 8.8; 192 rows of 5120 x 3072: 15.5 and 11.7).
+// (48 rows of 3072 x 3072: 5.8 us, the best tile 8.8; 192 rows of 5120 x 3072: 15.5 and 11.7).  And those with the norm inside (312
+// timings, 5% rms), which save its launch (48 rows 8.3 us, the tiles 11.8 with rows rounded once and 13.7 in two parts).
 struct Q4Cost {
   int bn, bm, wk, fit, step, full, rest;
 };
-constexpr Q4Cost Q4_COST[Q4_TILES + Q4_ROWS] = {
+constexpr Q4Cost Q4_COST[Q4_TILES + 2 * Q4_ROWS] = {
     {256, 128, 1, 2, 874, 1372, 3509}, {128, 128, 2, 1, 882, 882, 2404}, {128, 64, 2, 2, 551, 1142, 1853},
     {128, 32, 2, 2, 413, 741, 1582},   {64, 32, 4, 1, 484, 484, 1462},   {64, 64, 4, 1, 677, 677, 1732},
     {16, 16, 16, 1, 438, 363, 619},    {32, 16, 16, 1, 596, 516, 693},  {64, 16, 16, 1, 994, 961, 717},
+    {16, 16, 16, 1, 761, 777, 1780},   {32, 16, 16, 1, 936, 1013, 1926}, {64, 16, 16, 1, 1437, 1765, 1757},
 };
 
 // The choice of the shortest estimate.  Over the 96 shapes that the times were taken at it is 0.8% behind the fastest of all on
-// average, 11% at most; over 120 shapes with few rows as much, and 12%.  A split's join costs a launch and the passage of its sums through memory.
-int gemm_q4_plan(int M, int N, int K, bool rows) {
-  const int nch = K >> 6;
+// average, 11% at most; over 120 shapes with few rows as much, and 12%; over 104 with
+// a norm 0.2%, 10%, and before a SiLU 0.4%, 15%.  A split's join costs a launch and the passage of its sums through memory.
+int gemm_q4_plan(int M, int N, int K, Q4Among among) {
+  const bool norm = among >= Q4_NORM;
   long best = 0x7FFFFFFFFFFFFFFFL;
-  int plan = 1 + 256;
-  for (int t = 0; t < Q4_TILES + (rows ? Q4_ROWS : 0); ++t) {
-    const Q4Cost& c = Q4_COST[t];
+  int plan = 0;
+  for (int t = 0; t < Q4_TILES + (among == Q4_ONLY_TILES ? 0 : Q4_ROWS); ++t) {
+    const bool rows = t >= Q4_TILES, two = rows ? norm : among == Q4_NORM_SILU;
+    const Q4Cost& c = Q4_COST[rows && two ? t + Q4_ROWS : t];
+    const int nch = K >> 6 << (two && !rows);
     const long tiles = ((long)N + c.bn - 1) / c.bn * (((long)M + c.bm - 1) / c.bm);
-    for (int ks = 1; ks <= 12; ++ks) {
-      if (ks > 1 && (t >= Q4_TILES || tiles * ks > 1100 || nch < 4 * ks)) break;
+    for (int ks = 1; ks <= (rows ? 1 : 12); ++ks) {
+      if (ks > 1 && (tiles * ks > 1100 || nch < 4 * ks)) break;
       const long blocks = tiles * ks, steps = ((nch + ks - 1) / ks + c.wk - 1) / c.wk, per = 256L * c.fit, rem = blocks % per;
       long e = blocks / per * (steps * c.full + c.rest);
       // a last round of more than one workgroup per CU: 30% of the way to a full one at once, the rest with their number
       if (rem) e += steps * (c.step + (rem > 256 ? (c.full - c.step) * (77 + 179 * (rem - 256) / 256) / 256 : 0)) + c.rest;
       if (ks > 1) e += 2700 + 12L * (ks + 1) * M * N / 10000;
+      if (norm && !rows) e += 2700;  // the norm's launch
       if (e < best) {
         best = e;
-        plan = (t < Q4_TILES ? t + 1 : t + 1 - Q4_TILES + Q4_ROWS_AT) + 256 * ks;
+        plan = (rows ? t + 1 - Q4_TILES + Q4_ROWS_AT : t + 1) + (two ? Q4_TWO : 0) + 256 * ks;
       }
     }
   }

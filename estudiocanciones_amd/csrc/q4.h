@@ -54,14 +54,19 @@ struct Q4Args {
   long ldy;
   int M, N, K;
   int silu;  // pairs of rows (a, b) of the packed matrix give silu(a) b
+  int two;   // 1: rows of x are two fp16 parts, 64 of the first, 64 of the second, and so on (2 K in all); the tiles only
 };
 
 // The product by a tile (1 .. Q4_TILES) of gemm_q4.hip, K split ks ways (ws: ks M ceil8(N) floats where ks > 1); no norm.
-// go false: only whether the sizes fit.  And the choice for given sizes: tile + 256 ks; with rows also of the few-row
-// kernel's forms of 16, 32 and 64 features, which count as tiles Q4_ROWS_AT + 1 ..
-constexpr int Q4_TILES = 6, Q4_ROWS_AT = 16, Q4_ROWS = 3;
+// go false: only whether the sizes fit.  And the choice for given sizes: tile + 256 ks; the few-row
+// kernel's forms of 16, 32 and 64 features count as tiles Q4_ROWS_AT + 1 ..,
+// Q4_TWO more: with the rows' norm in two fp16 parts.
+// Q4_ONLY_TILES: the tiles; Q4_PLAIN: the few-row kernel's forms too; Q4_NORM: for products with a norm (the forms in two parts, the
+// tiles in one); Q4_NORM_SILU: in two parts.
+enum Q4Among { Q4_ONLY_TILES, Q4_PLAIN, Q4_NORM, Q4_NORM_SILU };
+constexpr int Q4_TILES = 6, Q4_ROWS_AT = 16, Q4_ROWS = 3, Q4_TWO = 32;
 int gemm_q4(const Q4Args& a, bool zp, int tile, float* ws, int ks, hipStream_t st, bool go);
-int gemm_q4_plan(int M, int N, int K, bool rows);
+int gemm_q4_plan(int M, int N, int K, Q4Among among);
 
 // silu(a) * b in fp32
 // (the exponential and the reciprocal by their instructions, 1 ulp of fp32 each)

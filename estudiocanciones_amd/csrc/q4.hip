@@ -486,8 +486,11 @@ static int rows_form(int N) {
 }
 
 // ---------------------------------------------------------------- norm of many rows
-// y = fp16(x / rms * nw), one rounding, for the matrix tiles, whose operands are fp16.  A workgroup per row; the second read of the
-// row comes from the caches.
+// y = fp16(x / rms * nw), one rounding, for the matrix tiles, whose operands are fp16: it adds about as much to a product's error as
+// the rounding of the result (2.1e-4 -> 2.9e-4 of the result, rms).  A SiLU multiplies two such products (3.7e-4), so before one
+// the rows go in as two parts, the second what the first's rounding left, 64 of each in turn (2.1e-4 again, for up to
+// twice the time: 384 rows of 16384 x 3072 92 us instead of 52).  A workgroup per row; the second read of the row comes from the caches.
+template <bool TWO>
 __global__ __launch_bounds__(256) void q4_norm_kernel(const f16* __restrict__ x, long ldx, const f16* __restrict__ nw, float eps,
                                                       f16* __restrict__ y, int K) {
   __shared__ float part[4];
@@ -504,10 +507,20 @@ __global__ __launch_bounds__(256) void q4_norm_kernel(const f16* __restrict__ x,
   const float inv = 1.0f / sqrtf((part[0] + part[1] + part[2] + part[3]) / (float)K + eps);
   for (int k = 8 * threadIdx.x; k < K; k += 2048) {
     const f16x8 v = *(const f16x8*)(xr + k), w = *(const f16x8*)(nw + k);
-    f16x8 o;
+    f16x8 o, rest;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (f16)((float)v[j] * inv * (float)w[j]);
-    *(f16x8*)(y + (long)blockIdx.x * K + k) = o;
+    for (int j = 0; j < 8; ++j) {
+      const float u = (float)v[j] * inv * (float)w[j];
+      o[j] = (f16)u;
+      rest[j] = (f16)(u - (float)o[j]);
+    }
+    if constexpr (TWO) {
+      f16* const d = y + (long)blockIdx.x * 2 * K + 2 * k - (k & 63);  // 128 (k / 64) + k % 64
+      *(f16x8*)d = o;
+      *(f16x8*)(d + 64) = rest;
+    } else {
+      *(f16x8*)(y + (long)blockIdx.x * K + k) = o;
+    }
   }
 }
 
@@ -561,44 +574,51 @@ int ecd_pack_q4(const void* q, const void* s, const void* z, int N, int K, int g
 
 // Up to 16 rows the few-row kernel with the norm inside (plan 0): 9 .. 16 rows of 3072 x 3072 4.0 us and with a norm 5.7, of
 // 1024 x 8192 5.9 and 10.0, where the matrix tiles take 7.7, 10.1, 8.2 and 11.4.
-static int mm_q4_plan(int M, int N, int K, bool rows) {
+static int mm_q4_plan(int M, int N, int K, Q4Among among) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 64) return ECD_EINVAL;
-  return M <= 16 ? 0 : gemm_q4_plan(M, N, K, rows);
+  return M <= 16 ? 0 : gemm_q4_plan(M, N, K, among);
 }
-int ecd_mm_q4_plan(int M, int N, int K) { return mm_q4_plan(M, N, K, false); }
-int ecd_mm_q4_choice(int M, int N, int K) { return mm_q4_plan(M, N, K, true); }
+int ecd_mm_q4_plan(int M, int N, int K) { return mm_q4_plan(M, N, K, Q4_ONLY_TILES); }
+int ecd_mm_q4_choice(int M, int N, int K) { return mm_q4_plan(M, N, K, Q4_PLAIN); }
+int ecd_mm_q4_norm_choice(int M, int N, int K, int silu) { return mm_q4_plan(M, N, K, silu ? Q4_NORM_SILU : Q4_NORM); }
 
 long ecd_mm_q4_ws_bytes(int M, int N, int K, int plan, int norm) {
   if (M <= 0 || N <= 0 || K <= 0 || plan <= 0) return 0;
   const long ks = plan >> 8, sums = ks > 1 ? ks * M * ((N + 7L) / 8 * 8) * 4 : 0;
-  return sums + (norm ? 2L * M * K : 0);
+  const bool rows = (plan & 31) > Q4_ROWS_AT, two = plan & Q4_TWO;
+  return sums + (!norm || (rows && two) ? 0 : (two ? 4L : 2L) * M * K);
 }
 
 int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* codes, const void* scales, int zeros, int group,
               const void* res, long ldr, void* y, long ldy, int M, int N, int K, int silu, int plan, void* ws, void* stream) {
   const int cols = silu ? N / 2 : N;
-  const int tile = plan & 255, ks = plan >> 8;
+  const bool two = plan & Q4_TWO;
+  const int tile = (plan & 255) - (two ? Q4_TWO : 0), ks = plan >> 8;
   const bool rows = tile > Q4_ROWS_AT && tile <= Q4_ROWS_AT + Q4_ROWS;
   if (!x || !codes || !scales || !y || M <= 0 || N <= 0 || K <= 0 || K % 64 || !group_ok(group) || ldx < K || ldx % 8 ||
       !al16(x) || (nw && !al16(nw)) || !al16(codes) || !al16(scales) || ldy < cols || (res && ldr < cols) ||
-      (silu && (N % 2 || res)) || (nw && !(eps >= 0.f)) || (plan ? !(rows ? ks == 1 : tile >= 1 && tile <= Q4_TILES && ks >= 1 && ks <= K / 64) : M > 16) ||
+      (silu && (N % 2 || res)) || (nw && !(eps >= 0.f)) || (plan ? !(rows ? ks == 1 : tile >= 1 && tile <= Q4_TILES && ks >= 1 && ks <= K / 64) || (two && !nw) : M > 16) ||
       (ecd_mm_q4_ws_bytes(M, N, K, plan, nw != nullptr) && (!ws || !al16(ws))))
     return ECD_EINVAL;
   if (N > 0x7FFFFFFF - 255 || K > 1 << 24 || ks > 65535) return ECD_ENOTSUP;
   Q4Args a{(const f16*)x, ldx, (const f16*)nw, eps, (const uint8_t*)codes, (const f16*)scales, log2_group(group),
-           (const f16*)res, ldr, (f16*)y, ldy, M, N, K, silu};
+           (const f16*)res, ldr, (f16*)y, ldy, M, N, K, silu, 0};
   const hipStream_t st = (hipStream_t)stream;
   if (!plan) return mm_rows(a, zeros, rows_form(N), st);
-  if (nw) {
+  if (nw && !(rows && two)) {
     a.x = (const f16*)((char*)ws + ecd_mm_q4_ws_bytes(M, N, K, plan, 0));
-    a.ldx = K;
+    a.ldx = two ? 2L * K : K;
+    a.two = two;
     if (!rows) {  // (refused sizes before the norm is launched)
       const int rc = gemm_q4(a, zeros, tile, (float*)ws, ks, nullptr, false);
       if (rc != ECD_OK) return rc;
     } else if ((M + 15) / 16 > 65535) {
       return ECD_ENOTSUP;
     }
-    hipLaunchKernelGGL(q4_norm_kernel, dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps, (f16*)a.x, K);
+    if (two)
+      hipLaunchKernelGGL(q4_norm_kernel<true>, dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps, (f16*)a.x, K);
+    else
+      hipLaunchKernelGGL(q4_norm_kernel<false>, dim3(M), dim3(256), 0, st, (const f16*)x, ldx, (const f16*)nw, eps, (f16*)a.x, K);
     const int err = ecd_launch_status();
     if (err != ECD_OK) return err;
     a.nw = nullptr;

@@ -1185,13 +1185,13 @@ class PackedQ4:
         self.N, self.K, self.group, self.zeros, self.interleave = N, K, group, zeros, interleave
         self.dev = codes.device
         self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
-        self.plans = {}  # rows -> plan(rows): they depend on sizes alone
+        self.plans = {}  # rows -> plan(rows): it depends on sizes alone
 
     def plan(self, M):
-        """(kernel choice, workspace bytes without and with a norm) of a product of M rows."""
-        lib = _ffi.lib()
-        n = lib.ecd_mm_q4_choice(M, self.N, self.K)
-        p = self.plans[M] = (n, *(lib.ecd_mm_q4_ws_bytes(M, self.N, self.K, n, f) for f in (0, 1)))
+        """(choice of the kernel, workspace bytes) of a product of M rows, and of one with a norm."""
+        lib, N, K = _ffi.lib(), self.N, self.K
+        n, f = lib.ecd_mm_q4_choice(M, N, K), lib.ecd_mm_q4_norm_choice(M, N, K, self.interleave)
+        p = self.plans[M] = ((n, lib.ecd_mm_q4_ws_bytes(M, N, K, n, 0)), (f, lib.ecd_mm_q4_ws_bytes(M, N, K, f, 1)))
         return p
 
     @property
@@ -1252,13 +1252,12 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         if _ends(out)[0] < _ends(x)[1] and _ends(x)[0] < _ends(out)[1]:
             raise ValueError(f"{name}: out must not overlap x")
     if M:
-        plan = w.plans.get(M) or w.plan(M)
-        nb = plan[1 if np is None else 2]
+        plan, nb = (w.plans.get(M) or w.plan(M))[0 if np is None else 1]
         if nb:
             ws = torch.empty(nb, device=dev, dtype=torch.uint8)  # (held until the launch)
             wp = ws.data_ptr()
         _call_on(dev, "ecd_mm_q4", x.data_ptr(), ldx, np, eps, w.codes_ptr, w.scales_ptr, w.zeros, w.group, rp, ldr,
-                 out.data_ptr(), ldy, M, w.N, K, silu, plan[0], wp)
+                 out.data_ptr(), ldy, M, w.N, K, silu, plan, wp)
     return out
 
 

@@ -704,10 +704,12 @@ int ecd_pack_q4(const void* q, const void* s, const void* z, int N, int K, int g
  *   x rows and nw 16-byte aligned; zeros: whether the weights were packed with zero points; y may be res, not x.
  *   plan: ecd_mm_q4_choice's kernel for these sizes, or 0 (few rows, M <= 16), or tile + 256 ks with tile 1 .. 6 and K split ks
  *   ways, or 17, 18 or 19 + 256 (few rows at a time, 16, 32 or 64 features a workgroup); ecd_mm_q4_plan: the choice among 0 and
- *   the tiles.  ws: 16-byte aligned workspace of ecd_mm_q4_ws_bytes (norm: whether nw is given; any contents).
+ *   the tiles.  With nw any of these but 0 takes x' rounded to fp16; 32 more takes it in two fp16 parts, as 0 does.  With nw:
+ *   ecd_mm_q4_norm_choice (silu: in two parts, as the roundings of both factors would add up).  ws: 16-byte aligned workspace of ecd_mm_q4_ws_bytes (norm: whether nw is given; any contents).
  * A row's result does not depend on the other rows; its last bits depend on the plan (the order of the sums). */
 int ecd_mm_q4_plan(int M, int N, int K);
 int ecd_mm_q4_choice(int M, int N, int K);
+int ecd_mm_q4_norm_choice(int M, int N, int K, int silu);
 long ecd_mm_q4_ws_bytes(int M, int N, int K, int plan, int norm);
 int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* codes, const void* scales, int zeros, int group,
               const void* res, long ldr, void* y, long ldy, int M, int N, int K, int silu, int plan, void* ws, void* stream);

@@ -256,6 +256,45 @@ def test_few_rows_at_a_time(dev, form, M, N, K, group, zeros, silu):
         assert (y[M] == 7.0).all() and (y[:, cols:] == 7.0).all()
 
 
+@pytest.mark.parametrize("plan", [1, 2 + 256, 3 + 512, 4, 5 + 512, 6 + 256, 17, 18, 19])
+@pytest.mark.parametrize("M,F,K", [(5, 20, 192), (37, 150, 320), (150, 65, 1088), (300, 260, 256)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
+def test_norm_in_two_parts(dev, plan, M, F, K, group, zeros):
+    """The norm before a SiLU in two fp16 parts, by the tiles (K whole and split, of odd and even numbers of chunks) and by the
+    few-row kernel: x' counts with 2^-22 of its value (what is left of the second part, 2^-25 of it where that is subnormal) and
+    the fp32 roundings of the norm (four of 2^-24), not with half a step of fp16."""
+    import torch
+    from estudiocanciones_amd import _ffi
+    tile, ks = plan & 255, 1 + (plan >> 8)
+    q, s, z, w = make(M + F + K, 2 * F, K, group, zeros)
+    wp = packed(dev, q, s, z, True)
+    x, nw = randn16(M, M, K), (1 + 0.1 * rng(K).standard_normal(K)).astype(np.float16)
+    xt, nt, st = _t(x, dev), _t(nw, dev), torch.cuda.current_stream().cuda_stream
+    plan = 32 + tile + 256 * ks
+    nb = _ffi.lib().ecd_mm_q4_ws_bytes(M, 2 * F, K, plan, 1)
+    assert nb == (0 if tile > 6 else 4 * M * K + (ks * M * (-(-2 * F // 8) * 8) * 4 if ks > 1 else 0))
+    ws = torch.full((nb // 4 + 64,), float("nan"), device=dev)
+    y = torch.full((M + 1, F), 7.0, device=dev, dtype=torch.float16)
+    _ffi.call("ecd_mm_q4", xt.data_ptr(), K, nt.data_ptr(), 1e-5, wp.codes_ptr, wp.scales_ptr, zeros, group, None, 0,
+              y.data_ptr(), F, M, 2 * F, K, True, plan, ws.data_ptr(), st)
+    xn = norm64(x, nw)
+    A = np.abs(xn) @ np.abs(w).T
+    want = xn @ w.T
+    # sums as in sums_tol (twice the additions), the quotients of scales (K / 16 at most, 2^-22 + 2^-24 each), and x'
+    tol = (2.0 ** -23 * (2 * 64 + 2 * K // 64 + 32) + K / 16 * 1.25 * 2.0 ** -22 + 2.0 ** -22 + 2.0 ** -22) * A
+    tol += 2.0 ** -25 * np.abs(w).sum(1)
+    a, b, ta, tb = want[:, :F], want[:, F:], tol[:, :F], tol[:, F:]
+    f = a / (1 + np.exp(-a))
+    want, tol = f * b, (1.1 * ta + 2.0 ** -20 * np.abs(f)) * (np.abs(b) + tb) + np.abs(f) * tb
+    got = y[:M].double().cpu().numpy()
+    err = np.abs(got - want)
+    bad = ~(err <= tol + H * (np.abs(want) + tol) + 2.0 ** -25)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[0])
+    assert (y[M] == 7.0).all() and torch.isnan(ws[nb // 4:]).all()
+    if want.size >= 2000:  # one rounding, of H / sqrt(3) at most in the mean (an x' rounded once adds as much twice)
+        assert np.sqrt((err ** 2).mean()) <= 0.6 * H * np.sqrt((want ** 2).mean()) + 2.0 ** -25
+
+
 @pytest.mark.parametrize("M,F,K", [(1, 1, 64), (1, 4099, 192), (3, 17, 192), (8, 512, 1024), (16, 40, 320), (30, 33, 64), (33, 500, 192),
                                    (64, 64, 128), (70, 65, 1024), (187, 1001, 320), (300, 256, 512)])
 @pytest.mark.parametrize("group,zeros,norm", [(32, True, True), (64, False, False), (128, False, True), (128, True, False)])

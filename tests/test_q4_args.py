@@ -114,3 +114,30 @@ def test_choices():
 def test_refused_few_row_plans(code, call):
     from estudiocanciones_amd import _ffi
     assert call(_ffi.lib()) == code
+
+
+def test_choices_with_two_parts():
+    """A norm in two parts: 32 more than a plan, and for the tiles twice the normed rows in the workspace; none without a norm."""
+    from estudiocanciones_amd import _ffi
+    L = _ffi.lib()
+    seen = set()
+    for M, N, K in [(1, 2, 64), (16, 1024, 8192), (17, 34, 64), (48, 3072, 3072), (2048, 16384, 3072), (1 << 24, 64, 64)]:
+        p = L.ecd_mm_q4_norm_choice(M, N, K, 1)
+        assert (p == 0) == (M <= 16)
+        if p:
+            tile, ks = (p & 255) - 32, p >> 8
+            seen.add(tile)
+            assert 1 <= ks <= K // 64 and (1 <= tile <= 6 or (17 <= tile <= 19 and ks == 1))
+            part = ks * M * (-(-N // 8) * 8) * 4 if ks > 1 else 0
+            assert L.ecd_mm_q4_ws_bytes(M, N, K, p, 1) == (part + 4 * M * K if tile <= 6 else 0)
+            assert mm(plan=p, M=M, N=N, K=K, ldx=K, ldy=N)(L) == I
+    assert seen & {17, 18, 19} and seen & set(range(1, 7))
+    # without a SiLU the tiles take rows rounded once
+    for M in (17, 48, 300, 2048):
+        p = L.ecd_mm_q4_norm_choice(M, 16384, 3072, 0)
+        assert (p & 32) == (32 if p & 16 else 0) and L.ecd_mm_q4_ws_bytes(M, 16384, 3072, p, 1) == (0 if p & 16 else 2 * M * 3072) + \
+            ((p >> 8) * M * 16384 * 4 if p >> 8 > 1 else 0)
+    assert mm(plan=32 + 1 + 256, nw=16)(L) == I and mm(plan=32 + 1 + 256, nw=16, ws=24)(L) == I  # no workspace for it
+    assert mm(plan=32, nw=16, ws=16)(L) == I and mm(plan=32 + 16 + 256, nw=16, ws=16)(L) == I
+    assert mm(plan=64 + 1 + 256, nw=16, ws=16)(L) == I
+    assert [L.ecd_mm_q4_norm_choice(*a) for a in ((0, 1, 64, 0), (1, 0, 64, 1), (1, 1, 65, 0), (1, 1, 0, 1))] == [-22] * 4
