@@ -149,7 +149,11 @@ class Linear:
         if self.q8 is None:
             if self.w4 is None:
                 self.pack()
-            return mm_q4(x, self.w4, res=res)
+            shape = (*x.shape[:-1], self.N)
+            x2 = x.reshape(-1, self.K)
+            if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+                x2 = x2.clone(memory_format=torch.contiguous_format)
+            return mm_q4(x2, self.w4, res=None if res is None else res.reshape(-1, self.N)).reshape(shape)
         if self.qp is not None and self.sp is self.s8 and x.dim() == 2 and x.stride(1) == 1 \
                 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
             if self.ks > 1:
@@ -969,7 +973,7 @@ class HeartMuLaLite:
 
     # -------------------------------------------------- logits before the sampler
     @staticmethod
-    def _check_rules(repetition, presence, frequency, window, bias, allowed):
+    def _check_rules(repetition, presence, frequency, window, bias, allowed, min_frames=0):
         for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
             if not math.isfinite(v) or (name == "repetition" and v <= 0):
                 raise ValueError(f"generate: {name} must be a finite number" + (" above 0" if name == "repetition" else ""))
@@ -978,6 +982,10 @@ class HeartMuLaLite:
         for name, t, dt in (("bias", bias, torch.float32), ("allowed", allowed, torch.bool)):
             if t is not None and (t.dtype != dt or tuple(t.shape) != (N_CB, AUDIO_VOCAB)):
                 raise ValueError(f"generate: {name} must be {dt} [{N_CB}, {AUDIO_VOCAB}]")
+        if bias is not None and not bias.isfinite().all():
+            raise ValueError("generate: bias must be finite (allowed forbids codes)")
+        if allowed is not None and not allowed[:, :AUDIO_EOS if min_frames > 0 else AUDIO_VOCAB].any(1).all():
+            raise ValueError("generate: allowed must leave every codebook a code" + (" that does not end the song" if min_frames > 0 else ""))
 
     def _song_rules(self, out, P, repetition, presence, frequency, window, bias, allowed, min_frames):
         """The arguments of process_logits for a song whose frames go to ``out`` [F, N, 8] (the history of codebook i is
@@ -1213,8 +1221,10 @@ class HeartMuLaLite:
 
         ``repetition``, ``presence``, ``frequency``: penalties for codes that a take's codebook has had in the last
         ``window`` frames (0: in the song so far): logits l > 0 become l / repetition, others l * repetition, then
-        l - (presence + frequency * count).  ``bias`` float32 [8, V] is added; ``allowed`` bool [8, V] forbids codes;
-        before ``min_ms`` no frame ends the song (process_logits, on the guided logits in fp32; teacher forcing ignores them)."""
+        l - (presence + frequency * count).  ``bias`` float32 [8, V], finite, is added; ``allowed`` bool [8, V] forbids codes (not
+        all of a codebook); before ``min_ms`` no frame ends the song.  process_logits does so on the guided logits in fp32;
+        teacher forcing ignores it.  A penalty or bias that takes every allowed logit of a codebook out of fp16's range leaves
+        nothing to draw, which ends the take."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
         if a8 and not self.backbone.eight():
@@ -1223,7 +1233,8 @@ class HeartMuLaLite:
             raise NotImplementedError("generate: int8 activations need a head_dim of 64, 128, 256 or 384 and 1, 2, 3, 4, 6 or 8 "
                                       "query heads per kv head")
         rules = float(repetition), float(presence), float(frequency), int(window)
-        self._check_rules(*rules, bias, allowed)
+        min_frames = -(-int(min_ms) // FRAME_MS)
+        self._check_rules(*rules, bias, allowed, min_frames)
         text = torch.as_tensor(text, dtype=torch.int64)
         P = int(text.numel())
         n_frames = max_ms // FRAME_MS
@@ -1258,7 +1269,7 @@ class HeartMuLaLite:
         if forced is not None:
             kw["forced"] = st["forced"]
         else:
-            kw["rules"] = st["rules"] = self._song_rules(st["out"], P, *rules, bias, allowed, -(-int(min_ms) // FRAME_MS))
+            kw["rules"] = st["rules"] = self._song_rules(st["out"], P, *rules, bias, allowed, min_frames)
         first = self._frame_fast(hb.contiguous(), cfg_scale, topk, temperature,
                                  pos=st["pos"], **kw)
         self._advance(first, st, P, n_frames)

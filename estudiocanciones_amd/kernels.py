@@ -1227,6 +1227,8 @@ def pack_q4(q4, s4, z4=None, interleave=False):
 
 
 def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
+    if x.dim() == 2 and x.shape[0] == 1 and x.stride(0) % 8 and x.shape[1] % 8 == 0:  # (one row: its stride says nothing)
+        x = x.as_strided(x.shape, (x.shape[1], x.stride(1)))
     dev, ldx = _rows16(x, name)
     M, K = x.shape
     if K != w.K or dev != w.dev or w.interleave is not silu or M > INT_MOST:
@@ -1251,6 +1253,10 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         ldy = _rows_of(out, M, cols, dev, name, "out")
         if _ends(out)[0] < _ends(x)[1] and _ends(x)[0] < _ends(out)[1]:
             raise ValueError(f"{name}: out must not overlap x")
+        if res is not None:
+            (lo, hi), (a, b) = _ends(out), _ends(res)
+            if lo < b and a < hi and not (lo == a and (ldy == ldr or M == 1)):
+                raise ValueError(f"{name}: out must be apart from res or the same rows")
     if M:
         plan, nb = (w.plans.get(M) or w.plan(M))[0 if np is None else 1]
         if nb:
@@ -1279,7 +1285,7 @@ def _rows_of(t, M, N, dev, call, name):
 def mm_q4(x, w, res=None, nw=None, eps=1e-5, out=None):
     """y = x @ w^T (+ res) -> [M, N] for 4-bit weights ``w`` (pack_q4) and x [M, K] fp16, or with ``nw`` [K] the RMS norm of
     x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end.  Any number of rows.
-    ``out`` may be ``res``, not x."""
+    ``out`` may be ``res``, or apart from it, and not x."""
     return _mm_q4("mm_q4", x, w, w.N, res, nw, eps, out, False)
 
 

@@ -467,3 +467,45 @@ def test_refusals(dev):
     ]:
         with pytest.raises(err):
             call()
+
+
+def test_out_and_res(dev):
+    """The sum may take the residual's place, or lie apart from it (between its rows too where ranges do not meet); other overlaps
+    are refused, as one thread would write what another has yet to read."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4
+    for M in (1, 8, 40):
+        N, K = 64, 128
+        q, s, z, w = make(M, N, K, 64, False)
+        wp = packed(dev, q, s, z)
+        x, res = _t(randn16(M, M, K), dev), _t(randn16(M + 1, M + 2, N), dev)
+        want = mm_q4(x, wp, res=res[:M])
+        buf = res.clone()
+        assert mm_q4(x, wp, res=buf[:M], out=buf[:M]).data_ptr() == buf.data_ptr() and torch.equal(buf[:M], want)
+        assert torch.equal(buf[M:], res[M:])
+        for a, b in ((slice(1, M + 1), slice(0, M)), (slice(0, M), slice(1, M + 1))):
+            buf = res.clone()
+            if M == 1:  # (rows next to each other)
+                assert torch.equal(mm_q4(x, wp, res=buf[a], out=buf[b]), mm_q4(x, wp, res=res[a]))
+                continue
+            with pytest.raises(ValueError, match="res"):
+                mm_q4(x, wp, res=buf[a], out=buf[b])
+            assert torch.equal(buf, res)
+        flat = torch.zeros((M + 1) * N, device=dev, dtype=torch.float16)
+        with pytest.raises(ValueError, match="res"):
+            mm_q4(x, wp, res=flat[:M * N].view(M, N), out=flat[8:8 + M * N].view(M, N))
+
+
+def test_one_row_of_any_stride(dev):
+    """A row's stride says nothing where there is one row, as of a transposed column."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4, mm_q4_silu
+    N, K = 70, 192
+    q, s, z, w = make(3, N, K, 32, True)
+    for il, f in ((False, mm_q4), (True, mm_q4_silu)):
+        wp = packed(dev, q, s, z, il)
+        x = _t(randn16(5, 1, K), dev)
+        col = x.reshape(K, 1).clone().t()
+        assert col.stride(0) == 1
+        assert torch.equal(f(col, wp), f(x, wp)) and torch.equal(f(x.as_strided((1, K), (3, 1)), wp), f(x, wp))
+

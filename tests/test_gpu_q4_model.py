@@ -256,3 +256,37 @@ def test_rules_refused_before_the_caches_go(dev):
         with pytest.raises(ValueError):
             m.generate(text, 1, max_ms=160, **kw)
     assert m.backbone.blocks[0].kc is kc
+
+
+def test_layer_of_any_input(dev):
+    """A single 4-bit layer takes what an 8-bit one takes: leading dimensions, strides, rows that start anywhere."""
+    import torch
+    from estudiocanciones_amd.engine import Linear
+    from estudiocanciones_amd.quant import q4_rows
+    N, K = 40, 128
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, s, z = q4_rows(torch.randn(N, K, generator=g, device=dev), 64, True)
+    lin = Linear(q4=q, s4=s, z4=z)
+    x = torch.randn(3, 2, K, generator=g, device=dev).half()
+    res = torch.randn(3, 2, N, generator=g, device=dev).half()
+    want = lin(x.reshape(6, K), res.reshape(6, N))
+    assert torch.equal(lin(x, res).reshape(6, N), want)
+    wide = torch.zeros(6, K + 5, device=dev, dtype=torch.float16)
+    wide[:, 3:K + 3] = x.reshape(6, K)
+    assert torch.equal(lin(wide[:, 3:K + 3], res.reshape(6, N)), want)
+    assert torch.equal(lin(x.reshape(6, K).t().contiguous().t(), res.reshape(6, N)), want)
+    assert torch.equal(lin(x[0, 0]), lin(x.reshape(6, K))[0]) and lin(x[:0]).shape == (0, 2, N)
+    q, s, _ = q4_rows(torch.randn(N, K, generator=g, device=dev), 128)
+    assert Linear(q4=q, s4=s)(x).shape == (3, 2, N)
+
+
+def test_a_codebook_with_nothing_to_draw_ends_the_take(dev, song):
+    """Penalties that take every allowed logit to -inf: the take ends at that frame, and nothing else happens."""
+    import torch
+    allowed = torch.zeros(N_CB, AUDIO_VOCAB, dtype=torch.bool)
+    allowed[:, 10:13] = True
+    for kw in (dict(), dict(use_graphs=False), dict(cfg_scale=1.0)):
+        got = song(presence=1e9, allowed=allowed, **kw)
+        assert all(1 <= t.shape[1] <= 3 and all(len(set(row.tolist())) == row.size for row in t) for t in got)
+        assert all(((t >= 10) & (t < 13)).all() for t in got)
+

@@ -141,3 +141,27 @@ def test_choices_with_two_parts():
     assert mm(plan=32, nw=16, ws=16)(L) == I and mm(plan=32 + 16 + 256, nw=16, ws=16)(L) == I
     assert mm(plan=64 + 1 + 256, nw=16, ws=16)(L) == I
     assert [L.ecd_mm_q4_norm_choice(*a) for a in ((0, 1, 64, 0), (1, 0, 64, 1), (1, 1, 65, 0), (1, 1, 0, 1))] == [-22] * 4
+
+
+def test_rules_that_leave_nothing_are_refused():
+    """A codebook without a code, or before the shortest length with none but end codes; biases that are not finite."""
+    from estudiocanciones_amd.engine import AUDIO_EOS, AUDIO_VOCAB, N_CB, HeartMuLaLite
+    check = HeartMuLaLite._check_rules
+    some = torch.zeros(N_CB, AUDIO_VOCAB, dtype=torch.bool)
+    some[:, 5] = True
+    check(1.0, 0.0, 0.0, 0, None, some, 10)
+    none = some.clone()
+    none[3] = False
+    ends = none.clone()
+    ends[3, AUDIO_EOS] = True
+    check(1.0, 0.0, 0.0, 0, None, ends)
+    check(1.0, 0.0, 0.0, 0, torch.full((N_CB, AUDIO_VOCAB), -1e30), ends, 0)
+    for allowed, first in ((none, 0), (none, 4), (ends, 1)):
+        with pytest.raises(ValueError, match="allowed"):
+            check(1.0, 0.0, 0.0, 0, None, allowed, first)
+    for v in (float("nan"), float("inf"), float("-inf")):
+        bias = torch.zeros(N_CB, AUDIO_VOCAB)
+        bias[7, -1] = v
+        with pytest.raises(ValueError, match="bias"):
+            check(1.0, 0.0, 0.0, 0, bias, None)
+
