@@ -5,9 +5,9 @@
 //
 // Packed codes: 32 rows x 64 k as 1 KB, blocks of a 32-row tile contiguous in k.  The 16 bytes at 16 l are row l & 31's; with
 // h = l >> 5, their dword 2 S + H holds octet 4 H + 2 h + S (k = 8 (4 H + 2 h + S) .. + 7).  So a lane of v_mfma_f32_32x32x16_f16
-// (row l & 31) takes its operands of four k-steps as 16 bytes, and so does one of v_mfma_f32_16x16x32_f16 (row l & 15) of one half of
-// the octets of a chunk, the other halves of the lanes from the next chunk.  An octet lies in a dword as pairs (k, k + 1) 16 bits apart, pair p at bits 4 p and 16 + 4 p, which
-// is how two halves of a register come out of one AND.
+// (row l & 31) takes its operands of four k-steps as 16 bytes, and so does one of v_mfma_f32_16x16x32_f16 (row l & 15): half the
+// octets of a chunk, the upper 32 lanes those of the next chunk.  An octet lies in a dword as pairs (k, k + 1) 16 bits apart,
+// pair p at bits 4 p and 16 + 4 p, which is how two halves of a register come out of one AND.
 // Scales: for each 32-row tile [K / G rounded up][32] fp16, or with zero points pairs (s, 1024 + z) of fp16.  Rows behind the
 // last have the scale 0.
 #pragma once

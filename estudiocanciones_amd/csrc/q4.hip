@@ -28,7 +28,8 @@ __device__ __forceinline__ int q4_nearest(float w, float s) {
   return (int)n;
 }
 
-// One thread per 8 consecutive weights, G / 8 neighbouring threads per group; the last group of a row may be short.
+// One thread per 8 consecutive weights, G / 8 neighbouring threads per group; the last group of a row may be short.  16384 x 3072
+// from fp32 62 us (3.6 TB/s, bound by memory), from 16 bits 60 to 64 (the quotients): set-up work, once per model.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_q4_kernel(const T* __restrict__ w, int N, int K, int lg, int ng,
                                                           uint32_t* __restrict__ q, f16* __restrict__ s,
@@ -142,6 +143,10 @@ __global__ __launch_bounds__(256) void pack_q4_scales_kernel(const f16* __restri
 // and what its rounding left (exact by the fused multiply-add), both multiplied by the codes.  Sums take 2^-e back in fp32, and
 // 1 / rms of the whole row at the end, when the waves' sums meet: nothing waits for the statistics.  Up to 8 rows the second
 // part takes the matrix instruction's rows 8 .. 15, which are idle otherwise.
+//
+// Measured in a graph (of it 2.2 us a launch): 1 x 8197 x 3072 with its norm 6.5 us, 8 x 5120 x 3072 with its norm 5.5, 8 x 3072 x 8192
+// with a residual 5.2 (2.5 TB/s), 8 x 16384 x 3072 with norm and SiLU 8.4 (3.1 TB/s), 48 x 3072 x 3072 in groups of 64 6.9.  What is
+// left is about 1 us to the first bytes, the address path, the conversion (9 instructions for 8 codes) and the sums' way through LDS.
 template <int NT, int XO, int GS, bool ZP, bool NORM>
 struct Q4Pair {
   static constexpr int SLOTS = NT * GS, SL = (SLOTS + 3) / 4;  // scales of 16 features each, and loads for them
@@ -168,7 +173,9 @@ __device__ __forceinline__ void spread16(uint32_t v, uint32_t* to) {
 
 // the sum over 16 neighbouring lanes, for all of them
 __device__ __forceinline__ float row_sum16(float v) {
-  auto ror = [&](auto n) { return __builtin_bit_cast(float, dpp_u32<0x120 + decltype(n)::value, 0xF>(__builtin_bit_cast(uint32_t, v), 0)); };
+  auto ror = [&](auto n) {
+    return __builtin_bit_cast(float, dpp_u32<0x120 + decltype(n)::value, 0xF>(__builtin_bit_cast(uint32_t, v), 0));
+  };
   v += ror(std::integral_constant<int, 8>());
   v += ror(std::integral_constant<int, 4>());
   v += ror(std::integral_constant<int, 2>());
@@ -349,9 +356,8 @@ __global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const f16* __restri
       for (int j = 0; j < 4; ++j) {
         f16x2 c0 = {(f16)-1032.f, (f16)-1032.f}, c1 = {(f16)-72.f, (f16)-72.f};
         if constexpr (ZP) {
-          const uint32_t* st = sc + t * GS;
-          const uint32_t v = GS == 1 ? st[0] : GS == 2 ? (cc ? st[GS / 2] : st[0]) : (cc ? st[GS / 2 + (j & 1) * (GS / 4)] : st[(j & 1) * (GS / 4)]);
-          const f16 z = __builtin_bit_cast(f16x2, v).y;
+          const uint32_t* st = sc + t * GS + (j & 1) * (GS / 4);  // (of the lane's chunk, and the dword's half of it)
+          const f16 z = __builtin_bit_cast(f16x2, cc ? st[GS / 2] : st[0]).y;
           c0 = (f16x2){-z, -z};
           c1 = c0 + (f16x2){(f16)960.f, (f16)960.f};
         }
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const f16* __restri
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (GS == 4 && (j & 1) != (g & 1)) continue;
-          const bool mine = GS == 1 || cc == g / (GS / 2 + (GS == 1));
+          const bool mine = GS == 1 || cc == 2 * g / GS;
           acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(mine ? xa[j] : none, w[j], acc, 0, 0, 0);
           if constexpr (LO > 0) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(mine ? xb[j] : none, w[j], acc, 0, 0, 0);
         }
@@ -595,9 +601,10 @@ int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* co
   const bool two = plan & Q4_TWO;
   const int tile = (plan & 255) - (two ? Q4_TWO : 0), ks = plan >> 8;
   const bool rows = tile > Q4_ROWS_AT && tile <= Q4_ROWS_AT + Q4_ROWS;
+  const bool planned = rows ? ks == 1 : tile >= 1 && tile <= Q4_TILES && ks >= 1 && ks <= K / 64;
   if (!x || !codes || !scales || !y || M <= 0 || N <= 0 || K <= 0 || K % 64 || !group_ok(group) || ldx < K || ldx % 8 ||
       !al16(x) || (nw && !al16(nw)) || !al16(codes) || !al16(scales) || ldy < cols || (res && ldr < cols) ||
-      (silu && (N % 2 || res)) || (nw && !(eps >= 0.f)) || (plan ? !(rows ? ks == 1 : tile >= 1 && tile <= Q4_TILES && ks >= 1 && ks <= K / 64) || (two && !nw) : M > 16) ||
+      (silu && (N % 2 || res)) || (nw && !(eps >= 0.f)) || (plan ? !planned || (two && !nw) : M > 16) ||
       (ecd_mm_q4_ws_bytes(M, N, K, plan, nw != nullptr) && (!ws || !al16(ws))))
     return ECD_EINVAL;
   if (N > 0x7FFFFFFF - 255 || K > 1 << 24 || ks > 65535) return ECD_ENOTSUP;
