@@ -13,8 +13,8 @@
 //
 // 2048 x 16384 x 3072 with SiLU: 172 to 179 us, 1.15 to 1.2 PFLOP/s (the library's product of fp16 matrices of these sizes: 175), matrix
 // units 64% busy; about 4 vector instructions hide behind each product, the rest of the conversion (30 us), the scales (15 to 20)
-// and the results' way out (10) add up.  187 x 3072 x 8192: 21 us, of it 4 the join; there a step's latency bounds (0.55 us for
-// 0.2 us of products).
+// and the results' way out (10) add up.  187 x 3072 x 8192: 21 us, of it 4 the join; there the latency of a
+// step bounds (1.3 us for 0.7 of products).
 #include "gemm_core.h"
 #include "q4.h"
 
@@ -345,9 +345,9 @@ template <bool ZP, int GS>
 static int by_tile(const Q4Args& a, int tile, float* ws, int ks, hipStream_t st, bool go) {
   switch (tile) {
     case 1: return launch<ZP, GS, 4, 1, 1, 2, 4, 3>(a, ws, ks, st, go);
-    case 2: return launch<ZP, GS, 4, 1, 2, 1, 4, 3>(a, ws, ks, st, go);
+    case 2: return launch<ZP, GS, 4, 1, 1, 2, 3, 3>(a, ws, ks, st, go);
     case 3: return launch<ZP, GS, 4, 1, 2, 1, 2, 3>(a, ws, ks, st, go);
-    case 4: return launch<ZP, GS, 4, 1, 2, 1, 1, 4>(a, ws, ks, st, go);
+    case 4: return launch<ZP, GS, 2, 1, 4, 2, 3, 2>(a, ws, ks, st, go);
     case 5: return launch<ZP, GS, 2, 1, 4, 1, 1, 4>(a, ws, ks, st, go);
     case 6: return launch<ZP, GS, 2, 1, 4, 1, 2, 3>(a, ws, ks, st, go);
     default: return ECD_EINVAL;
@@ -360,8 +360,10 @@ int gemm_q4(const Q4Args& a, bool zp, int tile, float* ws, int ks, hipStream_t s
 }
 
 // The tiles: features x rows, chunks of a step (WK), workgroups that a CU holds, and measured times in ns: a step of a workgroup
-// alone on its CU and of a full CU, and the rest of a workgroup's time.  Fitted to 2400 timings (12 to 3000 rows, 1001 to 16384
-// features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.  Then the
+// alone on its CU and of a full CU, and the rest of a workgroup's time.  Fitted to 2600 timings (12 to 3000 rows, 1001 to 16384
+// features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.  Tiles of 96 rows beside those
+// of 128 and 64 save padding (187 rows of 16384 x 3072 30 -> 25 us, 3000 of 3072 x 3072 79 -> 67); 128 x 128 and 128 x 32 were
+// the best nowhere by more than 5%.  Then the
 // few-row kernel's forms, whose 8 waves take a pair of chunks each in a step (360 timings of 16 to 256 rows, 7 to 9% rms): they
 // read the codes again for every 16 rows, but a CU starts on them with all loads in flight and ends without a split's join
 // (48 rows of 3072 x 3072: 5.8 us, the best tile 8.8; 192 rows of 5120 x 3072: 15.5 and 11.7).  And those with the norm inside (312
@@ -370,14 +372,14 @@ struct Q4Cost {
   int bn, bm, wk, fit, step, full, rest;
 };
 constexpr Q4Cost Q4_COST[Q4_TILES + 2 * Q4_ROWS] = {
-    {256, 128, 1, 2, 874, 1372, 3509}, {128, 128, 2, 1, 882, 882, 2404}, {128, 64, 2, 2, 551, 1142, 1853},
-    {128, 32, 2, 2, 413, 741, 1582},   {64, 32, 4, 1, 484, 484, 1462},   {64, 64, 4, 1, 677, 677, 1732},
+    {256, 128, 1, 2, 885, 1469, 3596}, {256, 96, 1, 2, 740, 1175, 2973}, {128, 64, 2, 2, 560, 1181, 1978},
+    {128, 96, 4, 1, 1342, 1342, 2681}, {64, 32, 4, 1, 499, 499, 1477},   {64, 64, 4, 1, 696, 696, 1767},
     {16, 16, 16, 1, 438, 363, 619},    {32, 16, 16, 1, 596, 516, 693},  {64, 16, 16, 1, 994, 961, 717},
     {16, 16, 16, 1, 761, 777, 1780},   {32, 16, 16, 1, 936, 1013, 1926}, {64, 16, 16, 1, 1437, 1765, 1757},
 };
 
 // The choice of the shortest estimate.  Over the 96 shapes that the times were taken at it is 0.8% behind the fastest of all on
-// average, 11% at most; over 120 shapes with few rows as much, and 12%; over 104 with
+// average, 17% at most; over 120 shapes with few rows as much, and 12%; over 104 with
 // a norm 0.2%, 10%, and before a SiLU 0.4%, 15%.  A split's join costs a launch and the passage of its sums through memory.
 int gemm_q4_plan(int M, int N, int K, Q4Among among) {
   const bool norm = among >= Q4_NORM;
