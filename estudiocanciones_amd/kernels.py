@@ -845,8 +845,10 @@ def _call_on(dev, name, *args):
     """_ffi.call with the tensors' device as the current one, on its current stream (asked for as its handle: a stream
     object costs as much as a launch)."""
     i = dev.index
-    if i == torch._C._cuda_getDevice():
-        _ffi.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
+    if i == torch._C._cuda_getDevice():  # (_ffi.call's steps, without passing the arguments on once more)
+        rc = getattr(_ffi.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i))
+        if rc:
+            _ffi.check(rc, name)
     else:
         with torch.cuda.device(dev):
             _ffi.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
@@ -1227,9 +1229,13 @@ def pack_q4(q4, s4, z4=None, interleave=False):
 
 
 def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
-    if x.dim() == 2 and x.shape[0] == 1 and x.stride(0) % 8 and x.shape[1] % 8 == 0:  # (one row: its stride says nothing)
-        x = x.as_strided(x.shape, (x.shape[1], x.stride(1)))
-    dev, ldx = _rows16(x, name)
+    try:
+        dev, ldx = _rows16(x, name)
+    except ValueError:
+        if x.dim() != 2 or x.shape[0] != 1 or x.shape[1] % 8:
+            raise
+        x = x.as_strided(x.shape, (x.shape[1], x.stride(1)))  # (one row: its stride says nothing)
+        dev, ldx = _rows16(x, name)
     M, K = x.shape
     if K != w.K or dev != w.dev or w.interleave is not silu or M > INT_MOST:
         if w.interleave is not silu:
@@ -1237,6 +1243,8 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         if dev != w.dev:
             raise ValueError(f"{name}: the weights are on {w.dev}, x on {dev}")
         raise ValueError(f"{name}: x must be [M, {w.K}]")
+    if ldx < K and M <= 1:
+        ldx = K
     np = rp = wp = None
     ldr = 0
     if nw is not None:

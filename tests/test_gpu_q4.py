@@ -508,4 +508,4 @@ def test_one_row_of_any_stride(dev):
         col = x.reshape(K, 1).clone().t()
         assert col.stride(0) == 1
         assert torch.equal(f(col, wp), f(x, wp)) and torch.equal(f(x.as_strided((1, K), (3, 1)), wp), f(x, wp))
-
+        assert torch.equal(f(x.as_strided((1, K), (8, 1)), wp), f(x, wp))
