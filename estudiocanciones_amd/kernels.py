@@ -1292,14 +1292,15 @@ def _rows_of(t, M, N, dev, call, name):
 
 def mm_q4(x, w, res=None, nw=None, eps=1e-5, out=None):
     """y = x @ w^T (+ res) -> [M, N] for 4-bit weights ``w`` (pack_q4) and x [M, K] fp16, or with ``nw`` [K] the RMS norm of
-    x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end.  Any number of rows.
+    x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end (normed rows of products of more
+    than 16 may be rounded to fp16 before).  Any number of rows.
     ``out`` may be ``res``, or apart from it, and not x."""
     return _mm_q4("mm_q4", x, w, w.N, res, nw, eps, out, False)
 
 
 def mm_q4_silu(x, w, nw=None, eps=1e-5, out=None):
     """silu(a) * b -> [M, N / 2] for the products a, b of mm_q4 on interleaved w1 | w3 (pack_q4(..., interleave=True)), in fp32
-    with one rounding at the end."""
+    with one rounding at the end (normed rows count in two fp16 parts)."""
     return _mm_q4("mm_q4_silu", x, w, w.N // 2, None, nw, eps, out, True)
 
 

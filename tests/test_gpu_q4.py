@@ -509,3 +509,32 @@ def test_one_row_of_any_stride(dev):
         assert col.stride(0) == 1
         assert torch.equal(f(col, wp), f(x, wp)) and torch.equal(f(x.as_strided((1, K), (3, 1)), wp), f(x, wp))
         assert torch.equal(f(x.as_strided((1, K), (8, 1)), wp), f(x, wp))
+
+
+@pytest.mark.parametrize("M", [12, 40, 700])
+def test_two_graphs_of_the_same_weights(dev, M):
+    """Two captured calls with a norm before a SiLU (with a workspace each, where many rows take one), replayed in turn, and an eager
+    call between them."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4_silu
+    q, s, z, w = make(M, 256, 1024, 64, True)
+    wi = packed(dev, q, s, z, True)
+    nw = _t((1 + 0.1 * rng(M).standard_normal(1024)).astype(np.float16), dev)
+    xs = [_t(randn16(i, M, 1024), dev) for i in range(3)]
+    want = [mm_q4_silu(x, wi, nw=nw) for x in xs]
+    ins, graphs, outs = [xs[0].clone(), xs[0].clone()], [], []
+    torch.cuda.synchronize()
+    for x in ins:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(mm_q4_silu(x, wi, nw=nw))
+        graphs.append(g)
+    for i in range(6):
+        for k in range(2):
+            ins[k].copy_(xs[(i + k) % 3])
+        graphs[0].replay()
+        assert torch.equal(mm_q4_silu(xs[2], wi, nw=nw), want[2])
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[k], want[(i + k) % 3]) for k in range(2))
+
