@@ -142,7 +142,9 @@ __global__ __launch_bounds__(256) void pack_q4_scales_kernel(const f16* __restri
 // The norm: x 2^e with 2^e a power of two near 1 / rms of the row's part at hand (exact), times nw in two fp16 parts, the product
 // and what its rounding left (exact by the fused multiply-add), both multiplied by the codes.  Sums take 2^-e back in fp32, and
 // 1 / rms of the whole row at the end, when the waves' sums meet: nothing waits for the statistics.  Up to 8 rows the second
-// part takes the matrix instruction's rows 8 .. 15, which are idle otherwise.
+// part takes the matrix instruction's rows 8 .. 15, which are idle otherwise.  A value is at most sqrt(128 CW) < 20 times the rms of
+// its part, so with weights below 2^11 every product fits fp16; where a part's weights reach more, all of them go in divided by
+// 2^5, and e tells the sums.
 //
 // Measured in a graph (of it 2.2 us a launch): 1 x 8197 x 3072 with its norm 6.5 us, 8 x 5120 x 3072 with its norm 5.5, 8 x 3072 x 8192
 // with a residual 5.2 (2.5 TB/s), 8 x 16384 x 3072 with norm and SiLU 8.4 (3.1 TB/s), 48 x 3072 x 3072 in groups of 64 6.9.  What is
@@ -295,8 +297,17 @@ __global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const f16* __restri
       if constexpr (PAIR) us[P * wv + 8 + 4 * o + xr] = u;
     }
   };
-  // 2^e of the rows' n pairs in the ring, and their sums of squares
+  // 2^e of the rows' n pairs in the ring, and their sums of squares; weights of 2^11 and more go 2^-5 times into the products.  The bits
+  // of all weights in one word rule those out while none is 2 or more (8 x 5120 x 3072 5.51 -> 5.63 us; by their maximum 5.74)
   auto scale_rows = [&](int n, bool first) {
+    int was[XO];
+#pragma unroll
+    for (int o = 0; o < XO; ++o) was[o] = e[o];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < CW; ++j)  // (all of the ring's, which are the row's in any case)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits |= __builtin_bit_cast(u32x4, ring[j].nw)[i];
 #pragma unroll
     for (int o = 0; o < XO; ++o) {
       float v = 0.f;
@@ -311,12 +322,30 @@ __global__ __launch_bounds__(64 * KW) void mm_q4_rows_kernel(const f16* __restri
       v = row_sum16(v);
       ss[o] += v;
       const float inv = __builtin_amdgcn_rsqf(v * (1.f / (128 * CW)));
-      const int was = e[o];
       e[o] = min(max((int)(__builtin_bit_cast(uint32_t, inv) >> 23) - 127, -14), 15);
       p2[o] = __builtin_bit_cast(f16, (uint16_t)((e[o] + 15) << 10));
-      if (!first) set_us(o, __builtin_bit_cast(float, (uint32_t)(127 + e[o] - was) << 23));
     }
-    if (!first) times_us();
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64((bits & 0x40004000u) != 0) != 0, 0)) {
+      f16x2 most = {(f16)0.f, (f16)0.f};  // of the magnitudes
+#pragma unroll
+      for (int j = 0; j < CW; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f16x2 w = {ring[j].nw[2 * i], ring[j].nw[2 * i + 1]};
+          asm("v_pk_maximum3_f16 %0, %0, %1, %1 neg_lo:[0,0,1] neg_hi:[0,0,1]" : "+v"(most) : "v"(w));
+        }
+      if (__builtin_amdgcn_ballot_w64(most.x >= (f16)2048.f || most.y >= (f16)2048.f)) {
+#pragma unroll
+        for (int j = 0; j < CW; ++j) ring[j].nw = ring[j].nw * (f16)0.03125f;
+#pragma unroll
+        for (int o = 0; o < XO; ++o) e[o] -= 5;
+      }
+    }
+    if (!first) {
+#pragma unroll
+      for (int o = 0; o < XO; ++o) set_us(o, __builtin_bit_cast(float, (uint32_t)(127 + e[o] - was[o]) << 23));
+      times_us();
+    }
   };
 
   f16x8* const put = ops + xj * PP + xr;
