@@ -7,6 +7,8 @@
 //     l = l > 0 ? l / rep[r] : l rep[r];  l = l - (presence[r] + frequency[r] n)
 //   l = l + bias[v]
 //   l = -inf                                   where the row's mask does not allow v
+// A finite l above fp16's largest number becomes that number: a softmax subtracts the largest value, and an infinity less itself is no
+// token's to draw.  One below the lowest becomes -inf, which is never drawn.
 // The history of a row are the last `window` (0: all) of its first length[r] tokens; tokens outside [0, V) count for nothing.
 //
 // A workgroup takes a segment of a row: its logits, biases and mask bits are loaded first; while they are in flight the row's
@@ -119,21 +121,32 @@ __global__ __launch_bounds__(TH) void process_logits_kernel(const LogitsArgs a) 
       n[4 + j] = n1[j];
     }
   }
-  f16x8 o;
+  float l[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    float l = (float)c[j];
+    l[j] = (float)c[j];
     if (a.guided) {
       const float w = (float)u[j];
-      l = w + (l - w) * a.cfg;
+      l[j] = w + (l[j] - w) * a.cfg;
     }
     if (n[j]) {
-      l = l > 0.f ? l / rep : l * rep;
-      l -= pres + freq * (float)n[j];
+      l[j] = l[j] > 0.f ? l[j] / rep : l[j] * rep;
+      l[j] -= pres + freq * (float)n[j];
     }
-    l += b[j];
-    o[j] = keep >> j & 1u ? (f16)l : (f16)-INFINITY;
+    l[j] += b[j];
   }
+  // above the range: rare, so one comparison for the eight (a vector instruction of a long row costs 15 ns)
+  float top = l[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = fmaxf(top, l[j]);
+  if (__builtin_expect(top > 65504.f, 0)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (l[j] < INFINITY) l[j] = fminf(l[j], 65504.f);
+  }
+  f16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = keep >> j & 1u ? (f16)l[j] : (f16)-INFINITY;
   f16* op = a.out + (long)r * a.ldo + i;
   if (full)
     *(f16x8u*)op = o;

@@ -1223,8 +1223,8 @@ class HeartMuLaLite:
         ``window`` frames (0: in the song so far): logits l > 0 become l / repetition, others l * repetition, then
         l - (presence + frequency * count).  ``bias`` float32 [8, V], finite, is added; ``allowed`` bool [8, V] forbids codes (not
         all of a codebook); before ``min_ms`` no frame ends the song.  process_logits does so on the guided logits in fp32;
-        teacher forcing ignores it.  A penalty or bias that takes every allowed logit of a codebook out of fp16's range leaves
-        nothing to draw, which ends the take."""
+        teacher forcing ignores it.  Logits above fp16's range count as its largest number, those below as -inf: a penalty or bias
+        that takes every allowed logit of a codebook there leaves nothing to draw, which ends the take."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
         if a8 and not self.backbone.eight():

@@ -1338,6 +1338,8 @@ def process_logits(logits, hist=None, length=None, window=0, repetition=None, pr
     l - (``presence`` + ``frequency`` * n) (each float32 [N] or [1], read on the device);
     l + ``bias`` (float32 [V], or [N, V]);
     -inf for tokens that the row's mask does not allow, whatever their logits hold (a row that may draw nothing is all -inf).
+    A finite result above fp16's range is 65504, its largest number (several such tokens are then equally likely); one below
+    it is -inf.
 
     ``hist`` int64 [N, T] with any strides: the row's tokens, of which the first ``length`` (int64 [N] on the device; None: T)
     are there and the last ``window`` of those count (0: all); tokens outside [0, V) count for nothing.  ``allowed`` int32

@@ -718,6 +718,7 @@ int ecd_mm_q4(const void* x, long ldx, const void* nw, float eps, const void* co
  * l = u + (logits[r, v] - u) cfg with u = logits[N + r, v];
  * where v occurs n > 0 times in the row's history: l = l > 0 ? l / rep : l * rep, l = l - (pres + freq n);
  * l = l + bias[r * ldb + v] (ldb 0: one bias for all rows); -inf where a mask does not allow v, whatever the logit is.
+ * A finite l above 65504 gives 65504 (a sampler's softmax has no use for an infinity); one that rounds below -65504 gives -inf.
  *   hist: token t of row r at hist[r hrow + t htok], t < T; the last `window` (0: all) of its first length[r] (NULL: T) tokens
  *   count, those outside [0, V) for nothing; rep, pres, freq: f32, bit 0, 1, 2 of per_row: an element per row (else one; NULL: 1, 0, 0);
  *   allowed [A] rows of ceil(V / 32) words (row stride lda), bit v & 31 of word v >> 5: v is allowed; state [N]: each row's mask,
