@@ -1224,7 +1224,8 @@ class HeartMuLaLite:
         l - (presence + frequency * count).  ``bias`` float32 [8, V], finite, is added; ``allowed`` bool [8, V] forbids codes (not
         all of a codebook); before ``min_ms`` no frame ends the song.  process_logits does so on the guided logits in fp32;
         teacher forcing ignores it.  Logits above fp16's range count as its largest number, those below as -inf: a penalty or bias
-        that takes every allowed logit of a codebook there leaves nothing to draw, which ends the take."""
+        that takes every allowed logit of a codebook there leaves nothing to draw, which ends the take (also before ``min_ms``; in
+        the first frame: a take of no frames, [8, 0])."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
         if a8 and not self.backbone.eight():
@@ -1273,6 +1274,8 @@ class HeartMuLaLite:
         first = self._frame_fast(hb.contiguous(), cfg_scale, topk, temperature,
                                  pos=st["pos"], **kw)
         self._advance(first, st, P, n_frames)
+        if forced is None:  # (a codebook with nothing to draw in the prompt's frame, which the bookkeeping does not scan for an end)
+            st["eos"].copy_((first[:N] < AUDIO_VOCAB).all(1).to(torch.int64).neg_())
 
         key = (B, cap, topk, float(temperature), float(cfg_scale), P if paged else None)
         done = n_frames

@@ -35,3 +35,24 @@ def test_a_bias_past_the_range_forces_its_code(dev, song, way):
     bias[torch.arange(N_CB), torch.from_numpy(codes)] = 1e5
     for t in song(bias=bias, min_ms=400, **WAYS[way]):
         assert t.shape == (N_CB, 1600 // 80 + 1) and (t == codes[:, None]).all()
+
+
+@pytest.mark.parametrize("way", range(len(WAYS)))
+def test_a_first_frame_with_nothing_to_draw_is_a_song_of_no_frames(dev, song, way):
+    """A bias that takes every code of a codebook out of fp16's range below: no frame, and no number that is not a code."""
+    import torch
+    for row in (0, 3, 7):
+        bias = torch.zeros(N_CB, AUDIO_VOCAB)
+        bias[row] = -1e30
+        for t in song(bias=bias, **WAYS[way]):
+            assert t.shape == (N_CB, 0)
+
+
+@pytest.mark.parametrize("use_graphs", [True, False])
+def test_a_song_that_may_only_end_later_does_not_start_with_nothing(dev, song, use_graphs):
+    """Codes out of the range below but for the end codes, which a shortest length forbids at first: no frames again."""
+    import torch
+    bias = torch.full((N_CB, AUDIO_VOCAB), -1e30)
+    bias[:, 8193:] = 0
+    for t in song(bias=bias, min_ms=400, use_graphs=use_graphs):
+        assert t.shape == (N_CB, 0)
