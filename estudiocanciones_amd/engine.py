@@ -974,16 +974,19 @@ class HeartMuLaLite:
     # -------------------------------------------------- logits before the sampler
     @staticmethod
     def _check_rules(repetition, presence, frequency, window, bias, allowed, min_frames=0):
+        # (up to 2^100 either way: a history's sums of them stay in fp32's range)
         for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-            if not math.isfinite(v) or (name == "repetition" and v <= 0):
-                raise ValueError(f"generate: {name} must be a finite number" + (" above 0" if name == "repetition" else ""))
+            if name == "repetition" and not 2.0 ** -100 <= v <= 2.0 ** 100:
+                raise ValueError("generate: repetition must be a number above 0, from 2^-100 to 2^100")
+            if not abs(v) <= 2.0 ** 100:
+                raise ValueError(f"generate: {name} must be a finite number of at most 2^100")
         if not 0 <= window <= INT_MOST:
             raise ValueError("generate: window must be 0 (the whole song) or a number of frames")
         for name, t, dt in (("bias", bias, torch.float32), ("allowed", allowed, torch.bool)):
             if t is not None and (t.dtype != dt or tuple(t.shape) != (N_CB, AUDIO_VOCAB)):
                 raise ValueError(f"generate: {name} must be {dt} [{N_CB}, {AUDIO_VOCAB}]")
-        if bias is not None and not bias.isfinite().all():
-            raise ValueError("generate: bias must be finite (allowed forbids codes)")
+        if bias is not None and not (bias.abs() <= 2.0 ** 100).all():
+            raise ValueError("generate: bias must be finite, of at most 2^100 (allowed forbids codes)")
         if allowed is not None and not allowed[:, :AUDIO_EOS if min_frames > 0 else AUDIO_VOCAB].any(1).all():
             raise ValueError("generate: allowed must leave every codebook a code" + (" that does not end the song" if min_frames > 0 else ""))
 
@@ -1221,11 +1224,11 @@ class HeartMuLaLite:
 
         ``repetition``, ``presence``, ``frequency``: penalties for codes that a take's codebook has had in the last
         ``window`` frames (0: in the song so far): logits l > 0 become l / repetition, others l * repetition, then
-        l - (presence + frequency * count).  ``bias`` float32 [8, V], finite, is added; ``allowed`` bool [8, V] forbids codes (not
+        l - (presence + frequency * count).  ``bias`` float32 [8, V] is added; ``allowed`` bool [8, V] forbids codes (not
         all of a codebook); before ``min_ms`` no frame ends the song.  process_logits does so on the guided logits in fp32;
-        teacher forcing ignores it.  Logits above fp16's range count as its largest number, those below as -inf: a penalty or bias
-        that takes every allowed logit of a codebook there leaves nothing to draw, which ends the take (also before ``min_ms``; in
-        the first frame: a take of no frames, [8, 0])."""
+        teacher forcing ignores it.  Penalties and biases are at most 2^100.  Logits above fp16's range count as its largest
+        number, those below as -inf: a penalty or bias that takes every allowed logit of a codebook there leaves nothing to draw,
+        which ends the take (also before ``min_ms``; in the first frame: a take of no frames, [8, 0])."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
         if a8 and not self.backbone.eight():
