@@ -385,7 +385,8 @@ int gemm_q4_plan(int M, int N, int K, Q4Among among) {
   const bool norm = among >= Q4_NORM;
   long best = 0x7FFFFFFFFFFFFFFFL;
   int plan = 0;
-  for (int t = 0; t < Q4_TILES + (among == Q4_ONLY_TILES ? 0 : Q4_ROWS); ++t) {
+  // (the few-row forms' launch counts at most 65535 blocks of 16 rows)
+  for (int t = 0; t < Q4_TILES + (among == Q4_ONLY_TILES || M > 16 * 65535 ? 0 : Q4_ROWS); ++t) {
     const bool rows = t >= Q4_TILES, two = rows ? norm : among == Q4_NORM_SILU;
     const Q4Cost& c = Q4_COST[rows && two ? t + Q4_ROWS : t];
     const int nch = K >> 6 << (two && !rows);
