@@ -1228,6 +1228,9 @@ def pack_q4(q4, s4, z4=None, interleave=False):
     return PackedQ4(codes, scales, N, K, group, z4 is not None, bool(interleave))
 
 
+Q4_TILE_LD = 1 << 23  # the largest stride of x's rows that every tile takes
+
+
 def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
     try:
         dev, ldx = _rows16(x, name)
@@ -1243,7 +1246,7 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         if dev != w.dev:
             raise ValueError(f"{name}: the weights are on {w.dev}, x on {dev}")
         raise ValueError(f"{name}: x must be [M, {w.K}]")
-    if ldx < K and M <= 1:
+    if M <= 1:
         ldx = K
     np = rp = wp = None
     ldr = 0
@@ -1267,6 +1270,8 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
                 raise ValueError(f"{name}: out must be apart from res or the same rows")
     if M:
         plan, nb = (w.plans.get(M) or w.plan(M))[0 if np is None else 1]
+        if ldx > Q4_TILE_LD and M > 16 and np is None:  # (the few-row kernel's offsets reach 8 times as far as a tile's)
+            plan, nb = 19 + 256, 0
         if nb:
             ws = torch.empty(nb, device=dev, dtype=torch.uint8)  # (held until the launch)
             wp = ws.data_ptr()

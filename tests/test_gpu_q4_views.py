@@ -8,6 +8,74 @@ from test_gpu_q4 import H, _t, make, packed
 pytestmark = pytest.mark.gpu
 
 
+def wide(dev, rows, ld, K, seed):
+    """[rows, K] of rows ld apart, in memory of which the rest is NaN around them."""
+    import torch
+    flat = torch.empty((rows - 1) * ld + K + 64, device=dev, dtype=torch.float16)
+    x = flat.as_strided((rows, K), (ld, 1))
+    flat.as_strided((rows, K + 64), (ld, 1)).fill_(float("nan"))
+    x.copy_(_t(randn16(seed, rows, K), dev))
+    return x
+
+
+@pytest.mark.parametrize("M", [2, 16, 17, 40, 130])
+@pytest.mark.parametrize("ld", [(1 << 23) + 8, (1 << 24) + 8])
+def test_rows_far_apart(dev, M, ld):
+    """Row strides that 32 bits of a tile's offsets do not reach: the values of a compact copy, within the kernels' sums."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4
+    for N, K, group in ((70, 192, 64), (3000, 128, 128)):
+        q, s, z, w = make(M, N, K, group, True)
+        wp = packed(dev, q, s, z)
+        x = wide(dev, M, ld, K, M)
+        res, nw = _t(randn16(M + 1, M, N), dev), torch.ones(K, device=dev, dtype=torch.float16)
+        x64 = x.double().cpu().numpy()
+        A = np.abs(x64) @ np.abs(w).T
+        tol = (2.0 ** -23 * (64 + K // 64 + 32) + K / 32 * 1.25 * 2.0 ** -22) * A
+        want = x64 @ w.T + res.double().cpu().numpy()
+        got = mm_q4(x, wp, res=res).double().cpu().numpy()
+        assert (np.abs(got - want) <= tol + H * (np.abs(want) + tol) + 2.0 ** -25).all()
+        assert torch.equal(mm_q4(x, wp, nw=nw), mm_q4(x.contiguous(), wp, nw=nw))
+        del x
+
+
+@pytest.mark.parametrize("M,N,K", [(130, 16384, 192), (200, 5120, 1024), (400, 8197, 1024)])
+def test_rows_too_far_apart_for_the_tiles(dev, M, N, K):
+    """Sizes that go by tiles where rows are close together."""
+    import torch
+    from estudiocanciones_amd import _ffi
+    from estudiocanciones_amd.kernels import mm_q4, mm_q4_silu
+    assert 1 <= _ffi.lib().ecd_mm_q4_choice(M, N, K) & 255 <= 6
+    q, s, z, w = make(M, N, K, 128, True)
+    x = wide(dev, M, (1 << 24) + 8, K, M)
+    x64 = x.double().cpu().numpy()
+    want = x64 @ w.T
+    tol = (2.0 ** -23 * (64 + K // 64 + 32) + K / 32 * 1.25 * 2.0 ** -22) * (np.abs(x64) @ np.abs(w).T)
+    got = mm_q4(x, packed(dev, q, s, z)).double().cpu().numpy()
+    assert (np.abs(got - want) <= tol + H * (np.abs(want) + tol) + 2.0 ** -25).all()
+    if N % 2 == 0:
+        a, b, ta, tb = want[:, :N // 2], want[:, N // 2:], tol[:, :N // 2], tol[:, N // 2:]
+        f = a / (1 + np.exp(-a))
+        want, tol = f * b, (1.1 * ta + 2.0 ** -20 * np.abs(f)) * (np.abs(b) + tb) + np.abs(f) * tb
+        wi, nw = packed(dev, q, s, z, True), torch.ones(K, device=dev, dtype=torch.float16)
+        got = mm_q4_silu(x, wi).double().cpu().numpy()
+        assert (np.abs(got - want) <= tol + H * (np.abs(want) + tol) + 2.0 ** -25).all()
+        assert torch.equal(mm_q4_silu(x, wi, nw=nw), mm_q4_silu(x.contiguous(), wi, nw=nw))
+
+
+def test_one_row_however_far_the_next(dev):
+    """A row's stride says nothing where there is one row: as of a view of a wide tensor."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4, mm_q4_silu
+    N, K = 70, 192
+    q, s, z, w = make(3, N, K, 32, True)
+    x = _t(randn16(5, 1, K), dev)
+    for il, f in ((False, mm_q4), (True, mm_q4_silu)):
+        wp = packed(dev, q, s, z, il)
+        for ld in (1 << 26, (1 << 26) + 8, 1 << 27, 1 << 40, (1 << 40) + 3):
+            assert torch.equal(f(x.as_strided((1, K), (ld, 1)), wp), f(x, wp))
+
+
 @pytest.mark.parametrize("silu", [False, True])
 def test_more_rows_than_blocks_of_a_launch(dev, silu):
     """1.1 million rows (of more than 2^31 bytes): the first, the last and some between them."""
