@@ -1262,12 +1262,10 @@ def _mm_q4(name, x, w, cols, res, nw, eps, out, silu):
         out, ldy = torch.empty(M, cols, device=dev, dtype=torch.float16), cols
     else:
         ldy = _rows_of(out, M, cols, dev, name, "out")
-        if _ends(out)[0] < _ends(x)[1] and _ends(x)[0] < _ends(out)[1]:
+        if _meet(out, ldy, x, ldx):
             raise ValueError(f"{name}: out must not overlap x")
-        if res is not None:
-            (lo, hi), (a, b) = _ends(out), _ends(res)
-            if lo < b and a < hi and not (lo == a and (ldy == ldr or M == 1)):
-                raise ValueError(f"{name}: out must be apart from res or the same rows")
+        if res is not None and _meet(out, ldy, res, ldr) and not (rp == out.data_ptr() and (ldy == ldr or M == 1)):
+            raise ValueError(f"{name}: out must be apart from res or the same rows")
     if M:
         plan, nb = (w.plans.get(M) or w.plan(M))[0 if np is None else 1]
         if ldx > Q4_TILE_LD and M > 16 and np is None:  # (the few-row kernel's offsets reach 8 times as far as a tile's)
@@ -1286,6 +1284,16 @@ def _ends(t):
     return a, a + (1 + sum((n - 1) * d for n, d in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else a
 
 
+def _meet(t, ldt, u, ldu):
+    """Whether fp16 matrices of row strides ldt and ldu (at least their width) share memory, or might: columns of the same wide
+    rows that do not meet share none."""
+    (lo, hi), (a, b) = _ends(t), _ends(u)
+    if lo >= b or a >= hi:
+        return False
+    at = (a - lo) // 2 % ldt  # where u's rows begin between t's
+    return ldt != ldu or (a - lo) % 2 != 0 or at < t.shape[1] or at + u.shape[1] > ldt
+
+
 def _rows_of(t, M, N, dev, call, name):
     """Row stride of an fp16 [M, N] tensor on dev with unit inner stride and rows that do not overlap."""
     if t.dtype is torch.float16 and t.device == dev and t.shape == (M, N):
@@ -1299,7 +1307,7 @@ def mm_q4(x, w, res=None, nw=None, eps=1e-5, out=None):
     """y = x @ w^T (+ res) -> [M, N] for 4-bit weights ``w`` (pack_q4) and x [M, K] fp16, or with ``nw`` [K] the RMS norm of
     x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end (normed rows of products of more
     than 16 may be rounded to fp16 before).  Any number of rows.
-    ``out`` may be ``res``, or apart from it, and not x."""
+    ``out`` may be ``res``, or apart from it, and not x (columns of the same rows that do not meet are apart)."""
     return _mm_q4("mm_q4", x, w, w.N, res, nw, eps, out, False)
 
 
@@ -1414,9 +1422,7 @@ def process_logits(logits, hist=None, length=None, window=0, repetition=None, pr
         out = torch.empty_strided((N, V), (ldo, 1), device=dev, dtype=torch.float16)
     else:
         ldo = _rows_of(out, N, V, dev, "process_logits", "out")
-        lo, hi = _ends(out)
-        a, b = _ends(logits)
-        if lo < b and a < hi and not (lo == a and (ldo == ld or N == 1)):
+        if _meet(out, ldo, logits, ld) and not (out.data_ptr() == logits.data_ptr() and (ldo == ld or N == 1)):
             raise ValueError("process_logits: out must be apart from logits or their first rows")
     if N:
         _call_on(dev, "ecd_process_logits", logits.data_ptr(), max(ld, V), guided, cfg if guided else 1.0, hp, hrow, htok, T, lp,

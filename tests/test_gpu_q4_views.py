@@ -97,3 +97,43 @@ def test_more_rows_than_blocks_of_a_launch(dev, silu):
             want, tol = f * b, (1.1 * tg + 2.0 ** -20 * np.abs(f)) * (np.abs(b) + tb) + np.abs(f) * tb
         got = y[a:a + 700].double().cpu().numpy()
         assert (np.abs(got - want) <= tol + H * (np.abs(want) + tol) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 12, 40, 200])
+def test_results_beside_their_inputs(dev, M):
+    """out in columns of the same wide rows as x or res, which do not meet; columns that do are refused, and nothing is written."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4, process_logits
+    N, K = 72, 192
+    q, s, z, w = make(M, N, K, 64, True)
+    wp = packed(dev, q, s, z)
+    for at in (0, N, K):  # out before x, behind it, and res behind out
+        room = torch.full((M, K + 2 * N + 8), 7.0, device=dev, dtype=torch.float16)
+        cols = {"x": K, "out": N, "res": N}
+        order = {0: ["out", "x", "res"], N: ["x", "out", "res"], K: ["res", "x", "out"]}[at]
+        v, c = {}, 0
+        for n in order:
+            v[n] = room[:, c:c + cols[n]]
+            c += cols[n]
+        v["x"].copy_(_t(randn16(M, M, K), dev))
+        v["res"].copy_(_t(randn16(M + 1, M, N), dev))
+        x, res = v["x"].clone(), v["res"].clone()
+        mm_q4(v["x"], wp, res=v["res"], out=v["out"])
+        assert torch.equal(v["out"], mm_q4(x, wp, res=res))
+        assert torch.equal(v["x"], x) and torch.equal(v["res"], res) and (room[:, c:] == 7.0).all()
+    if M > 1:
+        before = room.clone()
+        for out in (room[:, 1:1 + N], room[:, 100:100 + N], room[:, K + N - 1:K + 2 * N - 1]):
+            with pytest.raises(ValueError):
+                mm_q4(v["x"], wp, res=v["res"], out=out)
+        assert torch.equal(room, before)
+    lg = torch.full((2 * M, 300), 7.0, device=dev, dtype=torch.float16)
+    lg[:, :100] = _t(randn16(3, 2 * M, 100), dev)
+    src = lg[:, :100].clone()
+    process_logits(lg[:, :100], cfg=1.5, out=lg[:M, 100:200])
+    assert torch.equal(lg[:M, 100:200], process_logits(src, cfg=1.5))
+    assert torch.equal(lg[:, :100], src) and (lg[:, 200:] == 7.0).all() and (lg[M:, 100:] == 7.0).all()
+    for out in (lg[:M, 99:199], lg[M:, :100], lg[:M, 200:].as_strided((M, 100), (299, 1))):
+        if M > 1 or out.data_ptr() < lg[1].data_ptr() + 200 and out.storage_offset() % 300 < 100:
+            with pytest.raises(ValueError):
+                process_logits(lg[:, :100], cfg=1.5, out=out)

@@ -17,3 +17,26 @@ def test_blocks_of_few_rows_are_chosen_for_as_many_as_a_launch_takes():
                 p = choice(M)
                 assert p > 0 and not p & 16, (M, N, K, p)
     assert few  # (the rule above is what decides)
+
+
+def test_whether_matrices_meet():
+    """Against the sets of their elements: columns of rows of one stride are told apart, others that reach across each other are not."""
+    import random
+    from estudiocanciones_amd.kernels import _meet
+    r = random.Random(1)
+    flat = torch.zeros(4000, dtype=torch.float16)
+    told = 0
+    for _ in range(3000):
+        M, ld = r.randint(1, 6), r.randint(4, 60)
+        lds = [ld, ld if r.random() < 0.7 else r.randint(4, 60)]
+        w = [r.randint(1, d) for d in lds]
+        at = [r.randint(0, 200) for _ in range(2)]
+        rows = [M, r.choice([M, 2 * M])]
+        t, u = (flat.as_strided((n, k), (d, 1), o) for n, k, d, o in zip(rows, w, lds, at))
+        share = bool({o + i * d + j for n, k, d, o in [(rows[0], w[0], lds[0], at[0])] for i in range(n) for j in range(k)} &
+                     {o + i * d + j for n, k, d, o in [(rows[1], w[1], lds[1], at[1])] for i in range(n) for j in range(k)})
+        got = _meet(t, lds[0], u, lds[1])
+        assert got or not share
+        if lds[0] == lds[1] and at[0] + rows[0] * ld >= at[1] and not share and rows[0] > 1 and rows[1] > 1:
+            told += not got
+    assert told > 100
