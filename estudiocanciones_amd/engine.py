@@ -125,8 +125,11 @@ class Linear:
         """Add the lane-ordered tile copy used by the fused GEMVs (K % 64 == 0).  With
         ``interleave`` the w1 | w3 halves become (a_j, b_j) row pairs (scales likewise).
         ``stream``: the layer is read once per frame, so its loads bypass cache allocation.
-        4-bit weights are laid out for mm_q4 and not kept in the given form."""
+        4-bit weights are laid out for mm_q4 and not kept in the given form, at their first call if not before (and not
+        inside a capture)."""
         if self.q4 is not None:
+            if torch.cuda.is_current_stream_capturing():  # (it would run at the replays only, over memory given back by then)
+                raise RuntimeError("Linear: pack() 4-bit weights before a call of theirs is captured")
             self.w4 = pack_q4(self.q4, self.s4, self.z4, interleave)
             self.q4 = self.s4 = self.z4 = None
         if self.q8 is None:

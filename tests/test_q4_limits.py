@@ -40,3 +40,20 @@ def test_whether_matrices_meet():
         if lds[0] == lds[1] and at[0] + rows[0] * ld >= at[1] and not share and rows[0] > 1 and rows[1] > 1:
             told += not got
     assert told > 100
+
+
+def linear(N, K, bits):
+    from estudiocanciones_amd.engine import Linear
+    if bits == 8:
+        return Linear(q8=torch.zeros(N, K, dtype=torch.int8), s8=torch.ones(N, dtype=torch.float16))
+    return Linear(q4=torch.full((N, K // 2), 0x88, dtype=torch.uint8), s4=torch.ones(N, -(-K // 128), dtype=torch.float16))
+
+
+def test_a_layer_is_not_laid_out_inside_a_capture(monkeypatch):
+    """The layout would run at the replays only, over weights that are gone by then."""
+    lin = linear(32, 64, 4)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lin.pack, lambda: lin(torch.zeros(1, 64, dtype=torch.float16))):
+        with pytest.raises(RuntimeError, match="captur"):
+            call()
+    assert lin.q4 is not None and lin.w4 is None
