@@ -276,6 +276,8 @@ class Stack:
         dim = cfg.get("dim", DIM)
         self.blocks = [Block(p, f"{prefix}.layers.{i}.", cfg["heads"], cfg["kv_heads"], dim)
                        for i in range(cfg["layers"])]
+        if len({lin.q8 is None for b in self.blocks for lin in (b.qkv, b.o, b.w13, b.w2)}) > 1:
+            raise ValueError(f"{prefix}: linear layers in 4 bits beside others; a stack is of 4-bit layers throughout or of none")
         self.norm = p(f"{prefix}.norm.scale", norm=True)
         self.rope = None
         self.dim = dim

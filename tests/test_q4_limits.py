@@ -57,3 +57,20 @@ def test_a_layer_is_not_laid_out_inside_a_capture(monkeypatch):
         with pytest.raises(RuntimeError, match="captur"):
             call()
     assert lin.q4 is not None and lin.w4 is None
+
+
+@pytest.mark.parametrize("where", ["layers.1.", "attn.output_proj", "mlp.w2", "mlp.w1", "attn.", None])
+def test_a_stack_is_of_4_bits_throughout_or_not_at_all(where):
+    from estudiocanciones_amd.engine import Stack
+    cfg = dict(layers=2, heads=2, kv_heads=1, max_seq=64, dim=64)
+
+    def p(name, norm=False):
+        if norm:
+            return torch.ones(64, dtype=torch.float16)
+        return linear(64, 64, 8 if where is None or where not in name else 4)
+
+    if where is None:
+        assert len(Stack(p, "backbone", cfg).blocks) == 2
+    else:
+        with pytest.raises(ValueError, match="4-bit"):
+            Stack(p, "backbone", cfg)
