@@ -137,3 +137,60 @@ def test_results_beside_their_inputs(dev, M):
         if M > 1 or out.data_ptr() < lg[1].data_ptr() + 200 and out.storage_offset() % 300 < 100:
             with pytest.raises(ValueError):
                 process_logits(lg[:, :100], cfg=1.5, out=out)
+
+
+@pytest.mark.parametrize("silu", [False, True])
+def test_results_past_31_bits(dev, silu):
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4, mm_q4_silu
+    M, N, K = 66001, 32800 if silu else 16400, 64
+    cols = N // 2 if silu else N
+    q, s, z, w = make(2, N, K, 32, True)
+    wp = packed(dev, q, s, z, silu)
+    x = _t(randn16(1, M, K), dev)
+    y = (mm_q4_silu if silu else mm_q4)(x, wp)
+    assert y.numel() * 2 > 2 ** 31
+    wt, aw = _t(w.T, dev), _t(np.abs(w).T, dev)
+    for a in (0, 32768, M - 999):
+        x64 = x[a:a + 999].double()
+        want, A = x64 @ wt, x64.abs() @ aw
+        tol = (2.0 ** -23 * (64 + K // 64 + 32) + K / 32 * 1.25 * 2.0 ** -22) * A
+        if silu:
+            g, b, tg, tb = want[:, :cols], want[:, cols:], tol[:, :cols], tol[:, cols:]
+            f = g / (1 + (-g).exp())
+            want, tol = f * b, (1.1 * tg + 2.0 ** -20 * f.abs()) * (b.abs() + tb) + f.abs() * tb
+        assert ((y[a:a + 999].double() - want).abs() <= tol + H * (want.abs() + tol) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("silu", [False, True])
+def test_weights_past_31_bits(dev, silu):
+    """Weights to quantise, codes and packed codes of more than 2^31 bytes: the last features come out as on their own."""
+    import torch
+    from estudiocanciones_amd.kernels import mm_q4, mm_q4_silu, pack_q4
+    from estudiocanciones_amd.quant import q4_rows
+    N, K = 1_050_004, 4096
+    g = torch.Generator(device=dev).manual_seed(2)
+    t = torch.empty(N, K, device=dev, dtype=torch.bfloat16)
+    t.normal_(generator=g)
+    q, s, z = q4_rows(t, 128, True)
+    del t
+    assert q.numel() > 2 ** 31
+    w, half = pack_q4(q, s, z, silu), N // 2
+    for M in (3, 40):
+        x = _t(randn16(M, M, K), dev)
+        y = (mm_q4_silu if silu else mm_q4)(x, w)
+        for a in (0, half - 600, N - 600) if not silu else (0, half - 600):
+            rows = torch.arange(a, a + 600, device=dev)
+            rows = torch.cat([rows, rows + half]) if silu else rows
+            u = torch.stack([q[rows] & 15, q[rows] >> 4], -1).flatten(1).double()
+            wd = (u - z[rows].double().repeat_interleave(128, 1)) * s[rows].double().repeat_interleave(128, 1)
+            x64 = x.double()
+            want, A = x64 @ wd.t().contiguous(), x64.abs() @ wd.abs().t().contiguous()
+            tol = (2.0 ** -23 * (64 + K // 64 + 32) + K / 32 * 1.25 * 2.0 ** -22) * A
+            if silu:
+                ga, b, tg, tb = want[:, :600], want[:, 600:], tol[:, :600], tol[:, 600:]
+                f = ga / (1 + (-ga).exp())
+                want, tol = f * b, (1.1 * tg + 2.0 ** -20 * f.abs()) * (b.abs() + tb) + f.abs() * tb
+            assert ((y[:, a:a + 600].double() - want).abs() <= tol + H * (want.abs() + tol) + 2.0 ** -25).all()
+        assert y.shape[1] == (half if silu else N)
+    assert torch.equal(q4_rows(torch.zeros(1, K, device=dev), 128, True)[0], torch.zeros(1, K // 2, device=dev, dtype=torch.uint8))

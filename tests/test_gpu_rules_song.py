@@ -56,3 +56,17 @@ def test_a_song_that_may_only_end_later_does_not_start_with_nothing(dev, song, u
     bias[:, 8193:] = 0
     for t in song(bias=bias, min_ms=400, use_graphs=use_graphs):
         assert t.shape == (N_CB, 0)
+
+
+def test_int8_activations_need_eight_bits_in_the_backbone_alone(dev):
+    """A 4-bit decoder beside an int8 backbone sings with int8 activations; a 4-bit backbone refuses them."""
+    import torch
+    text = torch.arange(1, 13)
+    _, _, m = model(dev, 128, True, ("decoder",))
+    assert m.backbone.eight() and m.decoder.four()
+    for paged in (False, True):
+        for t in m.generate(text, 3, max_ms=800, seed=5, n=2, topk=20, a8=True, paged=paged):
+            assert t.shape[0] == N_CB and t.shape[1] >= 1 and ((t >= 0) & (t < AUDIO_VOCAB)).all()
+    _, _, m = model(dev, 128, True, ("backbone",))
+    with pytest.raises(NotImplementedError, match="int8 activations"):
+        m.generate(text, 3, max_ms=800, a8=True)
