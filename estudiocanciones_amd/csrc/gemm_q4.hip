@@ -11,8 +11,8 @@
 // K advances in 64-wide chunks through an NS-stage ring in LDS, loaded by LDS DMA: x rows with their 16-byte pieces swizzled
 // by row (x_swz), codes as packed, scales of the chunk's groups.
 //
-// 2048 x 16384 x 3072 with SiLU: 172 to 179 us, 1.15 to 1.2 PFLOP/s (the library's product of fp16 matrices of these sizes: 175), matrix
-// units 64% busy; about 4 vector instructions hide behind each product, the rest of the conversion (30 us), the scales (15 to 20)
+// 2048 x 16384 x 3072 with SiLU: 175 to 181 us for a few launches, 200 to 207 for sixty in a row, when the clock has fallen: 1.15 and 1.0
+// PFLOP/s (the library's product of fp16 matrices of these sizes: 153 and 172 to 177), matrix units 64% busy; about 4 vector instructions hide behind each product, the rest of the conversion (30 us), the scales (15 to 20)
 // and the results' way out (10) add up.  187 x 3072 x 8192: 21 us, of it 4 the join; there the latency of a
 // step bounds (1.3 us for 0.7 of products).
 #include "gemm_core.h"
@@ -363,7 +363,9 @@ int gemm_q4(const Q4Args& a, bool zp, int tile, float* ws, int ks, hipStream_t s
 // alone on its CU and of a full CU, and the rest of a workgroup's time.  Fitted to 2600 timings (12 to 3000 rows, 1001 to 16384
 // features, K 192 to 8192, up to 12 ways, groups of 128), which the estimate meets within 6 to 9% rms.  Tiles of 96 rows beside those
 // of 128 and 64 save padding (187 rows of 16384 x 3072 30 -> 25 us, 3000 of 3072 x 3072 79 -> 67); 128 x 128 and 128 x 32 were
-// the best nowhere by more than 5%.  Then the
+// the best nowhere by more than 5%.  Groups of 64 and 32 have the same choices: over 30 shapes of 24 to 1024 rows the mean is 5 to 6.5%
+// behind the best there (0.4 to 0.7% for 128), most where the few-row kernel's twice as many matrix instructions count: 24 rows of
+// 16384 x 3072 13.6 us (a tile 9.3), 100 of 3072 x 3072 12.8 (8.9).  Then the
 // few-row kernel's forms, whose 8 waves take a pair of chunks each in a step (360 timings of 16 to 256 rows, 7 to 9% rms): they
 // read the codes again for every 16 rows, but a CU starts on them with all loads in flight and ends without a split's join
 // (48 rows of 3072 x 3072: 5.8 us, the best tile 8.8; 192 rows of 5120 x 3072: 15.5 and 11.7).  And those with the norm inside (312

@@ -14,7 +14,7 @@
 // A workgroup takes a segment of a row: its logits, biases and mask bits are loaded first; while they are in flight the row's
 // history is counted for the segment with integer atomics in LDS (the order of their arrival cannot change a count), then
 // each thread finishes its 8 tokens.  Nothing is written in between, so one launch is one pass over the data.  1 row of 8197 tokens and
-// 64 of history 2.9 us (2.2 of it a launch), 32 rows of 100003 tokens with biases, masks and 4096 of history 9.3 (2.8 TB/s); histories of
+// 64 of history 3.0 us (2.2 of it a launch), 32 rows of 100003 tokens with biases, masks and 4096 of history 9.4 (2.8 TB/s); histories of
 // a song's frames cost a line of memory per token and segment.
 #include "gemm_core.h"
 

@@ -8,8 +8,9 @@
 // (row l & 31) takes its operands of four k-steps as 16 bytes, and so does one of v_mfma_f32_16x16x32_f16 (row l & 15): half the
 // octets of a chunk, the upper 32 lanes those of the next chunk.  An octet lies in a dword as pairs (k, k + 1) 16 bits apart,
 // pair p at bits 4 p and 16 + 4 p, which is how two halves of a register come out of one AND.
-// Scales: for each 32-row tile [K / G rounded up][32] fp16, or with zero points pairs (s, 1024 + z) of fp16.  Rows behind the
-// last have the scale 0.
+// Scales: for each 32-row tile [K / G rounded up][32] fp16, or with zero points pairs (s, 1024 + z) of fp16.  No scale is packed
+// as 0, since products take quotients of them: a group whose scale is 0, and the rows behind the last, get the scale 1 and codes that are
+// their zero point.
 #pragma once
 #include "common.h"
 

@@ -146,8 +146,8 @@ __global__ __launch_bounds__(256) void pack_q4_scales_kernel(const f16* __restri
 // its part, so with weights below 2^11 every product fits fp16; where a part's weights reach more, all of them go in divided by
 // 2^5, and e tells the sums.
 //
-// Measured in a graph (of it 2.2 us a launch): 1 x 8197 x 3072 with its norm 6.5 us, 8 x 5120 x 3072 with its norm 5.5, 8 x 3072 x 8192
-// with a residual 5.2 (2.5 TB/s), 8 x 16384 x 3072 with norm and SiLU 8.4 (3.1 TB/s), 48 x 3072 x 3072 in groups of 64 6.9.  What is
+// Measured in a graph (of it 2.2 us a launch): 1 x 8197 x 3072 with its norm 6.4 us, 8 x 5120 x 3072 with its norm 5.6, 8 x 3072 x 8192
+// with a residual 5.2 (2.5 TB/s), 8 x 16384 x 3072 with norm and SiLU 8.6 (3.0 TB/s), 48 x 3072 x 3072 in groups of 64 6.9.  What is
 // left is about 1 us to the first bytes, the address path, the conversion (9 instructions for 8 codes) and the sums' way through LDS.
 template <int NT, int XO, int GS, bool ZP, bool NORM>
 struct Q4Pair {
@@ -613,6 +613,7 @@ static int mm_q4_plan(int M, int N, int K, Q4Among among) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 64) return ECD_EINVAL;
   return M <= 16 ? 0 : gemm_q4_plan(M, N, K, among);
 }
+// (for tuning, as the few-row plans with a norm in one part are: no call of the package asks for them)
 int ecd_mm_q4_plan(int M, int N, int K) { return mm_q4_plan(M, N, K, Q4_ONLY_TILES); }
 int ecd_mm_q4_choice(int M, int N, int K) { return mm_q4_plan(M, N, K, Q4_PLAIN); }
 int ecd_mm_q4_norm_choice(int M, int N, int K, int silu) { return mm_q4_plan(M, N, K, silu ? Q4_NORM_SILU : Q4_NORM); }

@@ -1233,7 +1233,10 @@ class HeartMuLaLite:
         all of a codebook); before ``min_ms`` no frame ends the song.  process_logits does so on the guided logits in fp32;
         teacher forcing ignores it.  Penalties and biases are at most 2^100.  Logits above fp16's range count as its largest
         number, those below as -inf: a penalty or bias that takes every allowed logit of a codebook there leaves nothing to draw,
-        which ends the take (also before ``min_ms``; in the first frame: a take of no frames, [8, 0])."""
+        which ends the take (also before ``min_ms``; in the first frame: a take of no frames, [8, 0]).
+
+        4-bit layers: up to 16 rows of a step take the norms in two fp16 parts, more (and the prompt's) mostly rounded to fp16 once,
+        as int8 layers do."""
         if seed is not None and seed >= 0:
             torch.manual_seed(seed)
         if a8 and not self.backbone.eight():

@@ -707,7 +707,8 @@ int ecd_pack_q4(const void* q, const void* s, const void* z, int N, int K, int g
  *   the tiles.  With nw any of these but 0 takes x' rounded to fp16; 32 more takes it in two fp16 parts, as 0 does.  With nw:
  *   ecd_mm_q4_norm_choice (silu: in two parts, as the roundings of both factors would add up).  ws: 16-byte aligned workspace of ecd_mm_q4_ws_bytes (norm: whether nw is given; any contents).
  * ldx up to 2^26 (plans of tiles without nw: 2^23).
- * A row's result does not depend on the other rows; its last bits depend on the plan (the order of the sums). */
+ * A row's result does not depend on the other rows; its last bits depend on the plan (the order of the sums), and with nw in plan 0 on
+ * whether M is above 8.  ecd_mm_q4_plan and plans 17 .. 19 with nw but without the 32 are for tuning: no choice gives the latter. */
 int ecd_mm_q4_plan(int M, int N, int K);
 int ecd_mm_q4_choice(int M, int N, int K);
 int ecd_mm_q4_norm_choice(int M, int N, int K, int silu);
