@@ -107,8 +107,10 @@ if __name__ == "__main__":
     ap.add_argument("dst")
     ap.add_argument("--keep-emb-bf16", action="store_true")
     ap.add_argument("--int4", action="store_true")
-    ap.add_argument("--group", type=int, choices=(32, 64, 128), default=128)
+    ap.add_argument("--group", type=int, choices=(32, 64, 128))
     ap.add_argument("--zeros", action="store_true")
     a = ap.parse_args()
-    path = convert_file(a.src, a.dst, keep_emb=a.keep_emb_bf16, group=a.group if a.int4 else None, zeros=a.zeros)
+    if (a.zeros or a.group) and not a.int4:
+        ap.error("--group and --zeros are for --int4")
+    path = convert_file(a.src, a.dst, keep_emb=a.keep_emb_bf16, group=(a.group or 128) if a.int4 else None, zeros=a.zeros)
     print(path.name, round(path.stat().st_size / 1e9, 3), "GB")
