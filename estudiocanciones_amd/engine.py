@@ -1245,7 +1245,7 @@ class HeartMuLaLite:
             raise NotImplementedError("generate: int8 activations need a head_dim of 64, 128, 256 or 384 and 1, 2, 3, 4, 6 or 8 "
                                       "query heads per kv head")
         rules = float(repetition), float(presence), float(frequency), int(window)
-        min_frames = -(-int(min_ms) // FRAME_MS)
+        min_frames = math.ceil(min_ms / FRAME_MS)
         self._check_rules(*rules, bias, allowed, min_frames)
         text = torch.as_tensor(text, dtype=torch.int64)
         P = int(text.numel())

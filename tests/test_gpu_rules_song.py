@@ -70,3 +70,13 @@ def test_int8_activations_need_eight_bits_in_the_backbone_alone(dev):
     _, _, m = model(dev, 128, True, ("backbone",))
     with pytest.raises(NotImplementedError, match="int8 activations"):
         m.generate(text, 3, max_ms=800, a8=True)
+
+
+@pytest.mark.parametrize("min_ms,frames", [(80, 1), (80.5, 2), (159.9, 2), (160.25, 3)])
+def test_a_shortest_length_between_frames(dev, song, min_ms, frames):
+    """A bias towards the end codes: the song ends in the first frame at or past the shortest length."""
+    import torch
+    bias = torch.zeros(N_CB, AUDIO_VOCAB)
+    bias[:, 8193:] = 200.0
+    for t in song(bias=bias, min_ms=min_ms):
+        assert t.shape == (N_CB, frames) and (t < 8193).all()
