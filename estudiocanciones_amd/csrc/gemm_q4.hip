@@ -11,10 +11,10 @@
 // K advances in 64-wide chunks through an NS-stage ring in LDS, loaded by LDS DMA: x rows with their 16-byte pieces swizzled
 // by row (x_swz), codes as packed, scales of the chunk's groups.
 //
-// 2048 x 16384 x 3072 with SiLU: 175 to 181 us for a few launches, 200 to 207 for sixty in a row, when the clock has fallen: 1.15 and 1.0
-// PFLOP/s (the library's product of fp16 matrices of these sizes: 153 and 172 to 177), matrix units 64% busy; about 4 vector instructions hide behind each product, the rest of the conversion (30 us), the scales (15 to 20)
-// and the results' way out (10) add up.  187 x 3072 x 8192: 21 us, of it 4 the join; there the latency of a
-// step bounds (1.3 us for 0.7 of products).
+// 2048 x 16384 x 3072 with SiLU: 175 to 181 us for a few launches, 200 to 207 for sixty in a row, when the clock has fallen: 1.15 and
+// 1.0 PFLOP/s (the library's product of fp16 matrices of these sizes: 153 and 172 to 177), matrix units 64% busy; about 4 vector
+// instructions hide behind each product, the rest of the conversion (30 us), the scales (15 to 20) and the results' way out (10) add up.
+// 187 x 3072 x 8192: 21 us, of it 4 the join; there the latency of a step bounds (1.3 us for 0.7 of products).
 #include "gemm_core.h"
 #include "q4.h"
 

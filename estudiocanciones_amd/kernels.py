@@ -1305,8 +1305,9 @@ def _rows_of(t, M, N, dev, call, name):
 
 def mm_q4(x, w, res=None, nw=None, eps=1e-5, out=None):
     """y = x @ w^T (+ res) -> [M, N] for 4-bit weights ``w`` (pack_q4) and x [M, K] fp16, or with ``nw`` [K] the RMS norm of
-    x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end (of products of more than 16 rows
-    those that go by matrix tiles, most of them, round the normed rows to fp16 before: 2.9e-4 of the result for 2.1e-4).  Any number of rows.
+    x's rows: scales, sums, the norm's statistics and the residual in fp32, one rounding at the end (of products of more than 16
+    rows those that go by matrix tiles, most of them, round the normed rows to fp16 before: 2.9e-4 of the result for 2.1e-4).
+    Any number of rows.
     ``out`` may be ``res``, or apart from it, and not x (columns of the same rows that do not meet are apart)."""
     return _mm_q4("mm_q4", x, w, w.N, res, nw, eps, out, False)
 
